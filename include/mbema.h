@@ -339,6 +339,76 @@ int mbema_decode_update(const int64_t* tok, const float* rhos, float* state, int
  * mbema_decode_advance adds one to it, ordered on the stream. */
 int mbema_decode_advance(int32_t* t_now_dev, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Branches: several continuations of every sequence of a decode state, attended together.  The reference has no decode
+ * loop; the mathematics is that of the decode entry points above, for many rows at once.
+ *   B sequences, S branches of each; a branch holds `len` kept tokens of its own behind the sequence's prefix and up to
+ *   max_new (<= 32) staged ones.  Row (b, s, j) of a call with n staged tokens is step t0 + len + j: it sees the prefix, the
+ *   branch's kept tokens and its staged tokens before j.  All branches of a sequence have the same length.
+ * The prefix (state, last_t, active, n_active: the layout above) is read and left alone until mbema_branches_adopt; the other
+ * buffers belong to the branches and are filled by the calls below (no initial values needed).
+ *   mbema_branches_init    empty branches at step t_now (or *t_now_dev)
+ *   mbema_branches_extend  keeps the n_pending tokens staged by the call before (0 after mbema_branches_keep), then stages
+ *                          tok [B,S,n] i64 (-1: none; the step passes all the same): C_q [B,S,n,N] f32 = state of every token
+ *                          just before its own step
+ *   mbema_branches_keep    keeps the first counts[b] (i64, clamped to 0..n_pending) staged tokens of sequence b, drops the others
+ *   mbema_branches_attend  O[b,s,j,h,:] = softmax over all V_total slots of q.K/sqrt(hd) times V with the slot states that row
+ *                          sees; q, O [B,S,n,H,64] of q_dtype, E_k/E_v [V,H*64], n = the staged count.  mode
+ *                          MBEMA_MODE_TC_BF16: tensor cores (bf16 q and tables, N = 64 or 128), MBEMA_MODE_FP32: fp32 arithmetic
+ *   mbema_branches_adopt   moves branch[b] (i64) of every sequence into its prefix; step numbers move so that the next step of
+ *                          every sequence is t_next (>= t0 + len)
+ * *overflow: 1 an own or active list is full, 2 a token is outside [0, V) (and not -1), 3 branch[b] is outside [0, S),
+ * 4 t_next lies before a branch's end (that sequence stays as it was).
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct mbema_branches {
+    const float* rhos;      /* [N] */
+    float* state;           /* [B,V,N] */
+    int32_t* last_t;        /* [B,V] */
+    int32_t* active;        /* [B,Kcap] */
+    int32_t* n_active;      /* [B] */
+    int32_t* pos;           /* [B,V] place of a slot in the active list, -1: not listed */
+    int32_t* t0;            /* [1] */
+    int32_t* len;           /* [B,S] */
+    int32_t* own_n;         /* [B,S] slots a branch has touched */
+    int32_t* own_new;       /* [B,S] those of them that the prefix does not list */
+    int32_t* own_slot;      /* [B,S,cap] */
+    int32_t* own_t;         /* [B,S,cap] step of the last update */
+    float* own_state;       /* [B,S,cap,N] value right after it */
+    uint32_t* touched;      /* [B,S,ceil(Kcap/32)] bit per listed prefix slot */
+    int32_t* st_tok;        /* [B,S,max_new] staged tokens, -1: none */
+    int32_t* st_own;        /* [B,S,max_new] place in the own list, -1 */
+    int32_t* st_pos;        /* [B,S,max_new] place in the active list of a slot first touched here, -1 */
+    uint32_t* st_same;      /* [B,S,max_new] the staged places that hold the same token */
+    int32_t* st_new;        /* [B,S,max_new] 1: this place lists a slot that nothing before it lists */
+    float* st_state;        /* [B,S,max_new,N] C_q of the staged tokens */
+    void* pre_op;           /* [B,Kcap,N] fp16 or NULL: prefix states at the first staged step, operands of the tensor cores */
+    void* own_op;           /* [B,S,cap,N] fp16 or NULL: the same of the own slots */
+    int32_t* overflow;      /* [1] */
+    int64_t B, S, V, N, Kcap, cap, max_new;
+} mbema_branches;
+int mbema_branches_init(const mbema_branches* br, int64_t t_now, const int32_t* t_now_dev, void* stream);
+int mbema_branches_extend(const mbema_branches* br, const int64_t* tok, int64_t n, int64_t n_pending, float* C_q, void* stream);
+int mbema_branches_keep(const mbema_branches* br, const int64_t* counts, int64_t n_pending, void* stream);
+size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode);
+int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
+                          const float* W_pe, void* O, int64_t n, int64_t H, int64_t hd, int64_t V_total, int flags, int mode,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int mbema_branches_adopt(const mbema_branches* br, const int64_t* branch, int64_t t_next, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Verification of drafted tokens.  p [R,G+1,V] target probabilities (row stride p_row, position stride p_pos, in elements),
+ * q [R,G,V] those the drafts were drawn from, or NULL: drafts that were not drawn (q = 1 at the draft); both of `dtype`;
+ * drafted [R,G] i64 (a token outside [0, V) ends its row's drafts), uniforms [R,G+1] f32 in [0, 1).
+ *   draft j stands while uniforms[j] * q_j(x_j) < p_j(x_j); a = number of drafts that stand -> n_accepted [R] i64
+ *   next token: smallest i with sum_{k<=i} w_k > uniforms[G] * sum w, w = max(p_a - q_a, 0) where draft a was rejected (p_a if
+ *   that is zero everywhere), w = p_a where the drafts ended; entries that are negative or not finite count as 0; -1: no mass
+ *   tokens [R,G+1] i64: the drafts that stand, the next token, then -1
+ * Products, differences and sums in 64 bits.
+ * ---------------------------------------------------------------------------------------------- */
+int mbema_verify_drafts(const void* p, int64_t p_row, int64_t p_pos, const void* q, int64_t q_row, int64_t q_pos, int dtype,
+                        const int64_t* drafted, const float* uniforms, int64_t* n_accepted, int64_t* tokens, int64_t R,
+                        int64_t G, int64_t V, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,182 @@
+"""Branches of a decode state: several continuations or drafted tokens of every sequence, attended together.
+
+    br = st.fork(S, t_now)                       # st: DecodeState of B sequences, at step t_now
+    C_q = br.extend(tok)                         # tok int64 [B, S, n]: n new tokens a branch; C_q [B, S, n, N] for the query gate
+    O = br.attend(q, E_k, E_v, W_pe)             # q [B, S, n, H, 64] -> O, once a layer
+    br.keep(counts)                              # counts [B]: the first counts[b] of the n tokens stay
+    br.adopt(branch, t_next)                     # branch [B]: one branch of every sequence becomes the state of `st`
+
+Row j of a branch is one iteration of the reference's loop body (mathbrain/flash_ema_attention.py:46-82), as a decode step is: it
+sees the slots of the sequence's prefix, the branch's kept tokens and its staged tokens before j.  The prefix stays where it is
+and is read by all branches; a branch holds only the slots that it has touched.
+
+Sampling: S continuations of a prompt, `extend` with one token each; the tokens of the call before are kept by themselves.
+Drafts:   S = 1, `extend` with the last token and G drafted ones; `verify_drafts` (mathbrain_b200/verify.py) says how many stand,
+          `keep(n_accepted + 1)` drops the others.
+Scoring candidates: `extend`, `attend`, `keep` of zeros.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _dt, _ptr, _require_cuda, _stream, get_options
+
+_BY_REF = ctypes.byref
+
+
+class Branches:
+    """Made by DecodeState.fork.  While the branches live the state must not be updated (its own tokens are the branches'
+    prefix); a call on them after an update raises."""
+
+    def __init__(self, prefix, branches, t_now, capacity=1024, max_new=16):
+        B, V, N, Kcap = prefix.B, prefix.V, prefix.N, prefix.cap
+        S, cap, max_new = int(branches), int(capacity), int(max_new)
+        if S < 1 or cap < 1 or not 1 <= max_new <= 32:
+            raise _lib.MbemaError("fork: %d branches of capacity %d with %d new tokens at most (1 to 32)" % (S, cap, max_new))
+        self.prefix, self.B, self.S, self.V, self.N = prefix, B, S, V, N
+        self.capacity, self.max_new = cap, max_new
+        self._epoch = prefix._epoch
+        self._staged = 0             # tokens of the last extend that keep has not decided on
+        dev = prefix.state.device
+        expected = (("state", torch.float32, (B, V, N)), ("last_t", torch.int32, (B, V)), ("active", torch.int32, (B, Kcap)),
+                    ("n_active", torch.int32, (B,)), ("rhos", torch.float32, (N,)))
+        for name, dtype, shape in expected:
+            t = getattr(prefix, name)
+            if t.device != dev or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+                raise _lib.MbemaError("fork: the state's %s is %s %s on %s, expected contiguous %s %s on %s"
+                                      % (name, t.dtype, tuple(t.shape), t.device, dtype, shape, dev))
+        _require_cuda(prefix.state)
+        i32, f32 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.float32, device=dev)
+        self._hold = dict(
+            rhos=prefix.rhos, state=prefix.state, last_t=prefix.last_t, active=prefix.active, n_active=prefix.n_active,
+            pos=torch.empty(B, V, **i32), t0=torch.empty(1, **i32), len=torch.empty(B, S, **i32), own_n=torch.empty(B, S, **i32),
+            own_new=torch.empty(B, S, **i32), own_slot=torch.empty(B, S, cap, **i32), own_t=torch.empty(B, S, cap, **i32),
+            own_state=torch.empty(B, S, cap, N, **f32), touched=torch.empty(B, S, (Kcap + 31) // 32, **i32),
+            st_tok=torch.empty(B, S, max_new, **i32), st_own=torch.empty(B, S, max_new, **i32),
+            st_pos=torch.empty(B, S, max_new, **i32), st_same=torch.empty(B, S, max_new, **i32),
+            st_new=torch.empty(B, S, max_new, **i32), st_state=torch.empty(B, S, max_new, N, **f32), overflow=torch.empty(1, **i32))
+        self._c = _lib.BranchesStruct(**{k: _ptr(t) for k, t in self._hold.items()}, B=B, S=S, V=V, N=N, Kcap=Kcap, cap=cap,
+                                      max_new=max_new)
+        self._lib = _lib.load()
+        with torch.cuda.device(dev):
+            rc = self._lib.mbema_branches_init(_BY_REF(self._c), int(t_now), _ptr(prefix.t_dev), _stream())
+        _lib.check(rc, "mbema_branches_init")
+
+    def _alive(self, *operands):
+        if self.prefix is None:
+            raise _lib.MbemaError("branches: adopted already")
+        if self.prefix._epoch != self._epoch:
+            raise _lib.MbemaError("branches: the state they were forked from has been updated since")
+        dev = self._hold["state"].device
+        for t in operands:
+            if t.device != dev:
+                raise _lib.MbemaError("branches: operand on %s, state on %s" % (t.device, dev))
+
+    def _on_device(self, fn, *args):
+        dev = self._hold["state"].get_device()
+        if dev == torch.cuda.current_device():
+            return fn(*args)
+        with torch.cuda.device(dev):
+            return fn(*args)
+
+    def extend(self, tok):
+        """Stage n <= max_new new tokens of every branch (int64 [B, S, n]; -1: this branch has none at this step) and return
+        C_q [B, S, n, N] float32, the state of each token just before its own step (0 if never seen).  Tokens staged by the
+        call before are kept unless `keep` has decided on them."""
+        self._alive(tok)
+        if tok.dim() != 3 or tok.shape[:2] != (self.B, self.S) or not 1 <= tok.shape[2] <= self.max_new:
+            raise _lib.MbemaError("extend: tokens %s, expected [%d, %d, 1 to %d]" % (tuple(tok.shape), self.B, self.S, self.max_new))
+        if tok.dtype != torch.int64:
+            raise _lib.MbemaError("extend: tokens of %s, expected int64" % tok.dtype)
+        return self._on_device(self._extend, tok.contiguous())
+
+    def _extend(self, tok):
+        n = tok.shape[2]
+        C_q = torch.empty(self.B, self.S, n, self.N, dtype=torch.float32, device=tok.device)
+        rc = self._lib.mbema_branches_extend(_BY_REF(self._c), _ptr(tok), n, self._staged, _ptr(C_q), _stream())
+        _lib.check(rc, "mbema_branches_extend")
+        self._staged = n
+        return C_q
+
+    def keep(self, counts):
+        """Keep the first counts[b] of the staged tokens in every branch of sequence b and drop the others (integers [B] on
+        the GPU; clamped to 0..n).  The branches then have no staged tokens until the next `extend`."""
+        self._alive(counts)
+        if counts.shape != (self.B,) or counts.is_floating_point() or counts.dtype == torch.bool:
+            raise _lib.MbemaError("keep: counts %s of %s, expected [%d] integers" % (tuple(counts.shape), counts.dtype, self.B))
+        return self._on_device(self._keep, counts.long().contiguous())
+
+    def _keep(self, counts):
+        rc = self._lib.mbema_branches_keep(_BY_REF(self._c), _ptr(counts), self._staged, _stream())
+        _lib.check(rc, "mbema_branches_keep")
+        self._staged = 0
+
+    def attend(self, q, E_k, E_v, W_pe, V_total=None, use_silu=True, listed_only=False, mode=None):
+        """O [B, S, n, H, 64] of q's dtype for the n staged rows of every branch.  q [B, S, n, H, 64] float32 or bfloat16;
+        E_k, E_v [V, H*64] projected slot embeddings; W_pe [N, H*64].  Softmax over all V_total slots (the vocabulary by
+        default), those that a row does not see with score 0 and value 0; listed_only: over the seen ones alone (a row that
+        has seen none gets 0)."""
+        self._alive(q, E_k, E_v, W_pe)
+        n = self._staged
+        if n == 0:
+            raise _lib.MbemaError("attend: no staged tokens (call extend first)")
+        if q.dim() != 5 or q.shape[:3] != (self.B, self.S, n) or q.shape[4] != 64 or q.shape[3] < 1:
+            raise _lib.MbemaError("attend: q %s, expected [%d, %d, %d, H, 64]" % (tuple(q.shape), self.B, self.S, n))
+        D = q.shape[3] * 64
+        if E_k.shape != (self.V, D) or E_v.shape != (self.V, D) or W_pe.shape != (self.N, D):
+            raise _lib.MbemaError("attend: E_k %s, E_v %s, W_pe %s, expected [%d, %d] twice and [%d, %d]"
+                                  % (tuple(E_k.shape), tuple(E_v.shape), tuple(W_pe.shape), self.V, D, self.N, D))
+        return self._on_device(self._attend, q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode)
+
+    def _attend(self, q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode):
+        q, E_k, W = q.contiguous(), E_k.contiguous(), W_pe.float().contiguous()
+        E_v = E_v.to(E_k.dtype).contiguous()
+        if mode is None:
+            mode = get_options()["mode"]
+        if mode not in ("fp32", "tc_bf16", "auto"):
+            raise ValueError("mode must be 'fp32', 'tc_bf16' or 'auto'")
+        code = _lib.MODE_FP32
+        n, H = q.shape[2], q.shape[3]
+        O = torch.empty_like(q)
+        need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, n, H, self.prefix.cap, self.capacity, code)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        flags = (_lib.FLAG_SILU if use_silu else 0) | (_lib.FLAG_LISTED_ONLY if listed_only else 0)
+        rc = self._lib.mbema_branches_attend(_BY_REF(self._c), _ptr(q), _dt(q), _ptr(E_k), _ptr(E_v), _dt(E_k), _ptr(W), _ptr(O), n, H,
+                                             64, int(self.V if V_total is None else V_total), flags, code, _ptr(ws), need, _stream())
+        _lib.check(rc, "mbema_branches_attend")
+        return O
+
+    def adopt(self, branch, t_next):
+        """Branch branch[b] (integers [B] on the GPU) of every sequence becomes the state's own: its tokens join the resident
+        state and the active list.  Staged tokens are kept unless `keep` has decided on them.  The next step of every sequence
+        is t_next afterwards, whatever the branches' lengths (not before the longest one's end).  Ends these branches."""
+        self._alive(branch)
+        if branch.shape != (self.B,) or branch.is_floating_point() or branch.dtype == torch.bool:
+            raise _lib.MbemaError("adopt: branch %s of %s, expected [%d] integers" % (tuple(branch.shape), branch.dtype, self.B))
+        return self._on_device(self._adopt, branch.long().contiguous(), int(t_next))
+
+    def _adopt(self, branch, t_next):
+        st = self.prefix
+        if self._staged:
+            self._keep(torch.full((self.B,), self._staged, dtype=torch.int64, device=branch.device))
+        _lib.check(self._lib.mbema_branches_adopt(_BY_REF(self._c), _ptr(branch), t_next, _stream()), "mbema_branches_adopt")
+        st._epoch += 1
+        st.overflow.copy_(torch.where(self._hold["overflow"] == 1, self._hold["overflow"], st.overflow))
+        if st.t_dev is not None:
+            st.t_dev.fill_(t_next)
+        self.prefix = None
+
+    @property
+    def lengths(self):
+        """Kept tokens of the branches, int32 [B, S] on the GPU."""
+        return self._hold["len"]
+
+    def check_overflow(self):
+        """Synchronises; raises if a list overflowed, a token was out of range, or adopt was given a branch or a step that it
+        cannot take."""
+        code = int(self._hold["overflow"].item())
+        if code:
+            raise _lib.MbemaError("branches: " + {1: "a list of touched slots (or the state's active list) is full",
+                                                  2: "token outside the vocabulary", 3: "adopt: no such branch",
+                                                  4: "adopt: t_next lies before the end of a branch"}.get(code, "status %d" % code))

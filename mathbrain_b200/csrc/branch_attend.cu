@@ -1,0 +1,366 @@
+// Attention of the rows of a decode state's branches (mbema_branches_attend): fp32 arithmetic on the CUDA cores, and the merge.
+//
+// A slot of the prefix that a branch has not touched has the same state in every branch at the same step, so its gate
+// SiLU(M W_pe), K = E_k * gate and V = E_v * gate are formed once a (sequence, step) and read by all S branches; the slots that a
+// branch has touched are its own, and a row sees its prefix through a mask without them:
+//     softmax over {prefix slots not touched} + {own slots} + {tokens staged before the row} + {V_total - listed, score 0, value 0}.
+// A CTA takes one job (a chunk of slots) for one step and head: K and V tiles of 64 slots in shared memory, the scores of up to 64
+// branches against them, online softmax, one partial (m, l, o) per row.  k_branch_merge joins the partials, adds the few staged
+// tokens (each a dot product of N channels, in fp32) and the zero-score slots.
+#include <algorithm>
+
+#include "branches.cuh"
+
+namespace mbema {
+
+static constexpr int BA_THREADS = 256;
+static constexpr int BA_TILE = 64;       // slots a tile
+static constexpr int BA_ROWS = 64;       // branches a CTA
+static constexpr int BA_LD = 68;         // floats a row of the K and V tiles (16-byte rows, conflict-free columns)
+static constexpr int BM_WARPS = 4;
+static constexpr int BM_STAGED = 8;      // staged tokens at a time
+
+static size_t ba_smem(int N) {
+    return ((size_t)N * BR_HD + (size_t)BA_TILE * (N + 1) + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * BR_HD + BA_ROWS * (BA_TILE + 1) +
+            N + 3 * BA_ROWS + BA_TILE) * 4;
+}
+
+// grid: x = prefix jobs (B, blocks of 64 branches, chunks), then own jobs (B * S, chunks); y = head; z = step
+__global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    const mbema_branches& br = a.br;
+    const int N = (int)br.N, ldA = N + 1;
+    const int n = a.n, H = a.H, h = blockIdx.y, j = blockIdx.z;
+    const int SP = a.plan.SP, SO = a.plan.SO;
+    const int blocks = (int)((br.S + BA_ROWS - 1) / BA_ROWS);
+    const int64_t n_pre = (int64_t)br.B * blocks * SP;
+    const bool own = blockIdx.x >= n_pre;
+    int b, s0, rows, chunk, k_lo, k_hi;
+    if (!own) {
+        chunk = (int)(blockIdx.x % SP);
+        const int bb = (int)(blockIdx.x / SP);
+        b = bb / blocks;
+        s0 = (bb % blocks) * BA_ROWS;
+        rows = min(BA_ROWS, (int)br.S - s0);
+        k_lo = chunk * a.plan.chp;
+        k_hi = min(k_lo + a.plan.chp, min(br.n_active[b], (int)br.Kcap));
+    } else {
+        const int64_t x = blockIdx.x - n_pre;
+        chunk = (int)(x % SO);
+        const int64_t r = x / SO;
+        b = (int)(r / br.S);
+        s0 = (int)(r % br.S);
+        rows = 1;
+        k_lo = chunk * a.plan.cho;
+        k_hi = min(k_lo + a.plan.cho, br.own_n[r]);
+    }
+    if (k_lo >= k_hi) return;
+    const int64_t r0 = (int64_t)b * br.S + s0;
+    float* W_sh = smem;                                   // [N][64]
+    float* K_sh = W_sh + N * BR_HD;                       // [64][68]
+    float* V_sh = K_sh + BA_TILE * BA_LD;
+    float* q_sh = V_sh + BA_TILE * BA_LD;                 // [64][64], scaled to base-2 scores
+    float* P_sh = q_sh + BA_ROWS * BR_HD;                 // [64][65]
+    float* A_sh = P_sh + BA_ROWS * (BA_TILE + 1);         // [64][N+1]
+    float* l2r_sh = A_sh + BA_TILE * ldA;
+    float* m_sh = l2r_sh + N;
+    float* l_sh = m_sh + BA_ROWS;
+    float* al_sh = l_sh + BA_ROWS;
+    const int tid = threadIdx.x;
+    const int sr = tid >> 2, dg = tid & 3;
+    const int D = H * BR_HD;
+    for (int i = tid; i < N * BR_HD; i += BA_THREADS) W_sh[i] = a.W[(size_t)(i >> 6) * D + h * BR_HD + (i & 63)];
+    for (int i = tid; i < N; i += BA_THREADS) l2r_sh[i] = log2f(br.rhos[i]);
+    for (int i = tid; i < rows * BR_HD; i += BA_THREADS)
+        q_sh[i] = ld_dyn_f32(a.q, a.q_dt, ((((size_t)(r0 + (i >> 6))) * n + j) * H + h) * BR_HD + (i & 63)) * BR_SCORE_LOG2;
+    for (int i = tid; i < BA_ROWS; i += BA_THREADS) { m_sh[i] = -INFINITY; l_sh[i] = 0.f; }
+    const int tau = br.t0[0] + br.len[r0] + j;
+    const int oc = tid & 63, og = tid >> 6;               // output column, row group: rows og, og + 4, ...
+    float o[BA_ROWS / 4];
+#pragma unroll
+    for (int i = 0; i < BA_ROWS / 4; ++i) o[i] = 0.f;
+    for (int k0 = k_lo; k0 < k_hi; k0 += BA_TILE) {
+        const int tile = min(BA_TILE, k_hi - k0);
+        const int k = k0 + sr;
+        const bool ok = sr < tile;
+        int v = 0;
+        __syncthreads();                                  // the tile before is read
+        {
+            float dt = 0.f;
+            const float* row = nullptr;
+            if (ok && !own) {
+                v = br.active[(size_t)b * br.Kcap + k];
+                dt = (float)(tau - br.last_t[(size_t)b * br.V + v]);
+                row = br.state + ((size_t)b * br.V + v) * N;
+            } else if (ok) {
+                v = br.own_slot[(size_t)r0 * br.cap + k];
+                dt = (float)(tau - br.own_t[(size_t)r0 * br.cap + k]);
+                row = br.own_state + ((size_t)r0 * br.cap + k) * N;
+            }
+            for (int c = dg; c < N; c += 4) A_sh[sr * ldA + c] = ok ? row[c] * exp2f(dt * l2r_sh[c]) : 0.f;
+        }
+        __syncthreads();
+        float acc[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+        const float* arow = A_sh + sr * ldA;
+        const float* wcol = W_sh + dg * 16;
+#pragma unroll 4
+        for (int c = 0; c < N; ++c) {
+            const float av = arow[c];
+            const float4* wp = reinterpret_cast<const float4*>(wcol + c * BR_HD);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 w = wp[i];
+                acc[4 * i] = fmaf(av, w.x, acc[4 * i]);
+                acc[4 * i + 1] = fmaf(av, w.y, acc[4 * i + 1]);
+                acc[4 * i + 2] = fmaf(av, w.z, acc[4 * i + 2]);
+                acc[4 * i + 3] = fmaf(av, w.w, acc[4 * i + 3]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float4 ek = make_float4(0.f, 0.f, 0.f, 0.f), ev = ek;
+            if (ok) {
+                const size_t off = (size_t)v * D + h * BR_HD + dg * 16 + i;
+                ek = ld4_dyn_f32(a.Ek, a.e_dt, off);
+                ev = ld4_dyn_f32(a.Ev, a.e_dt, off);
+            }
+            float g[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) g[c] = a.silu ? acc[i + c] / (1.0f + expf(-acc[i + c])) : acc[i + c];
+            *reinterpret_cast<float4*>(K_sh + sr * BA_LD + dg * 16 + i) = make_float4(ek.x * g[0], ek.y * g[1], ek.z * g[2], ek.w * g[3]);
+            *reinterpret_cast<float4*>(V_sh + sr * BA_LD + dg * 16 + i) = make_float4(ev.x * g[0], ev.y * g[1], ev.z * g[2], ev.w * g[3]);
+        }
+        __syncthreads();
+        {   // scores: a thread holds one slot and takes every fourth row
+            const int slot = tid & 63;
+            const float4* kp = reinterpret_cast<const float4*>(K_sh + slot * BA_LD);
+            for (int row = tid >> 6; row < rows; row += 4) {
+                const float4* qp = reinterpret_cast<const float4*>(q_sh + row * BR_HD);
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float4 x = kp[i], y = qp[i];
+                    s = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
+                }
+                bool hide = slot >= tile;
+                if (!hide) hide = own ? br_hides_own(br, r0, j, k0 + slot) : br_hides_prefix(br, r0 + row, j, k0 + slot);
+                P_sh[row * (BA_TILE + 1) + slot] = hide ? -INFINITY : s;
+            }
+        }
+        __syncthreads();
+        for (int row = tid >> 5; row < rows; row += BA_THREADS / 32) {
+            const int lane = tid & 31;
+            float* p = P_sh + row * (BA_TILE + 1);
+            const float x = p[lane], y = p[lane + 32];
+            float mx = fmaxf(x, y);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float m_old = m_sh[row];
+            const float m_new = fmaxf(m_old, mx);
+            const float ref = m_new == -INFINITY ? 0.f : m_new;      // nothing visible so far: weights are zero all the same
+            const float ex = exp2f(x - ref), ey = exp2f(y - ref);
+            p[lane] = ex;
+            p[lane + 32] = ey;
+            const float sum = warp_sum(ex + ey);
+            if (lane == 0) {
+                const float alpha = exp2f(m_old - ref);
+                m_sh[row] = m_new;
+                l_sh[row] = l_sh[row] * alpha + sum;
+                al_sh[row] = alpha;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < BA_ROWS / 4; ++i) {
+            const int row = og + 4 * i;
+            if (row < rows) {
+                float x = o[i] * al_sh[row];
+                const float* p = P_sh + row * (BA_TILE + 1);
+                for (int c = 0; c < tile; ++c) x = fmaf(p[c], V_sh[c * BA_LD + oc], x);
+                o[i] = x;
+            }
+        }
+    }
+    __syncthreads();
+    const int slot = own ? SP + chunk : chunk;
+#pragma unroll
+    for (int i = 0; i < BA_ROWS / 4; ++i) {
+        const int row = og + 4 * i;
+        if (row < rows) {
+            const size_t at = ((((size_t)(r0 + row)) * n + j) * H + h) * (SP + SO) + slot;
+            a.po[at * BR_HD + oc] = o[i];
+            if (oc == 0) a.ml[at] = make_float2(m_sh[row], l_sh[row]);
+        }
+    }
+}
+
+// A warp per (row, head); a lane holds two output columns.
+__global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
+    __shared__ float s_c[BM_WARPS][BM_STAGED][128];
+    const mbema_branches& br = a.br;
+    const int N = (int)br.N, n = a.n, H = a.H, D = H * BR_HD;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t wid = (int64_t)blockIdx.x * BM_WARPS + warp;
+    if (wid >= (int64_t)br.B * br.S * n * H) return;
+    const int h = (int)(wid % H);
+    const int64_t row = wid / H;
+    const int j = (int)(row % n);
+    const int64_t r = row / n;
+    const int b = (int)(r / br.S);
+    const int SP = a.plan.SP, SO = a.plan.SO;
+    const int na = min(br.n_active[b], (int)br.Kcap), no = br.own_n[r];
+    const int np = (na + a.plan.chp - 1) / a.plan.chp, nq = (no + a.plan.cho - 1) / a.plan.cho;
+    const size_t base = (size_t)wid * (SP + SO);
+    float M = -INFINITY;
+    for (int p = lane; p < np + nq; p += 32) M = fmaxf(M, a.ml[base + (p < np ? p : SP + p - np)].x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    float rest = 0.f;
+    if (!a.listed_only) {
+        int listed = na + br.own_new[r];
+        for (int i = 0; i < j; ++i) listed += br.st_new[br_index(br, r, i)];
+        rest = fmaxf(a.v_total - (float)listed, 0.f);
+        if (rest > 0.f) M = fmaxf(M, 0.f);
+    }
+    float L = 0.f, o0 = 0.f, o1 = 0.f;
+    if (M > -INFINITY) {
+        L = rest > 0.f ? rest * exp2f(-M) : 0.f;
+        for (int p = 0; p < np + nq; ++p) {
+            const size_t at = base + (p < np ? p : SP + p - np);
+            const float2 ml = a.ml[at];
+            const float w = exp2f(ml.x - M);
+            const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
+            L = fmaf(ml.y, w, L);
+            o0 = fmaf(x.x, w, o0);
+            o1 = fmaf(x.y, w, o1);
+        }
+    }
+    if (j > 0) {
+        const size_t qoff = (size_t)wid * BR_HD + 2 * lane;
+        const float q0 = ld_dyn_f32(a.q, a.q_dt, qoff) * BR_SCORE_LOG2, q1 = ld_dyn_f32(a.q, a.q_dt, qoff + 1) * BR_SCORE_LOG2;
+        const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
+        for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
+            const int cnt = min(BM_STAGED, j - i0);
+            __syncwarp();
+            for (int c = lane; c < N; c += 32) {
+                const float l2r = log2f(br.rhos[c]);
+                for (int i = 0; i < cnt; ++i)
+                    s_c[warp][i][c] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * l2r);
+            }
+            __syncwarp();
+            float x0[BM_STAGED], x1[BM_STAGED];
+#pragma unroll
+            for (int i = 0; i < BM_STAGED; ++i) x0[i] = x1[i] = 0.f;
+            for (int c = 0; c < N; ++c) {
+                const float2 w = Wc[(size_t)c * (D / 2)];
+#pragma unroll
+                for (int i = 0; i < BM_STAGED; ++i) {
+                    if (i < cnt) {
+                        const float m = s_c[warp][i][c];
+                        x0[i] = fmaf(m, w.x, x0[i]);
+                        x1[i] = fmaf(m, w.y, x1[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < BM_STAGED; ++i) {
+                if (i >= cnt) continue;
+                const int place = i0 + i;
+                const size_t at = br_index(br, r, place);
+                const int v = br.st_tok[at];
+                const unsigned before = (1u << j) - 1u;                                  // j <= 31
+                if (v < 0 || ((br.st_same[at] & before) >> place) != 1u) continue;        // none, or repeated before this row
+                const float g0 = a.silu ? x0[i] / (1.0f + expf(-x0[i])) : x0[i], g1 = a.silu ? x1[i] / (1.0f + expf(-x1[i])) : x1[i];
+                const size_t e = (size_t)v * D + h * BR_HD + 2 * lane;
+                const float s = warp_sum(q0 * (ld_dyn_f32(a.Ek, a.e_dt, e) * g0) + q1 * (ld_dyn_f32(a.Ek, a.e_dt, e + 1) * g1));
+                const float m_new = fmaxf(M, s);
+                const float alpha = exp2f(M - m_new), p = exp2f(s - m_new);
+                L = fmaf(L, alpha, p);
+                o0 = fmaf(p, ld_dyn_f32(a.Ev, a.e_dt, e) * g0, o0 * alpha);
+                o1 = fmaf(p, ld_dyn_f32(a.Ev, a.e_dt, e + 1) * g1, o1 * alpha);
+                M = m_new;
+            }
+        }
+    }
+    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);      // no slot at all: zero; a NaN stays one
+    const size_t at = (size_t)wid * BR_HD + 2 * lane;
+    if (a.q_dt == MBEMA_F32) {
+        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.O) + at) = make_float2(o0 * inv, o1 * inv);
+    } else {
+        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.O) + at) = __floats2bfloat162_rn(o0 * inv, o1 * inv);
+    }
+}
+
+// Chunks: enough jobs for about four CTAs an SM, none shorter than a tile of 64 slots nor longer than sixteen.
+BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
+    (void)mode;
+    auto tiles = [&](int64_t lists, int64_t slots) {
+        const int64_t all = lists * n * H * ((slots + BA_TILE - 1) / BA_TILE);
+        return std::min<int64_t>(16, std::max<int64_t>(1, all / (4 * 148)));
+    };
+    BranchPlan p;
+    p.chp = (int)(BA_TILE * tiles(B * ((S + BA_ROWS - 1) / BA_ROWS), Kcap));
+    p.cho = (int)(BA_TILE * tiles(B * S, cap));
+    p.SP = (int)((Kcap + p.chp - 1) / p.chp);
+    p.SO = (int)((cap + p.cho - 1) / p.cho);
+    return p;
+}
+
+int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
+    const mbema_branches& br = a.br;
+    const int64_t jobs = br.B * ((br.S + BA_ROWS - 1) / BA_ROWS) * a.plan.SP + br.B * br.S * a.plan.SO;
+    if (jobs > 0x7fffffff || a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
+    const size_t smem = ba_smem((int)br.N);
+    MBEMA_CUDA_TRY(cudaFuncSetAttribute(k_branch_attend, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    k_branch_attend<<<dim3((unsigned)jobs, (unsigned)a.H, (unsigned)a.n), BA_THREADS, smem, st>>>(a);
+    return check_launch();
+}
+
+int launch_branch_merge(const BranchArgs& a, cudaStream_t st) {
+    const int64_t warps = a.br.B * a.br.S * a.n * a.H;
+    if (warps > (int64_t)0x7fffffff * BM_WARPS) return MBEMA_ERR_UNSUPPORTED;
+    k_branch_merge<<<(unsigned)((warps + BM_WARPS - 1) / BM_WARPS), BM_WARPS * 32, 0, st>>>(a);
+    return check_launch();
+}
+
+}  // namespace mbema
+
+using namespace mbema;
+
+static bool plan_sizes_ok(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap) {
+    return B >= 0 && S >= 1 && n >= 1 && n <= BR_MAX_NEW && H >= 1 && Kcap >= 1 && cap >= 1;
+}
+
+extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
+    if (!plan_sizes_ok(B, S, n, H, Kcap, cap)) return 0;
+    const BranchPlan p = branch_plan(B, S, n, H, Kcap, cap, mode);
+    return align_up((size_t)(B * S * n * H) * (p.SP + p.SO) * (2 + BR_HD) * 4, 256) + 256;
+}
+
+extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
+                                     const float* W_pe, void* O, int64_t n, int64_t H, int64_t hd, int64_t V_total, int flags, int mode,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+    if (!br) return MBEMA_ERR_NULL;
+    if (!plan_sizes_ok(br->B, br->S, n, H, br->Kcap, br->cap) || n > br->max_new || br->V < 1 || br->N < 1) return MBEMA_ERR_SHAPE;
+    if (hd != BR_HD || br->N > 128 || br->max_new > BR_MAX_NEW) return MBEMA_ERR_UNSUPPORTED;
+    if (br->B == 0) return MBEMA_OK;
+    if (!q || !E_k || !E_v || !W_pe || !O || !workspace || !br->state || !br->active || !br->own_state || !br->st_state) return MBEMA_ERR_NULL;
+    if ((q_dtype != MBEMA_F32 && q_dtype != MBEMA_BF16) || (e_dtype != MBEMA_F32 && e_dtype != MBEMA_BF16)) return MBEMA_ERR_DTYPE;
+    if (((uintptr_t)q | (uintptr_t)E_k | (uintptr_t)E_v | (uintptr_t)W_pe | (uintptr_t)O | (uintptr_t)workspace) & 15) return MBEMA_ERR_ALIGN;
+    if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
+    BranchArgs a;
+    a.br = *br;
+    a.q = q; a.Ek = E_k; a.Ev = E_v; a.W = W_pe; a.O = O;
+    a.q_dt = q_dtype; a.e_dt = e_dtype; a.n = (int)n; a.H = (int)H;
+    a.v_total = (float)V_total;
+    a.silu = (flags & MBEMA_FLAG_SILU) ? 1 : 0;
+    a.listed_only = (flags & MBEMA_FLAG_LISTED_ONLY) ? 1 : 0;
+    a.plan = branch_plan(br->B, br->S, n, H, br->Kcap, br->cap, mode);
+    const size_t parts = (size_t)(br->B * br->S * n * H) * (a.plan.SP + a.plan.SO);
+    a.po = reinterpret_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.po + parts * BR_HD);
+    int rc = launch_branch_attend_fp32(a, (cudaStream_t)stream);
+    return rc != MBEMA_OK ? rc : launch_branch_merge(a, (cudaStream_t)stream);
+}

@@ -1,0 +1,235 @@
+// Branches of a decode state: bookkeeping of kept and staged tokens (the attention over them: branch_attend.cu).
+//
+// A branch touches few of its sequence's slots, so it holds only those: their value right after the last update and the step
+// of it, as the resident state does.  A staged token's state is
+//     C_i = kept value * rho^(t_i - t_kept) + sum over staged i' < i with the same token of rho^(t_i - t_i'),
+// linear in its occurrences, so all staged tokens are independent of one another; powers and sums in double, rounded once (a
+// token repeated at every step amplifies a bias of rho by 1/(1 - rho)).
+// Bound by latency: chains of a few dependent loads for B S n rows of 4 N bytes.  The operand copies behind it move 6 N bytes a
+// listed slot.
+#include "branches.cuh"
+
+namespace mbema {
+
+static constexpr int BS_THREADS = 128;
+
+// pos[b, active[b, k]] = k over a buffer of -1; empty branches
+__global__ void k_branch_init(mbema_branches br, int t_host, const int* t_dev) {
+    const int b = blockIdx.y;
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < min(br.n_active[b], (int)br.Kcap)) {
+        const int v = br.active[(size_t)b * br.Kcap + i];
+        if (v >= 0 && v < br.V) br.pos[(size_t)b * br.V + v] = i;
+    }
+    const int words = (int)((br.Kcap + 31) / 32);
+    const size_t all = (size_t)br.S * words;
+    for (size_t w = i; w < all; w += (size_t)gridDim.x * blockDim.x) br.touched[(size_t)b * all + w] = 0u;
+    for (int s = i; s < br.S; s += gridDim.x * blockDim.x) {
+        br.len[b * br.S + s] = 0;
+        br.own_n[b * br.S + s] = 0;
+        br.own_new[b * br.S + s] = 0;
+    }
+    if (b == 0 && i == 0) {
+        br.t0[0] = t_dev ? *t_dev : t_host;
+        br.overflow[0] = 0;
+    }
+}
+
+// One CTA per branch: keeps staged tokens of the call before, then stages the new ones.
+__global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, const long long* __restrict__ tok, int n,
+                                                             const long long* __restrict__ counts, int pending, float* __restrict__ C_q) {
+    __shared__ int s_tok[BR_MAX_NEW], s_own[BR_MAX_NEW], s_dst[BR_MAX_NEW];
+    __shared__ unsigned s_same[BR_MAX_NEW];
+    __shared__ int s_n, s_len;
+    const int64_t r = blockIdx.x;
+    const int b = (int)(r / br.S);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int N = (int)br.N, cap = (int)br.cap;
+    const int t0 = br.t0[0];
+    const int words = (int)((br.Kcap + 31) / 32);
+    if (tid < 32) {
+        int own_n = br.own_n[r], len = br.len[r];
+        if (pending > 0) {
+            int c = pending;
+            if (counts) c = (int)min(max(counts[b], 0ll), (long long)pending);
+            const bool in = lane < c;
+            const size_t at = br_index(br, r, in ? lane : 0);
+            const int v = in ? br.st_tok[at] : -1;
+            const int own = in ? br.st_own[at] : -1, pos = in ? br.st_pos[at] : -1;
+            const unsigned kept = c >= 32 ? 0xffffffffu : (1u << c) - 1u;
+            const unsigned same = in ? br.st_same[at] & kept : 0u;
+            const bool some = in && v >= 0;
+            const int root = some ? __ffs(same) - 1 : 0;
+            const bool first = some && root == lane;
+            const bool last = some && (same >> lane) == 1u;              // no kept staged token behind this one repeats it
+            const unsigned fresh = __ballot_sync(0xffffffffu, first && own < 0);
+            const unsigned news = __ballot_sync(0xffffffffu, first && br.st_new[at] != 0);
+            const int dst = own >= 0 ? own : own_n + __popc(fresh & ((1u << root) - 1u));
+            s_dst[lane] = last && dst < cap ? dst : -1;
+            if (first && own < 0) {
+                if (dst < cap) br.own_slot[(size_t)r * cap + dst] = v;
+                else atomicExch(br.overflow, 1);
+            }
+            if (last && dst < cap) br.own_t[(size_t)r * cap + dst] = t0 + len + lane;
+            if (first && pos >= 0) atomicOr(&br.touched[(size_t)r * words + (pos >> 5)], 1u << (pos & 31));
+            own_n = min(own_n + __popc(fresh), cap);
+            len += c;
+            if (lane == 0) {
+                br.own_n[r] = own_n;
+                br.own_new[r] += __popc(news);
+                br.len[r] = len;
+            }
+        } else {
+            s_dst[lane] = -1;
+        }
+        if (lane == 0) { s_n = own_n; s_len = len; }
+    }
+    __syncthreads();
+    for (int i = 0; i < pending; ++i) {
+        const int dst = s_dst[i];
+        if (dst < 0) continue;
+        for (int c = tid; c < N; c += BS_THREADS)
+            br.own_state[((size_t)r * cap + dst) * N + c] = br.st_state[br_index(br, r, i) * N + c] + 1.0f;
+    }
+    if (n <= 0) return;
+    __syncthreads();              // the kept values are in place (this CTA alone reads them below)
+    int pos = -1;
+    if (tid < 32) {
+        const long long v = lane < n ? tok[r * n + lane] : -1;
+        const bool some = lane < n && v >= 0 && v < br.V;
+        if (lane < n && !some && v != -1) atomicExch(br.overflow, 2);
+        const unsigned same = __match_any_sync(0xffffffffu, some ? (int)v : -2 - lane);
+        s_tok[lane] = some ? (int)v : -1;
+        s_same[lane] = same;
+        s_own[lane] = -1;
+        if (some) pos = br.pos[(size_t)b * br.V + v];
+    }
+    __syncthreads();
+    const int own_n = s_n, base_t = t0 + s_len;
+    for (int u = tid; u < own_n; u += BS_THREADS) {
+        const int slot = br.own_slot[(size_t)r * cap + u];
+        for (int i = 0; i < n; ++i)
+            if (s_tok[i] == slot) s_own[i] = u;
+    }
+    __syncthreads();
+    if (tid < n) {
+        const bool first = s_tok[lane] >= 0 && __ffs(s_same[lane]) - 1 == lane;
+        const int own = s_own[lane];
+        const size_t at = br_index(br, r, lane);
+        br.st_tok[at] = s_tok[lane];
+        br.st_own[at] = own;
+        br.st_same[at] = s_same[lane];
+        br.st_pos[at] = first && own < 0 ? pos : -1;
+        br.st_new[at] = first && own < 0 && pos < 0;
+    }
+    for (int e = tid; e < n * N; e += BS_THREADS) {
+        const int i = e / N, c = e - i * N;
+        const int v = s_tok[i], own = s_own[i];
+        double x = 0.0;
+        if (v >= 0) {
+            const double l2 = log2((double)br.rhos[c]);
+            const int last = own >= 0 ? br.own_t[(size_t)r * cap + own] : br.last_t[(size_t)b * br.V + v];
+            if (own >= 0 || last >= 0) {
+                const float base = own >= 0 ? br.own_state[((size_t)r * cap + own) * N + c] : br.state[((size_t)b * br.V + v) * N + c];
+                x = (double)base * exp2((double)(base_t + i - last) * l2);
+            }
+            for (unsigned m = s_same[i] & ((1u << i) - 1u); m; m &= m - 1u) x += exp2((double)(i - (__ffs(m) - 1)) * l2);
+        }
+        br.st_state[br_index(br, r, i) * N + c] = (float)x;
+        C_q[((size_t)r * n + i) * N + c] = (float)x;
+    }
+}
+
+// One branch of every sequence moves into the prefix; step numbers move with it.
+__global__ void k_branch_adopt(mbema_branches br, const long long* __restrict__ branch, long long t_next) {
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const int N = (int)br.N, cap = (int)br.cap, Kcap = (int)br.Kcap;
+    const long long s = branch[b];
+    if (s < 0 || s >= br.S) { if (tid == 0) atomicExch(br.overflow, 3); return; }
+    const int64_t r = (int64_t)b * br.S + s;
+    const long long shift = t_next - ((long long)br.t0[0] + br.len[r]);
+    if (shift < 0) { if (tid == 0) atomicExch(br.overflow, 4); return; }
+    const int own_n = br.own_n[r];
+    for (size_t e = tid; e < (size_t)own_n * N; e += blockDim.x) {
+        const int u = (int)(e / N), c = (int)(e - (size_t)u * N);
+        br.state[((size_t)b * br.V + br.own_slot[(size_t)r * cap + u]) * N + c] = br.own_state[((size_t)r * cap + u) * N + c];
+    }
+    for (int u = tid; u < own_n; u += blockDim.x)
+        br.last_t[(size_t)b * br.V + br.own_slot[(size_t)r * cap + u]] = br.own_t[(size_t)r * cap + u];
+    __shared__ int s_na;
+    if (tid < 32) {                                  // slots that the prefix did not list, in the order the branch met them
+        int na = min(br.n_active[b], Kcap);
+        for (int u0 = 0; u0 < own_n; u0 += 32) {
+            const int u = u0 + tid;
+            const int v = u < own_n ? br.own_slot[(size_t)r * cap + u] : -1;
+            const bool add = v >= 0 && br.pos[(size_t)b * br.V + v] < 0;
+            const unsigned m = __ballot_sync(0xffffffffu, add);
+            const int at = na + __popc(m & ((1u << tid) - 1u));
+            if (add && at < Kcap) br.active[(size_t)b * Kcap + at] = v;
+            na += __popc(m);
+            if (na > Kcap) { na = Kcap; if (tid == 0) atomicExch(br.overflow, 1); }
+        }
+        if (tid == 0) { br.n_active[b] = na; s_na = na; }
+    }
+    __syncthreads();
+    for (int k = tid; k < s_na; k += blockDim.x) br.last_t[(size_t)b * br.V + br.active[(size_t)b * Kcap + k]] += (int)shift;
+}
+
+static int check_branches(const mbema_branches* br) {
+    if (!br) return MBEMA_ERR_NULL;
+    if (br->B < 0 || br->S < 1 || br->V < 1 || br->N < 1 || br->Kcap < 1 || br->cap < 1 || br->max_new < 1) return MBEMA_ERR_SHAPE;
+    if (br->N > 128 || br->max_new > BR_MAX_NEW || br->B > 65535 || br->B * br->S > 0x7fffffff / 2 || br->V > 0x7fffffff ||
+        br->Kcap > 0x7ffffff || br->cap > 0x7ffffff)
+        return MBEMA_ERR_UNSUPPORTED;
+    if (br->B == 0) return MBEMA_OK;
+    const void* need[] = {br->rhos, br->state, br->last_t, br->active, br->n_active, br->pos, br->t0, br->len, br->own_n, br->own_new,
+                          br->own_slot, br->own_t, br->own_state, br->touched, br->st_tok, br->st_own, br->st_pos, br->st_same,
+                          br->st_new, br->st_state, br->overflow};
+    for (const void* p : need)
+        if (!p) return MBEMA_ERR_NULL;
+    return MBEMA_OK;
+}
+
+}  // namespace mbema
+
+using namespace mbema;
+
+extern "C" int mbema_branches_init(const mbema_branches* br, int64_t t_now, const int32_t* t_now_dev, void* stream) {
+    int rc = check_branches(br);
+    if (rc != MBEMA_OK || br->B == 0) return rc;
+    MBEMA_CUDA_TRY(cudaMemsetAsync(br->pos, 0xff, (size_t)br->B * br->V * sizeof(int32_t), (cudaStream_t)stream));
+    dim3 grid((unsigned)((br->Kcap + 255) / 256), (unsigned)br->B);
+    k_branch_init<<<grid, 256, 0, (cudaStream_t)stream>>>(*br, (int)t_now, t_now_dev);
+    return check_launch();
+}
+
+extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* tok, int64_t n, int64_t n_pending, float* C_q, void* stream) {
+    int rc = check_branches(br);
+    if (rc != MBEMA_OK) return rc;
+    if (n < 1 || n > br->max_new || n_pending < 0 || n_pending > br->max_new) return MBEMA_ERR_SHAPE;
+    if (br->B == 0) return MBEMA_OK;
+    if (!tok || !C_q) return MBEMA_ERR_NULL;
+    k_branch_stage<<<(unsigned)(br->B * br->S), BS_THREADS, 0, (cudaStream_t)stream>>>(*br, (const long long*)tok, (int)n, nullptr,
+                                                                                   (int)n_pending, C_q);
+    return check_launch();
+}
+
+extern "C" int mbema_branches_keep(const mbema_branches* br, const int64_t* counts, int64_t n_pending, void* stream) {
+    int rc = check_branches(br);
+    if (rc != MBEMA_OK) return rc;
+    if (n_pending < 0 || n_pending > br->max_new) return MBEMA_ERR_SHAPE;
+    if (br->B == 0 || n_pending == 0) return MBEMA_OK;
+    if (!counts) return MBEMA_ERR_NULL;
+    k_branch_stage<<<(unsigned)(br->B * br->S), BS_THREADS, 0, (cudaStream_t)stream>>>(*br, nullptr, 0, (const long long*)counts,
+                                                                                   (int)n_pending, nullptr);
+    return check_launch();
+}
+
+extern "C" int mbema_branches_adopt(const mbema_branches* br, const int64_t* branch, int64_t t_next, void* stream) {
+    int rc = check_branches(br);
+    if (rc != MBEMA_OK || br->B == 0) return rc;
+    if (!branch) return MBEMA_ERR_NULL;
+    if (t_next < 0 || t_next > 0x7fffffff) return MBEMA_ERR_SHAPE;
+    k_branch_adopt<<<(unsigned)br->B, 256, 0, (cudaStream_t)stream>>>(*br, (const long long*)branch, (long long)t_next);
+    return check_launch();
+}

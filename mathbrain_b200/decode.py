@@ -26,6 +26,7 @@ class DecodeState:
         self.n_active = torch.zeros(self.B, dtype=torch.int32, device=dev)
         self.overflow = torch.zeros(1, dtype=torch.int32, device=dev)
         self._ws = None
+        self._epoch = 0          # updates so far: branches forked before one are stale
         self.t_dev = None        # device int32 step number (use_device_step): replaces the t_now arguments
 
     def use_device_step(self, t0=0):
@@ -139,12 +140,20 @@ class DecodeState:
         _require_cuda(tok)
         lib = _lib.load()
         tok = tok.long().contiguous()
+        self._epoch += 1
         C_q = torch.empty(self.B, self.N, dtype=torch.float32, device=tok.device)
         rc = lib.mbema_decode_update(_ptr(tok), _ptr(self.rhos), _ptr(self.state), _ptr(self.last_t), _ptr(self.active),
                                      _ptr(self.n_active), _ptr(C_q), _ptr(self.overflow), self.B, self.V, self.N,
                                      self.cap, int(t_now), _ptr(self.t_dev), _stream())
         _lib.check(rc, "mbema_decode_update")
         return C_q
+
+    def fork(self, branches, t_now, capacity=1024, max_new=16):
+        """Branches of every sequence from step t_now on (the device step, if use_device_step is on), each empty at first:
+        `branches` continuations that share this state, `capacity` distinct tokens a branch at most, `max_new` (up to 32) new
+        tokens a call.  See mathbrain_b200/branches.py."""
+        from .branches import Branches
+        return Branches(self, branches, t_now, capacity=capacity, max_new=max_new)
 
     def device_status(self):
         """Status word of the tensor-core attend kernels since this state was created (synchronises): 0 = ok, else a
