@@ -56,6 +56,10 @@ class Branches:
             st_tok=torch.empty(B, S, max_new, **i32), st_own=torch.empty(B, S, max_new, **i32),
             st_pos=torch.empty(B, S, max_new, **i32), st_same=torch.empty(B, S, max_new, **i32),
             st_new=torch.empty(B, S, max_new, **i32), st_state=torch.empty(B, S, max_new, N, **f32), overflow=torch.empty(1, **i32))
+        self._tensor_cores = N in (64, 128)
+        if self._tensor_cores:
+            self._hold.update(pre_op=torch.empty(B, Kcap, N, dtype=torch.float16, device=dev),
+                              own_op=torch.empty(B, S, cap, N, dtype=torch.float16, device=dev))
         self._c = _lib.BranchesStruct(**{k: _ptr(t) for k, t in self._hold.items()}, B=B, S=S, V=V, N=N, Kcap=Kcap, cap=cap,
                                       max_new=max_new)
         self._lib = _lib.load()
@@ -136,7 +140,11 @@ class Branches:
             mode = get_options()["mode"]
         if mode not in ("fp32", "tc_bf16", "auto"):
             raise ValueError("mode must be 'fp32', 'tc_bf16' or 'auto'")
-        code = _lib.MODE_FP32
+        fits = self._tensor_cores and q.dtype == torch.bfloat16 and E_k.dtype == torch.bfloat16
+        if mode == "tc_bf16" and not fits:
+            raise _lib.MbemaError("attend: mode 'tc_bf16' needs bfloat16 q and tables and 64 or 128 channels (%s, %s, %d)"
+                                  % (q.dtype, E_k.dtype, self.N))
+        code = _lib.MODE_TC_BF16 if fits and mode != "fp32" else _lib.MODE_FP32
         n, H = q.shape[2], q.shape[3]
         O = torch.empty_like(q)
         need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, n, H, self.prefix.cap, self.capacity, code)

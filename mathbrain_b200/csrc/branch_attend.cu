@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
 }
 
 // Chunks: enough jobs for about four CTAs an SM, none shorter than a tile of 64 slots nor longer than sixteen.
-BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
-    (void)mode;
+static BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
+    if (mode == MBEMA_MODE_TC_BF16) return branch_plan_tc(B, S, n, H, Kcap, cap);
     auto tiles = [&](int64_t lists, int64_t slots) {
         const int64_t all = lists * n * H * ((slots + BA_TILE - 1) / BA_TILE);
         return std::min<int64_t>(16, std::max<int64_t>(1, all / (4 * 148)));
@@ -344,13 +344,15 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
                                      void* workspace, size_t workspace_bytes, void* stream) {
     if (!br) return MBEMA_ERR_NULL;
     if (!plan_sizes_ok(br->B, br->S, n, H, br->Kcap, br->cap) || n > br->max_new || br->V < 1 || br->N < 1) return MBEMA_ERR_SHAPE;
-    if (hd != BR_HD || br->N > 128 || br->max_new > BR_MAX_NEW) return MBEMA_ERR_UNSUPPORTED;
+    if (hd != BR_HD || br->N > 128 || br->max_new > BR_MAX_NEW || (mode != MBEMA_MODE_FP32 && mode != MBEMA_MODE_TC_BF16)) return MBEMA_ERR_UNSUPPORTED;
+    if (mode == MBEMA_MODE_TC_BF16 && (!branch_tc_supported(br->N) || q_dtype != MBEMA_BF16 || e_dtype != MBEMA_BF16)) return MBEMA_ERR_UNSUPPORTED;
     if (br->B == 0) return MBEMA_OK;
     if (!q || !E_k || !E_v || !W_pe || !O || !workspace || !br->state || !br->active || !br->own_state || !br->st_state) return MBEMA_ERR_NULL;
     if ((q_dtype != MBEMA_F32 && q_dtype != MBEMA_BF16) || (e_dtype != MBEMA_F32 && e_dtype != MBEMA_BF16)) return MBEMA_ERR_DTYPE;
     if (((uintptr_t)q | (uintptr_t)E_k | (uintptr_t)E_v | (uintptr_t)W_pe | (uintptr_t)O | (uintptr_t)workspace) & 15) return MBEMA_ERR_ALIGN;
     if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
-    BranchArgs a;
+    if (mode == MBEMA_MODE_TC_BF16 && (!br->pre_op || !br->own_op)) return MBEMA_ERR_NULL;
+    BranchArgs a{};
     a.br = *br;
     a.q = q; a.Ek = E_k; a.Ev = E_v; a.W = W_pe; a.O = O;
     a.q_dt = q_dtype; a.e_dt = e_dtype; a.n = (int)n; a.H = (int)H;
@@ -361,6 +363,6 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     const size_t parts = (size_t)(br->B * br->S * n * H) * (a.plan.SP + a.plan.SO);
     a.po = reinterpret_cast<float*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.po + parts * BR_HD);
-    int rc = launch_branch_attend_fp32(a, (cudaStream_t)stream);
+    int rc = mode == MBEMA_MODE_TC_BF16 ? launch_branch_attend_tc(a, (cudaStream_t)stream) : launch_branch_attend_fp32(a, (cudaStream_t)stream);
     return rc != MBEMA_OK ? rc : launch_branch_merge(a, (cudaStream_t)stream);
 }

@@ -7,6 +7,8 @@
 // token repeated at every step amplifies a bias of rho by 1/(1 - rho)).
 // Bound by latency: chains of a few dependent loads for B S n rows of 4 N bytes.  The operand copies behind it move 6 N bytes a
 // listed slot.
+#include <algorithm>
+
 #include "branches.cuh"
 
 namespace mbema {
@@ -140,6 +142,46 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
     }
 }
 
+// Operand copies of all listed slots at the first staged step, state * rho^(t0 + len - last) / 64 in fp16 (11 significant bits; a
+// state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head.  grid: x = shares of a list,
+// y = sequence, z = 0: its prefix, s + 1: branch s.  A thread makes eight channels.
+__global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
+    const int b = blockIdx.y, z = blockIdx.z;
+    const int N = (int)br.N, per = N / 8;
+    const int64_t r = (int64_t)b * br.S + (z ? z - 1 : 0);
+    const int count = z ? br.own_n[r] : min(br.n_active[b], (int)br.Kcap);
+    const int now = br.t0[0] + br.len[r];
+    const int c = (threadIdx.x % per) * 8;
+    const int items = 256 / per;                        // a power of two of threads an item: 8 or 16
+    int k = blockIdx.x * items + threadIdx.x / per;
+    if (k >= count) return;
+    float l2r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l2r[i] = log2f(br.rhos[c + i]);
+    for (; k < count; k += gridDim.x * items) {
+        const float* src;
+        int last;
+        if (z) {
+            src = br.own_state + ((size_t)r * br.cap + k) * N;
+            last = br.own_t[(size_t)r * br.cap + k];
+        } else {
+            const int v = br.active[(size_t)b * br.Kcap + k];
+            src = br.state + ((size_t)b * br.V + v) * N;
+            last = br.last_t[(size_t)b * br.V + v];
+        }
+        const float dt = (float)(now - last);
+        const float4 x = *reinterpret_cast<const float4*>(src + c), y = *reinterpret_cast<const float4*>(src + c + 4);
+        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        __half2 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = __floats2half2_rn(fminf(f[2 * i] * exp2f(dt * l2r[2 * i]) * BR_OP_SCALE, 65504.f),
+                                     fminf(f[2 * i + 1] * exp2f(dt * l2r[2 * i + 1]) * BR_OP_SCALE, 65504.f));
+        __half* dst = reinterpret_cast<__half*>(z ? br.own_op : br.pre_op) + ((z ? (size_t)r * br.cap : (size_t)b * br.Kcap) + k) * N + c;
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(o);
+    }
+}
+
 // One branch of every sequence moves into the prefix; step numbers move with it.
 __global__ void k_branch_adopt(mbema_branches br, const long long* __restrict__ branch, long long t_next) {
     const int b = blockIdx.x, tid = threadIdx.x;
@@ -187,6 +229,7 @@ static int check_branches(const mbema_branches* br) {
                           br->st_new, br->st_state, br->overflow};
     for (const void* p : need)
         if (!p) return MBEMA_ERR_NULL;
+    if ((br->pre_op || br->own_op) && (!branch_tc_supported(br->N) || br->S >= 65535)) return MBEMA_ERR_UNSUPPORTED;
     return MBEMA_OK;
 }
 
@@ -211,6 +254,12 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
     if (!tok || !C_q) return MBEMA_ERR_NULL;
     k_branch_stage<<<(unsigned)(br->B * br->S), BS_THREADS, 0, (cudaStream_t)stream>>>(*br, (const long long*)tok, (int)n, nullptr,
                                                                                    (int)n_pending, C_q);
+    rc = check_launch();
+    if (rc != MBEMA_OK || !br->pre_op || !br->own_op) return rc;
+    // shares of a list: two CTAs an SM for a few sequences, one share of 32 or 16 slots where that is enough
+    const int64_t items = 256 / (br->N / 8), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
+    const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
+    k_branch_operands<<<dim3((unsigned)x, (unsigned)br->B, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream>>>(*br);
     return check_launch();
 }
 

@@ -32,6 +32,7 @@ struct BranchArgs {
     float v_total;
     int silu, listed_only;
     BranchPlan plan;
+    int wf_offset;           // tensor cores: floats of shared memory before the fragments of W
 };
 
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
@@ -50,7 +51,9 @@ __device__ __forceinline__ bool br_hides_own(const mbema_branches& br, int64_t r
     return false;
 }
 
-BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode);
+bool branch_tc_supported(int64_t N);
+BranchPlan branch_plan_tc(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap);
+int launch_branch_attend_tc(const BranchArgs& a, cudaStream_t st);
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st);
 int launch_branch_merge(const BranchArgs& a, cudaStream_t st);
 
