@@ -196,14 +196,17 @@ __global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
     }
 }
 
-// A warp per (row, head); a lane holds two output columns.
+// A CTA per (row, head): its four warps share the partials and, for the staged tokens, the state channels; a lane holds two output
+// columns.
 __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
-    __shared__ float s_c[BM_WARPS][BM_STAGED][128];
+    __shared__ float s_c[BM_STAGED][128];                       // states of the staged tokens at this row
+    __shared__ float2 s_x[BM_WARPS][BM_STAGED][32];             // partial pre-activations
+    __shared__ float s_m[BM_WARPS], s_l[BM_WARPS];
+    __shared__ float2 s_o[BM_WARPS][32];
     const mbema_branches& br = a.br;
     const int N = (int)br.N, n = a.n, H = a.H, D = H * BR_HD;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t wid = (int64_t)blockIdx.x * BM_WARPS + warp;
-    if (wid >= (int64_t)br.B * br.S * n * H) return;
+    const int64_t wid = blockIdx.x;
     const int h = (int)(wid % H);
     const int64_t row = wid / H;
     const int j = (int)(row % n);
@@ -213,83 +216,104 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     const int na = min(br.n_active[b], (int)br.Kcap), no = br.own_n[r];
     const int np = (na + a.plan.chp - 1) / a.plan.chp, nq = (no + a.plan.cho - 1) / a.plan.cho;
     const size_t base = (size_t)wid * (SP + SO);
-    float M = -INFINITY;
-    for (int p = lane; p < np + nq; p += 32) M = fmaxf(M, a.ml[base + (p < np ? p : SP + p - np)].x);
+    float M = -INFINITY, L = 0.f;
+    float2 o = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int p = warp; p < np + nq; p += BM_WARPS) {
+        const size_t at = base + (p < np ? p : SP + p - np);
+        const float2 ml = a.ml[at];
+        const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
+        if (ml.y == 0.f) continue;                              // every slot of the chunk is hidden
+        const float m_new = fmaxf(M, ml.x);
+        const float keep = exp2f(M - m_new), w = exp2f(ml.x - m_new);
+        L = fmaf(ml.y, w, L * keep);
+        o.x = fmaf(x.x, w, o.x * keep);
+        o.y = fmaf(x.y, w, o.y * keep);
+        M = m_new;
+    }
+    for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
+        const int cnt = min(BM_STAGED, j - i0);
+        __syncthreads();
+        for (int e = threadIdx.x; e < cnt * N; e += BM_WARPS * 32) {
+            const int i = e / N, c = e - i * N;
+            s_c[i][c] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * log2f(br.rhos[c]));
+        }
+        __syncthreads();
+        const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
+        float x0[BM_STAGED], x1[BM_STAGED];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        for (int i = 0; i < BM_STAGED; ++i) x0[i] = x1[i] = 0.f;
+#pragma unroll 4
+        for (int c = warp; c < N; c += BM_WARPS) {
+            const float2 w = Wc[(size_t)c * (D / 2)];
+#pragma unroll
+            for (int i = 0; i < BM_STAGED; ++i) {
+                if (i < cnt) {
+                    x0[i] = fmaf(s_c[i][c], w.x, x0[i]);
+                    x1[i] = fmaf(s_c[i][c], w.y, x1[i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < BM_STAGED; ++i)
+            if (i < cnt) s_x[warp][i][lane] = make_float2(x0[i], x1[i]);
+        __syncthreads();
+        for (int i = warp; i < cnt; i += BM_WARPS) {             // a staged token each
+            const int place = i0 + i;
+            const size_t at = br_index(br, r, place);
+            const int v = br.st_tok[at];
+            // none, or repeated before this row (j <= 31)
+            const bool see = v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
+            float s = -INFINITY;
+            float2 val = make_float2(0.f, 0.f);
+            if (see) {
+                float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+                for (int w = 0; w < BM_WARPS; ++w) { const float2 y = s_x[w][i][lane]; y0 += y.x; y1 += y.y; }
+                const float g0 = a.silu ? y0 / (1.0f + expf(-y0)) : y0, g1 = a.silu ? y1 / (1.0f + expf(-y1)) : y1;
+                const size_t e = (size_t)v * D + h * BR_HD + 2 * lane, qoff = (size_t)wid * BR_HD + 2 * lane;
+                s = warp_sum(ld_dyn_f32(a.q, a.q_dt, qoff) * (ld_dyn_f32(a.Ek, a.e_dt, e) * g0) +
+                             ld_dyn_f32(a.q, a.q_dt, qoff + 1) * (ld_dyn_f32(a.Ek, a.e_dt, e + 1) * g1)) * BR_SCORE_LOG2;
+                val = make_float2(ld_dyn_f32(a.Ev, a.e_dt, e) * g0, ld_dyn_f32(a.Ev, a.e_dt, e + 1) * g1);
+                const float m_new = fmaxf(M, s);
+                const float keep = exp2f(M - m_new), w = exp2f(s - m_new);
+                L = fmaf(L, keep, w);
+                o.x = fmaf(val.x, w, o.x * keep);
+                o.y = fmaf(val.y, w, o.y * keep);
+                M = m_new;
+            }
+        }
+    }
+    if (lane == 0) { s_m[warp] = M; s_l[warp] = L; }
+    s_o[warp][lane] = o;
+    __syncthreads();
+    if (warp != 0) return;
     float rest = 0.f;
     if (!a.listed_only) {
         int listed = na + br.own_new[r];
         for (int i = 0; i < j; ++i) listed += br.st_new[br_index(br, r, i)];
         rest = fmaxf(a.v_total - (float)listed, 0.f);
-        if (rest > 0.f) M = fmaxf(M, 0.f);
     }
-    float L = 0.f, o0 = 0.f, o1 = 0.f;
-    if (M > -INFINITY) {
-        L = rest > 0.f ? rest * exp2f(-M) : 0.f;
-        for (int p = 0; p < np + nq; ++p) {
-            const size_t at = base + (p < np ? p : SP + p - np);
-            const float2 ml = a.ml[at];
-            const float w = exp2f(ml.x - M);
-            const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
-            L = fmaf(ml.y, w, L);
-            o0 = fmaf(x.x, w, o0);
-            o1 = fmaf(x.y, w, o1);
-        }
-    }
-    if (j > 0) {
-        const size_t qoff = (size_t)wid * BR_HD + 2 * lane;
-        const float q0 = ld_dyn_f32(a.q, a.q_dt, qoff) * BR_SCORE_LOG2, q1 = ld_dyn_f32(a.q, a.q_dt, qoff + 1) * BR_SCORE_LOG2;
-        const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
-        for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
-            const int cnt = min(BM_STAGED, j - i0);
-            __syncwarp();
-            for (int c = lane; c < N; c += 32) {
-                const float l2r = log2f(br.rhos[c]);
-                for (int i = 0; i < cnt; ++i)
-                    s_c[warp][i][c] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * l2r);
-            }
-            __syncwarp();
-            float x0[BM_STAGED], x1[BM_STAGED];
+    M = rest > 0.f ? 0.f : -INFINITY;
 #pragma unroll
-            for (int i = 0; i < BM_STAGED; ++i) x0[i] = x1[i] = 0.f;
-            for (int c = 0; c < N; ++c) {
-                const float2 w = Wc[(size_t)c * (D / 2)];
+    for (int w = 0; w < BM_WARPS; ++w) M = fmaxf(M, s_m[w]);
+    L = rest > 0.f ? rest * exp2f(-M) : 0.f;
+    o = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < BM_STAGED; ++i) {
-                    if (i < cnt) {
-                        const float m = s_c[warp][i][c];
-                        x0[i] = fmaf(m, w.x, x0[i]);
-                        x1[i] = fmaf(m, w.y, x1[i]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < BM_STAGED; ++i) {
-                if (i >= cnt) continue;
-                const int place = i0 + i;
-                const size_t at = br_index(br, r, place);
-                const int v = br.st_tok[at];
-                const unsigned before = (1u << j) - 1u;                                  // j <= 31
-                if (v < 0 || ((br.st_same[at] & before) >> place) != 1u) continue;        // none, or repeated before this row
-                const float g0 = a.silu ? x0[i] / (1.0f + expf(-x0[i])) : x0[i], g1 = a.silu ? x1[i] / (1.0f + expf(-x1[i])) : x1[i];
-                const size_t e = (size_t)v * D + h * BR_HD + 2 * lane;
-                const float s = warp_sum(q0 * (ld_dyn_f32(a.Ek, a.e_dt, e) * g0) + q1 * (ld_dyn_f32(a.Ek, a.e_dt, e + 1) * g1));
-                const float m_new = fmaxf(M, s);
-                const float alpha = exp2f(M - m_new), p = exp2f(s - m_new);
-                L = fmaf(L, alpha, p);
-                o0 = fmaf(p, ld_dyn_f32(a.Ev, a.e_dt, e) * g0, o0 * alpha);
-                o1 = fmaf(p, ld_dyn_f32(a.Ev, a.e_dt, e + 1) * g1, o1 * alpha);
-                M = m_new;
-            }
-        }
+    for (int w = 0; w < BM_WARPS; ++w) {
+        if (s_l[w] == 0.f) continue;
+        const float e = exp2f(s_m[w] - M);
+        const float2 x = s_o[w][lane];
+        L = fmaf(s_l[w], e, L);
+        o.x = fmaf(x.x, e, o.x);
+        o.y = fmaf(x.y, e, o.y);
     }
     const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);      // no slot at all: zero; a NaN stays one
     const size_t at = (size_t)wid * BR_HD + 2 * lane;
     if (a.q_dt == MBEMA_F32) {
-        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.O) + at) = make_float2(o0 * inv, o1 * inv);
+        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.O) + at) = make_float2(o.x * inv, o.y * inv);
     } else {
-        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.O) + at) = __floats2bfloat162_rn(o0 * inv, o1 * inv);
+        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.O) + at) = __floats2bfloat162_rn(o.x * inv, o.y * inv);
     }
 }
 
@@ -319,9 +343,9 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
 }
 
 int launch_branch_merge(const BranchArgs& a, cudaStream_t st) {
-    const int64_t warps = a.br.B * a.br.S * a.n * a.H;
-    if (warps > (int64_t)0x7fffffff * BM_WARPS) return MBEMA_ERR_UNSUPPORTED;
-    k_branch_merge<<<(unsigned)((warps + BM_WARPS - 1) / BM_WARPS), BM_WARPS * 32, 0, st>>>(a);
+    const int64_t ctas = a.br.B * a.br.S * a.n * a.H;
+    if (ctas > 0x7fffffff) return MBEMA_ERR_UNSUPPORTED;
+    k_branch_merge<<<(unsigned)ctas, BM_WARPS * 32, 0, st>>>(a);
     return check_launch();
 }
 

@@ -5,8 +5,8 @@
 //     gate(j) = SiLU(A . (rho^j * W)),   16 slots x 64 channels of a head to a warp (mma.sync m16n8k16, fp32 accumulators).
 // A warp keeps its step's W in registers and its accumulators in the layout that the next operand needs: a thread holds the same
 // 16 channels of slots g and g + 8 in the gate, in the 16-byte pieces that it loads of the E rows, and in q and O.  So nothing goes
-// through shared memory on the way, the warps of a CTA (one per step and share of the slots) meet only at the end of a job, and
-// the E rows that one warp fetches are in L1 for the warps of the other steps.
+// through shared memory, a warp is a worker of its own with its own jobs, and the E rows that one warp fetches are in L1 for the
+// warps of the other steps, which take the same job.
 #include <algorithm>
 
 #include "branches.cuh"
@@ -15,7 +15,7 @@ namespace mbema {
 
 static constexpr int BT_WARPS = 8;
 static constexpr int BT_THREADS = BT_WARPS * 32;
-static constexpr int BT_LDW = 68;                 // floats a row of the staged W slice
+static constexpr int BT_LDW = 70;                 // floats a row of the staged W slice, which starts up to 6 floats in (w_row)
 static constexpr float BT_W_SCALE = 64.0f;        // undoes BR_OP_SCALE
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -53,11 +53,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {      // lane (g, 
 
 // Channel maps.  Lane = 4 g + t.  Gate column (tile nt, thread t, e) is channel 32 (nt / 4) + 8 t + 2 (nt % 4) + e of the head, and
 // contraction place (step ks, thread t, pair p, e) is state channel 32 (ks / 2) + 8 t + 4 (ks % 2) + 2 p + e: 16 bytes of a row each.
+// Rows 8, 16 and 24 behind one another start two banks apart: a fragment's lanes read four of them, 8 channels apart.
+__device__ __forceinline__ int w_row(int c) { return c * BT_LDW + 2 * ((c >> 3) & 3); }
+
 template <int KS>
 __device__ __forceinline__ void w_fragment(uint32_t (&w)[2], const float* W_sh, const float* pw, int ks, int nt, int g, int t) {
     const int c = 32 * (ks >> 1) + 8 * t + 4 * (ks & 1);
     const int d = 32 * (nt >> 2) + 8 * (g >> 1) + 2 * (nt & 3) + (g & 1);
-    const float* p = W_sh + c * BT_LDW + d;
+    const float* p = W_sh + w_row(c) + d;              // c .. c + 3 lie in one group of eight
     w[0] = pack_h2(p[0] * pw[0], p[BT_LDW] * pw[1]);
     w[1] = pack_h2(p[2 * BT_LDW] * pw[2], p[3 * BT_LDW] * pw[3]);
 }
@@ -105,24 +108,34 @@ struct WSource {
     }
 };
 
-// rows g and g + 8 of 16 operand rows
+// rows g and g + 8 of 16 operand rows, from this thread's first channel on
 template <int KS>
-__device__ __forceinline__ void load_A(uint32_t (&A)[KS][4], const __half* r0, const __half* r1, int t) {
+__device__ __forceinline__ void load_A(uint32_t (&A)[KS][4], const __half* r0, const __half* r1) {
 #pragma unroll
     for (int i = 0; i < KS / 2; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(r0 + 32 * i + 8 * t);
-        const uint4 y = *reinterpret_cast<const uint4*>(r1 + 32 * i + 8 * t);
+        const uint4 x = *reinterpret_cast<const uint4*>(r0 + 32 * i);
+        const uint4 y = *reinterpret_cast<const uint4*>(r1 + 32 * i);
         A[2 * i][0] = x.x; A[2 * i][2] = x.y; A[2 * i + 1][0] = x.z; A[2 * i + 1][2] = x.w;
         A[2 * i][1] = y.x; A[2 * i][3] = y.y; A[2 * i + 1][1] = y.z; A[2 * i + 1][3] = y.w;
     }
 }
 
-__device__ __forceinline__ void load_E(uint32_t (&E)[8], const __nv_bfloat16* row, int t) {
+__device__ __forceinline__ void load_E(uint32_t (&E)[8], const char* row) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(row + 32 * i + 8 * t);
+        const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i);
         E[4 * i] = x.x; E[4 * i + 1] = x.y; E[4 * i + 2] = x.z; E[4 * i + 3] = x.w;
     }
+}
+
+// products of the halves, exact in fp32 (mixed-precision FMA: no unpacking)
+__device__ __forceinline__ void mul_bf16x2(float& x, float& y, uint32_t a, uint32_t b) {
+    asm("{\n\t.reg .b16 al, ah, bl, bh;\n\t"
+        "mov.b32 {al, ah}, %2;\n\t"
+        "mov.b32 {bl, bh}, %3;\n\t"
+        "fma.rn.f32.bf16 %0, al, bl, 0f00000000;\n\t"
+        "fma.rn.f32.bf16 %1, ah, bh, 0f00000000;\n\t}"
+        : "=f"(x), "=f"(y) : "r"(a), "r"(b));
 }
 
 __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
@@ -229,94 +242,82 @@ __device__ __forceinline__ int quad_columns(int lane) {
 // ---------------------------------------------------------------------------------------------------------------------------
 // One or two branches at a time: q.K and P.V on the CUDA cores, in fp32, straight from the gate's accumulators.
 // ---------------------------------------------------------------------------------------------------------------------------
-template <int KS, int R>
-__device__ __forceinline__ void fma_job(const BranchArgs& a, const Job& job, const WSource<KS>& W, int j, int ig, int IG, int h,
-                                        float (&m)[R], float (&l)[R], float (&o)[R][16]) {
+template <int KS>
+__device__ __forceinline__ void fma_job(const BranchArgs& a, const Job& job, const WSource<KS>& W, int j, int h, float& m, float& l,
+                                        float (&o)[16]) {
     const mbema_branches& br = a.br;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int D = a.H * BR_HD;
-    const __nv_bfloat16* Ek = reinterpret_cast<const __nv_bfloat16*>(a.Ek) + h * BR_HD;
-    const __nv_bfloat16* Ev = reinterpret_cast<const __nv_bfloat16*>(a.Ev) + h * BR_HD;
-    float q[R][16];
-    int staged[R];
+    const uint32_t D2 = (uint32_t)a.H * BR_HD * 2;
+    const char* Ek = reinterpret_cast<const char*>(a.Ek) + h * (BR_HD * 2) + 16 * t;
+    const char* Ev = reinterpret_cast<const char*>(a.Ev) + h * (BR_HD * 2) + 16 * t;
+    uint32_t q[8];
+    load_E(q, reinterpret_cast<const char*>(a.q) + (((size_t)job.r0 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
+    int staged = -1;
+    if (lane < j) staged = (job.own ? br.st_own : br.st_pos)[br_index(br, job.r0, lane)];
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t row = job.r0 + min(r, job.rows - 1);
-        uint32_t x[8];
-        load_E(x, reinterpret_cast<const __nv_bfloat16*>(a.q) + (((size_t)row * a.n + j) * a.H + h) * BR_HD, t);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { q[r][2 * i] = bf_lo(x[i]) * BR_SCORE_LOG2; q[r][2 * i + 1] = bf_hi(x[i]) * BR_SCORE_LOG2; }
-        staged[r] = -1;
-        if (lane < j) staged[r] = (job.own ? br.st_own : br.st_pos)[br_index(br, row, lane)];
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[r][i] = 0.f;
-    }
-    const int step = 16 * IG;
-    int k0 = job.lo + 16 * ig;
-    if (k0 >= job.hi) return;
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
     const int last = job.hi - 1;
-    uint32_t A[KS][4];
-    load_A<KS>(A, job.op + (size_t)min(k0 + g, last) * br.N, job.op + (size_t)min(k0 + g + 8, last) * br.N, t);
-    int v0 = job.slots[min(k0 + g, last)], v1 = job.slots[min(k0 + g + 8, last)];
-    for (; k0 < job.hi; k0 += step) {
-        uint32_t ek0[8], ek1[8], ev0[8], ev1[8];
-        load_E(ek0, Ek + (size_t)v0 * D, t);
-        load_E(ek1, Ek + (size_t)v1 * D, t);
-        load_E(ev0, Ev + (size_t)v0 * D, t);
-        load_E(ev1, Ev + (size_t)v1 * D, t);
-        const int kn = k0 + step;
-        if (kn < job.hi) { v0 = job.slots[min(kn + g, last)]; v1 = job.slots[min(kn + g + 8, last)]; }
+    const __half* op = job.op + 8 * t;
+    // every load is for the unit behind: the operand rows follow the gate product that reads the registers, E_k the scores, E_v P.V
+    uint32_t A[KS][4], ek0[8], ek1[8], ev0[8], ev1[8];
+    int u0 = min(job.lo + g, last), u1 = min(job.lo + g + 8, last);
+    int v0 = job.slots[u0], v1 = job.slots[u1];
+    load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
+    load_E(ek0, Ek + (uint64_t)v0 * D2);
+    load_E(ek1, Ek + (uint64_t)v1 * D2);
+    load_E(ev0, Ev + (uint64_t)v0 * D2);
+    load_E(ev1, Ev + (uint64_t)v1 * D2);
+    u0 = min(job.lo + 16 + g, last);
+    u1 = min(job.lo + 24 + g, last);
+    v0 = job.slots[u0];
+    v1 = job.slots[u1];
+    for (int k0 = job.lo; k0 < job.hi; k0 += 16) {
         float acc[8][4];
         W.gate(acc, A);
-        if (kn < job.hi)
-            load_A<KS>(A, job.op + (size_t)min(kn + g, last) * br.N, job.op + (size_t)min(kn + g + 8, last) * br.N, t);
+        load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
         apply_gate(acc, a.silu);
-        float s0[R], s1[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) s0[r] = s1[r] = 0.f;
+        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            const float a0 = bf_lo(ek0[nt]) * acc[nt][0], a1 = bf_hi(ek0[nt]) * acc[nt][1];
-            const float b0 = bf_lo(ek1[nt]) * acc[nt][2], b1 = bf_hi(ek1[nt]) * acc[nt][3];
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                s0[r] = fmaf(a0, q[r][2 * nt], fmaf(a1, q[r][2 * nt + 1], s0[r]));
-                s1[r] = fmaf(b0, q[r][2 * nt], fmaf(b1, q[r][2 * nt + 1], s1[r]));
-            }
-            acc[nt][0] *= bf_lo(ev0[nt]);
-            acc[nt][1] *= bf_hi(ev0[nt]);
-            acc[nt][2] *= bf_lo(ev1[nt]);
-            acc[nt][3] *= bf_hi(ev1[nt]);
+            float x = 0.f, y = 0.f;
+            mul_bf16x2(x, y, ek0[nt], q[nt]);
+            s0 = fmaf(x, acc[nt][0], fmaf(y, acc[nt][1], s0));
+            mul_bf16x2(x, y, ek1[nt], q[nt]);
+            s1 = fmaf(x, acc[nt][2], fmaf(y, acc[nt][3], s1));
         }
-        const unsigned past = job.hi - k0 >= 16 ? 0u : 0xffffffffu << (job.hi - k0);
+        load_E(ek0, Ek + (uint64_t)v0 * D2);
+        load_E(ek1, Ek + (uint64_t)v1 * D2);
+        unsigned hide = hidden16(a, job, job.r0, k0, staged, j > 0);
+        if (job.hi - k0 < 16) hide |= 0xffffffffu << (job.hi - k0);
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+        s1 += __shfl_xor_sync(0xffffffffu, s1, 1);
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
+        s1 += __shfl_xor_sync(0xffffffffu, s1, 2);
+        const float x0 = (hide >> g) & 1u ? -INFINITY : s0 * BR_SCORE_LOG2, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s1 * BR_SCORE_LOG2;
+        const float m_new = fmaxf(m, fmaxf(x0, x1));
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float p0 = exp2f(x0 - ref), p1 = exp2f(x1 - ref);
+        if (__any_sync(0xffffffffu, m_new > m)) {
+            const float alpha = exp2f(m - ref);
+            l *= alpha;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const unsigned hide = hidden16(a, job, job.r0 + min(r, job.rows - 1), k0, staged[r], j > 0) | past;
-            s0[r] += __shfl_xor_sync(0xffffffffu, s0[r], 1);
-            s1[r] += __shfl_xor_sync(0xffffffffu, s1[r], 1);
-            s0[r] += __shfl_xor_sync(0xffffffffu, s0[r], 2);
-            s1[r] += __shfl_xor_sync(0xffffffffu, s1[r], 2);
-            const bool h0 = (hide >> g) & 1u, h1 = (hide >> (g + 8)) & 1u;
-            const float x0 = h0 ? -INFINITY : s0[r], x1 = h1 ? -INFINITY : s1[r];
-            const float m_new = fmaxf(m[r], fmaxf(x0, x1));
-            const float ref = m_new == -INFINITY ? 0.f : m_new;
-            const float p0 = exp2f(x0 - ref), p1 = exp2f(x1 - ref);
-            if (__any_sync(0xffffffffu, m_new > m[r])) {
-                const float alpha = exp2f(m[r] - ref);
-                l[r] *= alpha;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[r][i] *= alpha;
-            }
-            m[r] = m_new;
-            l[r] += p0 + p1;
-#pragma unroll
-            for (int nt = 0; nt < 8; ++nt) {      // (a value that is not finite stays in a row that hides it: the same slot is listed as the branch's own)
-                o[r][2 * nt] = fmaf(p0, acc[nt][0], fmaf(p1, acc[nt][2], o[r][2 * nt]));
-                o[r][2 * nt + 1] = fmaf(p0, acc[nt][1], fmaf(p1, acc[nt][3], o[r][2 * nt + 1]));
-            }
+            for (int i = 0; i < 16; ++i) o[i] *= alpha;
         }
+        m = m_new;
+        l += p0 + p1;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {      // (a value that is not finite stays in a row that hides it: the same slot is listed as the branch's own)
+            o[2 * nt] = fmaf(p0 * acc[nt][0], bf_lo(ev0[nt]), fmaf(p1 * acc[nt][2], bf_lo(ev1[nt]), o[2 * nt]));
+            o[2 * nt + 1] = fmaf(p0 * acc[nt][1], bf_hi(ev0[nt]), fmaf(p1 * acc[nt][3], bf_hi(ev1[nt]), o[2 * nt + 1]));
+        }
+        load_E(ev0, Ev + (uint64_t)v0 * D2);
+        load_E(ev1, Ev + (uint64_t)v1 * D2);
+        u0 = min(u0 + 16, last);
+        u1 = min(u1 + 16, last);
+        v0 = job.slots[u0];
+        v1 = job.slots[u1];
     }
 }
 
@@ -327,17 +328,17 @@ __device__ __forceinline__ void fma_job(const BranchArgs& a, const Job& job, con
 static constexpr int BT_ROWS = 16;
 
 template <int KS>
-__device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, const WSource<KS>& W, int j, int ig, int IG, int h,
-                                        float (&m)[2], float (&l)[2], float (&o)[8][4]) {
+__device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, const WSource<KS>& W, int j, int h, float (&m)[2],
+                                        float (&l)[2], float (&o)[8][4]) {
     const mbema_branches& br = a.br;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int D = a.H * BR_HD;
-    const __nv_bfloat16* Ek = reinterpret_cast<const __nv_bfloat16*>(a.Ek) + h * BR_HD;
-    const __nv_bfloat16* Ev = reinterpret_cast<const __nv_bfloat16*>(a.Ev) + h * BR_HD;
+    const uint32_t D2 = (uint32_t)a.H * BR_HD * 2;
+    const char* Ek = reinterpret_cast<const char*>(a.Ek) + h * (BR_HD * 2) + 16 * t;
+    const char* Ev = reinterpret_cast<const char*>(a.Ev) + h * (BR_HD * 2) + 16 * t;
     const int64_t row0 = job.r0 + min(g, job.rows - 1), row1 = job.r0 + min(g + 8, job.rows - 1);
     uint32_t q0[8], q1[8];
-    load_E(q0, reinterpret_cast<const __nv_bfloat16*>(a.q) + (((size_t)row0 * a.n + j) * a.H + h) * BR_HD, t);
-    load_E(q1, reinterpret_cast<const __nv_bfloat16*>(a.q) + (((size_t)row1 * a.n + j) * a.H + h) * BR_HD, t);
+    load_E(q0, reinterpret_cast<const char*>(a.q) + (((size_t)row0 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
+    load_E(q1, reinterpret_cast<const char*>(a.q) + (((size_t)row1 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
 #pragma unroll
@@ -345,22 +346,24 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
     const int words = (int)((br.Kcap + 31) / 32);
     const uint32_t* hid0 = br.touched + (size_t)row0 * words;
     const uint32_t* hid1 = br.touched + (size_t)row1 * words;
-    const int step = 16 * IG;
-    int k0 = job.lo + 16 * ig;
-    if (k0 >= job.hi) return;
     const int last = job.hi - 1;
-    uint32_t A[KS][4];
-    load_A<KS>(A, job.op + (size_t)min(k0 + g, last) * br.N, job.op + (size_t)min(k0 + g + 8, last) * br.N, t);
-    int v0 = job.slots[min(k0 + g, last)], v1 = job.slots[min(k0 + g + 8, last)];
-    for (; k0 < job.hi; k0 += step) {
-        uint32_t e0[8], e1[8];
-        load_E(e0, Ek + (size_t)v0 * D, t);
-        load_E(e1, Ek + (size_t)v1 * D, t);
+    const __half* op = job.op + 8 * t;
+    uint32_t A[KS][4], ek0[8], ek1[8], ev0[8], ev1[8];                // loads run a unit ahead, as in fma_job
+    int u0 = min(job.lo + g, last), u1 = min(job.lo + g + 8, last);
+    int v0 = job.slots[u0], v1 = job.slots[u1];
+    load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
+    load_E(ek0, Ek + (uint64_t)v0 * D2);
+    load_E(ek1, Ek + (uint64_t)v1 * D2);
+    load_E(ev0, Ev + (uint64_t)v0 * D2);
+    load_E(ev1, Ev + (uint64_t)v1 * D2);
+    u0 = min(job.lo + 16 + g, last);
+    u1 = min(job.lo + 24 + g, last);
+    v0 = job.slots[u0];
+    v1 = job.slots[u1];
+    for (int k0 = job.lo; k0 < job.hi; k0 += 16) {
         float acc[8][4];
         W.gate(acc, A);
-        const int kn = k0 + step;
-        if (kn < job.hi)
-            load_A<KS>(A, job.op + (size_t)min(kn + g, last) * br.N, job.op + (size_t)min(kn + g + 8, last) * br.N, t);
+        load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
         unsigned hide0 = (hid0[k0 >> 5] >> (k0 & 31)) & 0xffffu, hide1 = (hid1[k0 >> 5] >> (k0 & 31)) & 0xffffu;
         apply_gate(acc, a.silu);
         float sc[2][4];
@@ -373,8 +376,8 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int nt = 2 * c + p;
-                const float x0 = bf_lo(e0[nt]) * acc[nt][0], x1 = bf_hi(e0[nt]) * acc[nt][1];
-                const float y0 = bf_lo(e1[nt]) * acc[nt][2], y1 = bf_hi(e1[nt]) * acc[nt][3];
+                const float x0 = bf_lo(ek0[nt]) * acc[nt][0], x1 = bf_hi(ek0[nt]) * acc[nt][1];
+                const float y0 = bf_lo(ek1[nt]) * acc[nt][2], y1 = bf_hi(ek1[nt]) * acc[nt][3];
                 hi[0][p] = pack_bf2(x0, x1);
                 hi[1][p] = pack_bf2(y0, y1);
                 lo[0][p] = pack_bf2(x0 - bf_lo(hi[0][p]), x1 - bf_hi(hi[0][p]));
@@ -386,9 +389,8 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
                 mma_bf16(sc[x], Q, lo[x][0], lo[x][1]);
             }
         }
-        load_E(e0, Ev + (size_t)v0 * D, t);
-        load_E(e1, Ev + (size_t)v1 * D, t);
-        if (kn < job.hi) { v0 = job.slots[min(kn + g, last)]; v1 = job.slots[min(kn + g + 8, last)]; }
+        load_E(ek0, Ek + (uint64_t)v0 * D2);
+        load_E(ek1, Ek + (uint64_t)v1 * D2);
         if (j > 0) {
             unsigned x = 0u, y = 0u;
             for (int i = t; i < j; i += 4) {
@@ -440,10 +442,16 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
         }
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            const uint32_t b0 = transpose8x8(pack_bf2(bf_lo(e0[nt]) * acc[nt][0], bf_hi(e0[nt]) * acc[nt][1]));
-            const uint32_t b1 = transpose8x8(pack_bf2(bf_lo(e1[nt]) * acc[nt][2], bf_hi(e1[nt]) * acc[nt][3]));
+            const uint32_t b0 = transpose8x8(pack_bf2(bf_lo(ev0[nt]) * acc[nt][0], bf_hi(ev0[nt]) * acc[nt][1]));
+            const uint32_t b1 = transpose8x8(pack_bf2(bf_lo(ev1[nt]) * acc[nt][2], bf_hi(ev1[nt]) * acc[nt][3]));
             mma_bf16(o[nt], P, b0, b1);
         }
+        load_E(ev0, Ev + (uint64_t)v0 * D2);
+        load_E(ev1, Ev + (uint64_t)v1 * D2);
+        u0 = min(u0 + 16, last);
+        u1 = min(u1 + 16, last);
+        v0 = job.slots[u0];
+        v1 = job.slots[u1];
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -452,8 +460,8 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
     }
 }
 
-// grid: x = CTAs that share the jobs, y = head, z = block of JW steps.  Warp w: step z JW + w % JW, share w / JW of a job's slots.
-// ROWS: branches that a job of a prefix takes (1: fma_job, 16: mma_job).
+// grid: x = CTAs that share the jobs, y = head, z = block of JW steps.  Warp w takes step z JW + w % JW; the IG warps of a step
+// take jobs of their own.  ROWS: branches that a job of a prefix takes (1: fma_job, 16: mma_job).
 template <int KS, int ROWS>
 __global__ void __launch_bounds__(BT_THREADS, 1) k_branch_tc(BranchArgs a, int JW, int IG) {
     extern __shared__ __align__(16) float smem[];
@@ -462,88 +470,52 @@ __global__ void __launch_bounds__(BT_THREADS, 1) k_branch_tc(BranchArgs a, int J
     constexpr int N = 16 * KS;
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = a.H * BR_HD;
-    float* W_sh = smem;                                                     // [N][68]; behind the prologue:
-    float* red = W_sh;                                                      // [warps][ROWS][66]
-    uint2* Wf = reinterpret_cast<uint2*>(smem + a.wf_offset);               // KS = 8: [JW][KS * 8 * 32]
-    for (int i = tid; i < N * 16; i += BT_THREADS)
-        *reinterpret_cast<float4*>(W_sh + (i >> 4) * BT_LDW + (i & 15) * 4) =
-            *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
+    float* W_sh = smem;                                                     // [N] rows at w_row
+    uint2* Wf = reinterpret_cast<uint2*>(smem + (N * BT_LDW + 8));          // KS = 8: [JW][KS * 8 * 32]
+    for (int i = tid; i < N * 16; i += BT_THREADS) {
+        const float4 x = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
+        float2* dst = reinterpret_cast<float2*>(W_sh + w_row(i >> 4) + (i & 15) * 4);
+        dst[0] = make_float2(x.x, x.y);
+        dst[1] = make_float2(x.z, x.w);
+    }
     for (int i = tid; i < N; i += BT_THREADS) s_l2r[i] = log2f(br.rhos[i]);
     __syncthreads();
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;
-    const bool works = ig < IG && j < a.n;
-    WSource<KS> W;
+    if (ig >= IG || j >= a.n) return;
+    WSource<KS> W;                 // KS = 8: the IG warps of a step write the same fragments, each reads what it has written
     W.build(W_sh, s_l2r, Wf + (size_t)jj * KS * 8 * 32, j, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane);
-    __syncthreads();
     const int blocks = (int)((br.S + ROWS - 1) / ROWS);
     const int64_t jobs = br.B * blocks * a.plan.SP + br.B * br.S * a.plan.SO;
     const int parts = a.plan.SP + a.plan.SO;
-    for (int64_t x = blockIdx.x; x < jobs; x += gridDim.x) {
+    for (int64_t x = (int64_t)blockIdx.x * IG + ig; x < jobs; x += (int64_t)gridDim.x * IG) {
         Job job;
-        if (!find_job(job, a, x, ROWS)) continue;      // the same for all threads
-        const bool single = ROWS == 1 || job.own;
-        if (works) {
-            if (single) {
-                float m[1], l[1], o[1][16];
-                fma_job<KS, 1>(a, job, W, j, ig, IG, h, m, l, o);
-                float2 out;
-                join_quads(m[0], l[0], o[0], out);
-                if (IG == 1) {
-                    const size_t at = (((size_t)job.r0 * a.n + j) * a.H + h) * parts + job.part;
-                    *reinterpret_cast<float2*>(a.po + at * BR_HD + quad_columns(lane)) = out;
-                    if (lane == 0) a.ml[at] = make_float2(m[0], l[0]);
-                } else {
-                    float* dst = red + warp * 66;
-                    *reinterpret_cast<float2*>(dst + 2 + quad_columns(lane)) = out;
-                    if (lane == 0) { dst[0] = m[0]; dst[1] = l[0]; }
-                }
-            }
-            if constexpr (ROWS > 1) {
-                if (!single) {
-                    float m[2], l[2], o[8][4];
-                    mma_job<KS>(a, job, W, j, ig, IG, h, m, l, o);
-                    const int g = lane >> 2, t = lane & 3;
+        if (!find_job(job, a, x, ROWS)) continue;
+        if (ROWS == 1 || job.own) {
+            float m, l, o[16];
+            fma_job<KS>(a, job, W, j, h, m, l, o);
+            float2 out;
+            join_quads(m, l, o, out);
+            const size_t at = (((size_t)job.r0 * a.n + j) * a.H + h) * parts + job.part;
+            *reinterpret_cast<float2*>(a.po + at * BR_HD + quad_columns(lane)) = out;
+            if (lane == 0) a.ml[at] = make_float2(m, l);
+        } else if constexpr (ROWS > 1) {
+            float m[2], l[2], o[8][4];
+            mma_job<KS>(a, job, W, j, h, m, l, o);
+            const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int row = g + 8 * r;
-                        const size_t at = (((size_t)(job.r0 + min(row, job.rows - 1)) * a.n + j) * a.H + h) * parts + job.part;
-                        float* dst = IG == 1 ? a.po + at * BR_HD : red + (warp * ROWS + row) * 66 + 2;
-                        if (IG > 1 || row < job.rows) {
+            for (int r = 0; r < 2; ++r) {
+                const int row = g + 8 * r;
+                if (row < job.rows) {
+                    const size_t at = (((size_t)(job.r0 + row) * a.n + j) * a.H + h) * parts + job.part;
+                    float* dst = a.po + at * BR_HD + 8 * t;
 #pragma unroll
-                            for (int nt = 0; nt < 8; ++nt)
-                                *reinterpret_cast<float2*>(dst + 32 * (nt >> 2) + 8 * t + 2 * (nt & 3)) = make_float2(o[nt][2 * r], o[nt][2 * r + 1]);
-                            if (t == 0) {
-                                if (IG == 1) a.ml[at] = make_float2(m[r], l[r]);
-                                else { dst[-2] = m[r]; dst[-1] = l[r]; }
-                            }
-                        }
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4*>(dst + 32 * (i >> 1) + 4 * (i & 1)) =
+                            make_float4(o[2 * i][2 * r], o[2 * i][2 * r + 1], o[2 * i + 1][2 * r], o[2 * i + 1][2 * r + 1]);
+                    if (t == 0) a.ml[at] = make_float2(m[r], l[r]);
                 }
             }
-        }
-        if (IG > 1) {
-            __syncthreads();
-            const int R = single ? 1 : ROWS;
-            for (int i = warp; i < job.rows * JW; i += BT_WARPS) {                    // (row, step): a warp each
-                const int r = i / JW, jj2 = i - r * JW, j2 = blockIdx.z * JW + jj2;
-                if (j2 >= a.n) continue;
-                float M = -INFINITY;
-                for (int w = 0; w < IG; ++w) M = fmaxf(M, red[((w * JW + jj2) * R + r) * 66]);
-                float L = 0.f;
-                float2 s = make_float2(0.f, 0.f);
-                for (int w = 0; w < IG; ++w) {
-                    const float* src = red + ((w * JW + jj2) * R + r) * 66;
-                    const float e = M == -INFINITY ? 0.f : exp2f(src[0] - M);
-                    L = fmaf(src[1], e, L);
-                    s.x = fmaf(src[2 + 2 * lane], e, s.x);
-                    s.y = fmaf(src[3 + 2 * lane], e, s.y);
-                }
-                const size_t at = (((size_t)(job.r0 + r) * a.n + j2) * a.H + h) * parts + job.part;
-                *reinterpret_cast<float2*>(a.po + at * BR_HD + 2 * lane) = s;
-                if (lane == 0) a.ml[at] = make_float2(M, L);
-            }
-            __syncthreads();
         }
     }
 }
@@ -555,36 +527,36 @@ static void steps_and_shares(int n, int& JW, int& IG) {
     IG = BT_WARPS / JW;
 }
 
+// One CTA an SM (the registers allow no more), dealt to the heads and blocks of steps.
+static int64_t ctas_a_head(int64_t H, int64_t zb) { return std::max<int64_t>(1, 148 / (H * zb)); }
+
+// Chunks: about four jobs a worker if all lists were full, of 2 to 32 units of 16 slots (a job costs about one unit more than its
+// units: q, the joining of the quads, the partial).
 BranchPlan branch_plan_tc(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap) {
     int JW, IG;
     steps_and_shares((int)n, JW, IG);
-    const int unit = std::max(64, 16 * IG);
-    const int64_t zb = (n + JW - 1) / JW;
-    auto units = [&](int64_t lists, int64_t slots) {
-        const int64_t all = lists * zb * H * ((slots + unit - 1) / unit);
-        return std::min<int64_t>(16, std::max<int64_t>(1, all / (8 * 148)));
-    };
+    const int64_t zb = (n + JW - 1) / JW, workers = ctas_a_head(H, zb) * IG;
+    const int64_t lists = S == 1 ? B : B * ((S + BT_ROWS - 1) / BT_ROWS);
+    const int64_t units = lists * ((Kcap + 15) / 16) + B * S * ((cap + 15) / 16);
+    const int64_t chunk = 16 * std::min<int64_t>(32, std::max<int64_t>(2, units / (4 * workers)));
     BranchPlan p;
-    p.chp = (int)(unit * units(B, Kcap));
-    p.cho = (int)(unit * units(B * S, cap));
-    p.SP = (int)((Kcap + p.chp - 1) / p.chp);
-    p.SO = (int)((cap + p.cho - 1) / p.cho);
+    p.chp = p.cho = (int)chunk;
+    p.SP = (int)((Kcap + chunk - 1) / chunk);
+    p.SO = (int)((cap + chunk - 1) / chunk);
     return p;
 }
 
 template <int KS, int ROWS>
-static int launch_tc(BranchArgs a, cudaStream_t st) {
+static int launch_tc(const BranchArgs& a, cudaStream_t st) {
     int JW, IG;
     steps_and_shares(a.n, JW, IG);
     const mbema_branches& br = a.br;
     const int zb = (a.n + JW - 1) / JW;
     const int64_t jobs = br.B * ((br.S + ROWS - 1) / ROWS) * a.plan.SP + br.B * br.S * a.plan.SO;
-    const int64_t want = std::max<int64_t>(1, (2 * 148) / ((int64_t)a.H * zb));
-    const size_t area = std::max((size_t)16 * KS * BT_LDW, (size_t)BT_WARPS * ROWS * 66);
-    a.wf_offset = (int)area;
-    const size_t smem = area * 4 + (KS == 8 ? (size_t)JW * KS * 8 * 32 * sizeof(uint2) : 0);
+    const int64_t x = std::min((jobs + IG - 1) / IG, ctas_a_head(a.H, zb));
+    const size_t smem = ((size_t)16 * KS * BT_LDW + 8) * 4 + (KS == 8 ? (size_t)JW * KS * 8 * 32 * sizeof(uint2) : 0);
     MBEMA_CUDA_TRY(cudaFuncSetAttribute(k_branch_tc<KS, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k_branch_tc<KS, ROWS><<<dim3((unsigned)std::min(jobs, want), (unsigned)a.H, (unsigned)zb), BT_THREADS, smem, st>>>(a, JW, IG);
+    k_branch_tc<KS, ROWS><<<dim3((unsigned)x, (unsigned)a.H, (unsigned)zb), BT_THREADS, smem, st>>>(a, JW, IG);
     return check_launch();
 }
 

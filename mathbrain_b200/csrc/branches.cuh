@@ -32,7 +32,6 @@ struct BranchArgs {
     float v_total;
     int silu, listed_only;
     BranchPlan plan;
-    int wf_offset;           // tensor cores: floats of shared memory before the fragments of W
 };
 
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
