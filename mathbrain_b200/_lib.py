@@ -23,7 +23,7 @@ class BranchesStruct(ctypes.Structure):
     """mbema_branches of include/mbema.h."""
     _fields_ = [(name, _vp) for name in (
         "rhos", "state", "last_t", "active", "n_active", "pos", "t0", "len", "own_n", "own_new", "own_slot", "own_t", "own_state",
-        "touched", "st_tok", "st_own", "st_pos", "st_same", "st_new", "st_state", "pre_op", "own_op", "overflow")] + [
+        "touched", "st_tok", "st_own", "st_pos", "st_same", "st_new", "st_state", "pre_op", "own_op", "work", "overflow")] + [
         (name, _i64) for name in ("B", "S", "V", "N", "Kcap", "cap", "max_new")]
 
 

@@ -198,6 +198,8 @@ __global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
 
 // A CTA per (row, head): its four warps share the partials and, for the staged tokens, the state channels; a lane holds two output
 // columns.
+// PIECES: partials of the tensor-core kernel (a list's pieces, one a worker), else of the fp32 kernel (its chunks).
+template <bool PIECES>
 __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     __shared__ float s_c[BM_STAGED][128];                       // states of the staged tokens at this row
     __shared__ float2 s_x[BM_WARPS][BM_STAGED][32];             // partial pre-activations
@@ -211,19 +213,45 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     const int64_t row = wid / H;
     const int j = (int)(row % n);
     const int64_t r = row / n;
-    const int b = (int)(r / br.S);
-    const int SP = a.plan.SP, SO = a.plan.SO;
-    const int na = min(br.n_active[b], (int)br.Kcap), no = br.own_n[r];
-    const int np = (na + a.plan.chp - 1) / a.plan.chp, nq = (no + a.plan.cho - 1) / a.plan.cho;
-    const size_t base = (size_t)wid * (SP + SO);
+    const int b = (int)(r / br.S), s = (int)(r - (int64_t)b * br.S);
+    const int na = min(br.n_active[b], (int)br.Kcap);
+    // partials: np of the prefix from p0 on, then nq of the own slots from q0 on, p_step and q_step apart
+    int np, nq;
+    size_t p0, q0, p_step, q_step;
+    if constexpr (PIECES) {
+        const int64_t own = a.n_pre + r;
+        const int64_t pre = a.rows == 1 ? b : (int64_t)b * a.blocks + s / a.rows;
+        const long long total = br.work[a.n_pre + br.B * br.S], workers = branch_workers(total, a.max_workers);
+        auto pieces = [&](int64_t list, int cost, long long& first) {
+            const long long lo = br.work[list], hi = br.work[list + 1];
+            if (hi == lo) return 0;
+            first = branch_worker_of(total, workers, lo);
+            return (int)(branch_worker_of(total, workers, hi - cost) - first) + 1;
+        };
+        long long wp = 0, wq = 0;
+        np = pieces(pre, a.cost_pre, wp);
+        nq = pieces(own, BR_COST_OWN, wq);
+        const size_t each = (size_t)n * H, at = (size_t)j * H + h;
+        p_step = a.rows * each;
+        q_step = each;
+        p0 = ((size_t)(pre + wp) * a.rows + (a.rows == 1 ? 0 : s % a.rows)) * each + at;
+        q0 = (size_t)(a.own_piece0 + r + wq) * each + at;
+    } else {
+        const int SP = a.plan.SP, SO = a.plan.SO;
+        np = (na + a.plan.chp - 1) / a.plan.chp;
+        nq = (br.own_n[r] + a.plan.cho - 1) / a.plan.cho;
+        p_step = q_step = 1;
+        p0 = (size_t)wid * (SP + SO);
+        q0 = p0 + SP;
+    }
     float M = -INFINITY, L = 0.f;
     float2 o = make_float2(0.f, 0.f);
 #pragma unroll 4
     for (int p = warp; p < np + nq; p += BM_WARPS) {
-        const size_t at = base + (p < np ? p : SP + p - np);
+        const size_t at = p < np ? p0 + p * p_step : q0 + (p - np) * q_step;
         const float2 ml = a.ml[at];
         const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
-        if (ml.y == 0.f) continue;                              // every slot of the chunk is hidden
+        if (ml.y == 0.f) continue;                              // every slot of it is hidden
         const float m_new = fmaxf(M, ml.x);
         const float keep = exp2f(M - m_new), w = exp2f(ml.x - m_new);
         L = fmaf(ml.y, w, L * keep);
@@ -264,19 +292,17 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
             const int v = br.st_tok[at];
             // none, or repeated before this row (j <= 31)
             const bool see = v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
-            float s = -INFINITY;
-            float2 val = make_float2(0.f, 0.f);
             if (see) {
                 float y0 = 0.f, y1 = 0.f;
 #pragma unroll
                 for (int w = 0; w < BM_WARPS; ++w) { const float2 y = s_x[w][i][lane]; y0 += y.x; y1 += y.y; }
                 const float g0 = a.silu ? y0 / (1.0f + expf(-y0)) : y0, g1 = a.silu ? y1 / (1.0f + expf(-y1)) : y1;
                 const size_t e = (size_t)v * D + h * BR_HD + 2 * lane, qoff = (size_t)wid * BR_HD + 2 * lane;
-                s = warp_sum(ld_dyn_f32(a.q, a.q_dt, qoff) * (ld_dyn_f32(a.Ek, a.e_dt, e) * g0) +
+                const float score = warp_sum(ld_dyn_f32(a.q, a.q_dt, qoff) * (ld_dyn_f32(a.Ek, a.e_dt, e) * g0) +
                              ld_dyn_f32(a.q, a.q_dt, qoff + 1) * (ld_dyn_f32(a.Ek, a.e_dt, e + 1) * g1)) * BR_SCORE_LOG2;
-                val = make_float2(ld_dyn_f32(a.Ev, a.e_dt, e) * g0, ld_dyn_f32(a.Ev, a.e_dt, e + 1) * g1);
-                const float m_new = fmaxf(M, s);
-                const float keep = exp2f(M - m_new), w = exp2f(s - m_new);
+                const float2 val = make_float2(ld_dyn_f32(a.Ev, a.e_dt, e) * g0, ld_dyn_f32(a.Ev, a.e_dt, e + 1) * g1);
+                const float m_new = fmaxf(M, score);
+                const float keep = exp2f(M - m_new), w = exp2f(score - m_new);
                 L = fmaf(L, keep, w);
                 o.x = fmaf(val.x, w, o.x * keep);
                 o.y = fmaf(val.y, w, o.y * keep);
@@ -318,8 +344,7 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
 }
 
 // Chunks: enough jobs for about four CTAs an SM, none shorter than a tile of 64 slots nor longer than sixteen.
-static BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
-    if (mode == MBEMA_MODE_TC_BF16) return branch_plan_tc(B, S, n, H, Kcap, cap);
+static BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap) {
     auto tiles = [&](int64_t lists, int64_t slots) {
         const int64_t all = lists * n * H * ((slots + BA_TILE - 1) / BA_TILE);
         return std::min<int64_t>(16, std::max<int64_t>(1, all / (4 * 148)));
@@ -342,10 +367,11 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
     return check_launch();
 }
 
-int launch_branch_merge(const BranchArgs& a, cudaStream_t st) {
+int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st) {
     const int64_t ctas = a.br.B * a.br.S * a.n * a.H;
     if (ctas > 0x7fffffff) return MBEMA_ERR_UNSUPPORTED;
-    k_branch_merge<<<(unsigned)ctas, BM_WARPS * 32, 0, st>>>(a);
+    if (pieces) k_branch_merge<true><<<(unsigned)ctas, BM_WARPS * 32, 0, st>>>(a);
+    else k_branch_merge<false><<<(unsigned)ctas, BM_WARPS * 32, 0, st>>>(a);
     return check_launch();
 }
 
@@ -357,10 +383,29 @@ static bool plan_sizes_ok(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kc
     return B >= 0 && S >= 1 && n >= 1 && n <= BR_MAX_NEW && H >= 1 && Kcap >= 1 && cap >= 1;
 }
 
+// number of partials of a call
+static int64_t partials(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode, BranchArgs* a) {
+    if (mode != MBEMA_MODE_TC_BF16) {
+        const BranchPlan p = branch_plan(B, S, n, H, Kcap, cap);
+        if (a) a->plan = p;
+        return B * S * n * H * (p.SP + p.SO);
+    }
+    const BranchShape p = branch_shape(B, S, n, H);
+    const int64_t workers = (int64_t)p.ctas * p.IG, n_pre = B * p.blocks, own0 = (n_pre + workers) * p.rows;
+    if (a) {
+        a->n_pre = n_pre;
+        a->own_piece0 = own0;
+        a->max_workers = workers;
+        a->rows = p.rows;
+        a->blocks = p.blocks;
+        a->cost_pre = p.rows == 1 ? BR_COST_ONE : BR_COST_BLOCK;
+    }
+    return (own0 + B * S + workers) * n * H;
+}
+
 extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
     if (!plan_sizes_ok(B, S, n, H, Kcap, cap)) return 0;
-    const BranchPlan p = branch_plan(B, S, n, H, Kcap, cap, mode);
-    return align_up((size_t)(B * S * n * H) * (p.SP + p.SO) * (2 + BR_HD) * 4, 256) + 256;
+    return align_up((size_t)partials(B, S, n, H, Kcap, cap, mode, nullptr) * (2 + BR_HD) * 4, 256) + 256;
 }
 
 extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
@@ -375,7 +420,7 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     if ((q_dtype != MBEMA_F32 && q_dtype != MBEMA_BF16) || (e_dtype != MBEMA_F32 && e_dtype != MBEMA_BF16)) return MBEMA_ERR_DTYPE;
     if (((uintptr_t)q | (uintptr_t)E_k | (uintptr_t)E_v | (uintptr_t)W_pe | (uintptr_t)O | (uintptr_t)workspace) & 15) return MBEMA_ERR_ALIGN;
     if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
-    if (mode == MBEMA_MODE_TC_BF16 && (!br->pre_op || !br->own_op)) return MBEMA_ERR_NULL;
+    if (mode == MBEMA_MODE_TC_BF16 && (!br->pre_op || !br->own_op || !br->work)) return MBEMA_ERR_NULL;
     BranchArgs a{};
     a.br = *br;
     a.q = q; a.Ek = E_k; a.Ev = E_v; a.W = W_pe; a.O = O;
@@ -383,10 +428,10 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     a.v_total = (float)V_total;
     a.silu = (flags & MBEMA_FLAG_SILU) ? 1 : 0;
     a.listed_only = (flags & MBEMA_FLAG_LISTED_ONLY) ? 1 : 0;
-    a.plan = branch_plan(br->B, br->S, n, H, br->Kcap, br->cap, mode);
-    const size_t parts = (size_t)(br->B * br->S * n * H) * (a.plan.SP + a.plan.SO);
+    const int64_t parts = partials(br->B, br->S, n, H, br->Kcap, br->cap, mode, &a);
     a.po = reinterpret_cast<float*>(workspace);
-    a.ml = reinterpret_cast<float2*>(a.po + parts * BR_HD);
-    int rc = mode == MBEMA_MODE_TC_BF16 ? launch_branch_attend_tc(a, (cudaStream_t)stream) : launch_branch_attend_fp32(a, (cudaStream_t)stream);
-    return rc != MBEMA_OK ? rc : launch_branch_merge(a, (cudaStream_t)stream);
+    a.ml = reinterpret_cast<float2*>(a.po + (size_t)parts * BR_HD);
+    const bool tc = mode == MBEMA_MODE_TC_BF16;
+    int rc = tc ? launch_branch_attend_tc(a, branch_shape(br->B, br->S, n, H), (cudaStream_t)stream) : launch_branch_attend_fp32(a, (cudaStream_t)stream);
+    return rc != MBEMA_OK ? rc : launch_branch_merge(a, tc, (cudaStream_t)stream);
 }

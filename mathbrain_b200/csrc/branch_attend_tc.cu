@@ -4,17 +4,19 @@
 // (fp16, made once by mbema_branches_extend for all layers and steps) are the A operands of every step and rho^j goes into W:
 //     gate(j) = SiLU(A . (rho^j * W)),   16 slots x 64 channels of a head to a warp (mma.sync m16n8k16, fp32 accumulators).
 // A warp keeps its step's W in registers and its accumulators in the layout that the next operand needs: a thread holds the same
-// 16 channels of slots g and g + 8 in the gate, in the 16-byte pieces that it loads of the E rows, and in q and O.  So nothing goes
-// through shared memory, a warp is a worker of its own with its own jobs, and the E rows that one warp fetches are in L1 for the
-// warps of the other steps, which take the same job.
+// 16 channels of slots g and g + 8 in the gate, in the 16-byte pieces that it reads of the E rows, and in q and O.
+//
+// Work is dealt in units of 16 slots: mbema_branches_extend leaves the running sum of all lists' units, every worker (one warp, or
+// the warps of several steps together) takes an equal stretch of it and walks it without a stop; a list is cut where a stretch
+// ends, and each piece leaves a partial (m, l, o[64]) a row.  The operand and E rows of a unit come by cp.async into a ring of
+// shared memory, some units ahead across the ends of lists: they are gathered rows that mostly come from DRAM, and with them loaded
+// a unit ahead into registers half of all cycles were spent waiting.
 #include <algorithm>
 
 #include "branches.cuh"
 
 namespace mbema {
 
-static constexpr int BT_WARPS = 8;
-static constexpr int BT_THREADS = BT_WARPS * 32;
 static constexpr int BT_LDW = 70;                 // floats a row of the staged W slice, which starts up to 6 floats in (w_row)
 static constexpr float BT_W_SCALE = 64.0f;        // undoes BR_OP_SCALE
 
@@ -34,6 +36,28 @@ __device__ __forceinline__ float tanh_fast(float x) {
     float r;
     asm("tanh.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+template <int OFFSET>
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(OFFSET));
+    return v;
+}
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -93,34 +117,50 @@ struct WSource {
     }
     __device__ __forceinline__ void gate(float (&acc)[8][4], const uint32_t (&A)[KS][4]) const {
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int nt = 0; nt < 8; ++nt) {
+                uint32_t b0, b1;
                 if constexpr (KS == 4) {
-                    mma_f16(acc[nt], A[ks], w[ks][nt][0], w[ks][nt][1]);
+                    b0 = w[ks][nt][0];
+                    b1 = w[ks][nt][1];
                 } else {
                     const uint2 x = sh[(ks * 8 + nt) * 32];
-                    mma_f16(acc[nt], A[ks], x.x, x.y);
+                    b0 = x.x;
+                    b1 = x.y;
                 }
+                if (ks == 0) mma_f16_first(acc[nt], A[ks], b0, b1);
+                else mma_f16(acc[nt], A[ks], b0, b1);
             }
     }
 };
 
-// rows g and g + 8 of 16 operand rows, from this thread's first channel on
+// A unit in the ring: 16 rows of E_k, of E_v (128 bytes each; in odd rows the 16-byte pieces 0-3 and 4-7 change places, so that the
+// eight lanes that are served together, two rows and four pieces each, touch all banks), then the operands as the lanes' fragments.
 template <int KS>
-__device__ __forceinline__ void load_A(uint32_t (&A)[KS][4], const __half* r0, const __half* r1) {
-#pragma unroll
-    for (int i = 0; i < KS / 2; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(r0 + 32 * i);
-        const uint4 y = *reinterpret_cast<const uint4*>(r1 + 32 * i);
-        A[2 * i][0] = x.x; A[2 * i][2] = x.y; A[2 * i + 1][0] = x.z; A[2 * i + 1][2] = x.w;
-        A[2 * i][1] = y.x; A[2 * i][3] = y.y; A[2 * i + 1][1] = y.z; A[2 * i + 1][3] = y.w;
+struct UnitLayout {
+    static constexpr int EV = 2048, OP = 4096, OP_BYTES = 512 * KS;
+    static constexpr int BYTES = OP + OP_BYTES;
+};
+
+// rows g (at_lo, at_hi: this lane's pieces of channels 0-31 and 32-63) and g + 8, OFFSET bytes into the unit
+template <int OFFSET>
+__device__ __forceinline__ void load_E(uint32_t (&E0)[8], uint32_t (&E1)[8], uint32_t at_lo, uint32_t at_hi) {
+    const uint4 x = lds128<OFFSET>(at_lo), y = lds128<OFFSET>(at_hi), z = lds128<OFFSET + 1024>(at_lo), w = lds128<OFFSET + 1024>(at_hi);
+    E0[0] = x.x; E0[1] = x.y; E0[2] = x.z; E0[3] = x.w;
+    E0[4] = y.x; E0[5] = y.y; E0[6] = y.z; E0[7] = y.w;
+    E1[0] = z.x; E1[1] = z.y; E1[2] = z.z; E1[3] = z.w;
+    E1[4] = w.x; E1[5] = w.y; E1[6] = w.z; E1[7] = w.w;
+}
+template <int KS, int I = 0>
+__device__ __forceinline__ void load_A(uint32_t (&A)[KS][4], uint32_t at) {
+    if constexpr (I < KS) {
+        const uint4 x = lds128<UnitLayout<KS>::OP + 512 * I>(at);
+        A[I][0] = x.x; A[I][1] = x.y; A[I][2] = x.z; A[I][3] = x.w;
+        load_A<KS, I + 1>(A, at);
     }
 }
-
-__device__ __forceinline__ void load_E(uint32_t (&E)[8], const char* row) {
+__device__ __forceinline__ void load_q(uint32_t (&E)[8], const char* row) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i);
@@ -147,59 +187,39 @@ __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
     }
 }
 
-struct Job {
-    const int* slots;         // slot ids of the list
-    const __half* op;         // operand rows of the list
-    int64_t r0;               // first branch
-    int rows;                 // branches
-    int lo, hi;               // slots of this job
-    int part;                 // place of its partials
-    bool own;
+// A list of slots: the prefix of a sequence as 16 of its branches read it (all one, for one branch), or a branch's own slots.
+struct List {
+    const int* slots;
+    const char* op;           // operands, 16 slots after 16 slots
+    int count;
 };
 
-// chunk-major: lists shorter than their capacity leave empty jobs at the end, not between others
-__device__ __forceinline__ bool find_job(Job& job, const BranchArgs& a, int64_t x, int rows_a_job) {
+__device__ __forceinline__ List get_list(const BranchArgs& a, int64_t x) {
     const mbema_branches& br = a.br;
-    const int blocks = (int)((br.S + rows_a_job - 1) / rows_a_job);
-    const int64_t pre = br.B * blocks, n_pre = pre * a.plan.SP;
-    job.own = x >= n_pre;
-    if (!job.own) {
-        const int chunk = (int)(x / pre);
-        const int bb = (int)(x - chunk * pre);
-        const int b = bb / blocks, s0 = (bb - b * blocks) * rows_a_job;
-        job.slots = br.active + (size_t)b * br.Kcap;
-        job.op = reinterpret_cast<const __half*>(br.pre_op) + (size_t)b * br.Kcap * br.N;
-        job.r0 = (int64_t)b * br.S + s0;
-        job.rows = min(rows_a_job, (int)br.S - s0);
-        job.lo = chunk * a.plan.chp;
-        job.hi = min(job.lo + a.plan.chp, min(br.n_active[b], (int)br.Kcap));
-        job.part = chunk;
+    List t;
+    if (x < a.n_pre) {
+        const int b = (int)(x / a.blocks);
+        t.slots = br.active + (size_t)b * br.Kcap;
+        t.op = reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N);
+        t.count = min(br.n_active[b], (int)br.Kcap);
     } else {
-        const int64_t y = x - n_pre, all = br.B * br.S;
-        const int chunk = (int)(y / all);
-        const int64_t r = y - chunk * all;
-        job.slots = br.own_slot + (size_t)r * br.cap;
-        job.op = reinterpret_cast<const __half*>(br.own_op) + (size_t)r * br.cap * br.N;
-        job.r0 = r;
-        job.rows = 1;
-        job.lo = chunk * a.plan.cho;
-        job.hi = min(job.lo + a.plan.cho, br.own_n[r]);
-        job.part = a.plan.SP + chunk;
+        const int64_t r = x - a.n_pre;
+        t.slots = br.own_slot + (size_t)r * br.cap;
+        t.op = reinterpret_cast<const char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, br.N);
+        t.count = br.own_n[r];
     }
-    return job.lo < job.hi;
+    return t;
 }
 
-// bit i: slot k0 + i (i < 16) is hidden from row (r, j); staged: lane i holds the list place that staged token i < j hides, or -1
-__device__ __forceinline__ unsigned hidden16(const BranchArgs& a, const Job& job, int64_t r, int k0, int staged, bool any_staged) {
-    unsigned m = 0u;
-    if (!job.own) {
-        const int words = (int)((a.br.Kcap + 31) / 32);
-        m = (a.br.touched[(size_t)r * words + (k0 >> 5)] >> (k0 & 31)) & 0xffffu;
-    }
+// bit i: slot k0 + i (i < 16) is hidden; touched: word of the branch's bits (prefix), staged: lane i holds the list place that staged
+// token i < j hides, or -1
+__device__ __forceinline__ unsigned hidden16(unsigned touched, int k0, int staged, bool any_staged, int count) {
+    unsigned m = (touched >> (k0 & 31)) & 0xffffu;
     if (any_staged) {
         const unsigned d = (unsigned)(staged - k0);
         m |= __reduce_or_sync(0xffffffffu, d < 16u ? 1u << d : 0u);
     }
+    if (count - k0 < 16) m |= 0xffffffffu << (count - k0);
     return m;
 }
 
@@ -240,67 +260,49 @@ __device__ __forceinline__ int quad_columns(int lane) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// One or two branches at a time: q.K and P.V on the CUDA cores, in fp32, straight from the gate's accumulators.
+// One row: q.K and P.V on the CUDA cores, in fp32, straight from the gate's accumulators.  A quad of lanes has its own running
+// maximum and sums, joined at the end of the piece.
 // ---------------------------------------------------------------------------------------------------------------------------
-template <int KS>
-__device__ __forceinline__ void fma_job(const BranchArgs& a, const Job& job, const WSource<KS>& W, int j, int h, float& m, float& l,
-                                        float (&o)[16]) {
-    const mbema_branches& br = a.br;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t D2 = (uint32_t)a.H * BR_HD * 2;
-    const char* Ek = reinterpret_cast<const char*>(a.Ek) + h * (BR_HD * 2) + 16 * t;
-    const char* Ev = reinterpret_cast<const char*>(a.Ev) + h * (BR_HD * 2) + 16 * t;
+struct OneRow {
+    float m, l, o[16];
     uint32_t q[8];
-    load_E(q, reinterpret_cast<const char*>(a.q) + (((size_t)job.r0 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
-    int staged = -1;
-    if (lane < j) staged = (job.own ? br.st_own : br.st_pos)[br_index(br, job.r0, lane)];
-    m = -INFINITY;
-    l = 0.f;
+    int staged;
+    __device__ __forceinline__ void start(const BranchArgs& a, int64_t r, bool own, int j, int h, int lane) {
+        load_q(q, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
+        staged = -1;
+        if (lane < j) staged = (own ? a.br.st_own : a.br.st_pos)[br_index(a.br, r, lane)];
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = 0.f;
-    const int last = job.hi - 1;
-    const __half* op = job.op + 8 * t;
-    // every load is for the unit behind: the operand rows follow the gate product that reads the registers, E_k the scores, E_v P.V
-    uint32_t A[KS][4], ek0[8], ek1[8], ev0[8], ev1[8];
-    int u0 = min(job.lo + g, last), u1 = min(job.lo + g + 8, last);
-    int v0 = job.slots[u0], v1 = job.slots[u1];
-    load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
-    load_E(ek0, Ek + (uint64_t)v0 * D2);
-    load_E(ek1, Ek + (uint64_t)v1 * D2);
-    load_E(ev0, Ev + (uint64_t)v0 * D2);
-    load_E(ev1, Ev + (uint64_t)v1 * D2);
-    u0 = min(job.lo + 16 + g, last);
-    u1 = min(job.lo + 24 + g, last);
-    v0 = job.slots[u0];
-    v1 = job.slots[u1];
-    for (int k0 = job.lo; k0 < job.hi; k0 += 16) {
-        float acc[8][4];
-        W.gate(acc, A);
-        load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
-        apply_gate(acc, a.silu);
-        float s0 = 0.f, s1 = 0.f;
+        for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    }
+    __device__ __forceinline__ void unit(float (&acc)[8][4], uint32_t at_lo, uint32_t at_hi, unsigned hide, int g) {
+        uint32_t e0[8], e1[8];
+        load_E<0>(e0, e1, at_lo, at_hi);
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            float x = 0.f, y = 0.f;
-            mul_bf16x2(x, y, ek0[nt], q[nt]);
-            s0 = fmaf(x, acc[nt][0], fmaf(y, acc[nt][1], s0));
-            mul_bf16x2(x, y, ek1[nt], q[nt]);
-            s1 = fmaf(x, acc[nt][2], fmaf(y, acc[nt][3], s1));
+            float x, y;
+            mul_bf16x2(x, y, e0[nt], q[nt]);
+            s0 = fmaf(x, acc[nt][0], s0);
+            s1 = fmaf(y, acc[nt][1], s1);
+            mul_bf16x2(x, y, e1[nt], q[nt]);
+            s2 = fmaf(x, acc[nt][2], s2);
+            s3 = fmaf(y, acc[nt][3], s3);
         }
-        load_E(ek0, Ek + (uint64_t)v0 * D2);
-        load_E(ek1, Ek + (uint64_t)v1 * D2);
-        unsigned hide = hidden16(a, job, job.r0, k0, staged, j > 0);
-        if (job.hi - k0 < 16) hide |= 0xffffffffu << (job.hi - k0);
+        load_E<2048>(e0, e1, at_lo, at_hi);
+        s0 += s1;
+        s2 += s3;
         s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
-        s1 += __shfl_xor_sync(0xffffffffu, s1, 1);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
         s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
-        s1 += __shfl_xor_sync(0xffffffffu, s1, 2);
-        const float x0 = (hide >> g) & 1u ? -INFINITY : s0 * BR_SCORE_LOG2, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s1 * BR_SCORE_LOG2;
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
+        const float x0 = (hide >> g) & 1u ? -INFINITY : s0 * BR_SCORE_LOG2, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2 * BR_SCORE_LOG2;
         const float m_new = fmaxf(m, fmaxf(x0, x1));
         const float ref = m_new == -INFINITY ? 0.f : m_new;
-        const float p0 = exp2f(x0 - ref), p1 = exp2f(x1 - ref);
+        const float p0 = ex2(x0 - ref), p1 = ex2(x1 - ref);
         if (__any_sync(0xffffffffu, m_new > m)) {
-            const float alpha = exp2f(m - ref);
+            const float alpha = ex2(m - ref);
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= alpha;
@@ -309,63 +311,47 @@ __device__ __forceinline__ void fma_job(const BranchArgs& a, const Job& job, con
         l += p0 + p1;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {      // (a value that is not finite stays in a row that hides it: the same slot is listed as the branch's own)
-            o[2 * nt] = fmaf(p0 * acc[nt][0], bf_lo(ev0[nt]), fmaf(p1 * acc[nt][2], bf_lo(ev1[nt]), o[2 * nt]));
-            o[2 * nt + 1] = fmaf(p0 * acc[nt][1], bf_hi(ev0[nt]), fmaf(p1 * acc[nt][3], bf_hi(ev1[nt]), o[2 * nt + 1]));
+            o[2 * nt] = fmaf(p0 * acc[nt][0], bf_lo(e0[nt]), fmaf(p1 * acc[nt][2], bf_lo(e1[nt]), o[2 * nt]));
+            o[2 * nt + 1] = fmaf(p0 * acc[nt][1], bf_hi(e0[nt]), fmaf(p1 * acc[nt][3], bf_hi(e1[nt]), o[2 * nt + 1]));
         }
-        load_E(ev0, Ev + (uint64_t)v0 * D2);
-        load_E(ev1, Ev + (uint64_t)v1 * D2);
-        u0 = min(u0 + 16, last);
-        u1 = min(u1 + 16, last);
-        v0 = job.slots[u0];
-        v1 = job.slots[u1];
     }
-}
+    __device__ __forceinline__ void leave(const BranchArgs& a, int64_t piece, int j, int h, int lane) {
+        float2 out;
+        join_quads(m, l, o, out);
+        const size_t at = ((size_t)piece * a.n + j) * a.H + h;
+        *reinterpret_cast<float2*>(a.po + at * BR_HD + quad_columns(lane)) = out;
+        if (lane == 0) a.ml[at] = make_float2(m, l);
+    }
+};
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Sixteen branches at a time: q.K and P.V as products too.  K goes in as two bf16 terms (its rounding would come back
 // through the exponent as an error of the score's size), V and P as one.  V's 8 x 8 blocks are transposed in registers.
 // ---------------------------------------------------------------------------------------------------------------------------
-static constexpr int BT_ROWS = 16;
-
-template <int KS>
-__device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, const WSource<KS>& W, int j, int h, float (&m)[2],
-                                        float (&l)[2], float (&o)[8][4]) {
-    const mbema_branches& br = a.br;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t D2 = (uint32_t)a.H * BR_HD * 2;
-    const char* Ek = reinterpret_cast<const char*>(a.Ek) + h * (BR_HD * 2) + 16 * t;
-    const char* Ev = reinterpret_cast<const char*>(a.Ev) + h * (BR_HD * 2) + 16 * t;
-    const int64_t row0 = job.r0 + min(g, job.rows - 1), row1 = job.r0 + min(g + 8, job.rows - 1);
+struct SixteenRows {
+    float m[2], l[2], o[8][4];
     uint32_t q0[8], q1[8];
-    load_E(q0, reinterpret_cast<const char*>(a.q) + (((size_t)row0 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
-    load_E(q1, reinterpret_cast<const char*>(a.q) + (((size_t)row1 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+    const uint32_t* hid0;
+    const uint32_t* hid1;
+    int64_t row0, row1;
+    __device__ __forceinline__ void start(const BranchArgs& a, int64_t r0, int rows, int j, int h, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        row0 = r0 + min(g, rows - 1);
+        row1 = r0 + min(g + 8, rows - 1);
+        load_q(q0, reinterpret_cast<const char*>(a.q) + (((size_t)row0 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
+        load_q(q1, reinterpret_cast<const char*>(a.q) + (((size_t)row1 * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * t);
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
-    const int words = (int)((br.Kcap + 31) / 32);
-    const uint32_t* hid0 = br.touched + (size_t)row0 * words;
-    const uint32_t* hid1 = br.touched + (size_t)row1 * words;
-    const int last = job.hi - 1;
-    const __half* op = job.op + 8 * t;
-    uint32_t A[KS][4], ek0[8], ek1[8], ev0[8], ev1[8];                // loads run a unit ahead, as in fma_job
-    int u0 = min(job.lo + g, last), u1 = min(job.lo + g + 8, last);
-    int v0 = job.slots[u0], v1 = job.slots[u1];
-    load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
-    load_E(ek0, Ek + (uint64_t)v0 * D2);
-    load_E(ek1, Ek + (uint64_t)v1 * D2);
-    load_E(ev0, Ev + (uint64_t)v0 * D2);
-    load_E(ev1, Ev + (uint64_t)v1 * D2);
-    u0 = min(job.lo + 16 + g, last);
-    u1 = min(job.lo + 24 + g, last);
-    v0 = job.slots[u0];
-    v1 = job.slots[u1];
-    for (int k0 = job.lo; k0 < job.hi; k0 += 16) {
-        float acc[8][4];
-        W.gate(acc, A);
-        load_A<KS>(A, op + (size_t)u0 * br.N, op + (size_t)u1 * br.N);
-        unsigned hide0 = (hid0[k0 >> 5] >> (k0 & 31)) & 0xffffu, hide1 = (hid1[k0 >> 5] >> (k0 & 31)) & 0xffffu;
-        apply_gate(acc, a.silu);
+        for (int nt = 0; nt < 8; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
+        const int words = (int)((a.br.Kcap + 31) / 32);
+        hid0 = a.br.touched + (size_t)row0 * words;
+        hid1 = a.br.touched + (size_t)row1 * words;
+    }
+    __device__ __forceinline__ void unit(const BranchArgs& a, float (&acc)[8][4], uint32_t at_lo, uint32_t at_hi, int k0, int count,
+                                         unsigned touched0, unsigned touched1, int j, int t) {
+        uint32_t e0[8], e1[8];
+        load_E<0>(e0, e1, at_lo, at_hi);
         float sc[2][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[0][i] = sc[1][i] = 0.f;
@@ -376,8 +362,8 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int nt = 2 * c + p;
-                const float x0 = bf_lo(ek0[nt]) * acc[nt][0], x1 = bf_hi(ek0[nt]) * acc[nt][1];
-                const float y0 = bf_lo(ek1[nt]) * acc[nt][2], y1 = bf_hi(ek1[nt]) * acc[nt][3];
+                const float x0 = bf_lo(e0[nt]) * acc[nt][0], x1 = bf_hi(e0[nt]) * acc[nt][1];
+                const float y0 = bf_lo(e1[nt]) * acc[nt][2], y1 = bf_hi(e1[nt]) * acc[nt][3];
                 hi[0][p] = pack_bf2(x0, x1);
                 hi[1][p] = pack_bf2(y0, y1);
                 lo[0][p] = pack_bf2(x0 - bf_lo(hi[0][p]), x1 - bf_hi(hi[0][p]));
@@ -389,12 +375,12 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
                 mma_bf16(sc[x], Q, lo[x][0], lo[x][1]);
             }
         }
-        load_E(ek0, Ek + (uint64_t)v0 * D2);
-        load_E(ek1, Ek + (uint64_t)v1 * D2);
+        load_E<2048>(e0, e1, at_lo, at_hi);
+        unsigned hide0 = (touched0 >> (k0 & 31)) & 0xffffu, hide1 = (touched1 >> (k0 & 31)) & 0xffffu;
         if (j > 0) {
             unsigned x = 0u, y = 0u;
             for (int i = t; i < j; i += 4) {
-                const unsigned d0 = (unsigned)(br.st_pos[br_index(br, row0, i)] - k0), d1 = (unsigned)(br.st_pos[br_index(br, row1, i)] - k0);
+                const unsigned d0 = (unsigned)(a.br.st_pos[br_index(a.br, row0, i)] - k0), d1 = (unsigned)(a.br.st_pos[br_index(a.br, row1, i)] - k0);
                 if (d0 < 16u) x |= 1u << d0;
                 if (d1 < 16u) y |= 1u << d1;
             }
@@ -403,8 +389,8 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
             hide0 |= x | __shfl_xor_sync(0xffffffffu, x, 2);
             hide1 |= y | __shfl_xor_sync(0xffffffffu, y, 2);
         }
-        if (job.hi - k0 < 16) {
-            const unsigned past = 0xffffffffu << (job.hi - k0);
+        if (count - k0 < 16) {
+            const unsigned past = 0xffffffffu << (count - k0);
             hide0 |= past;
             hide1 |= past;
         }
@@ -423,10 +409,10 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
             const float m_new = fmaxf(m[r], mx);
             const float ref = m_new == -INFINITY ? 0.f : m_new;
             moved |= m_new > m[r];
-            alpha[r] = exp2f(m[r] - ref);
+            alpha[r] = ex2(m[r] - ref);
             m[r] = m_new;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = exp2f(x[i] - ref);
+            for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - ref);
             l[r] = l[r] * alpha[r] + ((x[0] + x[1]) + (x[2] + x[3]));
             P[r] = pack_bf2(x[0], x[1]);
             P[2 + r] = pack_bf2(x[2], x[3]);
@@ -442,129 +428,253 @@ __device__ __forceinline__ void mma_job(const BranchArgs& a, const Job& job, con
         }
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            const uint32_t b0 = transpose8x8(pack_bf2(bf_lo(ev0[nt]) * acc[nt][0], bf_hi(ev0[nt]) * acc[nt][1]));
-            const uint32_t b1 = transpose8x8(pack_bf2(bf_lo(ev1[nt]) * acc[nt][2], bf_hi(ev1[nt]) * acc[nt][3]));
+            const uint32_t b0 = transpose8x8(pack_bf2(bf_lo(e0[nt]) * acc[nt][0], bf_hi(e0[nt]) * acc[nt][1]));
+            const uint32_t b1 = transpose8x8(pack_bf2(bf_lo(e1[nt]) * acc[nt][2], bf_hi(e1[nt]) * acc[nt][3]));
             mma_bf16(o[nt], P, b0, b1);
         }
-        load_E(ev0, Ev + (uint64_t)v0 * D2);
-        load_E(ev1, Ev + (uint64_t)v1 * D2);
-        u0 = min(u0 + 16, last);
-        u1 = min(u1 + 16, last);
-        v0 = job.slots[u0];
-        v1 = job.slots[u1];
     }
+    __device__ __forceinline__ void leave(const BranchArgs& a, int64_t piece, int rows, int j, int h, int lane) {
+        const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            const int row = g + 8 * r;
+            if (row < rows) {
+                const size_t at = (((size_t)piece * BR_BLOCK + row) * a.n + j) * a.H + h;
+                float* dst = a.po + at * BR_HD + 8 * t;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4*>(dst + 32 * (i >> 1) + 4 * (i & 1)) =
+                        make_float4(o[2 * i][2 * r], o[2 * i][2 * r + 1], o[2 * i + 1][2 * r], o[2 * i + 1][2 * r + 1]);
+                if (t == 0) a.ml[at] = make_float2(m[r], l[r]);
+            }
+        }
     }
+};
+
+// Where a stretch begins: the first list whose units reach cost c, by 32 samples of the running sum at a time.
+__device__ __forceinline__ int64_t find_list(const long long* work, int64_t lists, long long c, int lane) {
+    int64_t lo = 0, hi = lists;                   // work[lo] <= c < work[hi]
+    while (hi - lo > 1) {
+        const int64_t step = (hi - lo + 31) / 32;
+        const int64_t at = lo + (lane + 1) * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at] <= c);
+        lo += __popc(below) * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
 }
 
-// grid: x = CTAs that share the jobs, y = head, z = block of JW steps.  Warp w takes step z JW + w % JW; the IG warps of a step
-// take jobs of their own.  ROWS: branches that a job of a prefix takes (1: fma_job, 16: mma_job).
-template <int KS, int ROWS>
-__global__ void __launch_bounds__(BT_THREADS, 1) k_branch_tc(BranchArgs a, int JW, int IG) {
-    extern __shared__ __align__(16) float smem[];
+// grid: x = CTAs that share the work, y = head, z = block of JW steps.  The CTA's warps are IG workers of JW warps each; warp w takes
+// step z JW + w % JW of worker w / JW.  ROWS: branches that read a prefix together (1 or 16).
+template <int KS, int ROWS, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int JW, int IG) {
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_l2r[16 * KS];
+    using Unit = UnitLayout<KS>;
     const mbema_branches& br = a.br;
     constexpr int N = 16 * KS;
-    const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.H * BR_HD;
-    float* W_sh = smem;                                                     // [N] rows at w_row
-    uint2* Wf = reinterpret_cast<uint2*>(smem + (N * BT_LDW + 8));          // KS = 8: [JW][KS * 8 * 32]
-    for (int i = tid; i < N * 16; i += BT_THREADS) {
+    // KS = 8: the fragments of W behind the ring, whose space the staged slice of W takes first
+    float* W_sh = reinterpret_cast<float*>(smem);
+    uint2* Wf = reinterpret_cast<uint2*>(smem + a.ring_bytes);
+    for (int i = tid; i < N * 16; i += WARPS * 32) {
         const float4 x = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
         float2* dst = reinterpret_cast<float2*>(W_sh + w_row(i >> 4) + (i & 15) * 4);
         dst[0] = make_float2(x.x, x.y);
         dst[1] = make_float2(x.z, x.w);
     }
-    for (int i = tid; i < N; i += BT_THREADS) s_l2r[i] = log2f(br.rhos[i]);
-    __syncthreads();
+    for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = log2f(br.rhos[i]);
+    const int64_t lists = a.n_pre + br.B * br.S;
+    const long long total = a.br.work[lists];
+    const long long workers = branch_workers(total, (long long)gridDim.x * IG);
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;
-    if (ig >= IG || j >= a.n) return;
-    WSource<KS> W;                 // KS = 8: the IG warps of a step write the same fragments, each reads what it has written
-    W.build(W_sh, s_l2r, Wf + (size_t)jj * KS * 8 * 32, j, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane);
-    const int blocks = (int)((br.S + ROWS - 1) / ROWS);
-    const int64_t jobs = br.B * blocks * a.plan.SP + br.B * br.S * a.plan.SO;
-    const int parts = a.plan.SP + a.plan.SO;
-    for (int64_t x = (int64_t)blockIdx.x * IG + ig; x < jobs; x += (int64_t)gridDim.x * IG) {
-        Job job;
-        if (!find_job(job, a, x, ROWS)) continue;
-        if (ROWS == 1 || job.own) {
-            float m, l, o[16];
-            fma_job<KS>(a, job, W, j, h, m, l, o);
-            float2 out;
-            join_quads(m, l, o, out);
-            const size_t at = (((size_t)job.r0 * a.n + j) * a.H + h) * parts + job.part;
-            *reinterpret_cast<float2*>(a.po + at * BR_HD + quad_columns(lane)) = out;
-            if (lane == 0) a.ml[at] = make_float2(m, l);
-        } else if constexpr (ROWS > 1) {
-            float m[2], l[2], o[8][4];
-            mma_job<KS>(a, job, W, j, h, m, l, o);
-            const int g = lane >> 2, t = lane & 3;
+    const int steps = min(JW, a.n - (int)blockIdx.z * JW);       // of this CTA
+    const long long me = (long long)blockIdx.x * IG + ig;
+    __syncthreads();
+    WSource<KS> W;                 // KS = 8: the workers write the same fragments of a step, each reads what it has written
+    if (ig < IG && jj < steps) W.build(W_sh, s_l2r, Wf + (size_t)jj * KS * 8 * 32, j, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane);
+    __syncthreads();
+    if (ig >= IG || jj >= steps || me >= workers) return;
+    const long long c_end = branch_cut(total, workers, me + 1);
+    const long long* work = reinterpret_cast<const long long*>(br.work);
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + ig * STAGES * Unit::BYTES;
+    const uint32_t ring_end = ring + STAGES * Unit::BYTES;
+
+    // producer: `left` units of list px from slot pk on; the ids of its next unit are a unit ahead
+    int64_t px;
+    int pk, left;
+    List pl;
+    auto units_to = [&](long long from, long long to, int cost) { return (int)((min(to, c_end) - from + cost - 1) / cost); };
+    auto cost_of = [&](int64_t list) { return list < a.n_pre ? a.cost_pre : BR_COST_OWN; };
+    auto next_list = [&](int64_t& list) {                        // the next list with units in this stretch: their number, or 0
+        for (;;) {
+            const long long lo = work[++list];
+            if (lo >= c_end) return 0;
+            const long long hi = work[list + 1];
+            if (hi > lo) return units_to(lo, hi, cost_of(list));
+        }
+    };
+    {
+        const long long c0 = branch_cut(total, workers, me);
+        px = find_list(work, lists, c0, lane);
+        const long long lo = work[px];
+        const int cost = cost_of(px), skip = (int)((c0 - lo + cost - 1) / cost);   // units of the list before this stretch
+        pk = skip * 16;
+        left = max(units_to(lo + (long long)skip * cost, work[px + 1], cost), 0);
+        if (left == 0) { pk = 0; left = next_list(px); }
+        if (left == 0) return;                                   // nothing is listed at all (the whole worker leaves)
+        pl = get_list(a, px);
+    }
+    int64_t x = px;                                              // consumer: c_left units of list x from slot k0 on
+    int k0 = pk, c_left = left, count = pl.count;
+    // a copy of this lane: a 16-byte piece of four rows (E_k 0-3, E_v 4-7) or of 512 bytes of fragments (8 on)
+    const int sub = lane >> 3;
+    const char* Ek = reinterpret_cast<const char*>(a.Ek) + h * (BR_HD * 2) + (lane & 7) * 16;
+    const char* Ev = reinterpret_cast<const char*>(a.Ev) + h * (BR_HD * 2) + (lane & 7) * 16;
+    const uint32_t D2 = (uint32_t)D * 2;
+    const uint32_t dst_E = sub * 128 + (((lane & 7) ^ ((sub & 1) << 2)) << 4), dst_A = Unit::OP + lane * 16;
+    int ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
+    uint32_t fill = ring;                                        // stage that the producer fills next
+    auto produce = [&]() {
+        if (left > 0) {
+            const char* op = pl.op + (size_t)(pk >> 4) * Unit::OP_BYTES + lane * 16;
+            const int now = ids;
+            pk += 16;
+            if (--left == 0) {
+                left = next_list(px);
+                if (left > 0) { pl = get_list(a, px); pk = 0; }
+            }
+            if (left > 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
+            if (steps == 1) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = g + 8 * r;
-                if (row < job.rows) {
-                    const size_t at = (((size_t)(job.r0 + row) * a.n + j) * a.H + h) * parts + job.part;
-                    float* dst = a.po + at * BR_HD + 8 * t;
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, now, i * 4 + sub);
+                    cp_async16(fill + dst_E + i * 512, Ek + (uint64_t)v * D2);
+                    cp_async16(fill + dst_E + Unit::EV + i * 512, Ev + (uint64_t)v * D2);
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<float4*>(dst + 32 * (i >> 1) + 4 * (i & 1)) =
-                            make_float4(o[2 * i][2 * r], o[2 * i][2 * r + 1], o[2 * i + 1][2 * r], o[2 * i + 1][2 * r + 1]);
-                    if (t == 0) a.ml[at] = make_float2(m[r], l[r]);
+                for (int i = 0; i < KS; ++i) cp_async16(fill + dst_A + i * 512, op + i * 512);
+            } else {                                             // the worker's warps share the copies
+                for (int i = jj; i < 8 + KS; i += steps) {
+                    if (i < 8) {
+                        const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, now, (i & 3) * 4 + sub);
+                        cp_async16(fill + dst_E + i * 512, (i < 4 ? Ek : Ev) + (uint64_t)v * D2);
+                    } else {
+                        cp_async16(fill + dst_A + (i - 8) * 512, op + (i - 8) * 512);
+                    }
                 }
             }
         }
+        cp_commit();
+        fill += Unit::BYTES;
+        if (fill == ring_end) fill = ring;
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) produce();
+    OneRow one;
+    SixteenRows many;
+    bool fresh = true, own = false, single = true;
+    int rows = 1;
+    const uint32_t* bits = nullptr;                              // one branch's bits over the prefix
+    uint32_t at = ring;
+    const uint32_t lane_lo = g * 128 + ((t ^ ((g & 1) << 2)) << 4), lane_hi = lane_lo ^ 64u;
+    for (;;) {
+        if (fresh) {
+            own = x >= a.n_pre;
+            single = ROWS == 1 || own;
+            if (single) {
+                const int64_t r = own ? x - a.n_pre : x;
+                one.start(a, r, own, j, h, lane);
+                bits = own ? nullptr : br.touched + (size_t)r * ((br.Kcap + 31) / 32);
+            } else if constexpr (ROWS > 1) {
+                const int b = (int)(x / a.blocks), s0 = (int)(x - (int64_t)b * a.blocks) * ROWS;
+                rows = min(ROWS, (int)br.S - s0);
+                many.start(a, (int64_t)b * br.S + s0, rows, j, h, lane);
+            }
+            fresh = false;
+        }
+        unsigned touched0 = 0u, touched1 = 0u;
+        if (single && bits) touched0 = bits[k0 >> 5];
+        if constexpr (ROWS > 1) {
+            if (!single) { touched0 = many.hid0[k0 >> 5]; touched1 = many.hid1[k0 >> 5]; }
+        }
+        cp_wait<STAGES - 2>();
+        if (steps == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(ig + 1), "r"(steps * 32) : "memory");
+        produce();
+        float acc[8][4];
+        {
+            uint32_t A[KS][4];
+            load_A<KS>(A, at + lane * 16);
+            W.gate(acc, A);
+        }
+        apply_gate(acc, a.silu);
+        if (single) one.unit(acc, at + lane_lo, at + lane_hi, hidden16(touched0, k0, one.staged, j > 0, count), g);
+        else if constexpr (ROWS > 1) many.unit(a, acc, at + lane_lo, at + lane_hi, k0, count, touched0, touched1, j, t);
+        at += Unit::BYTES;
+        if (at == ring_end) at = ring;
+        k0 += 16;
+        if (--c_left == 0) {                                     // end of the list or of the stretch
+            if (single) one.leave(a, own ? a.own_piece0 + (x - a.n_pre) + me : x + me, j, h, lane);
+            else if constexpr (ROWS > 1) many.leave(a, x + me, rows, j, h, lane);
+            c_left = next_list(x);
+            if (c_left == 0) break;
+            k0 = 0;
+            count = x < a.n_pre ? min(br.n_active[x / a.blocks], (int)br.Kcap) : br.own_n[x - a.n_pre];
+            fresh = true;
+        }
     }
+    cp_wait<0>();
 }
 
 bool branch_tc_supported(int64_t N) { return N == 64 || N == 128; }
 
-static void steps_and_shares(int n, int& JW, int& IG) {
-    JW = std::min(n, BT_WARPS);
-    IG = BT_WARPS / JW;
+// How the warps of a CTA are dealt: JW steps to a worker (they share its E and operand rows), IG workers.  Between three (all, of
+// fewer) and six steps, whichever keeps the most warps busy over all blocks of steps; more steps where that is equal.
+static void steps_and_workers(int n, int warps, int& JW, int& IG) {
+    double best = -1.0;
+    for (int jw = std::min(n, 3); jw <= std::min(n, 6); ++jw) {
+        const int zb = (n + jw - 1) / jw;
+        const double busy = (double)(warps / jw) * n / zb;
+        if (busy >= best) { best = busy; JW = jw; }
+    }
+    IG = warps / JW;
 }
 
-// One CTA an SM (the registers allow no more), dealt to the heads and blocks of steps.
-static int64_t ctas_a_head(int64_t H, int64_t zb) { return std::max<int64_t>(1, 148 / (H * zb)); }
+// Registers: W (64), accumulators (32) and one row's o and q let twelve warps run with 168 each, sixteen rows' o and q eight with
+// 255.  One step, one branch: eight, the ring of twelve workers is too large.
+static int tc_warps(int64_t S, int64_t n) { return S == 1 && n > 1 ? 12 : 8; }
 
-// Chunks: about four jobs a worker if all lists were full, of 2 to 32 units of 16 slots (a job costs about one unit more than its
-// units: q, the joining of the quads, the partial).
-BranchPlan branch_plan_tc(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap) {
-    int JW, IG;
-    steps_and_shares((int)n, JW, IG);
-    const int64_t zb = (n + JW - 1) / JW, workers = ctas_a_head(H, zb) * IG;
-    const int64_t lists = S == 1 ? B : B * ((S + BT_ROWS - 1) / BT_ROWS);
-    const int64_t units = lists * ((Kcap + 15) / 16) + B * S * ((cap + 15) / 16);
-    const int64_t chunk = 16 * std::min<int64_t>(32, std::max<int64_t>(2, units / (4 * workers)));
-    BranchPlan p;
-    p.chp = p.cho = (int)chunk;
-    p.SP = (int)((Kcap + chunk - 1) / chunk);
-    p.SO = (int)((cap + chunk - 1) / chunk);
+BranchShape branch_shape(int64_t B, int64_t S, int64_t n, int64_t H) {
+    BranchShape p;
+    p.rows = S == 1 ? 1 : BR_BLOCK;
+    p.blocks = (int)((S + p.rows - 1) / p.rows);
+    p.warps = tc_warps(S, n);
+    steps_and_workers((int)n, p.warps, p.JW, p.IG);
+    p.zb = (int)((n + p.JW - 1) / p.JW);
+    p.ctas = (int)std::max<int64_t>(1, 148 / (H * p.zb));       // one CTA an SM, dealt to the heads and blocks of steps
     return p;
 }
 
-template <int KS, int ROWS>
-static int launch_tc(const BranchArgs& a, cudaStream_t st) {
-    int JW, IG;
-    steps_and_shares(a.n, JW, IG);
-    const mbema_branches& br = a.br;
-    const int zb = (a.n + JW - 1) / JW;
-    const int64_t jobs = br.B * ((br.S + ROWS - 1) / ROWS) * a.plan.SP + br.B * br.S * a.plan.SO;
-    const int64_t x = std::min((jobs + IG - 1) / IG, ctas_a_head(a.H, zb));
-    const size_t smem = ((size_t)16 * KS * BT_LDW + 8) * 4 + (KS == 8 ? (size_t)JW * KS * 8 * 32 * sizeof(uint2) : 0);
-    MBEMA_CUDA_TRY(cudaFuncSetAttribute(k_branch_tc<KS, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k_branch_tc<KS, ROWS><<<dim3((unsigned)x, (unsigned)a.H, (unsigned)zb), BT_THREADS, smem, st>>>(a, JW, IG);
+template <int KS, int ROWS, int WARPS, int STAGES>
+static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
+    const size_t w_sh = ((size_t)16 * KS * BT_LDW + 8) * 4;
+    a.ring_bytes = (int)align_up(std::max(w_sh, (size_t)p.IG * STAGES * UnitLayout<KS>::BYTES), 128);
+    const size_t smem = a.ring_bytes + (KS == 8 ? (size_t)p.JW * KS * 8 * 32 * sizeof(uint2) : 0);
+    MBEMA_CUDA_TRY(cudaFuncSetAttribute(k_branch_tc<KS, ROWS, WARPS, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    k_branch_tc<KS, ROWS, WARPS, STAGES><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st>>>(a, p.JW, p.IG);
     return check_launch();
 }
 
-int launch_branch_attend_tc(const BranchArgs& a, cudaStream_t st) {
-    const bool one = a.br.S == 1;
+int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
-    if (a.br.N == 64) return one ? launch_tc<4, 1>(a, st) : launch_tc<4, BT_ROWS>(a, st);
-    return one ? launch_tc<8, 1>(a, st) : launch_tc<8, BT_ROWS>(a, st);
+    if (a.br.N == 64)
+        return p.rows > 1 ? launch_tc<4, BR_BLOCK, 8, 4>(a, p, st) : p.warps == 12 ? launch_tc<4, 1, 12, 4>(a, p, st) : launch_tc<4, 1, 8, 4>(a, p, st);
+    return p.rows > 1 ? launch_tc<8, BR_BLOCK, 8, 3>(a, p, st) : p.warps == 12 ? launch_tc<8, 1, 12, 3>(a, p, st) : launch_tc<8, 1, 8, 3>(a, p, st);
 }
 
 }  // namespace mbema

@@ -144,41 +144,91 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
 
 // Operand copies of all listed slots at the first staged step, state * rho^(t0 + len - last) / 64 in fp16 (11 significant bits; a
 // state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head.  grid: x = shares of a list,
-// y = sequence, z = 0: its prefix, s + 1: branch s.  A thread makes eight channels.
+// y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sum of
+// the lists' units that the attention deals its work by.
+__device__ void running_sum(const mbema_branches& br) {
+    __shared__ long long s_warp[8];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int blocks = br.S == 1 ? 1 : (int)((br.S + BR_BLOCK - 1) / BR_BLOCK);
+    const int64_t n_pre = br.B * blocks, lists = n_pre + br.B * br.S;
+    long long base = 0;
+    for (int64_t x0 = 0; x0 < lists; x0 += 256) {
+        const int64_t x = x0 + tid;
+        long long c = 0;
+        if (x < n_pre) c = (long long)((min(br.n_active[x / blocks], (int)br.Kcap) + 15) / 16) * (br.S == 1 ? BR_COST_ONE : BR_COST_BLOCK);
+        else if (x < lists) c = (long long)((br.own_n[x - n_pre] + 15) / 16) * BR_COST_OWN;
+        long long sum = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        if (lane == 31) s_warp[tid >> 5] = sum;
+        __syncthreads();
+        long long all = 0;
+        for (int w = 0; w < 8; ++w) {
+            if (w < (tid >> 5)) sum += s_warp[w];
+            all += s_warp[w];
+        }
+        if (x < lists) br.work[x] = base + sum - c;
+        base += all;
+        __syncthreads();
+    }
+    if (tid == 0) br.work[lists] = base;
+}
+
 __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
+    if (blockIdx.y == br.B) {
+        if (blockIdx.x == 0 && blockIdx.z == 0) running_sum(br);
+        return;
+    }
     const int b = blockIdx.y, z = blockIdx.z;
-    const int N = (int)br.N, per = N / 8;
+    const int N = (int)br.N, half = N / 32;             // pairs of fragments: a warp makes one of sixteen slots
     const int64_t r = (int64_t)b * br.S + (z ? z - 1 : 0);
     const int count = z ? br.own_n[r] : min(br.n_active[b], (int)br.Kcap);
     const int now = br.t0[0] + br.len[r];
-    const int c = (threadIdx.x % per) * 8;
-    const int items = 256 / per;                        // a power of two of threads an item: 8 or 16
-    int k = blockIdx.x * items + threadIdx.x / per;
-    if (k >= count) return;
+    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int i = warp % half, c = 32 * i + 8 * (lane & 3);
+    char* out = reinterpret_cast<char*>(z ? br.own_op : br.pre_op) + (z ? (size_t)r * br_operand_bytes(br.cap, N) : (size_t)b * br_operand_bytes(br.Kcap, N));
+    int k = warp / half * 16 + (lane >> 2);
+    if (k - (lane >> 2) >= count) return;
     float l2r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) l2r[i] = log2f(br.rhos[c + i]);
-    for (; k < count; k += gridDim.x * items) {
-        const float* src;
-        int last;
-        if (z) {
-            src = br.own_state + ((size_t)r * br.cap + k) * N;
-            last = br.own_t[(size_t)r * br.cap + k];
-        } else {
-            const int v = br.active[(size_t)b * br.Kcap + k];
-            src = br.state + ((size_t)b * br.V + v) * N;
-            last = br.last_t[(size_t)b * br.V + v];
-        }
-        const float dt = (float)(now - last);
-        const float4 x = *reinterpret_cast<const float4*>(src + c), y = *reinterpret_cast<const float4*>(src + c + 4);
-        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-        __half2 o[4];
+    for (int e = 0; e < 8; ++e) l2r[e] = log2f(br.rhos[c + e]);
+    for (; k - (lane >> 2) < count; k += gridDim.x * 8 / half * 16) {
+        uint32_t w[2][4];                               // slots k, k + 8
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            o[i] = __floats2half2_rn(fminf(f[2 * i] * exp2f(dt * l2r[2 * i]) * BR_OP_SCALE, 65504.f),
-                                     fminf(f[2 * i + 1] * exp2f(dt * l2r[2 * i + 1]) * BR_OP_SCALE, 65504.f));
-        __half* dst = reinterpret_cast<__half*>(z ? br.own_op : br.pre_op) + ((z ? (size_t)r * br.cap : (size_t)b * br.Kcap) + k) * N + c;
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(o);
+        for (int hi = 0; hi < 2; ++hi) {
+            const int slot = k + 8 * hi;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = 0.f;
+            if (slot < count) {
+                const float* src;
+                int last;
+                if (z) {
+                    src = br.own_state + ((size_t)r * br.cap + slot) * N;
+                    last = br.own_t[(size_t)r * br.cap + slot];
+                } else {
+                    const int v = br.active[(size_t)b * br.Kcap + slot];
+                    src = br.state + ((size_t)b * br.V + v) * N;
+                    last = br.last_t[(size_t)b * br.V + v];
+                }
+                const float dt = (float)(now - last);
+                const float4 x = *reinterpret_cast<const float4*>(src + c), y = *reinterpret_cast<const float4*>(src + c + 4);
+                const float in[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = fminf(in[e] * exp2f(dt * l2r[e]) * BR_OP_SCALE, 65504.f);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const __half2 o = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+                w[hi][e] = *reinterpret_cast<const uint32_t*>(&o);
+            }
+        }
+        char* dst = out + (size_t)(k >> 4) * N * 32 + (2 * i) * 512 + lane * 16;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
+        *reinterpret_cast<uint4*>(dst + 512) = make_uint4(w[0][2], w[1][2], w[0][3], w[1][3]);
     }
 }
 
@@ -229,7 +279,10 @@ static int check_branches(const mbema_branches* br) {
                           br->st_new, br->st_state, br->overflow};
     for (const void* p : need)
         if (!p) return MBEMA_ERR_NULL;
-    if ((br->pre_op || br->own_op) && (!branch_tc_supported(br->N) || br->S >= 65535)) return MBEMA_ERR_UNSUPPORTED;
+    if (br->pre_op || br->own_op || br->work) {              // all three or none
+        if (!branch_tc_supported(br->N) || br->S >= 65535 || br->B >= 65535) return MBEMA_ERR_UNSUPPORTED;
+        if (!br->pre_op || !br->own_op || !br->work) return MBEMA_ERR_NULL;
+    }
     return MBEMA_OK;
 }
 
@@ -255,11 +308,11 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
     k_branch_stage<<<(unsigned)(br->B * br->S), BS_THREADS, 0, (cudaStream_t)stream>>>(*br, (const long long*)tok, (int)n, nullptr,
                                                                                    (int)n_pending, C_q);
     rc = check_launch();
-    if (rc != MBEMA_OK || !br->pre_op || !br->own_op) return rc;
-    // shares of a list: two CTAs an SM for a few sequences, one share of 32 or 16 slots where that is enough
-    const int64_t items = 256 / (br->N / 8), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
+    if (rc != MBEMA_OK || !br->pre_op) return rc;
+    // shares of a list: eight CTAs an SM over all lists, one for every 64 or 32 slots where that is enough
+    const int64_t items = 16 * 8 / (br->N / 32), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
     const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
-    k_branch_operands<<<dim3((unsigned)x, (unsigned)br->B, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream>>>(*br);
+    k_branch_operands<<<dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream>>>(*br);
     return check_launch();
 }
 

@@ -11,11 +11,23 @@ static constexpr int BR_MAX_NEW = 32;              // staged tokens a branch: on
 static constexpr float BR_OP_SCALE = 1.0f / 64.0f;  // operand copies hold state / 64 in fp16: up to 4.19 million, saturated
 static constexpr float BR_SCORE_LOG2 = 0.125f * 1.4426950408889634f;   // 1 / sqrt(64), in powers of two
 
-// How the slot lists are cut into jobs.  A job is one chunk of a sequence's prefix for all its branches, or one chunk of a
-// branch's own slots; it leaves one partial (m, l, o[64]) for each of its rows, heads and steps, which k_branch_merge joins.
+static constexpr int BR_BLOCK = 16;                // branches that read a prefix together on the tensor cores
+// Cost of a unit (16 slots) of a list, in the running sum that mbema_branches_extend leaves: own slots, a prefix read by one branch,
+// a prefix read by sixteen.
+static constexpr int BR_COST_OWN = 2, BR_COST_ONE = 2, BR_COST_BLOCK = 3;
+
+// fp32 arithmetic: how the slot lists are cut into chunks.  A chunk of a sequence's prefix for all its branches, or one of a
+// branch's own slots, leaves one partial (m, l, o[64]) for each of its rows, heads and steps, which k_branch_merge joins.
 struct BranchPlan {
     int chp, cho;      // slots a chunk: prefix, own
     int SP, SO;        // chunks that the lists' capacities allow
+};
+
+// Tensor cores: workers, and the lists in the running sum: prefixes (as blocks of branches read them), then the branches' own.
+struct BranchShape {
+    int rows, blocks;      // branches that read a prefix together; such blocks a sequence
+    int warps, JW, IG;     // of a CTA: warps, steps a worker, workers
+    int zb, ctas;          // blocks of steps; CTAs a head and block of steps
 };
 
 struct BranchArgs {
@@ -25,16 +37,35 @@ struct BranchArgs {
     const void* Ev;
     const float* W;
     void* O;
-    float2* ml;              // [rows, H, SP + SO]: maximum (of base-2 scores), sum
-    float* po;               // [rows, H, SP + SO, 64]
+    float2* ml;              // maximum (of base-2 scores) and sum of every partial
+    float* po;               // [.., 64] its o
     int q_dt, e_dt;
     int n, H;
     float v_total;
     int silu, listed_only;
+    // fp32 arithmetic: partials [rows, H, SP + SO]
     BranchPlan plan;
+    // tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order; partials of the prefixes
+    // [piece, BR_BLOCK or 1, n, H], of the own lists [own_piece0 + piece, n, H]
+    int64_t n_pre, own_piece0, max_workers;
+    int rows, blocks, cost_pre, ring_bytes;
 };
 
+// The workers that a running sum of `total` occupies, each with two units or more, and where their stretches begin.
+__device__ __forceinline__ long long branch_workers(long long total, long long most) {
+    return max(1ll, min(most, total / (2 * BR_COST_BLOCK)));
+}
+__device__ __forceinline__ long long branch_cut(long long total, long long workers, long long w) { return total * w / workers; }
+// the worker whose stretch holds cost c < total
+__device__ __forceinline__ long long branch_worker_of(long long total, long long workers, long long c) {
+    return ((c + 1) * workers - 1) / total;
+}
+
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
+
+// Operands of a list: fp16 fragments of the gate product, 16 slots after 16 slots.  Slot k, channel c = 32 i + 8 t + 4 u + 2 p + e is half e
+// of word (row / 8) + 2 p (row = k % 16) of lane 4 (row % 8) + t in fragment 2 i + u of its sixteen (512 bytes each).
+__host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + 15) / 16) * N * 32; }
 
 // Row j of branch r cannot see slot k of the prefix: the branch has touched it, or does so with a staged token before j.
 __device__ __forceinline__ bool br_hides_prefix(const mbema_branches& br, int64_t r, int j, int k) {
@@ -51,9 +82,9 @@ __device__ __forceinline__ bool br_hides_own(const mbema_branches& br, int64_t r
 }
 
 bool branch_tc_supported(int64_t N);
-BranchPlan branch_plan_tc(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap);
-int launch_branch_attend_tc(const BranchArgs& a, cudaStream_t st);
+BranchShape branch_shape(int64_t B, int64_t S, int64_t n, int64_t H);
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st);
-int launch_branch_merge(const BranchArgs& a, cudaStream_t st);
+int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st);
+int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st);
 
 }  // namespace mbema
