@@ -221,14 +221,14 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     if constexpr (PIECES) {
         const int64_t own = a.n_pre + r;
         const int64_t pre = a.rows == 1 ? b : (int64_t)b * a.blocks + s / a.rows;
-        const long long total = br.work[a.n_pre + br.B * br.S], workers = branch_workers(total, a.max_workers);
-        auto pieces = [&](int64_t list, int cost, long long& first) {
-            const long long lo = br.work[list], hi = br.work[list + 1];
+        const int total = br.work[a.n_pre + br.B * br.S], workers = branch_workers(total, (int)a.max_workers);
+        auto pieces = [&](int64_t list, int cost, int& first) {
+            const int lo = br.work[list], hi = br.work[list + 1];
             if (hi == lo) return 0;
             first = branch_worker_of(total, workers, lo);
-            return (int)(branch_worker_of(total, workers, hi - cost) - first) + 1;
+            return branch_worker_of(total, workers, hi - cost) - first + 1;
         };
-        long long wp = 0, wq = 0;
+        int wp = 0, wq = 0;
         np = pieces(pre, a.cost_pre, wp);
         nq = pieces(own, BR_COST_OWN, wq);
         const size_t each = (size_t)n * H, at = (size_t)j * H + h;

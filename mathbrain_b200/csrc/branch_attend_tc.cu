@@ -194,16 +194,16 @@ struct List {
     int count;
 };
 
-__device__ __forceinline__ List get_list(const BranchArgs& a, int64_t x) {
+__device__ __forceinline__ List get_list(const BranchArgs& a, int x) {
     const mbema_branches& br = a.br;
     List t;
-    if (x < a.n_pre) {
-        const int b = (int)(x / a.blocks);
+    if (x < (int)a.n_pre) {
+        const int b = x / a.blocks;
         t.slots = br.active + (size_t)b * br.Kcap;
         t.op = reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N);
         t.count = min(br.n_active[b], (int)br.Kcap);
     } else {
-        const int64_t r = x - a.n_pre;
+        const int r = x - (int)a.n_pre;
         t.slots = br.own_slot + (size_t)r * br.cap;
         t.op = reinterpret_cast<const char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, br.N);
         t.count = br.own_n[r];
@@ -454,11 +454,11 @@ struct SixteenRows {
 };
 
 // Where a stretch begins: the first list whose units reach cost c, by 32 samples of the running sum at a time.
-__device__ __forceinline__ int64_t find_list(const long long* work, int64_t lists, long long c, int lane) {
-    int64_t lo = 0, hi = lists;                   // work[lo] <= c < work[hi]
+__device__ __forceinline__ int find_list(const int* work, int lists, int c, int lane) {
+    int lo = 0, hi = lists;                       // work[lo] <= c < work[hi]
     while (hi - lo > 1) {
-        const int64_t step = (hi - lo + 31) / 32;
-        const int64_t at = lo + (lane + 1) * step;
+        const int step = (hi - lo + 31) / 32;
+        const int at = lo + (lane + 1) * step;
         const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at] <= c);
         lo += __popc(below) * step;
         hi = min(hi, lo + step);
@@ -487,69 +487,69 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         dst[1] = make_float2(x.z, x.w);
     }
     for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = log2f(br.rhos[i]);
-    const int64_t lists = a.n_pre + br.B * br.S;
-    const long long total = a.br.work[lists];
-    const long long workers = branch_workers(total, (long long)gridDim.x * IG);
+    const int lists = (int)(a.n_pre + br.B * br.S), n_pre = (int)a.n_pre;
+    const int total = br.work[lists];
+    const int workers = branch_workers(total, (int)gridDim.x * IG);
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;
     const int steps = min(JW, a.n - (int)blockIdx.z * JW);       // of this CTA
-    const long long me = (long long)blockIdx.x * IG + ig;
+    const int me = (int)blockIdx.x * IG + ig;
     __syncthreads();
     WSource<KS> W;                 // KS = 8: the workers write the same fragments of a step, each reads what it has written
     if (ig < IG && jj < steps) W.build(W_sh, s_l2r, Wf + (size_t)jj * KS * 8 * 32, j, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane);
     __syncthreads();
     if (ig >= IG || jj >= steps || me >= workers) return;
-    const long long c_end = branch_cut(total, workers, me + 1);
-    const long long* work = reinterpret_cast<const long long*>(br.work);
+    const int c_end = branch_cut(total, workers, me + 1);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + ig * STAGES * Unit::BYTES;
     const uint32_t ring_end = ring + STAGES * Unit::BYTES;
 
     // producer: `left` units of list px from slot pk on; the ids of its next unit are a unit ahead
-    int64_t px;
-    int pk, left;
+    int px, pk, left;
     List pl;
-    auto units_to = [&](long long from, long long to, int cost) { return (int)((min(to, c_end) - from + cost - 1) / cost); };
-    auto cost_of = [&](int64_t list) { return list < a.n_pre ? a.cost_pre : BR_COST_OWN; };
-    auto next_list = [&](int64_t& list) {                        // the next list with units in this stretch: their number, or 0
+    auto units_to = [&](int from, int to, int cost) { return (min(to, c_end) - from + cost - 1) / cost; };
+    auto cost_of = [&](int list) { return list < n_pre ? a.cost_pre : BR_COST_OWN; };
+    auto next_list = [&](int& list) {                            // the next list with units in this stretch: their number, or 0
         for (;;) {
-            const long long lo = work[++list];
+            const int lo = br.work[++list];
             if (lo >= c_end) return 0;
-            const long long hi = work[list + 1];
+            const int hi = br.work[list + 1];
             if (hi > lo) return units_to(lo, hi, cost_of(list));
         }
     };
     {
-        const long long c0 = branch_cut(total, workers, me);
-        px = find_list(work, lists, c0, lane);
-        const long long lo = work[px];
-        const int cost = cost_of(px), skip = (int)((c0 - lo + cost - 1) / cost);   // units of the list before this stretch
+        const int c0 = branch_cut(total, workers, me);
+        px = find_list(br.work, lists, c0, lane);
+        const int lo = br.work[px], cost = cost_of(px), skip = (c0 - lo + cost - 1) / cost;      // units of the list before this stretch
         pk = skip * 16;
-        left = max(units_to(lo + (long long)skip * cost, work[px + 1], cost), 0);
+        left = max(units_to(lo + skip * cost, br.work[px + 1], cost), 0);
         if (left == 0) { pk = 0; left = next_list(px); }
         if (left == 0) return;                                   // nothing is listed at all (the whole worker leaves)
         pl = get_list(a, px);
     }
-    int64_t x = px;                                              // consumer: c_left units of list x from slot k0 on
+    int x = px;                                                  // consumer: c_left units of list x from slot k0 on
     int k0 = pk, c_left = left, count = pl.count;
-    // a copy of this lane: a 16-byte piece of four rows (E_k 0-3, E_v 4-7) or of 512 bytes of fragments (8 on)
+    // copies of a lane: 16-byte pieces of rows 4 i + sub of E_k and E_v, and of the fragments
     const int sub = lane >> 3;
     const char* Ek = reinterpret_cast<const char*>(a.Ek) + h * (BR_HD * 2) + (lane & 7) * 16;
     const char* Ev = reinterpret_cast<const char*>(a.Ev) + h * (BR_HD * 2) + (lane & 7) * 16;
     const uint32_t D2 = (uint32_t)D * 2;
     const uint32_t dst_E = sub * 128 + (((lane & 7) ^ ((sub & 1) << 2)) << 4), dst_A = Unit::OP + lane * 16;
-    int ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
+    int ids = 0, turn = 0;                                       // the worker's warps copy a unit each in turn
+    if (jj == 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
     uint32_t fill = ring;                                        // stage that the producer fills next
     auto produce = [&]() {
         if (left > 0) {
             const char* op = pl.op + (size_t)(pk >> 4) * Unit::OP_BYTES + lane * 16;
             const int now = ids;
+            const bool mine = turn == jj;
+            turn = turn + 1 == steps ? 0 : turn + 1;
             pk += 16;
             if (--left == 0) {
                 left = next_list(px);
                 if (left > 0) { pl = get_list(a, px); pk = 0; }
             }
-            if (left > 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
-            if (steps == 1) {
+            if (turn == jj && left > 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
+            if (mine) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, now, i * 4 + sub);
@@ -558,15 +558,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
                 }
 #pragma unroll
                 for (int i = 0; i < KS; ++i) cp_async16(fill + dst_A + i * 512, op + i * 512);
-            } else {                                             // the worker's warps share the copies
-                for (int i = jj; i < 8 + KS; i += steps) {
-                    if (i < 8) {
-                        const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, now, (i & 3) * 4 + sub);
-                        cp_async16(fill + dst_E + i * 512, (i < 4 ? Ek : Ev) + (uint64_t)v * D2);
-                    } else {
-                        cp_async16(fill + dst_A + (i - 8) * 512, op + (i - 8) * 512);
-                    }
-                }
             }
         }
         cp_commit();
@@ -584,14 +575,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     const uint32_t lane_lo = g * 128 + ((t ^ ((g & 1) << 2)) << 4), lane_hi = lane_lo ^ 64u;
     for (;;) {
         if (fresh) {
-            own = x >= a.n_pre;
+            own = x >= n_pre;
             single = ROWS == 1 || own;
             if (single) {
-                const int64_t r = own ? x - a.n_pre : x;
+                const int64_t r = own ? x - n_pre : x;
                 one.start(a, r, own, j, h, lane);
                 bits = own ? nullptr : br.touched + (size_t)r * ((br.Kcap + 31) / 32);
             } else if constexpr (ROWS > 1) {
-                const int b = (int)(x / a.blocks), s0 = (int)(x - (int64_t)b * a.blocks) * ROWS;
+                const int b = x / a.blocks, s0 = (x - b * a.blocks) * ROWS;
                 rows = min(ROWS, (int)br.S - s0);
                 many.start(a, (int64_t)b * br.S + s0, rows, j, h, lane);
             }
@@ -619,12 +610,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         if (at == ring_end) at = ring;
         k0 += 16;
         if (--c_left == 0) {                                     // end of the list or of the stretch
-            if (single) one.leave(a, own ? a.own_piece0 + (x - a.n_pre) + me : x + me, j, h, lane);
-            else if constexpr (ROWS > 1) many.leave(a, x + me, rows, j, h, lane);
+            if (single) one.leave(a, own ? a.own_piece0 + (x - n_pre) + me : (int64_t)x + me, j, h, lane);
+            else if constexpr (ROWS > 1) many.leave(a, (int64_t)x + me, rows, j, h, lane);
             c_left = next_list(x);
             if (c_left == 0) break;
             k0 = 0;
-            count = x < a.n_pre ? min(br.n_active[x / a.blocks], (int)br.Kcap) : br.own_n[x - a.n_pre];
+            count = x < n_pre ? min(br.n_active[x / a.blocks], (int)br.Kcap) : br.own_n[x - n_pre];
             fresh = true;
         }
     }

@@ -147,25 +147,25 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
 // y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sum of
 // the lists' units that the attention deals its work by.
 __device__ void running_sum(const mbema_branches& br) {
-    __shared__ long long s_warp[8];
+    __shared__ int s_warp[8];
     const int tid = threadIdx.x, lane = tid & 31;
     const int blocks = br.S == 1 ? 1 : (int)((br.S + BR_BLOCK - 1) / BR_BLOCK);
-    const int64_t n_pre = br.B * blocks, lists = n_pre + br.B * br.S;
-    long long base = 0;
-    for (int64_t x0 = 0; x0 < lists; x0 += 256) {
-        const int64_t x = x0 + tid;
-        long long c = 0;
-        if (x < n_pre) c = (long long)((min(br.n_active[x / blocks], (int)br.Kcap) + 15) / 16) * (br.S == 1 ? BR_COST_ONE : BR_COST_BLOCK);
-        else if (x < lists) c = (long long)((br.own_n[x - n_pre] + 15) / 16) * BR_COST_OWN;
-        long long sum = c;
+    const int n_pre = (int)br.B * blocks, lists = n_pre + (int)(br.B * br.S);
+    int base = 0;
+    for (int x0 = 0; x0 < lists; x0 += 256) {
+        const int x = x0 + tid;
+        int c = 0;
+        if (x < n_pre) c = (min(br.n_active[x / blocks], (int)br.Kcap) + 15) / 16 * (br.S == 1 ? BR_COST_ONE : BR_COST_BLOCK);
+        else if (x < lists) c = (br.own_n[x - n_pre] + 15) / 16 * BR_COST_OWN;
+        int sum = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += y;
         }
         if (lane == 31) s_warp[tid >> 5] = sum;
         __syncthreads();
-        long long all = 0;
+        int all = 0;
         for (int w = 0; w < 8; ++w) {
             if (w < (tid >> 5)) sum += s_warp[w];
             all += s_warp[w];
@@ -282,6 +282,9 @@ static int check_branches(const mbema_branches* br) {
     if (br->pre_op || br->own_op || br->work) {              // all three or none
         if (!branch_tc_supported(br->N) || br->S >= 65535 || br->B >= 65535) return MBEMA_ERR_UNSUPPORTED;
         if (!br->pre_op || !br->own_op || !br->work) return MBEMA_ERR_NULL;
+        const int64_t blocks = (br->S + BR_BLOCK - 1) / BR_BLOCK;                   // the running sum stays below 2^30
+        if (br->B * blocks * (br->Kcap / 16 + 1) * BR_COST_BLOCK + br->B * br->S * (br->cap / 16 + 1) * BR_COST_OWN >= 1ll << 30)
+            return MBEMA_ERR_UNSUPPORTED;
     }
     return MBEMA_OK;
 }

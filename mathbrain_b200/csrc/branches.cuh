@@ -52,20 +52,18 @@ struct BranchArgs {
 };
 
 // The workers that a running sum of `total` occupies, each with two units or more, and where their stretches begin.
-__device__ __forceinline__ long long branch_workers(long long total, long long most) {
-    return max(1ll, min(most, total / (2 * BR_COST_BLOCK)));
-}
-__device__ __forceinline__ long long branch_cut(long long total, long long workers, long long w) { return total * w / workers; }
+__device__ __forceinline__ int branch_workers(int total, int most) { return max(1, min(most, total / (2 * BR_COST_BLOCK))); }
+__device__ __forceinline__ int branch_cut(int total, int workers, int w) { return (int)((long long)total * w / workers); }
 // the worker whose stretch holds cost c < total
-__device__ __forceinline__ long long branch_worker_of(long long total, long long workers, long long c) {
-    return ((c + 1) * workers - 1) / total;
+__device__ __forceinline__ int branch_worker_of(int total, int workers, int c) {
+    return (int)((((long long)c + 1) * workers - 1) / total);
 }
-
-__host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
 
 // Operands of a list: fp16 fragments of the gate product, 16 slots after 16 slots.  Slot k, channel c = 32 i + 8 t + 4 u + 2 p + e is half e
 // of word (row / 8) + 2 p (row = k % 16) of lane 4 (row % 8) + t in fragment 2 i + u of its sixteen (512 bytes each).
 __host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + 15) / 16) * N * 32; }
+
+__host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
 
 // Row j of branch r cannot see slot k of the prefix: the branch has touched it, or does so with a staged token before j.
 __device__ __forceinline__ bool br_hides_prefix(const mbema_branches& br, int64_t r, int j, int k) {
