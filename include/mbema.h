@@ -390,7 +390,7 @@ typedef struct mbema_branches {
 int mbema_branches_init(const mbema_branches* br, int64_t t_now, const int32_t* t_now_dev, void* stream);
 int mbema_branches_extend(const mbema_branches* br, const int64_t* tok, int64_t n, int64_t n_pending, float* C_q, void* stream);
 int mbema_branches_keep(const mbema_branches* br, const int64_t* counts, int64_t n_pending, void* stream);
-size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode);
+size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode);
 int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
                           const float* W_pe, void* O, int64_t n, int64_t H, int64_t hd, int64_t V_total, int flags, int mode,
                           void* workspace, size_t workspace_bytes, void* stream);

@@ -65,7 +65,7 @@ SIGNATURES = {
     "mbema_branches_init": (_i32, [_vp, _i64, _vp, _vp]),
     "mbema_branches_extend": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "mbema_branches_keep": (_i32, [_vp, _vp, _i64, _vp]),
-    "mbema_branches_attend_workspace_bytes": (_sz, [_i64] * 6 + [_i32]),
+    "mbema_branches_attend_workspace_bytes": (_sz, [_i64] * 7 + [_i32]),
     "mbema_branches_attend": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
     "mbema_branches_adopt": (_i32, [_vp, _vp, _i64, _vp]),
     "mbema_verify_drafts": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),

@@ -20,9 +20,9 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _dt, _ptr, _require_cuda, _stream, get_options
+from .ops import _OPTIONS, _current_device, _dt, _ptr, _raw_stream, _require_cuda
 
-_BY_REF = ctypes.byref
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 class Branches:
@@ -63,105 +63,135 @@ class Branches:
                               work=torch.empty(B * ((S + 15) // 16 + S) + 1, **i32))
         self._c = _lib.BranchesStruct(**{k: _ptr(t) for k, t in self._hold.items()}, B=B, S=S, V=V, N=N, Kcap=Kcap, cap=cap,
                                       max_new=max_new)
+        self._ref = ctypes.byref(self._c)
         self._lib = _lib.load()
+        self._device, self._dev = dev, prefix.state.get_device()
+        self._plans = {}
         with torch.cuda.device(dev):
-            rc = self._lib.mbema_branches_init(_BY_REF(self._c), int(t_now), _ptr(prefix.t_dev), _stream())
+            rc = self._lib.mbema_branches_init(self._ref, int(t_now), _ptr(prefix.t_dev), _raw_stream(self._dev))
         _lib.check(rc, "mbema_branches_init")
 
-    def _alive(self, *operands):
+    def _alive(self):
         if self.prefix is None:
             raise _lib.MbemaError("branches: adopted already")
         if self.prefix._epoch != self._epoch:
             raise _lib.MbemaError("branches: the state they were forked from has been updated since")
-        dev = self._hold["state"].device
+
+    def _refuse(self, *operands):
         for t in operands:
-            if t.device != dev:
-                raise _lib.MbemaError("branches: operand on %s, state on %s" % (t.device, dev))
+            if t.get_device() != self._dev:
+                raise _lib.MbemaError("branches: operand on %s, state on %s" % (t.device, self._hold["state"].device))
 
     def _on_device(self, fn, *args):
-        dev = self._hold["state"].get_device()
-        if dev == torch.cuda.current_device():
+        if self._dev == _current_device():
             return fn(*args)
-        with torch.cuda.device(dev):
+        with torch.cuda.device(self._dev):
             return fn(*args)
 
     def extend(self, tok):
         """Stage n <= max_new new tokens of every branch (int64 [B, S, n]; -1: this branch has none at this step) and return
         C_q [B, S, n, N] float32, the state of each token just before its own step (0 if never seen).  Tokens staged by the
         call before are kept unless `keep` has decided on them."""
-        self._alive(tok)
-        if tok.dim() != 3 or tok.shape[:2] != (self.B, self.S) or not 1 <= tok.shape[2] <= self.max_new:
-            raise _lib.MbemaError("extend: tokens %s, expected [%d, %d, 1 to %d]" % (tuple(tok.shape), self.B, self.S, self.max_new))
+        self._alive()
+        if tok.get_device() != self._dev:
+            self._refuse(tok)
+        shape = tok.shape
+        if len(shape) != 3 or shape[0] != self.B or shape[1] != self.S or not 1 <= shape[2] <= self.max_new:
+            raise _lib.MbemaError("extend: tokens %s, expected [%d, %d, 1 to %d]" % (tuple(shape), self.B, self.S, self.max_new))
         if tok.dtype != torch.int64:
             raise _lib.MbemaError("extend: tokens of %s, expected int64" % tok.dtype)
         return self._on_device(self._extend, tok.contiguous())
 
     def _extend(self, tok):
         n = tok.shape[2]
-        C_q = torch.empty(self.B, self.S, n, self.N, dtype=torch.float32, device=tok.device)
-        rc = self._lib.mbema_branches_extend(_BY_REF(self._c), _ptr(tok), n, self._staged, _ptr(C_q), _stream())
-        _lib.check(rc, "mbema_branches_extend")
+        C_q = torch.empty((self.B, self.S, n, self.N), dtype=torch.float32, device=self._device)
+        rc = self._lib.mbema_branches_extend(self._ref, tok.data_ptr(), n, self._staged, C_q.data_ptr(), _raw_stream(self._dev))
+        if rc:
+            _lib.check(rc, "mbema_branches_extend")
         self._staged = n
         return C_q
 
     def keep(self, counts):
         """Keep the first counts[b] of the staged tokens in every branch of sequence b and drop the others (integers [B] on
         the GPU; clamped to 0..n).  The branches then have no staged tokens until the next `extend`."""
-        self._alive(counts)
-        if counts.shape != (self.B,) or counts.is_floating_point() or counts.dtype == torch.bool:
+        self._alive()
+        if counts.get_device() != self._dev:
+            self._refuse(counts)
+        if counts.dim() != 1 or counts.shape[0] != self.B or counts.dtype not in _INTEGERS:
             raise _lib.MbemaError("keep: counts %s of %s, expected [%d] integers" % (tuple(counts.shape), counts.dtype, self.B))
         return self._on_device(self._keep, counts.long().contiguous())
 
     def _keep(self, counts):
-        rc = self._lib.mbema_branches_keep(_BY_REF(self._c), _ptr(counts), self._staged, _stream())
-        _lib.check(rc, "mbema_branches_keep")
+        rc = self._lib.mbema_branches_keep(self._ref, counts.data_ptr(), self._staged, _raw_stream(self._dev))
+        if rc:
+            _lib.check(rc, "mbema_branches_keep")
         self._staged = 0
 
     def attend(self, q, E_k, E_v, W_pe, V_total=None, use_silu=True, listed_only=False, mode=None):
         """O [B, S, n, H, 64] of q's dtype for the n staged rows of every branch.  q [B, S, n, H, 64] float32 or bfloat16;
         E_k, E_v [V, H*64] projected slot embeddings; W_pe [N, H*64].  Softmax over all V_total slots (the vocabulary by
         default), those that a row does not see with score 0 and value 0; listed_only: over the seen ones alone (a row that
-        has seen none gets 0)."""
-        self._alive(q, E_k, E_v, W_pe)
+        has seen none gets 0).  mode: "fp32", "tc_bf16" or "auto" (the package option `mode` by default): the tensor cores
+        take bfloat16 q and tables with 64 or 128 channels, "auto" runs anything else in fp32 arithmetic."""
+        self._alive()
+        dev = self._dev
+        if q.get_device() != dev or E_k.get_device() != dev or E_v.get_device() != dev or W_pe.get_device() != dev:
+            self._refuse(q, E_k, E_v, W_pe)
+        if mode is None:
+            mode = _OPTIONS["mode"]
+        # checked and sized once for operands of the same shapes, types and options
+        key = (q.shape, q.dtype, E_k.shape, E_k.dtype, E_v.shape, W_pe.shape, self._staged, V_total, use_silu, listed_only, mode)
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plan(q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode)
+            if len(self._plans) >= 64:
+                self._plans.clear()
+            self._plans[key] = plan
+        return self._on_device(self._attend, q, E_k, E_v, W_pe, plan)
+
+    def _plan(self, q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode):
+        """(arguments of the C call behind O, workspace bytes)."""
         n = self._staged
         if n == 0:
             raise _lib.MbemaError("attend: no staged tokens (call extend first)")
         if q.dim() != 5 or q.shape[:3] != (self.B, self.S, n) or q.shape[4] != 64 or q.shape[3] < 1:
             raise _lib.MbemaError("attend: q %s, expected [%d, %d, %d, H, 64]" % (tuple(q.shape), self.B, self.S, n))
-        D = q.shape[3] * 64
+        H = q.shape[3]
+        D = H * 64
         if E_k.shape != (self.V, D) or E_v.shape != (self.V, D) or W_pe.shape != (self.N, D):
             raise _lib.MbemaError("attend: E_k %s, E_v %s, W_pe %s, expected [%d, %d] twice and [%d, %d]"
                                   % (tuple(E_k.shape), tuple(E_v.shape), tuple(W_pe.shape), self.V, D, self.N, D))
-        return self._on_device(self._attend, q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode)
-
-    def _attend(self, q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode):
-        q, E_k, W = q.contiguous(), E_k.contiguous(), W_pe.float().contiguous()
-        E_v = E_v.to(E_k.dtype).contiguous()
-        if mode is None:
-            mode = get_options()["mode"]
+        q_dt, e_dt = _dt(q), _dt(E_k)
         if mode not in ("fp32", "tc_bf16", "auto"):
             raise ValueError("mode must be 'fp32', 'tc_bf16' or 'auto'")
-        fits = self._tensor_cores and q.dtype == torch.bfloat16 and E_k.dtype == torch.bfloat16
+        fits = self._tensor_cores and q_dt == _lib.BF16 and e_dt == _lib.BF16
         if mode == "tc_bf16" and not fits:
             raise _lib.MbemaError("attend: mode 'tc_bf16' needs bfloat16 q and tables and 64 or 128 channels (%s, %s, %d)"
                                   % (q.dtype, E_k.dtype, self.N))
         code = _lib.MODE_TC_BF16 if fits and mode != "fp32" else _lib.MODE_FP32
-        n, H = q.shape[2], q.shape[3]
-        O = torch.empty_like(q)
-        need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, n, H, self.prefix.cap, self.capacity, code)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         flags = (_lib.FLAG_SILU if use_silu else 0) | (_lib.FLAG_LISTED_ONLY if listed_only else 0)
-        rc = self._lib.mbema_branches_attend(_BY_REF(self._c), _ptr(q), _dt(q), _ptr(E_k), _ptr(E_v), _dt(E_k), _ptr(W), _ptr(O), n, H,
-                                             64, int(self.V if V_total is None else V_total), flags, code, _ptr(ws), need, _stream())
-        _lib.check(rc, "mbema_branches_attend")
+        need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, self.N, n, H, self.prefix.cap, self.capacity, code)
+        return q_dt, e_dt, n, H, int(self.V if V_total is None else V_total), flags, code, need
+
+    def _attend(self, q, E_k, E_v, W_pe, plan):
+        q_dt, e_dt, n, H, V_total, flags, code, need = plan
+        q, E_k, W = q.contiguous(), E_k.contiguous(), W_pe.float().contiguous()
+        E_v = E_v.to(E_k.dtype).contiguous()
+        O = torch.empty_like(q)
+        ws = torch.empty(need, dtype=torch.uint8, device=self._device)
+        rc = self._lib.mbema_branches_attend(self._ref, q.data_ptr(), q_dt, E_k.data_ptr(), E_v.data_ptr(), e_dt, W.data_ptr(), O.data_ptr(),
+                                             n, H, 64, V_total, flags, code, ws.data_ptr(), need, _raw_stream(self._dev))
+        if rc:
+            _lib.check(rc, "mbema_branches_attend")
         return O
 
     def adopt(self, branch, t_next):
         """Branch branch[b] (integers [B] on the GPU) of every sequence becomes the state's own: its tokens join the resident
         state and the active list.  Staged tokens are kept unless `keep` has decided on them.  The next step of every sequence
         is t_next afterwards, whatever the branches' lengths (not before the longest one's end).  Ends these branches."""
-        self._alive(branch)
-        if branch.shape != (self.B,) or branch.is_floating_point() or branch.dtype == torch.bool:
+        self._alive()
+        self._refuse(branch)
+        if branch.shape != (self.B,) or branch.dtype not in _INTEGERS:
             raise _lib.MbemaError("adopt: branch %s of %s, expected [%d] integers" % (tuple(branch.shape), branch.dtype, self.B))
         return self._on_device(self._adopt, branch.long().contiguous(), int(t_next))
 
@@ -169,7 +199,7 @@ class Branches:
         st = self.prefix
         if self._staged:
             self._keep(torch.full((self.B,), self._staged, dtype=torch.int64, device=branch.device))
-        _lib.check(self._lib.mbema_branches_adopt(_BY_REF(self._c), _ptr(branch), t_next, _stream()), "mbema_branches_adopt")
+        _lib.check(self._lib.mbema_branches_adopt(self._ref, _ptr(branch), t_next, _raw_stream(self._dev)), "mbema_branches_adopt")
         st._epoch += 1
         st.overflow.copy_(torch.where(self._hold["overflow"] == 1, self._hold["overflow"], st.overflow))
         if st.t_dev is not None:

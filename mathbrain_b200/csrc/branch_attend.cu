@@ -362,7 +362,8 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
     const int64_t jobs = br.B * ((br.S + BA_ROWS - 1) / BA_ROWS) * a.plan.SP + br.B * br.S * a.plan.SO;
     if (jobs > 0x7fffffff || a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
     const size_t smem = ba_smem((int)br.N);
-    MBEMA_CUDA_TRY(cudaFuncSetAttribute(k_branch_attend, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<unsigned long long> done{0};
+    MBEMA_CUDA_TRY(allow_smem(k_branch_attend, ba_smem(128), done));
     k_branch_attend<<<dim3((unsigned)jobs, (unsigned)a.H, (unsigned)a.n), BA_THREADS, smem, st>>>(a);
     return check_launch();
 }
@@ -384,13 +385,13 @@ static bool plan_sizes_ok(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kc
 }
 
 // number of partials of a call
-static int64_t partials(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode, BranchArgs* a) {
+static int64_t partials(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode, BranchArgs* a) {
     if (mode != MBEMA_MODE_TC_BF16) {
         const BranchPlan p = branch_plan(B, S, n, H, Kcap, cap);
         if (a) a->plan = p;
         return B * S * n * H * (p.SP + p.SO);
     }
-    const BranchShape p = branch_shape(B, S, n, H);
+    const BranchShape p = branch_shape(B, S, N, n, H);
     const int64_t workers = (int64_t)p.ctas * p.IG, n_pre = B * p.blocks, own0 = (n_pre + workers) * p.rows;
     if (a) {
         a->n_pre = n_pre;
@@ -403,9 +404,9 @@ static int64_t partials(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap
     return (own0 + B * S + workers) * n * H;
 }
 
-extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
-    if (!plan_sizes_ok(B, S, n, H, Kcap, cap)) return 0;
-    return align_up((size_t)partials(B, S, n, H, Kcap, cap, mode, nullptr) * (2 + BR_HD) * 4, 256) + 256;
+extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
+    if (!plan_sizes_ok(B, S, n, H, Kcap, cap) || N < 1) return 0;
+    return align_up((size_t)partials(B, S, N, n, H, Kcap, cap, mode, nullptr) * (2 + BR_HD) * 4, 256) + 256;
 }
 
 extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
@@ -419,7 +420,7 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     if (!q || !E_k || !E_v || !W_pe || !O || !workspace || !br->state || !br->active || !br->own_state || !br->st_state) return MBEMA_ERR_NULL;
     if ((q_dtype != MBEMA_F32 && q_dtype != MBEMA_BF16) || (e_dtype != MBEMA_F32 && e_dtype != MBEMA_BF16)) return MBEMA_ERR_DTYPE;
     if (((uintptr_t)q | (uintptr_t)E_k | (uintptr_t)E_v | (uintptr_t)W_pe | (uintptr_t)O | (uintptr_t)workspace) & 15) return MBEMA_ERR_ALIGN;
-    if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
+    if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, br->N, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
     if (mode == MBEMA_MODE_TC_BF16 && (!br->pre_op || !br->own_op || !br->work)) return MBEMA_ERR_NULL;
     BranchArgs a{};
     a.br = *br;
@@ -428,10 +429,10 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     a.v_total = (float)V_total;
     a.silu = (flags & MBEMA_FLAG_SILU) ? 1 : 0;
     a.listed_only = (flags & MBEMA_FLAG_LISTED_ONLY) ? 1 : 0;
-    const int64_t parts = partials(br->B, br->S, n, H, br->Kcap, br->cap, mode, &a);
+    const int64_t parts = partials(br->B, br->S, br->N, n, H, br->Kcap, br->cap, mode, &a);
     a.po = reinterpret_cast<float*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.po + (size_t)parts * BR_HD);
     const bool tc = mode == MBEMA_MODE_TC_BF16;
-    int rc = tc ? launch_branch_attend_tc(a, branch_shape(br->B, br->S, n, H), (cudaStream_t)stream) : launch_branch_attend_fp32(a, (cudaStream_t)stream);
+    int rc = tc ? launch_branch_attend_tc(a, branch_shape(br->B, br->S, br->N, n, H), (cudaStream_t)stream) : launch_branch_attend_fp32(a, (cudaStream_t)stream);
     return rc != MBEMA_OK ? rc : launch_branch_merge(a, tc, (cudaStream_t)stream);
 }

@@ -89,51 +89,59 @@ __device__ __forceinline__ void w_fragment(uint32_t (&w)[2], const float* W_sh, 
     w[1] = pack_h2(p[2 * BT_LDW] * pw[2], p[3 * BT_LDW] * pw[3]);
 }
 
-// The gate product's W: in registers for 64 channels (64 of them a thread), in shared memory for 128.
+// The gate product's W, as fragments in shared memory: [KS][4 pairs of column tiles][32 lanes] of 16 bytes.
 template <int KS>
-struct WSource {
-    uint32_t w[KS == 4 ? 4 : 1][8][2];
-    const uint2* sh;
-    __device__ __forceinline__ void build(const float* W_sh, const float* l2r, uint2* dst, int j, float scale, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-        sh = dst + lane;
+__device__ __forceinline__ void build_W(uint32_t dst, const float* W_sh, const float* l2r, int j, float scale, int lane, int part, int parts) {
+    const int g = lane >> 2, t = lane & 3;
+    for (int i = part; i < KS * 4; i += parts) {
+        const int ks = i >> 2, c = 32 * (ks >> 1) + 8 * t + 4 * (ks & 1);
+        float pw[4];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int c = 32 * (ks >> 1) + 8 * t + 4 * (ks & 1);
-            float pw[4];
+        for (int e = 0; e < 4; ++e) pw[e] = exp2f((float)j * l2r[c + e]) * scale;
+        uint32_t x[2], y[2];
+        w_fragment<KS>(x, W_sh, pw, ks, 2 * (i & 3), g, t);
+        w_fragment<KS>(y, W_sh, pw, ks, 2 * (i & 3) + 1, g, t);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * 512 + lane * 16), "r"(x[0]), "r"(x[1]), "r"(y[0]), "r"(y[1]) : "memory");
+    }
+}
+// A warp's copy of them in registers (64 a thread for 64 channels): twelve rows of sixteen bytes fewer to read a unit, for eight warps
+// an SM instead of sixteen.
+template <int KS, int I = 0>
+__device__ __forceinline__ void read_W(uint4 (&w)[KS * 4], uint32_t at) {
+    if constexpr (I < KS * 4) {
+        w[I] = lds128<512 * I>(at);
+        read_W<KS, I + 1>(w, at);
+    }
+}
+template <int KS>
+__device__ __forceinline__ void gate(float (&acc)[8][4], const uint32_t (&A)[KS][4], const uint4 (&w)[KS * 4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pw[i] = exp2f((float)j * l2r[c + i]) * scale;
-#pragma unroll
-            for (int nt = 0; nt < 8; ++nt) {
-                if constexpr (KS == 4) {
-                    w_fragment<KS>(w[ks][nt], W_sh, pw, ks, nt, g, t);
-                } else {
-                    uint32_t x[2];
-                    w_fragment<KS>(x, W_sh, pw, ks, nt, g, t);
-                    dst[(ks * 8 + nt) * 32 + lane] = make_uint2(x[0], x[1]);
-                }
-            }
+    for (int i = 0; i < KS * 4; ++i) {
+        const int ks = i / 4, nt = 2 * (i % 4);
+        if (ks == 0) {
+            mma_f16_first(acc[nt], A[ks], w[i].x, w[i].y);
+            mma_f16_first(acc[nt + 1], A[ks], w[i].z, w[i].w);
+        } else {
+            mma_f16(acc[nt], A[ks], w[i].x, w[i].y);
+            mma_f16(acc[nt + 1], A[ks], w[i].z, w[i].w);
         }
     }
-    __device__ __forceinline__ void gate(float (&acc)[8][4], const uint32_t (&A)[KS][4]) const {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int nt = 0; nt < 8; ++nt) {
-                uint32_t b0, b1;
-                if constexpr (KS == 4) {
-                    b0 = w[ks][nt][0];
-                    b1 = w[ks][nt][1];
-                } else {
-                    const uint2 x = sh[(ks * 8 + nt) * 32];
-                    b0 = x.x;
-                    b1 = x.y;
-                }
-                if (ks == 0) mma_f16_first(acc[nt], A[ks], b0, b1);
-                else mma_f16(acc[nt], A[ks], b0, b1);
-            }
+}
+template <int KS, int I = 0>
+__device__ __forceinline__ void gate(float (&acc)[8][4], const uint32_t (&A)[KS][4], uint32_t w) {
+    if constexpr (I < KS * 4) {
+        constexpr int ks = I / 4, nt = 2 * (I % 4);
+        const uint4 b = lds128<512 * I>(w);
+        if (ks == 0) {
+            mma_f16_first(acc[nt], A[ks], b.x, b.y);
+            mma_f16_first(acc[nt + 1], A[ks], b.z, b.w);
+        } else {
+            mma_f16(acc[nt], A[ks], b.x, b.y);
+            mma_f16(acc[nt + 1], A[ks], b.z, b.w);
+        }
+        gate<KS, I + 1>(acc, A, w);
     }
-};
+}
 
 // A unit in the ring: 16 rows of E_k, of E_v (128 bytes each; in odd rows the 16-byte pieces 0-3 and 4-7 change places, so that the
 // eight lanes that are served together, two rows and four pieces each, touch all banks), then the operands as the lanes' fragments.
@@ -166,16 +174,6 @@ __device__ __forceinline__ void load_q(uint32_t (&E)[8], const char* row) {
         const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i);
         E[4 * i] = x.x; E[4 * i + 1] = x.y; E[4 * i + 2] = x.z; E[4 * i + 3] = x.w;
     }
-}
-
-// products of the halves, exact in fp32 (mixed-precision FMA: no unpacking)
-__device__ __forceinline__ void mul_bf16x2(float& x, float& y, uint32_t a, uint32_t b) {
-    asm("{\n\t.reg .b16 al, ah, bl, bh;\n\t"
-        "mov.b32 {al, ah}, %2;\n\t"
-        "mov.b32 {bl, bh}, %3;\n\t"
-        "fma.rn.f32.bf16 %0, al, bl, 0f00000000;\n\t"
-        "fma.rn.f32.bf16 %1, ah, bh, 0f00000000;\n\t}"
-        : "=f"(x), "=f"(y) : "r"(a), "r"(b));
 }
 
 __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
@@ -264,11 +262,13 @@ __device__ __forceinline__ int quad_columns(int lane) {
 // maximum and sums, joined at the end of the piece.
 // ---------------------------------------------------------------------------------------------------------------------------
 struct OneRow {
-    float m, l, o[16];
-    uint32_t q[8];
+    float m, l, o[16], q[16];
     int staged;
     __device__ __forceinline__ void start(const BranchArgs& a, int64_t r, bool own, int j, int h, int lane) {
-        load_q(q, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
+        uint32_t x[8];
+        load_q(x, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { q[2 * i] = bf_lo(x[i]) * BR_SCORE_LOG2; q[2 * i + 1] = bf_hi(x[i]) * BR_SCORE_LOG2; }
         staged = -1;
         if (lane < j) staged = (own ? a.br.st_own : a.br.st_pos)[br_index(a.br, r, lane)];
         m = -INFINITY;
@@ -282,13 +282,10 @@ struct OneRow {
         float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            float x, y;
-            mul_bf16x2(x, y, e0[nt], q[nt]);
-            s0 = fmaf(x, acc[nt][0], s0);
-            s1 = fmaf(y, acc[nt][1], s1);
-            mul_bf16x2(x, y, e1[nt], q[nt]);
-            s2 = fmaf(x, acc[nt][2], s2);
-            s3 = fmaf(y, acc[nt][3], s3);
+            s0 = fmaf(bf_lo(e0[nt]) * q[2 * nt], acc[nt][0], s0);
+            s1 = fmaf(bf_hi(e0[nt]) * q[2 * nt + 1], acc[nt][1], s1);
+            s2 = fmaf(bf_lo(e1[nt]) * q[2 * nt], acc[nt][2], s2);
+            s3 = fmaf(bf_hi(e1[nt]) * q[2 * nt + 1], acc[nt][3], s3);
         }
         load_E<2048>(e0, e1, at_lo, at_hi);
         s0 += s1;
@@ -297,7 +294,7 @@ struct OneRow {
         s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
         s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
         s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
-        const float x0 = (hide >> g) & 1u ? -INFINITY : s0 * BR_SCORE_LOG2, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2 * BR_SCORE_LOG2;
+        const float x0 = (hide >> g) & 1u ? -INFINITY : s0, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2;
         const float m_new = fmaxf(m, fmaxf(x0, x1));
         const float ref = m_new == -INFINITY ? 0.f : m_new;
         const float p0 = ex2(x0 - ref), p1 = ex2(x1 - ref);
@@ -477,9 +474,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     constexpr int N = 16 * KS;
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.H * BR_HD;
-    // KS = 8: the fragments of W behind the ring, whose space the staged slice of W takes first
+    // the steps' fragments of W behind the ring, whose space the staged slice of W takes first
     float* W_sh = reinterpret_cast<float*>(smem);
-    uint2* Wf = reinterpret_cast<uint2*>(smem + a.ring_bytes);
     for (int i = tid; i < N * 16; i += WARPS * 32) {
         const float4 x = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
         float2* dst = reinterpret_cast<float2*>(W_sh + w_row(i >> 4) + (i & 15) * 4);
@@ -495,10 +491,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     const int steps = min(JW, a.n - (int)blockIdx.z * JW);       // of this CTA
     const int me = (int)blockIdx.x * IG + ig;
     __syncthreads();
-    WSource<KS> W;                 // KS = 8: the workers write the same fragments of a step, each reads what it has written
-    if (ig < IG && jj < steps) W.build(W_sh, s_l2r, Wf + (size_t)jj * KS * 8 * 32, j, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane);
+    const uint32_t w_all = (uint32_t)__cvta_generic_to_shared(smem) + a.ring_bytes;
+    for (int i = 0; i < steps; ++i)
+        build_W<KS>(w_all + i * KS * 2048, W_sh, s_l2r, blockIdx.z * JW + i, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane, warp, WARPS);
     __syncthreads();
     if (ig >= IG || jj >= steps || me >= workers) return;
+    const uint32_t w_at = w_all + jj * KS * 2048 + lane * 16;
+    constexpr bool W_REGS = KS == 4 && WARPS == 8;
+    uint4 w[KS * 4];
+    if constexpr (W_REGS) read_W<KS>(w, w_at);
     const int c_end = branch_cut(total, workers, me + 1);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + ig * STAGES * Unit::BYTES;
     const uint32_t ring_end = ring + STAGES * Unit::BYTES;
@@ -601,7 +602,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         {
             uint32_t A[KS][4];
             load_A<KS>(A, at + lane * 16);
-            W.gate(acc, A);
+            if constexpr (W_REGS) gate<KS>(acc, A, w);
+            else gate<KS>(acc, A, w_at);
         }
         apply_gate(acc, a.silu);
         if (single) one.unit(acc, at + lane_lo, at + lane_hi, hidden16(touched0, k0, one.staged, j > 0, count), g);
@@ -624,27 +626,27 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
 
 bool branch_tc_supported(int64_t N) { return N == 64 || N == 128; }
 
-// How the warps of a CTA are dealt: JW steps to a worker (they share its E and operand rows), IG workers.  Between three (all, of
-// fewer) and six steps, whichever keeps the most warps busy over all blocks of steps; more steps where that is equal.
+// How the warps of a CTA are dealt: JW steps to a worker (they share its E and operand rows), IG workers, whichever keeps the most
+// warps busy over all blocks of steps; a worker of fewer steps fetches its rows more often.
 static void steps_and_workers(int n, int warps, int& JW, int& IG) {
     double best = -1.0;
-    for (int jw = std::min(n, 3); jw <= std::min(n, 6); ++jw) {
+    for (int jw = 1; jw <= std::min(n, 8); ++jw) {
         const int zb = (n + jw - 1) / jw;
-        const double busy = (double)(warps / jw) * n / zb;
+        const double busy = (double)(warps / jw) * n / zb / (1.0 + 0.25 / jw);
         if (busy >= best) { best = busy; JW = jw; }
     }
     IG = warps / JW;
 }
 
-// Registers: W (64), accumulators (32) and one row's o and q let twelve warps run with 168 each, sixteen rows' o and q eight with
-// 255.  One step, one branch: eight, the ring of twelve workers is too large.
-static int tc_warps(int64_t S, int64_t n) { return S == 1 && n > 1 ? 12 : 8; }
+// Single rows: sixteen warps with W in shared memory (64 sequences with 6 rows 486 us; twelve with W in registers 566, eight 645), for
+// 128 channels the twelve whose rings fit.  Sixteen rows: eight, with W in registers (64 samples 25 us; twelve 31).
+static int tc_warps(int64_t S, int64_t N) { return S > 1 ? 8 : N == 64 ? 16 : 12; }
 
-BranchShape branch_shape(int64_t B, int64_t S, int64_t n, int64_t H) {
+BranchShape branch_shape(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H) {
     BranchShape p;
     p.rows = S == 1 ? 1 : BR_BLOCK;
     p.blocks = (int)((S + p.rows - 1) / p.rows);
-    p.warps = tc_warps(S, n);
+    p.warps = tc_warps(S, N);
     steps_and_workers((int)n, p.warps, p.JW, p.IG);
     p.zb = (int)((n + p.JW - 1) / p.JW);
     p.ctas = (int)std::max<int64_t>(1, 148 / (H * p.zb));       // one CTA an SM, dealt to the heads and blocks of steps
@@ -655,17 +657,17 @@ template <int KS, int ROWS, int WARPS, int STAGES>
 static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     const size_t w_sh = ((size_t)16 * KS * BT_LDW + 8) * 4;
     a.ring_bytes = (int)align_up(std::max(w_sh, (size_t)p.IG * STAGES * UnitLayout<KS>::BYTES), 128);
-    const size_t smem = a.ring_bytes + (KS == 8 ? (size_t)p.JW * KS * 8 * 32 * sizeof(uint2) : 0);
-    MBEMA_CUDA_TRY(cudaFuncSetAttribute(k_branch_tc<KS, ROWS, WARPS, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const size_t smem = a.ring_bytes + (size_t)p.JW * KS * 2048;
+    static std::atomic<unsigned long long> done{0};
+    MBEMA_CUDA_TRY(allow_smem(k_branch_tc<KS, ROWS, WARPS, STAGES>, 232448 - 1024, done));
     k_branch_tc<KS, ROWS, WARPS, STAGES><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st>>>(a, p.JW, p.IG);
     return check_launch();
 }
 
 int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
-    if (a.br.N == 64)
-        return p.rows > 1 ? launch_tc<4, BR_BLOCK, 8, 4>(a, p, st) : p.warps == 12 ? launch_tc<4, 1, 12, 4>(a, p, st) : launch_tc<4, 1, 8, 4>(a, p, st);
-    return p.rows > 1 ? launch_tc<8, BR_BLOCK, 8, 3>(a, p, st) : p.warps == 12 ? launch_tc<8, 1, 12, 3>(a, p, st) : launch_tc<8, 1, 8, 3>(a, p, st);
+    if (a.br.N == 64) return p.rows > 1 ? launch_tc<4, BR_BLOCK, 8, 4>(a, p, st) : launch_tc<4, 1, 16, 2>(a, p, st);
+    return p.rows > 1 ? launch_tc<8, BR_BLOCK, 8, 3>(a, p, st) : launch_tc<8, 1, 12, 2>(a, p, st);
 }
 
 }  // namespace mbema

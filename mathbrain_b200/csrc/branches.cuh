@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace mbema {
@@ -79,8 +81,21 @@ __device__ __forceinline__ bool br_hides_own(const mbema_branches& br, int64_t r
     return false;
 }
 
+// cudaFuncAttributeMaxDynamicSharedMemorySize raised to what every later call needs, once a device (the call costs the host as much
+// as a launch)
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel kernel, size_t most, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 bool branch_tc_supported(int64_t N);
-BranchShape branch_shape(int64_t B, int64_t S, int64_t n, int64_t H);
+BranchShape branch_shape(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H);
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st);
 int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st);
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st);

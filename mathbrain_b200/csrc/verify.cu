@@ -2,12 +2,13 @@
 //
 // Draft j, drawn from q_j, stands with probability min(1, p_j(x) / q_j(x)): u q < p.  Behind the drafts that stand one token is
 // drawn by inversion, from max(p - q, 0) where a draft was rejected, else from p; the whole then has the target's distribution.
-// Products of two fp32 values, differences and sums are taken in double, so that the token does not depend on how the sum over
-// the vocabulary is split (a border between tokens lies within the rounding of an fp32 sum of 50 000 terms once in a hundred draws).
+// Products of two fp32 values, differences and sums are taken in (or with the exactness of) double, so that the token does not depend on
+// how the sum over the vocabulary is split (a border between tokens lies within the rounding of an fp32 sum of 50 000 terms once in a
+// hundred draws).
 // Bound by the bytes of one row of p (and of q) per sequence, behind a chain of three dependent loads that finds the row.  A
-// cluster of eight CTAs takes a sequence, so that one sequence alone is not bound by what one SM can load: a warp sums its
-// stretch of the vocabulary, the stretches' sums are exchanged through distributed shared memory, and the warp whose stretch
-// holds the threshold walks it again.
+// cluster of CTAs takes a sequence, so that one sequence alone is not bound by what one SM can load: a warp sums its
+// stretch of the vocabulary, the stretches' sums are exchanged through distributed shared memory, and the CTA whose
+// stretch holds the threshold deals it to its warps once more, so that no warp walks more than a hundred tokens one after another.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -16,10 +17,9 @@ namespace cg = cooperative_groups;
 
 namespace mbema {
 
-static constexpr int VD_CTAS = 8;         // a cluster: the portable size
 static constexpr int VD_THREADS = 512;
 static constexpr int VD_WARPS = VD_THREADS / 32;
-static constexpr int VD_LANE = VD_CTAS * VD_WARPS / 32;   // stretches a lane holds
+static constexpr int VD_BATCH = 8;         // loads of p and of q that a lane has in flight
 
 struct VerifyArgs {
     const void* p; const void* q;
@@ -29,12 +29,21 @@ struct VerifyArgs {
     int G, V;
 };
 
-// weight of token i: one that is negative or not finite is none
-template <int DT>
-__device__ __forceinline__ double vd_weight(const void* p, const void* q, size_t po, size_t qo, int i, int onehot, bool minus_q) {
-    double w = (double)ld_as_f32<DT>(p, po + i);
-    if (minus_q) w -= q ? (double)ld_as_f32<DT>(q, qo + i) : (i == onehot ? 1.0 : 0.0);
-    return w > 0.0 && w <= 3.4028234663852886e38 ? w : 0.0;
+// weight of a token: one that is negative or not finite is none
+__device__ __forceinline__ double vd_weight(double w) { return w > 0.0 && w <= 3.4028234663852886e38 ? w : 0.0; }
+
+// s + e += weight of (p - q), as a lane's sum of a few dozen of them: the difference and every sum with its rounding error kept (Knuth's
+// two-sum; relative error about 2^-47).  In double, the conversions and the compares of a whole row took longer than its bytes.
+__device__ __forceinline__ void add_weight(float& s, float& e, float p, float q) {
+    float d = __fsub_rn(p, q);
+    const float b = __fsub_rn(d, p);
+    float r = __fsub_rn(__fsub_rn(p, __fsub_rn(d, b)), __fadd_rn(q, b));
+    const bool ok = d > 0.f && d <= 3.402823466e38f;
+    d = ok ? d : 0.f;
+    r = ok ? r : 0.f;
+    const float t = __fadd_rn(s, d), c = __fsub_rn(t, s);
+    e = __fadd_rn(e, __fadd_rn(__fadd_rn(__fsub_rn(s, __fsub_rn(t, c)), __fsub_rn(d, c)), r));
+    s = t;
 }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -43,9 +52,44 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     return v;
 }
 
-template <int DT>
-__global__ void __cluster_dims__(VD_CTAS, 1, 1) __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
+// Of 32 EACH sums, in shared memory: the first at which the running sum (from `before` on) passes the threshold; without one (a number
+// of 1 or more, or the rounding of another order of summing) the last that is not empty; -1 if all are.  `before`: the running sum there.
+template <int EACH>
+__device__ __forceinline__ int pick(const double* sums, double thr, double& before) {
+    const int lane = threadIdx.x & 31;
+    double own[EACH], lane_sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) lane_sum += own[i] = sums[lane * EACH + i];
+    double run = lane_sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+    }
+    run += before - lane_sum;
+    int hit = -1, some = -1;
+    double hit_before = 0.0, some_before = 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        if (own[i] > 0.0) {
+            if (hit < 0 && run + own[i] > thr) { hit = lane * EACH + i; hit_before = run; }
+            some = lane * EACH + i;
+            some_before = run;
+        }
+        run += own[i];
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), somes = __ballot_sync(0xffffffffu, some >= 0);
+    const int from = hits ? __ffs(hits) - 1 : 31 - __clz(somes | 1u);
+    before = __shfl_sync(0xffffffffu, hits ? hit_before : some_before, from);
+    return __shfl_sync(0xffffffffu, hits ? hit : some, from);
+}
+
+// CTAS: of a cluster, 2 to 8
+template <int DT, int VD_CTAS>
+__global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
+    constexpr int VD_LANE = VD_CTAS * VD_WARPS / 32;     // stretches a lane holds
     __shared__ double s_sum[VD_CTAS * VD_WARPS];         // sums of all stretches of the row, in vocabulary order
+    __shared__ double s_sub[32];
     __shared__ int s_acc[2];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank();
@@ -81,54 +125,42 @@ __global__ void __cluster_dims__(VD_CTAS, 1, 1) __launch_bounds__(VD_THREADS) k_
     const int stretch = (V + VD_CTAS * VD_WARPS - 1) / (VD_CTAS * VD_WARPS);
     const int w_id = rank * VD_WARPS + warp;
     const int lo = min(w_id * stretch, V), hi = min(lo + stretch, V);
-    bool minus_q = rejected;
+    // what is taken off p: q, or 1 at the draft, or (not rejected; p <= q everywhere) nothing
+    bool from_q = rejected && a.q, minus = rejected;
+    int spike = rejected && !a.q ? onehot : -1;
+    auto weight = [&](int i) {
+        const double taken = from_q ? (double)ld_as_f32<DT>(a.q, qo + i) : (i == spike ? 1.0 : 0.0);
+        return vd_weight((double)ld_as_f32<DT>(a.p, po + i) - taken);
+    };
     double total = 0.0;
     for (int pass = 0; pass < 2; ++pass) {
-        double sum = 0.0;
-#pragma unroll 8
-        for (int i = lo + lane; i < hi; i += 32) sum += vd_weight<DT>(a.p, a.q, po, qo, i, onehot, minus_q);
-        sum = warp_sum_d(sum);
+        float s = 0.f, e = 0.f;
+        for (int i0 = lo + lane; i0 < hi; i0 += 32 * VD_BATCH) {         // a batch of loads is in flight, the last one too
+            float x[VD_BATCH], y[VD_BATCH];
+#pragma unroll
+            for (int k = 0; k < VD_BATCH; ++k) {
+                const int i = i0 + 32 * k;
+                x[k] = i < hi ? ld_as_f32<DT>(a.p, po + i) : 0.f;
+                y[k] = i < hi && from_q ? ld_as_f32<DT>(a.q, qo + i) : (i == spike ? 1.f : 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < VD_BATCH; ++k) add_weight(s, e, x[k], y[k]);
+        }
+        const double sum = warp_sum_d((double)s + (double)e);
         if (lane < VD_CTAS) cluster.map_shared_rank(s_sum, lane)[w_id] = sum;
         cluster.sync();
         total = 0.0;                                     // a lane holds four stretches; the same sums in every thread
 #pragma unroll
         for (int i = 0; i < VD_LANE; ++i) total += s_sum[lane * VD_LANE + i];
         total = warp_sum_d(total);
-        if (total > 0.0 || !minus_q) break;              // the same in every CTA of the cluster
-        minus_q = false;                                 // p <= q everywhere: draw from p
+        if (total > 0.0 || !minus) break;                // the same in every CTA of the cluster
+        minus = from_q = false;                          // p <= q everywhere: draw from p
+        spike = -1;
         cluster.sync();                                  // every CTA has read the sums
     }
-    // the first stretch whose running sum passes the threshold; without one (a number of 1 or more) the last that holds a token
     const double thr = (double)a.u[r * (G + 1) + G] * total;
     double before = 0.0;
-    int mine;
-    {
-        double own[VD_LANE], lane_sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < VD_LANE; ++i) lane_sum += own[i] = s_sum[lane * VD_LANE + i];
-        double run = lane_sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += y;
-        }
-        run -= lane_sum;
-        int hit = -1, some = -1;
-        double hit_before = 0.0, some_before = 0.0;
-#pragma unroll
-        for (int i = 0; i < VD_LANE; ++i) {
-            if (own[i] > 0.0) {
-                if (hit < 0 && run + own[i] > thr) { hit = lane * VD_LANE + i; hit_before = run; }
-                some = lane * VD_LANE + i;
-                some_before = run;
-            }
-            run += own[i];
-        }
-        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), somes = __ballot_sync(0xffffffffu, some >= 0);
-        const int from = hits ? __ffs(hits) - 1 : 31 - __clz(somes | 1u);
-        mine = __shfl_sync(0xffffffffu, hits ? hit : some, from);
-        before = __shfl_sync(0xffffffffu, hits ? hit_before : some_before, from);
-    }
+    const int mine = pick<VD_LANE>(s_sum, thr, before);
     if (rank == 0) {
         for (int j = tid; j <= G; j += VD_THREADS)
             if (j != acc) a.tokens[r * (G + 1) + j] = j < acc ? a.drafted[r * G + j] : -1;
@@ -137,11 +169,24 @@ __global__ void __cluster_dims__(VD_CTAS, 1, 1) __launch_bounds__(VD_THREADS) k_
             if (mine < 0) a.tokens[r * (G + 1) + acc] = -1;
         }
     }
-    if (w_id != mine) return;
+    if (mine < 0 || mine / VD_WARPS != rank) return;
+    // the CTA whose warp summed that stretch deals it to all its warps again; the one whose share passes the threshold walks it
+    const int first = min(mine * stretch, V), behind = min(first + stretch, V);
+    const int share = (stretch + VD_WARPS - 1) / VD_WARPS;
+    const int from = min(first + warp * share, behind), to = min(from + share, behind);
+    {
+        double sum = 0.0;
+        for (int i = from + lane; i < to; i += 32) sum += weight(i);
+        sum = warp_sum_d(sum);
+        if (lane == 0) s_sub[warp] = sum;
+    }
+    if (tid < 32 && tid >= VD_WARPS) s_sub[tid] = 0.0;
+    __syncthreads();
+    if (pick<1>(s_sub, thr, before) != warp) return;
     int found = -1, tail = -1;
-    for (int i0 = lo; i0 < hi && found < 0; i0 += 32) {
+    for (int i0 = from; i0 < to && found < 0; i0 += 32) {
         const int i = i0 + lane;
-        const double w = i < hi ? vd_weight<DT>(a.p, a.q, po, qo, i, onehot, minus_q) : 0.0;
+        const double w = i < to ? weight(i) : 0.0;
         double x = w;                                    // inclusive sum over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -157,6 +202,22 @@ __global__ void __cluster_dims__(VD_CTAS, 1, 1) __launch_bounds__(VD_THREADS) k_
     if (lane == 0) a.tokens[r * (G + 1) + acc] = found >= 0 ? found : tail;
 }
 
+template <int DT, int CTAS>
+static int launch(const VerifyArgs& a, int64_t R, void* stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(R * CTAS));
+    cfg.blockDim = dim3(VD_THREADS);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MBEMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_verify<DT, CTAS>, a));
+    return check_launch();
+}
+
 }  // namespace mbema
 
 using namespace mbema;
@@ -165,13 +226,15 @@ extern "C" int mbema_verify_drafts(const void* p, int64_t p_row, int64_t p_pos, 
                                    const int64_t* drafted, const float* uniforms, int64_t* n_accepted, int64_t* tokens, int64_t R,
                                    int64_t G, int64_t V, void* stream) {
     if (R < 0 || G < 0 || V < 1) return MBEMA_ERR_SHAPE;
-    if (V > 0x3fffffff || G > 4096 || R > 0x7fffffff / VD_CTAS) return MBEMA_ERR_UNSUPPORTED;
+    if (V > 0x3fffffff || G > 4096 || R > 0x7fffffff / 8) return MBEMA_ERR_UNSUPPORTED;
     if (dtype != MBEMA_F32 && dtype != MBEMA_BF16) return MBEMA_ERR_DTYPE;
     if (R == 0) return MBEMA_OK;
     if (!p || (G > 0 && !drafted) || !uniforms || !n_accepted || !tokens) return MBEMA_ERR_NULL;
     VerifyArgs a{p, q, p_row, p_pos, q_row, q_pos, (const long long*)drafted, uniforms, (long long*)n_accepted, (long long*)tokens, (int)G, (int)V};
-    const unsigned grid = (unsigned)(R * VD_CTAS);
-    if (dtype == MBEMA_F32) k_verify<MBEMA_F32><<<grid, VD_THREADS, 0, (cudaStream_t)stream>>>(a);
-    else k_verify<MBEMA_BF16><<<grid, VD_THREADS, 0, (cudaStream_t)stream>>>(a);
-    return check_launch();
+    // the largest cluster with which all rows are resident at once (four CTAs an SM): behind one another, rows pay their chain of
+    // loads again (256 rows of 50257: clusters of eight 51 us)
+    int64_t ctas = 8;
+    while (ctas > 2 && R * ctas > 4 * 148) ctas >>= 1;
+    if (dtype == MBEMA_F32) return ctas == 8 ? launch<MBEMA_F32, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_F32, 4>(a, R, stream) : launch<MBEMA_F32, 2>(a, R, stream);
+    return ctas == 8 ? launch<MBEMA_BF16, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_BF16, 4>(a, R, stream) : launch<MBEMA_BF16, 2>(a, R, stream);
 }

@@ -127,6 +127,8 @@ def _f32_or_bf16(t):
 # Raw handle of a device's current stream: torch.cuda.current_stream() builds a Stream object, 4 us a call, several times
 # what the launch itself costs the host.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+# The current device without torch.cuda.current_device's check that CUDA is up (callers hold CUDA tensors).
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream():

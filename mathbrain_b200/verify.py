@@ -8,10 +8,9 @@ max(p_j - q_j, 0), and behind drafts that all stand one more token is drawn from
 import torch
 
 from . import _lib
-from .ops import _dt, _on_tensor_device, _ptr, _require_cuda, _stream
+from .ops import _current_device, _dt, _raw_stream, _require_cuda
 
 
-@_on_tensor_device
 def verify_drafts(p_target, drafted, uniforms, p_draft=None):
     """(n_accepted int64 [R], tokens int64 [R, G + 1]): the drafts that stand, the next token, then -1.
 
@@ -24,28 +23,47 @@ def verify_drafts(p_target, drafted, uniforms, p_draft=None):
 
     A draw takes the smallest i whose running sum of weights passes uniform * their total; probabilities that are negative or
     not finite count as 0 there.  G = 0 draws from p_target alone."""
-    _require_cuda(p_target, drafted, uniforms, p_draft)
-    if p_target.dim() != 3 or p_target.shape[1] < 1 or p_target.shape[2] < 1:
-        raise _lib.MbemaError("verify_drafts: p_target %s, expected [R, G + 1, V]" % (tuple(p_target.shape),))
-    R, G, V = p_target.shape[0], p_target.shape[1] - 1, p_target.shape[2]
+    dev = p_target.get_device()
+    if dev < 0 or drafted.get_device() != dev or uniforms.get_device() != dev or (p_draft is not None and p_draft.get_device() != dev):
+        _require_cuda(p_target, drafted, uniforms, p_draft)
+        raise _lib.MbemaError("verify_drafts: operands live on different devices")
+    shape, dtype = p_target.shape, p_target.dtype
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
+        raise _lib.MbemaError("verify_drafts: p_target %s, expected [R, G + 1, V]" % (tuple(shape),))
+    R, places, V = shape
+    G = places - 1
     if drafted.shape != (R, G) or drafted.dtype != torch.int64:
         raise _lib.MbemaError("verify_drafts: drafted %s of %s, expected [%d, %d] int64" % (tuple(drafted.shape), drafted.dtype, R, G))
-    if uniforms.shape != (R, G + 1) or uniforms.dtype != torch.float32:
+    if uniforms.shape != (R, places) or uniforms.dtype != torch.float32:
         raise _lib.MbemaError("verify_drafts: uniforms %s of %s, expected [%d, %d] float32"
-                              % (tuple(uniforms.shape), uniforms.dtype, R, G + 1))
-    if p_draft is not None and (p_draft.shape != (R, G, V) or p_draft.dtype != p_target.dtype):
+                              % (tuple(uniforms.shape), uniforms.dtype, R, places))
+    if p_draft is not None and (p_draft.shape != (R, G, V) or p_draft.dtype != dtype):
         raise _lib.MbemaError("verify_drafts: p_draft %s of %s, expected [%d, %d, %d] %s"
-                              % (tuple(p_draft.shape), p_draft.dtype, R, G, V, p_target.dtype))
+                              % (tuple(p_draft.shape), p_draft.dtype, R, G, V, dtype))
     dt = _dt(p_target)
-    if V > 1 and p_target.stride(2) != 1:
-        p_target = p_target.contiguous()
-    if p_draft is not None and V > 1 and p_draft.stride(2) != 1:
-        p_draft = p_draft.contiguous()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _verify(p_target, drafted, uniforms, p_draft, dt, dev, R, G, V)
+    return _verify(p_target, drafted, uniforms, p_draft, dt, dev, R, G, V)
+
+
+def _verify(p, drafted, uniforms, q, dt, dev, R, G, V):
+    p_row, p_pos, one = p.stride()
+    if one != 1 and V > 1:
+        p = p.contiguous()
+        p_row, p_pos, _ = p.stride()
+    q_ptr, q_row, q_pos = None, 0, 0
+    if q is not None:
+        q_row, q_pos, one = q.stride()
+        if one != 1 and V > 1:
+            q = q.contiguous()
+            q_row, q_pos, _ = q.stride()
+        q_ptr = q.data_ptr()
     drafted, uniforms = drafted.contiguous(), uniforms.contiguous()
-    n_accepted = torch.empty(R, dtype=torch.int64, device=p_target.device)
-    tokens = torch.empty(R, G + 1, dtype=torch.int64, device=p_target.device)
-    q_row, q_pos = (p_draft.stride(0), p_draft.stride(1)) if p_draft is not None else (0, 0)
-    rc = _lib.load().mbema_verify_drafts(_ptr(p_target), p_target.stride(0), p_target.stride(1), _ptr(p_draft), q_row, q_pos, dt,
-                                         _ptr(drafted), _ptr(uniforms), _ptr(n_accepted), _ptr(tokens), R, G, V, _stream())
-    _lib.check(rc, "mbema_verify_drafts")
+    n_accepted = torch.empty(R, dtype=torch.int64, device=p.device)
+    tokens = torch.empty((R, G + 1), dtype=torch.int64, device=p.device)
+    rc = _lib.load().mbema_verify_drafts(p.data_ptr(), p_row, p_pos, q_ptr, q_row, q_pos, dt, drafted.data_ptr(), uniforms.data_ptr(),
+                                         n_accepted.data_ptr(), tokens.data_ptr(), R, G, V, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "mbema_verify_drafts")
     return n_accepted, tokens
