@@ -28,6 +28,7 @@ static size_t ba_smem(int N) {
 // grid: x = prefix jobs (B, blocks of 64 branches, chunks), then own jobs (B * S, chunks); y = head; z = step
 __global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
     extern __shared__ __align__(16) float smem[];
+    br_let_next_kernel_start();
     const mbema_branches& br = a.br;
     const int N = (int)br.N, ldA = N + 1;
     const int n = a.n, H = a.H, h = blockIdx.y, j = blockIdx.z;
@@ -214,51 +215,9 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     const int j = (int)(row % n);
     const int64_t r = row / n;
     const int b = (int)(r / br.S), s = (int)(r - (int64_t)b * br.S);
-    const int na = min(br.n_active[b], (int)br.Kcap);
-    // partials: np of the prefix from p0 on, then nq of the own slots from q0 on, p_step and q_step apart
-    int np, nq;
-    size_t p0, q0, p_step, q_step;
-    if constexpr (PIECES) {
-        const int64_t own = a.n_pre + r;
-        const int64_t pre = a.rows == 1 ? b : (int64_t)b * a.blocks + s / a.rows;
-        const int total = br.work[a.n_pre + br.B * br.S], workers = branch_workers(total, (int)a.max_workers);
-        auto pieces = [&](int64_t list, int cost, int& first) {
-            const int lo = br.work[list], hi = br.work[list + 1];
-            if (hi == lo) return 0;
-            first = branch_worker_of(total, workers, lo);
-            return branch_worker_of(total, workers, hi - cost) - first + 1;
-        };
-        int wp = 0, wq = 0;
-        np = pieces(pre, a.cost_pre, wp);
-        nq = pieces(own, BR_COST_OWN, wq);
-        const size_t each = (size_t)n * H, at = (size_t)j * H + h;
-        p_step = a.rows * each;
-        q_step = each;
-        p0 = ((size_t)(pre + wp) * a.rows + (a.rows == 1 ? 0 : s % a.rows)) * each + at;
-        q0 = (size_t)(a.own_piece0 + r + wq) * each + at;
-    } else {
-        const int SP = a.plan.SP, SO = a.plan.SO;
-        np = (na + a.plan.chp - 1) / a.plan.chp;
-        nq = (br.own_n[r] + a.plan.cho - 1) / a.plan.cho;
-        p_step = q_step = 1;
-        p0 = (size_t)wid * (SP + SO);
-        q0 = p0 + SP;
-    }
     float M = -INFINITY, L = 0.f;
     float2 o = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int p = warp; p < np + nq; p += BM_WARPS) {
-        const size_t at = p < np ? p0 + p * p_step : q0 + (p - np) * q_step;
-        const float2 ml = a.ml[at];
-        const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
-        if (ml.y == 0.f) continue;                              // every slot of it is hidden
-        const float m_new = fmaxf(M, ml.x);
-        const float keep = exp2f(M - m_new), w = exp2f(ml.x - m_new);
-        L = fmaf(ml.y, w, L * keep);
-        o.x = fmaf(x.x, w, o.x * keep);
-        o.y = fmaf(x.y, w, o.y * keep);
-        M = m_new;
-    }
+    // the staged tokens do not wait for the kernel before, which has seen the calls before it end
     for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
         const int cnt = min(BM_STAGED, j - i0);
         __syncthreads();
@@ -309,6 +268,51 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
                 M = m_new;
             }
         }
+    }
+    const int na = min(br.n_active[b], (int)br.Kcap);
+    // partials: np of the prefix from p0 on, then nq of the own slots from q0 on, p_step and q_step apart
+    int np, nq;
+    size_t p0, q0, p_step, q_step;
+    if constexpr (PIECES) {
+        const int2* work = reinterpret_cast<const int2*>(br.work);
+        const int64_t own = a.n_pre + r;
+        const int64_t pre = a.rows == 1 ? b : (int64_t)b * a.blocks + s / a.rows;
+        const int total = work[a.n_pre + br.B * br.S].x, workers = branch_workers(total, (int)a.max_workers);
+        auto pieces = [&](int64_t list, int cost, int& first) {
+            const int lo = work[list].x, hi = work[list + 1].x;
+            if (hi == lo) return 0;
+            first = branch_worker_of(total, workers, lo);
+            return branch_worker_of(total, workers, hi - cost) - first + 1;
+        };
+        int wp = 0, wq = 0;
+        np = pieces(pre, a.cost_pre, wp);
+        nq = pieces(own, BR_COST_OWN, wq);
+        const size_t each = (size_t)n * H, at = (size_t)j * H + h;
+        p_step = a.rows * each;
+        q_step = each;
+        p0 = ((size_t)(pre + wp) * a.rows + (a.rows == 1 ? 0 : s % a.rows)) * each + at;
+        q0 = (size_t)(a.own_piece0 + r + wq) * each + at;
+    } else {
+        const int SP = a.plan.SP, SO = a.plan.SO;
+        np = (na + a.plan.chp - 1) / a.plan.chp;
+        nq = (br.own_n[r] + a.plan.cho - 1) / a.plan.cho;
+        p_step = q_step = 1;
+        p0 = (size_t)wid * (SP + SO);
+        q0 = p0 + SP;
+    }
+    br_wait_for_kernel_before();
+#pragma unroll 4
+    for (int p = warp; p < np + nq; p += BM_WARPS) {
+        const size_t at = p < np ? p0 + p * p_step : q0 + (p - np) * q_step;
+        const float2 ml = a.ml[at];
+        const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
+        if (ml.y == 0.f) continue;                              // every slot of it is hidden
+        const float m_new = fmaxf(M, ml.x);
+        const float keep = exp2f(M - m_new), w = exp2f(ml.x - m_new);
+        L = fmaf(ml.y, w, L * keep);
+        o.x = fmaf(x.x, w, o.x * keep);
+        o.y = fmaf(x.y, w, o.y * keep);
+        M = m_new;
     }
     if (lane == 0) { s_m[warp] = M; s_l[warp] = L; }
     s_o[warp][lane] = o;
@@ -371,8 +375,7 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st) {
     const int64_t ctas = a.br.B * a.br.S * a.n * a.H;
     if (ctas > 0x7fffffff) return MBEMA_ERR_UNSUPPORTED;
-    if (pieces) k_branch_merge<true><<<(unsigned)ctas, BM_WARPS * 32, 0, st>>>(a);
-    else k_branch_merge<false><<<(unsigned)ctas, BM_WARPS * 32, 0, st>>>(a);
+    MBEMA_CUDA_TRY(launch_early(pieces ? k_branch_merge<true> : k_branch_merge<false>, dim3((unsigned)ctas), BM_WARPS * 32, st, a));
     return check_launch();
 }
 

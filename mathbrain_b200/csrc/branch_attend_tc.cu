@@ -192,19 +192,18 @@ struct List {
     int count;
 };
 
-__device__ __forceinline__ List get_list(const BranchArgs& a, int x) {
+__device__ __forceinline__ List get_list(const BranchArgs& a, int x, int count) {
     const mbema_branches& br = a.br;
     List t;
+    t.count = count;
     if (x < (int)a.n_pre) {
         const int b = x / a.blocks;
         t.slots = br.active + (size_t)b * br.Kcap;
         t.op = reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N);
-        t.count = min(br.n_active[b], (int)br.Kcap);
     } else {
         const int r = x - (int)a.n_pre;
         t.slots = br.own_slot + (size_t)r * br.cap;
         t.op = reinterpret_cast<const char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, br.N);
-        t.count = br.own_n[r];
     }
     return t;
 }
@@ -451,12 +450,12 @@ struct SixteenRows {
 };
 
 // Where a stretch begins: the first list whose units reach cost c, by 32 samples of the running sum at a time.
-__device__ __forceinline__ int find_list(const int* work, int lists, int c, int lane) {
-    int lo = 0, hi = lists;                       // work[lo] <= c < work[hi]
+__device__ __forceinline__ int find_list(const int2* work, int lists, int c, int lane) {
+    int lo = 0, hi = lists;                       // work[lo].x <= c < work[hi].x
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32;
         const int at = lo + (lane + 1) * step;
-        const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at] <= c);
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at].x <= c);
         lo += __popc(below) * step;
         hi = min(hi, lo + step);
     }
@@ -474,8 +473,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     constexpr int N = 16 * KS;
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.H * BR_HD;
-    // the steps' fragments of W behind the ring, whose space the staged slice of W takes first
-    float* W_sh = reinterpret_cast<float*>(smem);
+    br_let_next_kernel_start();
+    const int lists = (int)(a.n_pre + br.B * br.S), n_pre = (int)a.n_pre;
+    const int2* work = reinterpret_cast<const int2*>(br.work);
+    const int total = work[lists].x;
+    // behind the ring the steps' fragments of W, then (or in the ring, where there is no room) the staged slice of W
+    const uint32_t w_all = (uint32_t)__cvta_generic_to_shared(smem) + a.ring_bytes;
+    float* W_sh = reinterpret_cast<float*>(smem + a.w_offset);
     for (int i = tid; i < N * 16; i += WARPS * 32) {
         const float4 x = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
         float2* dst = reinterpret_cast<float2*>(W_sh + w_row(i >> 4) + (i & 15) * 4);
@@ -483,49 +487,41 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         dst[1] = make_float2(x.z, x.w);
     }
     for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = log2f(br.rhos[i]);
-    const int lists = (int)(a.n_pre + br.B * br.S), n_pre = (int)a.n_pre;
-    const int total = br.work[lists];
     const int workers = branch_workers(total, (int)gridDim.x * IG);
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;
     const int steps = min(JW, a.n - (int)blockIdx.z * JW);       // of this CTA
     const int me = (int)blockIdx.x * IG + ig;
-    __syncthreads();
-    const uint32_t w_all = (uint32_t)__cvta_generic_to_shared(smem) + a.ring_bytes;
-    for (int i = 0; i < steps; ++i)
-        build_W<KS>(w_all + i * KS * 2048, W_sh, s_l2r, blockIdx.z * JW + i, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane, warp, WARPS);
-    __syncthreads();
-    if (ig >= IG || jj >= steps || me >= workers) return;
-    const uint32_t w_at = w_all + jj * KS * 2048 + lane * 16;
-    constexpr bool W_REGS = KS == 4 && WARPS == 8;
-    uint4 w[KS * 4];
-    if constexpr (W_REGS) read_W<KS>(w, w_at);
-    const int c_end = branch_cut(total, workers, me + 1);
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + ig * STAGES * Unit::BYTES;
+    const bool works = ig < IG && jj < steps && me < workers && total > 0;
+    if ((int)blockIdx.x * IG >= workers || total == 0) return;   // the whole CTA has nothing to do
+    const int c_end = works ? branch_cut(total, workers, me + 1) : 0;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (works ? ig : 0) * STAGES * Unit::BYTES;
     const uint32_t ring_end = ring + STAGES * Unit::BYTES;
 
     // producer: `left` units of list px from slot pk on; the ids of its next unit are a unit ahead
-    int px, pk, left;
-    List pl;
+    int px = 0, pk = 0, left = 0;
+    List pl = {nullptr, nullptr, 0};
     auto units_to = [&](int from, int to, int cost) { return (min(to, c_end) - from + cost - 1) / cost; };
     auto cost_of = [&](int list) { return list < n_pre ? a.cost_pre : BR_COST_OWN; };
-    auto next_list = [&](int& list) {                            // the next list with units in this stretch: their number, or 0
+    auto next_list = [&](int& list, int& count) {                // the next list with units in this stretch: their number, or 0
         for (;;) {
-            const int lo = br.work[++list];
-            if (lo >= c_end) return 0;
-            const int hi = br.work[list + 1];
-            if (hi > lo) return units_to(lo, hi, cost_of(list));
+            const int2 at = work[++list];
+            if (at.x >= c_end) return 0;
+            const int hi = work[list + 1].x;
+            count = at.y;
+            if (hi > at.x) return units_to(at.x, hi, cost_of(list));
         }
     };
-    {
+    if (works) {
         const int c0 = branch_cut(total, workers, me);
-        px = find_list(br.work, lists, c0, lane);
-        const int lo = br.work[px], cost = cost_of(px), skip = (c0 - lo + cost - 1) / cost;      // units of the list before this stretch
+        px = find_list(work, lists, c0, lane);
+        const int2 lo = work[px];
+        const int hi = work[px + 1].x, cost = cost_of(px), skip = (c0 - lo.x + cost - 1) / cost;     // units of the list before this stretch
+        int count = lo.y;
         pk = skip * 16;
-        left = max(units_to(lo + skip * cost, br.work[px + 1], cost), 0);
-        if (left == 0) { pk = 0; left = next_list(px); }
-        if (left == 0) return;                                   // nothing is listed at all (the whole worker leaves)
-        pl = get_list(a, px);
+        left = max(units_to(lo.x + skip * cost, hi, cost), 0);
+        if (left == 0) { pk = 0; left = next_list(px, count); }
+        pl = get_list(a, px, count);
     }
     int x = px;                                                  // consumer: c_left units of list x from slot k0 on
     int k0 = pk, c_left = left, count = pl.count;
@@ -536,7 +532,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     const uint32_t D2 = (uint32_t)D * 2;
     const uint32_t dst_E = sub * 128 + (((lane & 7) ^ ((sub & 1) << 2)) << 4), dst_A = Unit::OP + lane * 16;
     int ids = 0, turn = 0;                                       // the worker's warps copy a unit each in turn
-    if (jj == 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
+    if (works && jj == 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
     uint32_t fill = ring;                                        // stage that the producer fills next
     auto produce = [&]() {
         if (left > 0) {
@@ -546,8 +542,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
             turn = turn + 1 == steps ? 0 : turn + 1;
             pk += 16;
             if (--left == 0) {
-                left = next_list(px);
-                if (left > 0) { pl = get_list(a, px); pk = 0; }
+                int next = 0;
+                left = next_list(px, next);
+                if (left > 0) { pl = get_list(a, px, next); pk = 0; }
             }
             if (turn == jj && left > 0) ids = pl.slots[min(pk + (lane & 15), pl.count - 1)];
             if (mine) {
@@ -565,8 +562,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         fill += Unit::BYTES;
         if (fill == ring_end) fill = ring;
     };
+    const bool in_ring = a.w_offset == 0;
+    auto fill_ring = [&]() {
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) produce();
+        for (int i = 0; i < STAGES - 1; ++i) produce();
+    };
+    if (works && !in_ring) fill_ring();
+    __syncthreads();
+    for (int i = 0; i < steps; ++i)
+        build_W<KS>(w_all + i * KS * 2048, W_sh, s_l2r, blockIdx.z * JW + i, a.silu ? 0.5f * BT_W_SCALE : BT_W_SCALE, lane, warp, WARPS);
+    __syncthreads();
+    if (!works) return;
+    if (in_ring) fill_ring();
+    const uint32_t w_at = w_all + jj * KS * 2048 + lane * 16;
+    constexpr bool W_REGS = KS == 4 && WARPS == 8;
+    uint4 w[KS * 4];
+    if constexpr (W_REGS) read_W<KS>(w, w_at);
     OneRow one;
     SixteenRows many;
     bool fresh = true, own = false, single = true;
@@ -614,10 +625,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         if (--c_left == 0) {                                     // end of the list or of the stretch
             if (single) one.leave(a, own ? a.own_piece0 + (x - n_pre) + me : (int64_t)x + me, j, h, lane);
             else if constexpr (ROWS > 1) many.leave(a, (int64_t)x + me, rows, j, h, lane);
-            c_left = next_list(x);
+            c_left = next_list(x, count);
             if (c_left == 0) break;
             k0 = 0;
-            count = x < n_pre ? min(br.n_active[x / a.blocks], (int)br.Kcap) : br.own_n[x - n_pre];
             fresh = true;
         }
     }
@@ -655,11 +665,14 @@ BranchShape branch_shape(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H) 
 
 template <int KS, int ROWS, int WARPS, int STAGES>
 static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
-    const size_t w_sh = ((size_t)16 * KS * BT_LDW + 8) * 4;
-    a.ring_bytes = (int)align_up(std::max(w_sh, (size_t)p.IG * STAGES * UnitLayout<KS>::BYTES), 128);
-    const size_t smem = a.ring_bytes + (size_t)p.JW * KS * 2048;
+    const size_t w_sh = align_up(((size_t)16 * KS * BT_LDW + 8) * 4, 128), w_all = (size_t)p.JW * KS * 2048;
+    const size_t ring = (size_t)p.IG * STAGES * UnitLayout<KS>::BYTES, most = 232448 - 1024;
+    const bool in_ring = ring + w_all + w_sh > most;
+    a.ring_bytes = (int)(in_ring ? std::max(ring, w_sh) : ring);
+    a.w_offset = in_ring ? 0 : a.ring_bytes + (int)w_all;
+    const size_t smem = a.ring_bytes + w_all + (in_ring ? 0 : w_sh);
     static std::atomic<unsigned long long> done{0};
-    MBEMA_CUDA_TRY(allow_smem(k_branch_tc<KS, ROWS, WARPS, STAGES>, 232448 - 1024, done));
+    MBEMA_CUDA_TRY(allow_smem(k_branch_tc<KS, ROWS, WARPS, STAGES>, most, done));
     k_branch_tc<KS, ROWS, WARPS, STAGES><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st>>>(a, p.JW, p.IG);
     return check_launch();
 }

@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
     __shared__ int s_tok[BR_MAX_NEW], s_own[BR_MAX_NEW], s_dst[BR_MAX_NEW];
     __shared__ unsigned s_same[BR_MAX_NEW];
     __shared__ int s_n, s_len;
+    br_let_next_kernel_start();
     const int64_t r = blockIdx.x;
     const int b = (int)(r / br.S);
     const int tid = threadIdx.x, lane = tid & 31;
@@ -154,9 +155,8 @@ __device__ void running_sum(const mbema_branches& br) {
     int base = 0;
     for (int x0 = 0; x0 < lists; x0 += 256) {
         const int x = x0 + tid;
-        int c = 0;
-        if (x < n_pre) c = (min(br.n_active[x / blocks], (int)br.Kcap) + 15) / 16 * (br.S == 1 ? BR_COST_ONE : BR_COST_BLOCK);
-        else if (x < lists) c = (br.own_n[x - n_pre] + 15) / 16 * BR_COST_OWN;
+        const int count = x < n_pre ? min(br.n_active[x / blocks], (int)br.Kcap) : x < lists ? br.own_n[x - n_pre] : 0;
+        const int c = (count + 15) / 16 * (x >= n_pre ? BR_COST_OWN : br.S == 1 ? BR_COST_ONE : BR_COST_BLOCK);
         int sum = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -170,14 +170,15 @@ __device__ void running_sum(const mbema_branches& br) {
             if (w < (tid >> 5)) sum += s_warp[w];
             all += s_warp[w];
         }
-        if (x < lists) br.work[x] = base + sum - c;
+        if (x < lists) reinterpret_cast<int2*>(br.work)[x] = make_int2(base + sum - c, count);
         base += all;
         __syncthreads();
     }
-    if (tid == 0) br.work[lists] = base;
+    if (tid == 0) reinterpret_cast<int2*>(br.work)[lists] = make_int2(base, 0);
 }
 
 __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
+    br_wait_for_kernel_before();
     if (blockIdx.y == br.B) {
         if (blockIdx.x == 0 && blockIdx.z == 0) running_sum(br);
         return;
@@ -315,7 +316,7 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
     // shares of a list: eight CTAs an SM over all lists, one for every 64 or 32 slots where that is enough
     const int64_t items = 16 * 8 / (br->N / 32), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
     const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
-    k_branch_operands<<<dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream>>>(*br);
+    MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, (cudaStream_t)stream, *br));
     return check_launch();
 }
 

@@ -50,7 +50,7 @@ struct BranchArgs {
     // tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order; partials of the prefixes
     // [piece, BR_BLOCK or 1, n, H], of the own lists [own_piece0 + piece, n, H]
     int64_t n_pre, own_piece0, max_workers;
-    int rows, blocks, cost_pre, ring_bytes;
+    int rows, blocks, cost_pre, ring_bytes, w_offset;
 };
 
 // The workers that a running sum of `total` occupies, each with two units or more, and where their stretches begin.
@@ -93,6 +93,23 @@ inline cudaError_t allow_smem(Kernel kernel, size_t most, std::atomic<unsigned l
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
 }
+
+// A kernel whose CTAs may start while the kernel before it still runs (it waits for it with br_wait_for_kernel_before).
+template <typename... Params, typename... Args>
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+__device__ __forceinline__ void br_wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void br_let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 bool branch_tc_supported(int64_t N);
 BranchShape branch_shape(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H);

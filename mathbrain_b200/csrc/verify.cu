@@ -231,10 +231,10 @@ extern "C" int mbema_verify_drafts(const void* p, int64_t p_row, int64_t p_pos, 
     if (R == 0) return MBEMA_OK;
     if (!p || (G > 0 && !drafted) || !uniforms || !n_accepted || !tokens) return MBEMA_ERR_NULL;
     VerifyArgs a{p, q, p_row, p_pos, q_row, q_pos, (const long long*)drafted, uniforms, (long long*)n_accepted, (long long*)tokens, (int)G, (int)V};
-    // the largest cluster with which all rows are resident at once (four CTAs an SM): behind one another, rows pay their chain of
-    // loads again (256 rows of 50257: clusters of eight 51 us)
+    // the largest cluster with which all rows are resident at once, two CTAs an SM (one sequence and 20: 8 or 2 make no difference; 64: 8 17 us,
+    // 4 12.7, 2 14.5; 256: 8 48 us, 4 37, 2 34)
     int64_t ctas = 8;
-    while (ctas > 2 && R * ctas > 4 * 148) ctas >>= 1;
+    while (ctas > 2 && R * ctas > 2 * 148) ctas >>= 1;
     if (dtype == MBEMA_F32) return ctas == 8 ? launch<MBEMA_F32, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_F32, 4>(a, R, stream) : launch<MBEMA_F32, 2>(a, R, stream);
     return ctas == 8 ? launch<MBEMA_BF16, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_BF16, 4>(a, R, stream) : launch<MBEMA_BF16, 2>(a, R, stream);
 }
