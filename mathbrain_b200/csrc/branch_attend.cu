@@ -15,22 +15,23 @@ namespace mbema {
 
 static constexpr int BA_THREADS = 256;
 static constexpr int BA_TILE = 64;       // slots a tile
-static constexpr int BA_ROWS = 64;       // branches a CTA
-static constexpr int BA_LD = 68;         // floats a row of the K and V tiles (16-byte rows, conflict-free columns)
+static constexpr int BA_ROWS = 32;       // branches a CTA
+static constexpr int BA_LD = 68;         // floats a row of 64 in shared memory: 16-byte pieces of eight rows lie in different banks
 static constexpr int BM_WARPS = 4;
 static constexpr int BM_STAGED = 8;      // staged tokens at a time
 
 static size_t ba_smem(int N) {
-    return ((size_t)N * BR_HD + (size_t)BA_TILE * (N + 1) + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * BR_HD + BA_ROWS * (BA_TILE + 1) +
-            N + 3 * BA_ROWS + BA_TILE) * 4;
+    return ((size_t)N * BR_HD + (size_t)N * BA_LD + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * (BR_HD + BA_LD) + ((N + 3) & ~3) + 3 * BA_ROWS + 2 * BA_TILE) * 4;
 }
 
-// grid: x = prefix jobs (B, blocks of 64 branches, chunks), then own jobs (B * S, chunks); y = head; z = step
-__global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
+// grid: x = prefix jobs (B, blocks of 32 branches, chunks), then own jobs (B * S, chunks); y = head; z = step.
+// The gate product is tiled 4 slots x 4 channels to a thread (three wavefronts of shared memory for 16 FMAs a warp; with one slot and 16
+// channels it was nine, and the kernel took 82 us where it takes now 33: 2 x 5 branches of 701 slots, 3 steps, 8 heads).
+__global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     extern __shared__ __align__(16) float smem[];
     br_let_next_kernel_start();
     const mbema_branches& br = a.br;
-    const int N = (int)br.N, ldA = N + 1;
+    const int N = (int)br.N;
     const int n = a.n, H = a.H, h = blockIdx.y, j = blockIdx.z;
     const int SP = a.plan.SP, SO = a.plan.SO;
     const int blocks = (int)((br.S + BA_ROWS - 1) / BA_ROWS);
@@ -58,102 +59,117 @@ __global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
     if (k_lo >= k_hi) return;
     const int64_t r0 = (int64_t)b * br.S + s0;
     float* W_sh = smem;                                   // [N][64]
-    float* K_sh = W_sh + N * BR_HD;                       // [64][68]
+    float* A_sh = W_sh + N * BR_HD;                       // [N][68]: states, transposed
+    float* K_sh = A_sh + N * BA_LD;                       // [64][68]
     float* V_sh = K_sh + BA_TILE * BA_LD;
-    float* q_sh = V_sh + BA_TILE * BA_LD;                 // [64][64], scaled to base-2 scores
-    float* P_sh = q_sh + BA_ROWS * BR_HD;                 // [64][65]
-    float* A_sh = P_sh + BA_ROWS * (BA_TILE + 1);         // [64][N+1]
-    float* l2r_sh = A_sh + BA_TILE * ldA;
-    float* m_sh = l2r_sh + N;
+    float* q_sh = V_sh + BA_TILE * BA_LD;                 // [32][64], scaled to base-2 scores
+    float* P_sh = q_sh + BA_ROWS * BR_HD;                 // [32][68]
+    float* l2r_sh = P_sh + BA_ROWS * BA_LD;
+    float* m_sh = l2r_sh + ((N + 3) & ~3);
     float* l_sh = m_sh + BA_ROWS;
     float* al_sh = l_sh + BA_ROWS;
+    int* v_sh = reinterpret_cast<int*>(al_sh + BA_ROWS);  // the tile's slots, and their ages
+    float* dt_sh = reinterpret_cast<float*>(v_sh + BA_TILE);
     const int tid = threadIdx.x;
-    const int sr = tid >> 2, dg = tid & 3;
     const int D = H * BR_HD;
-    for (int i = tid; i < N * BR_HD; i += BA_THREADS) W_sh[i] = a.W[(size_t)(i >> 6) * D + h * BR_HD + (i & 63)];
+    const int tau = br.t0[0] + br.len[r0] + j;
+    auto slots_of = [&](int k0) {                         // (the first 64 threads)
+        const int k = k0 + tid;
+        int v = 0;
+        float dt = 0.f;
+        if (k < k_hi) {
+            v = own ? br.own_slot[(size_t)r0 * br.cap + k] : br.active[(size_t)b * br.Kcap + k];
+            dt = (float)(tau - (own ? br.own_t[(size_t)r0 * br.cap + k] : br.last_t[(size_t)b * br.V + v]));
+        }
+        v_sh[tid] = v;
+        dt_sh[tid] = dt;
+    };
+    if (tid < BA_TILE) slots_of(k_lo);
+    for (int i = tid; i < N * (BR_HD / 4); i += BA_THREADS)
+        *reinterpret_cast<float4*>(W_sh + i * 4) = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
     for (int i = tid; i < N; i += BA_THREADS) l2r_sh[i] = log2f(br.rhos[i]);
     for (int i = tid; i < rows * BR_HD; i += BA_THREADS)
         q_sh[i] = ld_dyn_f32(a.q, a.q_dt, ((((size_t)(r0 + (i >> 6))) * n + j) * H + h) * BR_HD + (i & 63)) * BR_SCORE_LOG2;
     for (int i = tid; i < BA_ROWS; i += BA_THREADS) { m_sh[i] = -INFINITY; l_sh[i] = 0.f; }
-    const int tau = br.t0[0] + br.len[r0] + j;
-    const int oc = tid & 63, og = tid >> 6;               // output column, row group: rows og, og + 4, ...
+    const int tx = tid & 15, ty = tid >> 4;               // gate: channels 4 tx.., slots 4 ty..
+    const int slot = tid & 63, group = tid >> 6;          // states and scores: a slot, every fourth row; output: a column, every fourth row
     float o[BA_ROWS / 4];
 #pragma unroll
     for (int i = 0; i < BA_ROWS / 4; ++i) o[i] = 0.f;
     for (int k0 = k_lo; k0 < k_hi; k0 += BA_TILE) {
         const int tile = min(BA_TILE, k_hi - k0);
-        const int k = k0 + sr;
-        const bool ok = sr < tile;
-        int v = 0;
-        __syncthreads();                                  // the tile before is read
+        __syncthreads();                                  // the slots are there
         {
-            float dt = 0.f;
-            const float* row = nullptr;
-            if (ok && !own) {
-                v = br.active[(size_t)b * br.Kcap + k];
-                dt = (float)(tau - br.last_t[(size_t)b * br.V + v]);
-                row = br.state + ((size_t)b * br.V + v) * N;
-            } else if (ok) {
-                v = br.own_slot[(size_t)r0 * br.cap + k];
-                dt = (float)(tau - br.own_t[(size_t)r0 * br.cap + k]);
-                row = br.own_state + ((size_t)r0 * br.cap + k) * N;
+            const bool ok = slot < tile;
+            const float dt = dt_sh[slot];
+            const float* row = own ? br.own_state + ((size_t)r0 * br.cap + min(k0 + slot, k_hi - 1)) * N : br.state + ((size_t)b * br.V + v_sh[slot]) * N;
+            for (int c = group; c < N; c += 4) A_sh[c * BA_LD + slot] = ok ? row[c] * exp2f(dt * l2r_sh[c]) : 0.f;
+        }
+        float4 ek[4], ev[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ek[i] = ev[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (4 * ty + i < tile) {
+                const size_t off = (size_t)v_sh[4 * ty + i] * D + h * BR_HD + 4 * tx;
+                ek[i] = ld4_dyn_f32(a.Ek, a.e_dt, off);
+                ev[i] = ld4_dyn_f32(a.Ev, a.e_dt, off);
             }
-            for (int c = dg; c < N; c += 4) A_sh[sr * ldA + c] = ok ? row[c] * exp2f(dt * l2r_sh[c]) : 0.f;
         }
         __syncthreads();
-        float acc[16];
+        float acc[4][4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-        const float* arow = A_sh + sr * ldA;
-        const float* wcol = W_sh + dg * 16;
-#pragma unroll 4
+        for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll 8
         for (int c = 0; c < N; ++c) {
-            const float av = arow[c];
-            const float4* wp = reinterpret_cast<const float4*>(wcol + c * BR_HD);
+            const float4 x = *reinterpret_cast<const float4*>(A_sh + c * BA_LD + 4 * ty), w = *reinterpret_cast<const float4*>(W_sh + c * BR_HD + 4 * tx);
+            const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4 w = wp[i];
-                acc[4 * i] = fmaf(av, w.x, acc[4 * i]);
-                acc[4 * i + 1] = fmaf(av, w.y, acc[4 * i + 1]);
-                acc[4 * i + 2] = fmaf(av, w.z, acc[4 * i + 2]);
-                acc[4 * i + 3] = fmaf(av, w.w, acc[4 * i + 3]);
+                acc[i][0] = fmaf(xs[i], w.x, acc[i][0]);
+                acc[i][1] = fmaf(xs[i], w.y, acc[i][1]);
+                acc[i][2] = fmaf(xs[i], w.z, acc[i][2]);
+                acc[i][3] = fmaf(xs[i], w.w, acc[i][3]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            float4 ek = make_float4(0.f, 0.f, 0.f, 0.f), ev = ek;
-            if (ok) {
-                const size_t off = (size_t)v * D + h * BR_HD + dg * 16 + i;
-                ek = ld4_dyn_f32(a.Ek, a.e_dt, off);
-                ev = ld4_dyn_f32(a.Ev, a.e_dt, off);
-            }
+        for (int i = 0; i < 4; ++i) {
             float g[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) g[c] = a.silu ? acc[i + c] / (1.0f + expf(-acc[i + c])) : acc[i + c];
-            *reinterpret_cast<float4*>(K_sh + sr * BA_LD + dg * 16 + i) = make_float4(ek.x * g[0], ek.y * g[1], ek.z * g[2], ek.w * g[3]);
-            *reinterpret_cast<float4*>(V_sh + sr * BA_LD + dg * 16 + i) = make_float4(ev.x * g[0], ev.y * g[1], ev.z * g[2], ev.w * g[3]);
+            for (int c = 0; c < 4; ++c) g[c] = a.silu ? __fdividef(acc[i][c], 1.0f + expf(-acc[i][c])) : acc[i][c];
+            const int at = (4 * ty + i) * BA_LD + 4 * tx;
+            *reinterpret_cast<float4*>(K_sh + at) = make_float4(ek[i].x * g[0], ek[i].y * g[1], ek[i].z * g[2], ek[i].w * g[3]);
+            *reinterpret_cast<float4*>(V_sh + at) = make_float4(ev[i].x * g[0], ev[i].y * g[1], ev[i].z * g[2], ev[i].w * g[3]);
         }
         __syncthreads();
-        {   // scores: a thread holds one slot and takes every fourth row
-            const int slot = tid & 63;
+        if (tid < BA_TILE && k0 + BA_TILE < k_hi) slots_of(k0 + BA_TILE);
+        for (int row0 = group; row0 < rows; row0 += 16) {        // rows row0, row0 + 4, + 8, + 12 against one slot's K
             const float4* kp = reinterpret_cast<const float4*>(K_sh + slot * BA_LD);
-            for (int row = tid >> 6; row < rows; row += 4) {
-                const float4* qp = reinterpret_cast<const float4*>(q_sh + row * BR_HD);
-                float s = 0.f;
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const float4 x = kp[i];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float4 x = kp[i], y = qp[i];
-                    s = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
+                for (int e = 0; e < 4; ++e) {
+                    if (row0 + 4 * e < rows) {
+                        const float4 y = *reinterpret_cast<const float4*>(q_sh + (row0 + 4 * e) * BR_HD + 4 * i);
+                        s[e] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[e]))));
+                    }
                 }
-                bool hide = slot >= tile;
-                if (!hide) hide = own ? br_hides_own(br, r0, j, k0 + slot) : br_hides_prefix(br, r0 + row, j, k0 + slot);
-                P_sh[row * (BA_TILE + 1) + slot] = hide ? -INFINITY : s;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = row0 + 4 * e;
+                if (row < rows) {
+                    bool hide = slot >= tile;
+                    if (!hide) hide = own ? br_hides_own(br, r0, j, k0 + slot) : br_hides_prefix(br, r0 + row, j, k0 + slot);
+                    P_sh[row * BA_LD + slot] = hide ? -INFINITY : s[e];
+                }
             }
         }
         __syncthreads();
         for (int row = tid >> 5; row < rows; row += BA_THREADS / 32) {
             const int lane = tid & 31;
-            float* p = P_sh + row * (BA_TILE + 1);
+            float* p = P_sh + row * BA_LD;
             const float x = p[lane], y = p[lane + 32];
             float mx = fmaxf(x, y);
 #pragma unroll
@@ -173,26 +189,44 @@ __global__ void __launch_bounds__(BA_THREADS) k_branch_attend(BranchArgs a) {
             }
         }
         __syncthreads();
+        if (rows == 1) {                                  // the groups share the slots: 16 each
+            float x = o[0] * al_sh[0];
 #pragma unroll
-        for (int i = 0; i < BA_ROWS / 4; ++i) {
-            const int row = og + 4 * i;
-            if (row < rows) {
-                float x = o[i] * al_sh[row];
-                const float* p = P_sh + row * (BA_TILE + 1);
-                for (int c = 0; c < tile; ++c) x = fmaf(p[c], V_sh[c * BA_LD + oc], x);
-                o[i] = x;
+            for (int c = 0; c < 16; ++c) x = fmaf(P_sh[16 * group + c], V_sh[(16 * group + c) * BA_LD + slot], x);
+            o[0] = x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < BA_ROWS / 4; ++i)
+                if (group + 4 * i < rows) o[i] *= al_sh[group + 4 * i];
+            for (int c = 0; c < BA_TILE; c += 4) {        // (slots past the list: weight 0, value 0)
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = V_sh[(c + e) * BA_LD + slot];
+#pragma unroll
+                for (int i = 0; i < BA_ROWS / 4; ++i) {
+                    if (group + 4 * i < rows) {
+                        const float4 p = *reinterpret_cast<const float4*>(P_sh + (group + 4 * i) * BA_LD + c);
+                        o[i] = fmaf(p.x, v[0], fmaf(p.y, v[1], fmaf(p.z, v[2], fmaf(p.w, v[3], o[i]))));
+                    }
+                }
             }
         }
     }
     __syncthreads();
-    const int slot = own ? SP + chunk : chunk;
+    const int part = own ? SP + chunk : chunk;
+    if (rows == 1) {
+        K_sh[tid] = o[0];
+        __syncthreads();
+        if (group > 0) return;
+        o[0] = (K_sh[slot] + K_sh[64 + slot]) + (K_sh[128 + slot] + K_sh[192 + slot]);
+    }
 #pragma unroll
     for (int i = 0; i < BA_ROWS / 4; ++i) {
-        const int row = og + 4 * i;
+        const int row = group + 4 * i;
         if (row < rows) {
-            const size_t at = ((((size_t)(r0 + row)) * n + j) * H + h) * (SP + SO) + slot;
-            a.po[at * BR_HD + oc] = o[i];
-            if (oc == 0) a.ml[at] = make_float2(m_sh[row], l_sh[row]);
+            const size_t at = ((((size_t)(r0 + row)) * n + j) * H + h) * (SP + SO) + part;
+            a.po[at * BR_HD + slot] = o[i];
+            if (slot == 0) a.ml[at] = make_float2(m_sh[row], l_sh[row]);
         }
     }
 }
