@@ -4,8 +4,8 @@
 // SiLU(M W_pe), K = E_k * gate and V = E_v * gate are formed once a (sequence, step) and read by all S branches; the slots that a
 // branch has touched are its own, and a row sees its prefix through a mask without them:
 //     softmax over {prefix slots not touched} + {own slots} + {tokens staged before the row} + {V_total - listed, score 0, value 0}.
-// A CTA takes one job (a chunk of slots) for one step and head: K and V tiles of 64 slots in shared memory, the scores of up to 64
-// branches against them, online softmax, one partial (m, l, o) per row.  k_branch_merge joins the partials, adds the few staged
+// A CTA takes one job (a chunk of slots, up to 32 rows) for one head: K and V tiles of 64 slots in shared memory, the branches' scores
+// against them, online softmax, one partial (m, l, o) per row.  k_branch_merge joins the partials, adds the few staged
 // tokens (each a dot product of N channels, in fp32) and the zero-score slots.
 #include <algorithm>
 
@@ -21,29 +21,34 @@ static constexpr int BM_WARPS = 4;
 static constexpr int BM_STAGED = 8;      // staged tokens at a time
 
 static size_t ba_smem(int N) {
-    return ((size_t)N * BR_HD + (size_t)N * BA_LD + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * (BR_HD + BA_LD) + ((N + 3) & ~3) + 3 * BA_ROWS + 2 * BA_TILE) * 4;
+    return ((size_t)N * BR_HD + (size_t)N * BA_LD + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * (2 * BR_HD + BA_LD) + 2 * ((N + 3) & ~3) + 3 * BA_ROWS +
+            2 * BA_TILE) * 4;
 }
 
-// grid: x = prefix jobs (B, blocks of 32 branches, chunks), then own jobs (B * S, chunks); y = head; z = step.
-// The gate product is tiled 4 slots x 4 channels to a thread (three wavefronts of shared memory for 16 FMAs a warp; with one slot and 16
-// channels it was nine, and the kernel took 82 us where it takes now 33: 2 x 5 branches of 701 slots, 3 steps, 8 heads).
+// grid: x = prefix jobs (B, blocks of 32 branches, chunks; then blocks of steps), then own jobs (B * S, chunks; all steps); y = head.
+// A job's rows are (step, branch) pairs, 32 at most: the tile's states and E rows, loaded once, serve as many steps as that allows.
+// The gate product is tiled 4 slots x 4 channels to a thread (three wavefronts of shared memory for 16 FMAs a warp; one slot and 16
+// channels take nine).  Bound by latency at small sizes: nine meetings of the CTA a tile and step.
 __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     extern __shared__ __align__(16) float smem[];
     br_let_next_kernel_start();
     const mbema_branches& br = a.br;
     const int N = (int)br.N;
-    const int n = a.n, H = a.H, h = blockIdx.y, j = blockIdx.z;
+    const int n = a.n, H = a.H, h = blockIdx.y;
     const int SP = a.plan.SP, SO = a.plan.SO;
     const int blocks = (int)((br.S + BA_ROWS - 1) / BA_ROWS);
-    const int64_t n_pre = (int64_t)br.B * blocks * SP;
+    const int64_t n_pre = (int64_t)br.B * blocks * SP * a.plan.JP;
     const bool own = blockIdx.x >= n_pre;
-    int b, s0, rows, chunk, k_lo, k_hi;
+    int b, s0, branches, chunk, k_lo, k_hi, j0, steps;
     if (!own) {
         chunk = (int)(blockIdx.x % SP);
-        const int bb = (int)(blockIdx.x / SP);
-        b = bb / blocks;
-        s0 = (bb % blocks) * BA_ROWS;
-        rows = min(BA_ROWS, (int)br.S - s0);
+        int y = (int)(blockIdx.x / SP);
+        j0 = (y % a.plan.JP) * a.plan.steps;
+        steps = min(a.plan.steps, n - j0);
+        y /= a.plan.JP;
+        b = y / blocks;
+        s0 = (y % blocks) * BA_ROWS;
+        branches = min(BA_ROWS, (int)br.S - s0);
         k_lo = chunk * a.plan.chp;
         k_hi = min(k_lo + a.plan.chp, min(br.n_active[b], (int)br.Kcap));
     } else {
@@ -52,27 +57,38 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
         const int64_t r = x / SO;
         b = (int)(r / br.S);
         s0 = (int)(r % br.S);
-        rows = 1;
+        branches = 1;
+        j0 = 0;
+        steps = n;
         k_lo = chunk * a.plan.cho;
         k_hi = min(k_lo + a.plan.cho, br.own_n[r]);
     }
     if (k_lo >= k_hi) return;
     const int64_t r0 = (int64_t)b * br.S + s0;
+    const int rows = branches * steps;                    // row = step * branches + branch
     float* W_sh = smem;                                   // [N][64]
-    float* A_sh = W_sh + N * BR_HD;                       // [N][68]: states, transposed
+    float* A_sh = W_sh + N * BR_HD;                       // [N][68]: states at step j0, transposed; groups of four slots change places by the channel (state_row's stores)
     float* K_sh = A_sh + N * BA_LD;                       // [64][68]
     float* V_sh = K_sh + BA_TILE * BA_LD;
     float* q_sh = V_sh + BA_TILE * BA_LD;                 // [32][64], scaled to base-2 scores
-    float* P_sh = q_sh + BA_ROWS * BR_HD;                 // [32][68]
+    float* o_sh = q_sh + BA_ROWS * BR_HD;                 // [32][64]
+    float* P_sh = o_sh + BA_ROWS * BR_HD;                 // [32][68]
     float* l2r_sh = P_sh + BA_ROWS * BA_LD;
-    float* m_sh = l2r_sh + ((N + 3) & ~3);
+    float* pw_sh = l2r_sh + ((N + 3) & ~3);               // rho^(step - j0)
+    float* m_sh = pw_sh + ((N + 3) & ~3);
     float* l_sh = m_sh + BA_ROWS;
     float* al_sh = l_sh + BA_ROWS;
     int* v_sh = reinterpret_cast<int*>(al_sh + BA_ROWS);  // the tile's slots, and their ages
     float* dt_sh = reinterpret_cast<float*>(v_sh + BA_TILE);
+    __shared__ unsigned hid_sh[2 * BA_ROWS];              // bits of the tile's slots that a branch has touched
+    __shared__ int pos_sh[BA_ROWS * BR_MAX_NEW];          // the list places that its staged tokens hide from the rows behind them
     const int tid = threadIdx.x;
     const int D = H * BR_HD;
-    const int tau = br.t0[0] + br.len[r0] + j;
+    const int tau = br.t0[0] + br.len[r0] + j0;
+    for (int i = tid; i < branches * (j0 + steps); i += BA_THREADS) {
+        const int branch = i / (j0 + steps), place = i - branch * (j0 + steps);
+        pos_sh[branch * BR_MAX_NEW + place] = (own ? br.st_own : br.st_pos)[br_index(br, r0 + branch, place)];
+    }
     auto slots_of = [&](int k0) {                         // (the first 64 threads)
         const int k = k0 + tid;
         int v = 0;
@@ -84,26 +100,46 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
         v_sh[tid] = v;
         dt_sh[tid] = dt;
     };
+    auto state_row = [&](int k0, int k) {
+        return own ? br.own_state + ((size_t)r0 * br.cap + k0 + k) * N : br.state + ((size_t)b * br.V + v_sh[k]) * N;
+    };
     if (tid < BA_TILE) slots_of(k_lo);
     for (int i = tid; i < N * (BR_HD / 4); i += BA_THREADS)
         *reinterpret_cast<float4*>(W_sh + i * 4) = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
     for (int i = tid; i < N; i += BA_THREADS) l2r_sh[i] = log2f(br.rhos[i]);
-    for (int i = tid; i < rows * BR_HD; i += BA_THREADS)
-        q_sh[i] = ld_dyn_f32(a.q, a.q_dt, ((((size_t)(r0 + (i >> 6))) * n + j) * H + h) * BR_HD + (i & 63)) * BR_SCORE_LOG2;
+    for (int i = tid; i < rows * BR_HD; i += BA_THREADS) {
+        const int row = i >> 6, st = row / branches;
+        q_sh[i] = ld_dyn_f32(a.q, a.q_dt, ((((size_t)(r0 + row - st * branches)) * n + j0 + st) * H + h) * BR_HD + (i & 63)) * BR_SCORE_LOG2;
+        o_sh[i] = 0.f;
+    }
     for (int i = tid; i < BA_ROWS; i += BA_THREADS) { m_sh[i] = -INFINITY; l_sh[i] = 0.f; }
     const int tx = tid & 15, ty = tid >> 4;               // gate: channels 4 tx.., slots 4 ty..
-    const int slot = tid & 63, group = tid >> 6;          // states and scores: a slot, every fourth row; output: a column, every fourth row
-    float o[BA_ROWS / 4];
-#pragma unroll
-    for (int i = 0; i < BA_ROWS / 4; ++i) o[i] = 0.f;
+    const int slot = tid & 63, group = tid >> 6;          // states and scores: a slot, every fourth branch; output: a column, every fourth branch
     for (int k0 = k_lo; k0 < k_hi; k0 += BA_TILE) {
         const int tile = min(BA_TILE, k_hi - k0);
         __syncthreads();                                  // the slots are there
-        {
-            const bool ok = slot < tile;
-            const float dt = dt_sh[slot];
-            const float* row = own ? br.own_state + ((size_t)r0 * br.cap + min(k0 + slot, k_hi - 1)) * N : br.state + ((size_t)b * br.V + v_sh[slot]) * N;
-            for (int c = group; c < N; c += 4) A_sh[c * BA_LD + slot] = ok ? row[c] * exp2f(dt * l2r_sh[c]) : 0.f;
+        if (tid < 2 * branches) {
+            const int words = (int)((br.Kcap + 31) / 32), word = (k0 >> 5) + (tid & 1);
+            hid_sh[tid] = !own && word < words ? br.touched[(size_t)(r0 + (tid >> 1)) * words + word] : 0u;
+        }
+        if (N % 4 == 0) {                                 // whole rows, 16 bytes a thread
+            for (int i = tid; i < BA_TILE * (N / 4); i += BA_THREADS) {
+                const int k = i / (N / 4), c = (i - k * (N / 4)) * 4;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k < tile) {
+                    const float dt = dt_sh[k];
+                    x = *reinterpret_cast<const float4*>(state_row(k0, k) + c);
+                    x.x *= exp2f(dt * l2r_sh[c]); x.y *= exp2f(dt * l2r_sh[c + 1]);
+                    x.z *= exp2f(dt * l2r_sh[c + 2]); x.w *= exp2f(dt * l2r_sh[c + 3]);
+                }
+                float* dst = A_sh + c * BA_LD + (k ^ (((c >> 2) & 7) << 2));
+                dst[0] = x.x; dst[BA_LD] = x.y; dst[2 * BA_LD] = x.z; dst[3 * BA_LD] = x.w;
+            }
+        } else {
+            for (int i = tid; i < BA_TILE * N; i += BA_THREADS) {
+                const int k = i / N, c = i - k * N;
+                A_sh[c * BA_LD + (k ^ (((c >> 2) & 7) << 2))] = k < tile ? state_row(k0, k)[c] * exp2f(dt_sh[k] * l2r_sh[c]) : 0.f;
+            }
         }
         float4 ek[4], ev[4];
 #pragma unroll
@@ -115,119 +151,130 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
                 ev[i] = ld4_dyn_f32(a.Ev, a.e_dt, off);
             }
         }
-        __syncthreads();
-        float acc[4][4];
+        for (int st = 0; st < steps; ++st) {
+            const int j = j0 + st, base = st * branches;
+            for (int c = tid; c < N; c += BA_THREADS) pw_sh[c] = exp2f((float)st * l2r_sh[c]);
+            __syncthreads();                              // states and powers are there, the step before has read K, V and P
+            float acc[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll 8
-        for (int c = 0; c < N; ++c) {
-            const float4 x = *reinterpret_cast<const float4*>(A_sh + c * BA_LD + 4 * ty), w = *reinterpret_cast<const float4*>(W_sh + c * BR_HD + 4 * tx);
-            const float xs[4] = {x.x, x.y, x.z, x.w};
+            for (int c = 0; c < N; ++c) {
+                const float4 x = *reinterpret_cast<const float4*>(A_sh + c * BA_LD + 4 * (ty ^ ((c >> 2) & 7)));
+                float4 w = *reinterpret_cast<const float4*>(W_sh + c * BR_HD + 4 * tx);
+                const float pw = pw_sh[c];
+                w.x *= pw; w.y *= pw; w.z *= pw; w.w *= pw;
+                const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[i][0] = fmaf(xs[i], w.x, acc[i][0]);
+                    acc[i][1] = fmaf(xs[i], w.y, acc[i][1]);
+                    acc[i][2] = fmaf(xs[i], w.z, acc[i][2]);
+                    acc[i][3] = fmaf(xs[i], w.w, acc[i][3]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                acc[i][0] = fmaf(xs[i], w.x, acc[i][0]);
-                acc[i][1] = fmaf(xs[i], w.y, acc[i][1]);
-                acc[i][2] = fmaf(xs[i], w.z, acc[i][2]);
-                acc[i][3] = fmaf(xs[i], w.w, acc[i][3]);
+                float g[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) g[c] = a.silu ? __fdividef(acc[i][c], 1.0f + expf(-acc[i][c])) : acc[i][c];
+                const int at = (4 * ty + i) * BA_LD + 4 * tx;
+                *reinterpret_cast<float4*>(K_sh + at) = make_float4(ek[i].x * g[0], ek[i].y * g[1], ek[i].z * g[2], ek[i].w * g[3]);
+                *reinterpret_cast<float4*>(V_sh + at) = make_float4(ev[i].x * g[0], ev[i].y * g[1], ev[i].z * g[2], ev[i].w * g[3]);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float g[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) g[c] = a.silu ? __fdividef(acc[i][c], 1.0f + expf(-acc[i][c])) : acc[i][c];
-            const int at = (4 * ty + i) * BA_LD + 4 * tx;
-            *reinterpret_cast<float4*>(K_sh + at) = make_float4(ek[i].x * g[0], ek[i].y * g[1], ek[i].z * g[2], ek[i].w * g[3]);
-            *reinterpret_cast<float4*>(V_sh + at) = make_float4(ev[i].x * g[0], ev[i].y * g[1], ev[i].z * g[2], ev[i].w * g[3]);
-        }
-        __syncthreads();
-        if (tid < BA_TILE && k0 + BA_TILE < k_hi) slots_of(k0 + BA_TILE);
-        for (int row0 = group; row0 < rows; row0 += 16) {        // rows row0, row0 + 4, + 8, + 12 against one slot's K
-            const float4* kp = reinterpret_cast<const float4*>(K_sh + slot * BA_LD);
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            __syncthreads();
+            if (st + 1 == steps && tid < BA_TILE && k0 + BA_TILE < k_hi) slots_of(k0 + BA_TILE);
+            for (int br0 = group; br0 < branches; br0 += 16) {        // branches br0, br0 + 4, + 8, + 12 against one slot's K
+                const float4* kp = reinterpret_cast<const float4*>(K_sh + slot * BA_LD);
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                const float4 x = kp[i];
+                for (int i = 0; i < 16; ++i) {
+                    const float4 x = kp[i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (br0 + 4 * e < branches) {
+                            const float4 y = *reinterpret_cast<const float4*>(q_sh + (base + br0 + 4 * e) * BR_HD + 4 * i);
+                            s[e] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[e]))));
+                        }
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (row0 + 4 * e < rows) {
-                        const float4 y = *reinterpret_cast<const float4*>(q_sh + (row0 + 4 * e) * BR_HD + 4 * i);
-                        s[e] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[e]))));
+                    const int branch = br0 + 4 * e;
+                    if (branch < branches) {
+                        bool hide = slot >= tile || ((hid_sh[2 * branch + (slot >> 5)] >> (slot & 31)) & 1u);
+                        for (int i = 0; i < j; ++i) hide |= pos_sh[branch * BR_MAX_NEW + i] == k0 + slot;
+                        P_sh[(base + branch) * BA_LD + slot] = hide ? -INFINITY : s[e];
                     }
                 }
             }
+            __syncthreads();
+            for (int row = base + (tid >> 5); row < base + branches; row += BA_THREADS / 32) {
+                const int lane = tid & 31;
+                float* p = P_sh + row * BA_LD;
+                const float x = p[lane], y = p[lane + 32];
+                float mx = fmaxf(x, y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = row0 + 4 * e;
-                if (row < rows) {
-                    bool hide = slot >= tile;
-                    if (!hide) hide = own ? br_hides_own(br, r0, j, k0 + slot) : br_hides_prefix(br, r0 + row, j, k0 + slot);
-                    P_sh[row * BA_LD + slot] = hide ? -INFINITY : s[e];
+                for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                const float m_old = m_sh[row];
+                const float m_new = fmaxf(m_old, mx);
+                const float ref = m_new == -INFINITY ? 0.f : m_new;      // nothing visible so far: weights are zero all the same
+                const float ex = exp2f(x - ref), ey = exp2f(y - ref);
+                p[lane] = ex;
+                p[lane + 32] = ey;
+                const float sum = warp_sum(ex + ey);
+                if (lane == 0) {
+                    const float alpha = exp2f(m_old - ref);
+                    m_sh[row] = m_new;
+                    l_sh[row] = l_sh[row] * alpha + sum;
+                    al_sh[row] = alpha;
                 }
             }
-        }
-        __syncthreads();
-        for (int row = tid >> 5; row < rows; row += BA_THREADS / 32) {
-            const int lane = tid & 31;
-            float* p = P_sh + row * BA_LD;
-            const float x = p[lane], y = p[lane + 32];
-            float mx = fmaxf(x, y);
+            __syncthreads();
+            if (branches == 1) {                          // the groups share the slots, 16 each; joined in the row's old scores' place
+                float x = 0.f;
 #pragma unroll
-            for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float m_old = m_sh[row];
-            const float m_new = fmaxf(m_old, mx);
-            const float ref = m_new == -INFINITY ? 0.f : m_new;      // nothing visible so far: weights are zero all the same
-            const float ex = exp2f(x - ref), ey = exp2f(y - ref);
-            p[lane] = ex;
-            p[lane + 32] = ey;
-            const float sum = warp_sum(ex + ey);
-            if (lane == 0) {
-                const float alpha = exp2f(m_old - ref);
-                m_sh[row] = m_new;
-                l_sh[row] = l_sh[row] * alpha + sum;
-                al_sh[row] = alpha;
-            }
-        }
-        __syncthreads();
-        if (rows == 1) {                                  // the groups share the slots: 16 each
-            float x = o[0] * al_sh[0];
+                for (int c = 0; c < 16; ++c) x = fmaf(P_sh[base * BA_LD + 16 * group + c], V_sh[(16 * group + c) * BA_LD + slot], x);
+                K_sh[tid] = x;                            // (the scores have been read off K)
+                __syncthreads();
+                if (group == 0)
+                    o_sh[base * BR_HD + slot] = o_sh[base * BR_HD + slot] * al_sh[base] + ((K_sh[slot] + K_sh[64 + slot]) + (K_sh[128 + slot] + K_sh[192 + slot]));
+            } else {
+                for (int br0 = group; br0 < branches; br0 += 16) {
+                    float o[4];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) x = fmaf(P_sh[16 * group + c], V_sh[(16 * group + c) * BA_LD + slot], x);
-            o[0] = x;
-        } else {
-#pragma unroll
-            for (int i = 0; i < BA_ROWS / 4; ++i)
-                if (group + 4 * i < rows) o[i] *= al_sh[group + 4 * i];
-            for (int c = 0; c < BA_TILE; c += 4) {        // (slots past the list: weight 0, value 0)
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = V_sh[(c + e) * BA_LD + slot];
-#pragma unroll
-                for (int i = 0; i < BA_ROWS / 4; ++i) {
-                    if (group + 4 * i < rows) {
-                        const float4 p = *reinterpret_cast<const float4*>(P_sh + (group + 4 * i) * BA_LD + c);
-                        o[i] = fmaf(p.x, v[0], fmaf(p.y, v[1], fmaf(p.z, v[2], fmaf(p.w, v[3], o[i]))));
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = base + br0 + 4 * e;
+                        o[e] = br0 + 4 * e < branches ? o_sh[row * BR_HD + slot] * al_sh[row] : 0.f;
                     }
+#pragma unroll 4
+                    for (int c = 0; c < BA_TILE; c += 4) {                // (slots past the list: weight 0, value 0)
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = V_sh[(c + e) * BA_LD + slot];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (br0 + 4 * e < branches) {
+                                const float4 p = *reinterpret_cast<const float4*>(P_sh + (base + br0 + 4 * e) * BA_LD + c);
+                                o[e] = fmaf(p.x, v[0], fmaf(p.y, v[1], fmaf(p.z, v[2], fmaf(p.w, v[3], o[e]))));
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (br0 + 4 * e < branches) o_sh[(base + br0 + 4 * e) * BR_HD + slot] = o[e];
                 }
             }
+            // (the next step's K, V and P follow the meeting at its start)
         }
     }
     __syncthreads();
     const int part = own ? SP + chunk : chunk;
-    if (rows == 1) {
-        K_sh[tid] = o[0];
-        __syncthreads();
-        if (group > 0) return;
-        o[0] = (K_sh[slot] + K_sh[64 + slot]) + (K_sh[128 + slot] + K_sh[192 + slot]);
-    }
-#pragma unroll
-    for (int i = 0; i < BA_ROWS / 4; ++i) {
-        const int row = group + 4 * i;
-        if (row < rows) {
-            const size_t at = ((((size_t)(r0 + row)) * n + j) * H + h) * (SP + SO) + part;
-            a.po[at * BR_HD + slot] = o[i];
-            if (slot == 0) a.ml[at] = make_float2(m_sh[row], l_sh[row]);
-        }
+    for (int i = tid; i < rows * BR_HD; i += BA_THREADS) {
+        const int row = i >> 6, st = row / branches;
+        const size_t at = ((((size_t)(r0 + row - st * branches)) * n + j0 + st) * H + h) * (SP + SO) + part;
+        a.po[at * BR_HD + (i & 63)] = o_sh[i];
+        if ((i & 63) == 0) a.ml[at] = make_float2(m_sh[row], l_sh[row]);
     }
 }
 
@@ -381,14 +428,17 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     }
 }
 
-// Chunks: enough jobs for about four CTAs an SM, none shorter than a tile of 64 slots nor longer than sixteen.
+// Steps a job: as many as leave it 32 rows.  Chunks: enough jobs for about four CTAs an SM, none shorter than a tile of 64 slots nor
+// longer than sixteen.
 static BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap) {
+    BranchPlan p;
+    p.steps = (int)std::max<int64_t>(1, std::min<int64_t>(n, BA_ROWS / std::min<int64_t>(S, BA_ROWS)));
+    p.JP = (int)((n + p.steps - 1) / p.steps);
     auto tiles = [&](int64_t lists, int64_t slots) {
-        const int64_t all = lists * n * H * ((slots + BA_TILE - 1) / BA_TILE);
+        const int64_t all = lists * H * ((slots + BA_TILE - 1) / BA_TILE);
         return std::min<int64_t>(16, std::max<int64_t>(1, all / (4 * 148)));
     };
-    BranchPlan p;
-    p.chp = (int)(BA_TILE * tiles(B * ((S + BA_ROWS - 1) / BA_ROWS), Kcap));
+    p.chp = (int)(BA_TILE * tiles(B * ((S + BA_ROWS - 1) / BA_ROWS) * p.JP, Kcap));
     p.cho = (int)(BA_TILE * tiles(B * S, cap));
     p.SP = (int)((Kcap + p.chp - 1) / p.chp);
     p.SO = (int)((cap + p.cho - 1) / p.cho);
@@ -397,12 +447,12 @@ static BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_
 
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
     const mbema_branches& br = a.br;
-    const int64_t jobs = br.B * ((br.S + BA_ROWS - 1) / BA_ROWS) * a.plan.SP + br.B * br.S * a.plan.SO;
+    const int64_t jobs = br.B * ((br.S + BA_ROWS - 1) / BA_ROWS) * a.plan.SP * a.plan.JP + br.B * br.S * a.plan.SO;
     if (jobs > 0x7fffffff || a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
     const size_t smem = ba_smem((int)br.N);
     static std::atomic<unsigned long long> done{0};
     MBEMA_CUDA_TRY(allow_smem(k_branch_attend, ba_smem(128), done));
-    k_branch_attend<<<dim3((unsigned)jobs, (unsigned)a.H, (unsigned)a.n), BA_THREADS, smem, st>>>(a);
+    k_branch_attend<<<dim3((unsigned)jobs, (unsigned)a.H), BA_THREADS, smem, st>>>(a);
     return check_launch();
 }
 

@@ -23,6 +23,7 @@ static constexpr int BR_COST_OWN = 2, BR_COST_ONE = 2, BR_COST_BLOCK = 3;
 struct BranchPlan {
     int chp, cho;      // slots a chunk: prefix, own
     int SP, SO;        // chunks that the lists' capacities allow
+    int steps, JP;     // steps a job of a prefix, blocks of steps
 };
 
 // Tensor cores: workers, and the lists in the running sum: prefixes (as blocks of branches read them), then the branches' own.
@@ -66,20 +67,6 @@ __device__ __forceinline__ int branch_worker_of(int total, int workers, int c) {
 __host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + 15) / 16) * N * 32; }
 
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
-
-// Row j of branch r cannot see slot k of the prefix: the branch has touched it, or does so with a staged token before j.
-__device__ __forceinline__ bool br_hides_prefix(const mbema_branches& br, int64_t r, int j, int k) {
-    const int words = (int)((br.Kcap + 31) / 32);
-    if ((br.touched[(size_t)r * words + (k >> 5)] >> (k & 31)) & 1u) return true;
-    for (int i = 0; i < j; ++i)
-        if (br.st_pos[br_index(br, r, i)] == k) return true;
-    return false;
-}
-__device__ __forceinline__ bool br_hides_own(const mbema_branches& br, int64_t r, int j, int u) {
-    for (int i = 0; i < j; ++i)
-        if (br.st_own[br_index(br, r, i)] == u) return true;
-    return false;
-}
 
 // cudaFuncAttributeMaxDynamicSharedMemorySize raised to what every later call needs, once a device (the call costs the host as much
 // as a launch)
