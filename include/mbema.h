@@ -381,16 +381,17 @@ typedef struct mbema_branches {
     uint32_t* st_same;      /* [B,S,max_new] the staged places that hold the same token */
     int32_t* st_new;        /* [B,S,max_new] 1: this place lists a slot that nothing before it lists */
     float* st_state;        /* [B,S,max_new,N] C_q of the staged tokens */
-    void* pre_op;           /* [B,ceil16(Kcap),N] fp16 or NULL (with the next two): prefix states at the first staged step */
-    void* own_op;           /* [B,S,ceil16(cap),N] fp16 or NULL: the same of the own slots; operands of the tensor cores */
-    int32_t* work;          /* [B (ceil(S/16) + S) + 1, 2] or NULL: running sum of the lists' units, by which the work is dealt, and lengths */
+    void* pre_op;           /* [B,ceil128(Kcap),N] fp16 or NULL (with the next three): prefix states at the first staged step, */
+    void* own_op;           /* [B,S,ceil128(cap),N] fp16 or NULL: the same of the own slots; operands of the tensor cores, 16-byte aligned */
+    int32_t* work;          /* [B (ceil(S/16) + S) + 2, 2] or NULL: running sums of the lists' units, by which the work is dealt, and lengths */
+    int32_t* status;        /* [1] or NULL: status word of the tensor-core attends (see the conventions above) */
     int32_t* overflow;      /* [1] */
     int64_t B, S, V, N, Kcap, cap, max_new;
 } mbema_branches;
 int mbema_branches_init(const mbema_branches* br, int64_t t_now, const int32_t* t_now_dev, void* stream);
 int mbema_branches_extend(const mbema_branches* br, const int64_t* tok, int64_t n, int64_t n_pending, float* C_q, void* stream);
 int mbema_branches_keep(const mbema_branches* br, const int64_t* counts, int64_t n_pending, void* stream);
-size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode);
+size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode);
 int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
                           const float* W_pe, void* O, int64_t n, int64_t H, int64_t hd, int64_t V_total, int flags, int mode,
                           void* workspace, size_t workspace_bytes, void* stream);

@@ -23,7 +23,7 @@ class BranchesStruct(ctypes.Structure):
     """mbema_branches of include/mbema.h."""
     _fields_ = [(name, _vp) for name in (
         "rhos", "state", "last_t", "active", "n_active", "pos", "t0", "len", "own_n", "own_new", "own_slot", "own_t", "own_state",
-        "touched", "st_tok", "st_own", "st_pos", "st_same", "st_new", "st_state", "pre_op", "own_op", "work", "overflow")] + [
+        "touched", "st_tok", "st_own", "st_pos", "st_same", "st_new", "st_state", "pre_op", "own_op", "work", "status", "overflow")] + [
         (name, _i64) for name in ("B", "S", "V", "N", "Kcap", "cap", "max_new")]
 
 
@@ -65,7 +65,7 @@ SIGNATURES = {
     "mbema_branches_init": (_i32, [_vp, _i64, _vp, _vp]),
     "mbema_branches_extend": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "mbema_branches_keep": (_i32, [_vp, _vp, _i64, _vp]),
-    "mbema_branches_attend_workspace_bytes": (_sz, [_i64] * 7 + [_i32]),
+    "mbema_branches_attend_workspace_bytes": (_sz, [_i64] * 6 + [_i32]),
     "mbema_branches_attend": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
     "mbema_branches_adopt": (_i32, [_vp, _vp, _i64, _vp]),
     "mbema_verify_drafts": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),

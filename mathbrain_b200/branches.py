@@ -58,9 +58,9 @@ class Branches:
             st_new=torch.empty(B, S, max_new, **i32), st_state=torch.empty(B, S, max_new, N, **f32), overflow=torch.empty(1, **i32))
         self._tensor_cores = N in (64, 128)
         if self._tensor_cores:
-            self._hold.update(pre_op=torch.empty(B, (Kcap + 15) // 16 * 16, N, dtype=torch.float16, device=dev),
-                              own_op=torch.empty(B, S, (cap + 15) // 16 * 16, N, dtype=torch.float16, device=dev),
-                              work=torch.empty(B * ((S + 15) // 16 + S) + 1, 2, **i32))
+            self._hold.update(pre_op=torch.empty(B, (Kcap + 127) // 128 * 128, N, dtype=torch.float16, device=dev),
+                              own_op=torch.empty(B, S, (cap + 127) // 128 * 128, N, dtype=torch.float16, device=dev),
+                              work=torch.empty(B * ((S + 15) // 16 + S) + 2, 2, **i32), status=torch.zeros(1, **i32))
         self._c = _lib.BranchesStruct(**{k: _ptr(t) for k, t in self._hold.items()}, B=B, S=S, V=V, N=N, Kcap=Kcap, cap=cap,
                                       max_new=max_new)
         self._ref = ctypes.byref(self._c)
@@ -170,7 +170,7 @@ class Branches:
                                   % (q.dtype, E_k.dtype, self.N))
         code = _lib.MODE_TC_BF16 if fits and mode != "fp32" else _lib.MODE_FP32
         flags = (_lib.FLAG_SILU if use_silu else 0) | (_lib.FLAG_LISTED_ONLY if listed_only else 0)
-        need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, self.N, n, H, self.prefix.cap, self.capacity, code)
+        need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, n, H, self.prefix.cap, self.capacity, code)
         return q_dt, e_dt, n, H, int(self.V if V_total is None else V_total), flags, code, need
 
     def _attend(self, q, E_k, E_v, W_pe, plan):
@@ -210,6 +210,11 @@ class Branches:
     def lengths(self):
         """Kept tokens of the branches, int32 [B, S] on the GPU."""
         return self._hold["len"]
+
+    def device_status(self):
+        """Status word of the tensor-core attends of these branches (synchronises): 0 = ok, else a bounded wait inside a kernel
+        gave up and the outputs since then are invalid."""
+        return int(self._hold["status"].item()) if self._tensor_cores else 0
 
     def check_overflow(self):
         """Synchronises; raises if a list overflowed, a token was out of range, or adopt was given a branch or a step that it

@@ -356,23 +356,30 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     size_t p0, q0, p_step, q_step;
     if constexpr (PIECES) {
         const int2* work = reinterpret_cast<const int2*>(br.work);
-        const int64_t own = a.n_pre + r;
-        const int64_t pre = a.rows == 1 ? b : (int64_t)b * a.blocks + s / a.rows;
-        const int total = work[a.n_pre + br.B * br.S].x, workers = branch_workers(total, (int)a.max_workers);
-        auto pieces = [&](int64_t list, int cost, int& first) {
-            const int lo = work[list].x, hi = work[list + 1].x;
-            if (hi == lo) return 0;
-            first = branch_worker_of(total, workers, lo);
-            return branch_worker_of(total, workers, hi - cost) - first + 1;
-        };
-        int wp = 0, wq = 0;
-        np = pieces(pre, a.cost_pre, wp);
-        nq = pieces(own, BR_COST_OWN, wq);
         const size_t each = (size_t)n * H, at = (size_t)j * H + h;
-        p_step = a.rows * each;
+        auto pieces = [&](const int2* sum, int lists, int list, int most, int least, int& first) {
+            const int lo = sum[list].x, hi = sum[list + 1].x, total = sum[lists].x;
+            first = 0;
+            if (hi == lo) return 0;
+            const int workers = branch_workers(total, most, least);
+            first = branch_worker_of(total, workers, lo);
+            return branch_worker_of(total, workers, hi - 1) - first + 1;
+        };
+        int first;
+        if (br.S == 1) {
+            np = 4 * pieces(work + a.row_work, a.row_lists, b, a.row_workers, 1, first);
+            p_step = each;
+            p0 = (size_t)a.row_part0 + (size_t)(b + first) * 4 * each + at;
+        } else {
+            const int list = b * a.blocks + s / BR_BLOCK;
+            np = pieces(work, a.n_pre, list, a.pre_workers, BR_LEAST_UNITS, first);
+            p_step = BR_BLOCK * each;
+            p0 = ((size_t)(list + first) * BR_BLOCK + s % BR_BLOCK) * each + at;
+        }
+        const int list = (br.S == 1 ? (int)br.B : 0) + (int)r;
+        nq = 4 * pieces(work + a.row_work, a.row_lists, list, a.row_workers, 1, first);
         q_step = each;
-        p0 = ((size_t)(pre + wp) * a.rows + (a.rows == 1 ? 0 : s % a.rows)) * each + at;
-        q0 = (size_t)(a.own_piece0 + r + wq) * each + at;
+        q0 = (size_t)a.row_part0 + (size_t)(list + first) * 4 * each + at;
     } else {
         const int SP = a.plan.SP, SO = a.plan.SO;
         np = (na + a.plan.chp - 1) / a.plan.chp;
@@ -471,29 +478,33 @@ static bool plan_sizes_ok(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kc
     return B >= 0 && S >= 1 && n >= 1 && n <= BR_MAX_NEW && H >= 1 && Kcap >= 1 && cap >= 1;
 }
 
-// number of partials of a call
-static int64_t partials(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode, BranchArgs* a) {
+// number of partials of a call, and how it is dealt
+static int64_t partials(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode, BranchArgs* a) {
     if (mode != MBEMA_MODE_TC_BF16) {
         const BranchPlan p = branch_plan(B, S, n, H, Kcap, cap);
         if (a) a->plan = p;
         return B * S * n * H * (p.SP + p.SO);
     }
-    const BranchShape p = branch_shape(B, S, N, n, H);
-    const int64_t workers = (int64_t)p.ctas * p.IG, n_pre = B * p.blocks, own0 = (n_pre + workers) * p.rows;
+    const BranchShape p = branch_shape(S, n, H);
+    const BranchRows q = branch_rows(n, H);
+    const int64_t n_pre = S > 1 ? B * p.blocks : 0, pre_workers = (int64_t)p.ctas * p.IG;
+    const int64_t rows = (S == 1 ? B : 0) + B * S, row_workers = (int64_t)q.ctas * q.IG;
+    const int64_t part0 = n_pre ? (n_pre + pre_workers) * BR_BLOCK * n * H : 0;
     if (a) {
-        a->n_pre = n_pre;
-        a->own_piece0 = own0;
-        a->max_workers = workers;
-        a->rows = p.rows;
+        a->n_pre = (int)n_pre;
         a->blocks = p.blocks;
-        a->cost_pre = p.rows == 1 ? BR_COST_ONE : BR_COST_BLOCK;
+        a->pre_workers = (int)pre_workers;
+        a->row_lists = (int)rows;
+        a->row_work = (int)n_pre + 1;
+        a->row_workers = (int)row_workers;
+        a->row_part0 = part0;
     }
-    return (own0 + B * S + workers) * n * H;
+    return part0 + (rows + row_workers) * 4 * n * H;
 }
 
-extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
-    if (!plan_sizes_ok(B, S, n, H, Kcap, cap) || N < 1) return 0;
-    return align_up((size_t)partials(B, S, N, n, H, Kcap, cap, mode, nullptr) * (2 + BR_HD) * 4, 256) + 256;
+extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
+    if (!plan_sizes_ok(B, S, n, H, Kcap, cap)) return 0;
+    return align_up((size_t)partials(B, S, n, H, Kcap, cap, mode, nullptr) * (2 + BR_HD) * 4, 256) + 256;
 }
 
 extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
@@ -507,8 +518,8 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     if (!q || !E_k || !E_v || !W_pe || !O || !workspace || !br->state || !br->active || !br->own_state || !br->st_state) return MBEMA_ERR_NULL;
     if ((q_dtype != MBEMA_F32 && q_dtype != MBEMA_BF16) || (e_dtype != MBEMA_F32 && e_dtype != MBEMA_BF16)) return MBEMA_ERR_DTYPE;
     if (((uintptr_t)q | (uintptr_t)E_k | (uintptr_t)E_v | (uintptr_t)W_pe | (uintptr_t)O | (uintptr_t)workspace) & 15) return MBEMA_ERR_ALIGN;
-    if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, br->N, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
-    if (mode == MBEMA_MODE_TC_BF16 && (!br->pre_op || !br->own_op || !br->work)) return MBEMA_ERR_NULL;
+    if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
+    if (mode == MBEMA_MODE_TC_BF16 && (!br->pre_op || !br->own_op || !br->work || !br->status)) return MBEMA_ERR_NULL;
     BranchArgs a{};
     a.br = *br;
     a.q = q; a.Ek = E_k; a.Ev = E_v; a.W = W_pe; a.O = O;
@@ -516,10 +527,17 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     a.v_total = (float)V_total;
     a.silu = (flags & MBEMA_FLAG_SILU) ? 1 : 0;
     a.listed_only = (flags & MBEMA_FLAG_LISTED_ONLY) ? 1 : 0;
-    const int64_t parts = partials(br->B, br->S, br->N, n, H, br->Kcap, br->cap, mode, &a);
+    const int64_t parts = partials(br->B, br->S, n, H, br->Kcap, br->cap, mode, &a);
     a.po = reinterpret_cast<float*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.po + (size_t)parts * BR_HD);
+    cudaStream_t st = (cudaStream_t)stream;
     const bool tc = mode == MBEMA_MODE_TC_BF16;
-    int rc = tc ? launch_branch_attend_tc(a, branch_shape(br->B, br->S, br->N, n, H), (cudaStream_t)stream) : launch_branch_attend_fp32(a, (cudaStream_t)stream);
-    return rc != MBEMA_OK ? rc : launch_branch_merge(a, tc, (cudaStream_t)stream);
+    int rc = MBEMA_OK;
+    if (tc) {
+        if (br->S > 1) rc = launch_branch_attend_tc(a, branch_shape(br->S, n, H), st);
+        if (rc == MBEMA_OK) rc = launch_branch_rows(a, branch_rows(n, H), br->S > 1, st);
+    } else {
+        rc = launch_branch_attend_fp32(a, st);
+    }
+    return rc != MBEMA_OK ? rc : launch_branch_merge(a, tc, st);
 }

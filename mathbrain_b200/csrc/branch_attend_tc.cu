@@ -1,10 +1,12 @@
-// Attention of the rows of a decode state's branches on the tensor cores (mbema_branches_attend, MBEMA_MODE_TC_BF16).
+// Attention over the prefix of sequences that several branches share, on the tensor cores (mbema_branches_attend,
+// MBEMA_MODE_TC_BF16).  (The branches' own slots, and the prefix of a single branch: branch_rows_tc.cu.)
 //
 // The states that the rows of one call see differ from the ones at the call's first step by rho^j alone, so the operand copies
 // (fp16, made once by mbema_branches_extend for all layers and steps) are the A operands of every step and rho^j goes into W:
 //     gate(j) = SiLU(A . (rho^j * W)),   16 slots x 64 channels of a head to a warp (mma.sync m16n8k16, fp32 accumulators).
-// A warp keeps its step's W in registers and its accumulators in the layout that the next operand needs: a thread holds the same
-// 16 channels of slots g and g + 8 in the gate, in the 16-byte pieces that it reads of the E rows, and in q and O.
+// The accumulators, K = E_k gate and V = E_v gate stay in registers: the layout of the gate's accumulators is the layout of K as the
+// operand of q.K for sixteen branches, V's 8 x 8 blocks are transposed in registers for P.V, and a thread holds the same 16 channels
+// of slots g and g + 8 in the gate, in the 16-byte pieces that it reads of the E rows, and in q and O.
 //
 // Work is dealt in units of 16 slots: mbema_branches_extend leaves the running sum of all lists' units, every worker (one warp, or
 // the warps of several steps together) takes an equal stretch of it and walks it without a stop; a list is cut where a stretch
@@ -17,6 +19,7 @@
 
 namespace mbema {
 
+static constexpr int WARPS = 8;                   // of 255 registers: W (64), accumulators (32), sixteen rows' o (32) and q (16), E rows
 static constexpr int BT_LDW = 70;                 // floats a row of the staged W slice, which starts up to 6 floats in (w_row)
 static constexpr float BT_W_SCALE = 64.0f;        // undoes BR_OP_SCALE
 
@@ -104,8 +107,7 @@ __device__ __forceinline__ void build_W(uint32_t dst, const float* W_sh, const f
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * 512 + lane * 16), "r"(x[0]), "r"(x[1]), "r"(y[0]), "r"(y[1]) : "memory");
     }
 }
-// A warp's copy of them in registers (64 a thread for 64 channels): twelve rows of sixteen bytes fewer to read a unit, for eight warps
-// an SM instead of sixteen.
+// A warp's copy of them in registers (64 a thread for 64 channels; 128 channels have no room for it).
 template <int KS, int I = 0>
 __device__ __forceinline__ void read_W(uint4 (&w)[KS * 4], uint32_t at) {
     if constexpr (I < KS * 4) {
@@ -185,7 +187,7 @@ __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
     }
 }
 
-// A list of slots: the prefix of a sequence as 16 of its branches read it (all one, for one branch), or a branch's own slots.
+// The prefix of a sequence as a block of its branches reads it.
 struct List {
     const int* slots;
     const char* op;           // operands, 16 slots after 16 slots
@@ -194,131 +196,9 @@ struct List {
 
 __device__ __forceinline__ List get_list(const BranchArgs& a, int x, int count) {
     const mbema_branches& br = a.br;
-    List t;
-    t.count = count;
-    if (x < (int)a.n_pre) {
-        const int b = x / a.blocks;
-        t.slots = br.active + (size_t)b * br.Kcap;
-        t.op = reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N);
-    } else {
-        const int r = x - (int)a.n_pre;
-        t.slots = br.own_slot + (size_t)r * br.cap;
-        t.op = reinterpret_cast<const char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, br.N);
-    }
-    return t;
+    const int b = x / a.blocks;
+    return List{br.active + (size_t)b * br.Kcap, reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N), count};
 }
-
-// bit i: slot k0 + i (i < 16) is hidden; touched: word of the branch's bits (prefix), staged: lane i holds the list place that staged
-// token i < j hides, or -1
-__device__ __forceinline__ unsigned hidden16(unsigned touched, int k0, int staged, bool any_staged, int count) {
-    unsigned m = (touched >> (k0 & 31)) & 0xffffu;
-    if (any_staged) {
-        const unsigned d = (unsigned)(staged - k0);
-        m |= __reduce_or_sync(0xffffffffu, d < 16u ? 1u << d : 0u);
-    }
-    if (count - k0 < 16) m |= 0xffffffffu << (count - k0);
-    return m;
-}
-
-// One partial of a warp: the eight quads' (m, l, o[16]) joined.  A lane is left with o of channels 32 (x / 4) + 8 t + 2 (x % 4) + {0, 1},
-// x = g with its bits reversed in place: see quad_columns.
-__device__ __forceinline__ void join_quads(float& m, float& l, float (&o)[16], float2& out) {
-    float M = m;
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-    const float w = M == -INFINITY ? 0.f : exp2f(m - M);
-    l *= w;
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] *= w;
-    const bool b0 = lane & 4, b1 = lane & 8, b2 = lane & 16;
-    float x[8], y[4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {          // keep the half that bit 0 of g names
-        const float send = b0 ? o[i] : o[8 + i], keep = b0 ? o[8 + i] : o[i];
-        x[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float send = b1 ? x[i] : x[4 + i], keep = b1 ? x[4 + i] : x[i];
-        y[i] = keep + __shfl_xor_sync(0xffffffffu, send, 8);
-    }
-    const float s0 = b2 ? y[0] : y[2], s1 = b2 ? y[1] : y[3], k0 = b2 ? y[2] : y[0], k1 = b2 ? y[3] : y[1];
-    out.x = k0 + __shfl_xor_sync(0xffffffffu, s0, 16);
-    out.y = k1 + __shfl_xor_sync(0xffffffffu, s1, 16);
-    m = M;
-}
-// first of the two head channels that join_quads leaves in this lane
-__device__ __forceinline__ int quad_columns(int lane) {
-    const int t = lane & 3, i = ((lane >> 2) & 1) * 8 + ((lane >> 3) & 1) * 4 + ((lane >> 4) & 1) * 2;    // index into o[16]
-    return 32 * (i >> 3) + 8 * t + (i & 7);
-}
-
-// ---------------------------------------------------------------------------------------------------------------------------
-// One row: q.K and P.V on the CUDA cores, in fp32, straight from the gate's accumulators.  A quad of lanes has its own running
-// maximum and sums, joined at the end of the piece.
-// ---------------------------------------------------------------------------------------------------------------------------
-struct OneRow {
-    float m, l, o[16], q[16];
-    int staged;
-    __device__ __forceinline__ void start(const BranchArgs& a, int64_t r, bool own, int j, int h, int lane) {
-        uint32_t x[8];
-        load_q(x, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { q[2 * i] = bf_lo(x[i]) * BR_SCORE_LOG2; q[2 * i + 1] = bf_hi(x[i]) * BR_SCORE_LOG2; }
-        staged = -1;
-        if (lane < j) staged = (own ? a.br.st_own : a.br.st_pos)[br_index(a.br, r, lane)];
-        m = -INFINITY;
-        l = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = 0.f;
-    }
-    __device__ __forceinline__ void unit(float (&acc)[8][4], uint32_t at_lo, uint32_t at_hi, unsigned hide, int g) {
-        uint32_t e0[8], e1[8];
-        load_E<0>(e0, e1, at_lo, at_hi);
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-            s0 = fmaf(bf_lo(e0[nt]) * q[2 * nt], acc[nt][0], s0);
-            s1 = fmaf(bf_hi(e0[nt]) * q[2 * nt + 1], acc[nt][1], s1);
-            s2 = fmaf(bf_lo(e1[nt]) * q[2 * nt], acc[nt][2], s2);
-            s3 = fmaf(bf_hi(e1[nt]) * q[2 * nt + 1], acc[nt][3], s3);
-        }
-        load_E<2048>(e0, e1, at_lo, at_hi);
-        s0 += s1;
-        s2 += s3;
-        s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
-        s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
-        const float x0 = (hide >> g) & 1u ? -INFINITY : s0, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2;
-        const float m_new = fmaxf(m, fmaxf(x0, x1));
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        const float p0 = ex2(x0 - ref), p1 = ex2(x1 - ref);
-        if (__any_sync(0xffffffffu, m_new > m)) {
-            const float alpha = ex2(m - ref);
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= alpha;
-        }
-        m = m_new;
-        l += p0 + p1;
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {      // (a value that is not finite stays in a row that hides it: the same slot is listed as the branch's own)
-            o[2 * nt] = fmaf(p0 * acc[nt][0], bf_lo(e0[nt]), fmaf(p1 * acc[nt][2], bf_lo(e1[nt]), o[2 * nt]));
-            o[2 * nt + 1] = fmaf(p0 * acc[nt][1], bf_hi(e0[nt]), fmaf(p1 * acc[nt][3], bf_hi(e1[nt]), o[2 * nt + 1]));
-        }
-    }
-    __device__ __forceinline__ void leave(const BranchArgs& a, int64_t piece, int j, int h, int lane) {
-        float2 out;
-        join_quads(m, l, o, out);
-        const size_t at = ((size_t)piece * a.n + j) * a.H + h;
-        *reinterpret_cast<float2*>(a.po + at * BR_HD + quad_columns(lane)) = out;
-        if (lane == 0) a.ml[at] = make_float2(m, l);
-    }
-};
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Sixteen branches at a time: q.K and P.V as products too.  K goes in as two bf16 terms (its rounding would come back
@@ -449,22 +329,9 @@ struct SixteenRows {
     }
 };
 
-// Where a stretch begins: the first list whose units reach cost c, by 32 samples of the running sum at a time.
-__device__ __forceinline__ int find_list(const int2* work, int lists, int c, int lane) {
-    int lo = 0, hi = lists;                       // work[lo].x <= c < work[hi].x
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
-        const int at = lo + (lane + 1) * step;
-        const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at].x <= c);
-        lo += __popc(below) * step;
-        hi = min(hi, lo + step);
-    }
-    return lo;
-}
-
 // grid: x = CTAs that share the work, y = head, z = block of JW steps.  The CTA's warps are IG workers of JW warps each; warp w takes
-// step z JW + w % JW of worker w / JW.  ROWS: branches that read a prefix together (1 or 16).
-template <int KS, int ROWS, int WARPS, int STAGES>
+// step z JW + w % JW of worker w / JW.
+template <int KS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int JW, int IG) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_l2r[16 * KS];
@@ -474,7 +341,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.H * BR_HD;
     br_let_next_kernel_start();
-    const int lists = (int)(a.n_pre + br.B * br.S), n_pre = (int)a.n_pre;
+    const int lists = a.n_pre;
     const int2* work = reinterpret_cast<const int2*>(br.work);
     const int total = work[lists].x;
     // behind the ring the steps' fragments of W, then (or in the ring, where there is no room) the staged slice of W
@@ -487,7 +354,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         dst[1] = make_float2(x.z, x.w);
     }
     for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = log2f(br.rhos[i]);
-    const int workers = branch_workers(total, (int)gridDim.x * IG);
+    const int workers = branch_workers(total, (int)gridDim.x * IG, BR_LEAST_UNITS);
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;
     const int steps = min(JW, a.n - (int)blockIdx.z * JW);       // of this CTA
@@ -501,27 +368,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     // producer: `left` units of list px from slot pk on; the ids of its next unit are a unit ahead
     int px = 0, pk = 0, left = 0;
     List pl = {nullptr, nullptr, 0};
-    auto units_to = [&](int from, int to, int cost) { return (min(to, c_end) - from + cost - 1) / cost; };
-    auto cost_of = [&](int list) { return list < n_pre ? a.cost_pre : BR_COST_OWN; };
     auto next_list = [&](int& list, int& count) {                // the next list with units in this stretch: their number, or 0
         for (;;) {
             const int2 at = work[++list];
             if (at.x >= c_end) return 0;
             const int hi = work[list + 1].x;
             count = at.y;
-            if (hi > at.x) return units_to(at.x, hi, cost_of(list));
+            if (hi > at.x) return min(hi, c_end) - at.x;
         }
     };
     if (works) {
         const int c0 = branch_cut(total, workers, me);
         px = find_list(work, lists, c0, lane);
         const int2 lo = work[px];
-        const int hi = work[px + 1].x, cost = cost_of(px), skip = (c0 - lo.x + cost - 1) / cost;     // units of the list before this stretch
-        int count = lo.y;
-        pk = skip * 16;
-        left = max(units_to(lo.x + skip * cost, hi, cost), 0);
-        if (left == 0) { pk = 0; left = next_list(px, count); }
-        pl = get_list(a, px, count);
+        pk = (c0 - lo.x) * 16;
+        left = min(work[px + 1].x, c_end) - c0;
+        pl = get_list(a, px, lo.y);
     }
     int x = px;                                                  // consumer: c_left units of list x from slot k0 on
     int k0 = pk, c_left = left, count = pl.count;
@@ -575,36 +437,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     if (!works) return;
     if (in_ring) fill_ring();
     const uint32_t w_at = w_all + jj * KS * 2048 + lane * 16;
-    constexpr bool W_REGS = KS == 4 && WARPS == 8;
+    constexpr bool W_REGS = KS == 4;
     uint4 w[KS * 4];
     if constexpr (W_REGS) read_W<KS>(w, w_at);
-    OneRow one;
     SixteenRows many;
-    bool fresh = true, own = false, single = true;
+    bool fresh = true;
     int rows = 1;
-    const uint32_t* bits = nullptr;                              // one branch's bits over the prefix
     uint32_t at = ring;
     const uint32_t lane_lo = g * 128 + ((t ^ ((g & 1) << 2)) << 4), lane_hi = lane_lo ^ 64u;
     for (;;) {
         if (fresh) {
-            own = x >= n_pre;
-            single = ROWS == 1 || own;
-            if (single) {
-                const int64_t r = own ? x - n_pre : x;
-                one.start(a, r, own, j, h, lane);
-                bits = own ? nullptr : br.touched + (size_t)r * ((br.Kcap + 31) / 32);
-            } else if constexpr (ROWS > 1) {
-                const int b = x / a.blocks, s0 = (x - b * a.blocks) * ROWS;
-                rows = min(ROWS, (int)br.S - s0);
-                many.start(a, (int64_t)b * br.S + s0, rows, j, h, lane);
-            }
+            const int b = x / a.blocks, s0 = (x - b * a.blocks) * BR_BLOCK;
+            rows = min(BR_BLOCK, (int)br.S - s0);
+            many.start(a, (int64_t)b * br.S + s0, rows, j, h, lane);
             fresh = false;
         }
-        unsigned touched0 = 0u, touched1 = 0u;
-        if (single && bits) touched0 = bits[k0 >> 5];
-        if constexpr (ROWS > 1) {
-            if (!single) { touched0 = many.hid0[k0 >> 5]; touched1 = many.hid1[k0 >> 5]; }
-        }
+        const unsigned touched0 = many.hid0[k0 >> 5], touched1 = many.hid1[k0 >> 5];
         cp_wait<STAGES - 2>();
         if (steps == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(ig + 1), "r"(steps * 32) : "memory");
@@ -617,14 +465,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
             else gate<KS>(acc, A, w_at);
         }
         apply_gate(acc, a.silu);
-        if (single) one.unit(acc, at + lane_lo, at + lane_hi, hidden16(touched0, k0, one.staged, j > 0, count), g);
-        else if constexpr (ROWS > 1) many.unit(a, acc, at + lane_lo, at + lane_hi, k0, count, touched0, touched1, j, t);
+        many.unit(a, acc, at + lane_lo, at + lane_hi, k0, count, touched0, touched1, j, t);
         at += Unit::BYTES;
         if (at == ring_end) at = ring;
         k0 += 16;
         if (--c_left == 0) {                                     // end of the list or of the stretch
-            if (single) one.leave(a, own ? a.own_piece0 + (x - n_pre) + me : (int64_t)x + me, j, h, lane);
-            else if constexpr (ROWS > 1) many.leave(a, (int64_t)x + me, rows, j, h, lane);
+            many.leave(a, (int64_t)x + me, rows, j, h, lane);
             c_left = next_list(x, count);
             if (c_left == 0) break;
             k0 = 0;
@@ -648,22 +494,16 @@ static void steps_and_workers(int n, int warps, int& JW, int& IG) {
     IG = warps / JW;
 }
 
-// Single rows: sixteen warps with W in shared memory (64 sequences with 6 rows 486 us; twelve with W in registers 566, eight 645), for
-// 128 channels the twelve whose rings fit.  Sixteen rows: eight, with W in registers (64 samples 25 us; twelve 31).
-static int tc_warps(int64_t S, int64_t N) { return S > 1 ? 8 : N == 64 ? 16 : 12; }
-
-BranchShape branch_shape(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H) {
+BranchShape branch_shape(int64_t S, int64_t n, int64_t H) {
     BranchShape p;
-    p.rows = S == 1 ? 1 : BR_BLOCK;
-    p.blocks = (int)((S + p.rows - 1) / p.rows);
-    p.warps = tc_warps(S, N);
-    steps_and_workers((int)n, p.warps, p.JW, p.IG);
+    p.blocks = (int)((S + BR_BLOCK - 1) / BR_BLOCK);
+    steps_and_workers((int)n, WARPS, p.JW, p.IG);
     p.zb = (int)((n + p.JW - 1) / p.JW);
     p.ctas = (int)std::max<int64_t>(1, 148 / (H * p.zb));       // one CTA an SM, dealt to the heads and blocks of steps
     return p;
 }
 
-template <int KS, int ROWS, int WARPS, int STAGES>
+template <int KS, int STAGES>
 static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     const size_t w_sh = align_up(((size_t)16 * KS * BT_LDW + 8) * 4, 128), w_all = (size_t)p.JW * KS * 2048;
     const size_t ring = (size_t)p.IG * STAGES * UnitLayout<KS>::BYTES, most = 232448 - 1024;
@@ -672,15 +512,14 @@ static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     a.w_offset = in_ring ? 0 : a.ring_bytes + (int)w_all;
     const size_t smem = a.ring_bytes + w_all + (in_ring ? 0 : w_sh);
     static std::atomic<unsigned long long> done{0};
-    MBEMA_CUDA_TRY(allow_smem(k_branch_tc<KS, ROWS, WARPS, STAGES>, most, done));
-    k_branch_tc<KS, ROWS, WARPS, STAGES><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st>>>(a, p.JW, p.IG);
+    MBEMA_CUDA_TRY(allow_smem(k_branch_tc<KS, STAGES>, most, done));
+    k_branch_tc<KS, STAGES><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st>>>(a, p.JW, p.IG);
     return check_launch();
 }
 
 int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
-    if (a.br.N == 64) return p.rows > 1 ? launch_tc<4, BR_BLOCK, 8, 4>(a, p, st) : launch_tc<4, 1, 16, 2>(a, p, st);
-    return p.rows > 1 ? launch_tc<8, BR_BLOCK, 8, 3>(a, p, st) : launch_tc<8, 1, 12, 2>(a, p, st);
+    return a.br.N == 64 ? launch_tc<4, 4>(a, p, st) : launch_tc<8, 3>(a, p, st);
 }
 
 }  // namespace mbema

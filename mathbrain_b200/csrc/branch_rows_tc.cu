@@ -1,0 +1,469 @@
+// Attention of single rows over lists of slots on tcgen05 (mbema_branches_attend, MBEMA_MODE_TC_BF16): the branches' own slots, and the
+// prefix of a sequence with one branch.
+//
+// A tile is 128 slots of a list; its operands lie in memory as the gate product wants them in shared memory (mbema_branches_extend),
+// so one bulk copy fetches them, and rho^j of staged step j is in that step's W:  gate(j) = SiLU(A (rho^j W)),  M = 128 slots, N = 64
+// channels of one head, accumulators in TMEM.  A thread owns a slot and all 64 channels: its score is a sum in the thread, it keeps its
+// own running maximum, sum and o[64] over the tiles of a list, and only where the list (or the worker's stretch) ends do the 32 lanes of
+// a warp join.  The gate goes back to TMEM between the two passes (q.K; P.V), since 64 of its values beside o[64] do not fit the registers.
+//
+// Roles: three epilogue groups of four warps; two warps gather the E_k and E_v rows (cp.async, mbarrier arrivals), one lane copies the
+// operands and issues the products.  With one step the groups are workers with stretches of their own, a tile each in turn; with
+// two or three steps they take the same tile, a step each.
+// Bound by the FMA and ALU instructions of the two passes (eight a slot, channel and step, one MUFU among them).
+#include <algorithm>
+
+#include "branches.cuh"
+#include "sm100_ptx.cuh"
+
+namespace mbema {
+namespace brows {
+
+using namespace ptx;
+
+static constexpr int TILE = BR_TILE, GROUPS = 3, EPI_WARPS = 4 * GROUPS, THREADS = (EPI_WARPS + 4) * 32;
+static constexpr int WARP_K = EPI_WARPS, WARP_V = EPI_WARPS + 1, WARP_MMA = EPI_WARPS + 2;
+// setmaxnreg: 12 * 32 * 152 (epilogue) + 4 * 32 * 56 (producers) = the launch allocation 512 * 128
+static constexpr float W_SCALE = 64.0f;           // undoes BR_OP_SCALE
+
+template <int ATOMS>                               // of 64 state channels
+struct Smem {
+    static constexpr int A_STAGES = 2, E_STAGES = ATOMS == 1 ? 5 : 3, OP_BYTES = ATOMS * 16384;
+    static constexpr int EK = A_STAGES * OP_BYTES, EV = EK + 16384, E_STAGE = 32768;
+    static constexpr int B = EK + E_STAGES * E_STAGE, B_STEP = ATOMS * 8192, Q = B + GROUPS * B_STEP, BARS = Q + EPI_WARPS * 256, BYTES = BARS + 256 + 1024;
+};
+
+struct Bars {
+    uint64_t a_full[2];            // operands have landed                                     (1 arrival and their bytes)
+    uint64_t a_empty[2];           // every product that reads them has completed              (1 commit)
+    uint64_t e_full[5];            // E rows have landed                                       (64: the lanes of both gathering warps)
+    uint64_t e_empty[5];           // every epilogue warp of the tile has read them            (4 a step)
+    uint64_t acc_full[GROUPS][2];  // gate product of a group's tile done                      (1 commit)
+    uint64_t acc_empty[GROUPS][2]; // the group's warps have read its accumulators a second time (4)
+    uint64_t drain;                // every product has completed (teardown)                   (1 commit)
+    uint32_t tmem_base;
+    int abort_flag;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+struct Cursor {                    // a worker's place in the lists
+    int list, left, k, count, end; // left tiles of this list from slot k on; end: of the stretch, in tiles
+    __device__ __forceinline__ void start(const int2* work, int lists, int total, int workers, int me, int lane) {
+        const int c0 = branch_cut(total, workers, me);
+        end = branch_cut(total, workers, me + 1);
+        list = find_list(work, lists, c0, lane);
+        const int2 at = work[list];
+        count = at.y;
+        k = (c0 - at.x) * TILE;
+        left = min(work[list + 1].x, end) - c0;
+    }
+    __device__ __forceinline__ bool next(const int2* work) {       // false: the stretch ends
+        k += TILE;
+        if (--left > 0) return true;
+        for (;;) {
+            const int2 at = work[++list];
+            if (at.x >= end) return false;
+            const int hi = work[list + 1].x;
+            if (hi > at.x) { left = min(hi, end) - at.x; k = 0; count = at.y; return true; }
+        }
+    }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {        // once this thread's copies so far have landed
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// lists: [B prefixes (S = 1)] [B S own]
+template <int ATOMS, int IG, bool SILU>
+__global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW) {
+    using L = Smem<ATOMS>;
+    extern __shared__ unsigned char smem_raw[];
+    br_let_next_kernel_start();
+    unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    Bars* bars = reinterpret_cast<Bars*>(sm + L::BARS);
+    volatile int* abort_flag = &bars->abort_flag;
+    const mbema_branches& br = a.br;
+    constexpr int N = 64 * ATOMS;
+    const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int D = a.H * BR_HD;
+    const int steps = min(JW, a.n - (int)blockIdx.z * JW), j0 = blockIdx.z * JW;
+    const int lists = a.row_lists;
+    const int2* work = reinterpret_cast<const int2*>(br.work) + a.row_work;
+    const int total = work[lists].x;
+    const int workers = max(1, min((int)gridDim.x * IG, total));
+    const int me0 = blockIdx.x * IG;
+    if (total == 0 || me0 >= workers) {                           // nothing to do (the same for all threads)
+        if (tid == 0) br_wait_for_kernel_before();                // the merge waits for this kernel alone
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < L::A_STAGES; ++i) {
+            mbar_init(&bars->a_full[i], 1);
+            mbar_init(&bars->a_empty[i], 1);
+        }
+        for (int i = 0; i < L::E_STAGES; ++i) {
+            mbar_init(&bars->e_full[i], 64);
+            mbar_init(&bars->e_empty[i], 4 * steps);
+        }
+        for (int g = 0; g < GROUPS; ++g)
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&bars->acc_full[g][i], 1);
+                mbar_init(&bars->acc_empty[g][i], 4);
+            }
+        mbar_init(&bars->drain, 1);
+        bars->abort_flag = *reinterpret_cast<volatile int*>(br.status);
+        fence_barrier_init();
+    }
+    if (warp == WARP_MMA) {
+        tmem_alloc(&bars->tmem_base, 512);
+        tmem_relinquish();
+    }
+    {   // W of every step, fp16, K-major rows of 64 state channels, 128-byte swizzle: a thread packs 8 channels of one output column
+        const float scale = SILU ? 0.5f * W_SCALE : W_SCALE;      // SiLU(x) = h + h tanh(h), h = x / 2
+        for (int i = tid; i < N * 8; i += THREADS) {
+            const int d = i & 63, c = (i >> 6) * 8;
+            float w[8], l2r[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = a.W[(size_t)(c + e) * D + h * BR_HD + d] * scale;
+                l2r[e] = log2f(br.rhos[c + e]);
+            }
+            unsigned char* dst = sm + L::B + (c >> 6) * 8192 + d * 128 + ((((c & 63) >> 3) ^ (d & 7)) << 4);
+            for (int s = 0; s < steps; ++s) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = w[e] * exp2f((float)(j0 + s) * l2r[e]);
+                *reinterpret_cast<uint4*>(dst + s * L::B_STEP) = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
+            }
+        }
+    }
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = bars->tmem_base;
+    // tiles of this CTA's workers; the CTA's tiles are numbered round by round
+    int tiles[IG], rounds = 0;
+#pragma unroll
+    for (int g = 0; g < IG; ++g) {
+        tiles[g] = me0 + g < workers ? branch_cut(total, workers, me0 + g + 1) - branch_cut(total, workers, me0 + g) : 0;
+        rounds = max(rounds, tiles[g]);
+    }
+
+    if (warp >= EPI_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp <= WARP_V) {
+            // ------------------------------------------------------------ gathering warps: E_k or E_v rows, 8 lanes a row
+            const char* table = reinterpret_cast<const char*>(warp == WARP_K ? a.Ek : a.Ev) + h * (BR_HD * 2) + (lane & 7) * 16;
+            const uint32_t D2 = (uint32_t)D * 2;
+            const int sub = lane >> 3;
+            const uint32_t base = smem_u32(sm) + (warp == WARP_K ? L::EK : L::EV);
+            const uint32_t even = base + sub * 128 + (((lane & 7) ^ sub) << 4), odd = base + (sub + 4) * 128 + (((lane & 7) ^ (sub + 4)) << 4);
+            Cursor cur[IG];
+#pragma unroll
+            for (int g = 0; g < IG; ++g)
+                if (tiles[g] > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
+            int it = 0;
+            bool go = true;
+            for (int r = 0; r < rounds && go; ++r) {
+#pragma unroll
+                for (int g = 0; g < IG; ++g) {
+                    if (r >= tiles[g] || !go) continue;
+                    const int* slots = a.row_slots(cur[g].list);
+                    int ids[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ids[i] = slots[min(cur[g].k + 32 * i + lane, cur[g].count - 1)];
+                    const int st = it % L::E_STAGES, use = it / L::E_STAGES;
+                    if (use > 0) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 1));
+                    if (!go) continue;
+                    const uint32_t at = st * L::E_STAGE;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {                // rows 4 i + sub
+                        const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, ids[i >> 3], (i & 7) * 4 + sub);
+                        cp_async16(at + ((i & 1) ? odd : even) + (i >> 1) * 1024, table + (uint64_t)v * D2);
+                    }
+                    cp_async_arrive(&bars->e_full[st]);
+                    ++it;
+                    cur[g].next(work);
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else if (warp == WARP_MMA) {
+            // ------------------------------------------------------------ one lane: operand copies, a stage or more ahead, and all products
+            Cursor cur[IG];
+#pragma unroll
+            for (int g = 0; g < IG; ++g)
+                if (tiles[g] > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
+            if (lane == 0) {
+                int all = 0;
+#pragma unroll
+                for (int g = 0; g < IG; ++g) all += tiles[g];
+                const uint32_t idesc = umma_idesc_16(TILE, BR_HD, 0, 0, 0, 0);
+                int it = 0, copied = 0, cr = 0, cg = 0;
+                bool go = true;
+                auto copy_next = [&]() {                          // operands of the next tile in order, into a stage that is free
+                    for (;;) {                                    // (cr, cg): the next tile that exists
+                        bool there = false;
+#pragma unroll
+                        for (int g = 0; g < IG; ++g) there |= g == cg && cr < tiles[g];
+                        if (there) break;
+                        if (++cg == IG) { cg = 0; ++cr; }
+                    }
+                    const int st = copied % L::A_STAGES;
+#pragma unroll
+                    for (int g = 0; g < IG; ++g) {
+                        if (g != cg) continue;
+                        mbar_expect_tx(&bars->a_full[st], L::OP_BYTES);
+                        bulk_load(sm + st * L::OP_BYTES, a.row_operands(cur[g].list) + (size_t)(cur[g].k / TILE) * L::OP_BYTES, L::OP_BYTES, &bars->a_full[st]);
+                        cur[g].next(work);
+                    }
+                    ++copied;
+                    if (++cg == IG) { cg = 0; ++cr; }
+                };
+                while (copied < min(L::A_STAGES, all)) copy_next();
+                for (int r = 0; r < rounds && go; ++r) {
+                    for (int g = 0; g < IG && go; ++g) {
+                        bool there = false;
+#pragma unroll
+                        for (int x = 0; x < IG; ++x) there |= x == g && r < tiles[x];
+                        if (!there) continue;
+                        const int st = it % L::A_STAGES;
+                        go = mbar_wait(&bars->a_full[st], (uint32_t)((it / L::A_STAGES) & 1), abort_flag, 3);
+                        const uint64_t da = umma_desc_k_sw128(smem_u32(sm + st * L::OP_BYTES));
+                        for (int s = 0; s < steps && go; ++s) {
+                            const int w = IG == 1 ? s : g;
+                            if (r >= 2) go = mbar_wait(&bars->acc_empty[w][r & 1], (uint32_t)(((r >> 1) - 1) & 1), abort_flag, 4);
+                            if (!go) break;
+                            tc_fence_after_sync();
+                            const uint64_t db = umma_desc_k_sw128(smem_u32(sm + L::B + s * L::B_STEP));
+#pragma unroll
+                            for (int k16 = 0; k16 < 4 * ATOMS; ++k16)
+                                umma_bf16_ss(tmem + (uint32_t)((w * 2 + (r & 1)) * BR_HD), da + (uint64_t)(((k16 >> 2) * 16384 + (k16 & 3) * 32) >> 4),
+                                             db + (uint64_t)(((k16 >> 2) * 8192 + (k16 & 3) * 32) >> 4), idesc, k16 != 0 ? 1u : 0u);
+                            umma_commit(&bars->acc_full[w][r & 1]);
+                        }
+                        if (!go) break;
+                        umma_commit(&bars->a_empty[st]);
+                        ++it;
+                        if (copied < all) {                       // the stage just read serves tile it + 1 (products take a few hundred cycles)
+                            go = mbar_wait(&bars->a_empty[st], (uint32_t)(((it - 1) / L::A_STAGES) & 1), abort_flag, 2);
+                            if (go) copy_next();
+                        }
+                    }
+                }
+                umma_commit(&bars->drain);
+                for (; !go && it < copied; ++it)                  // given up: operand copies still on their way
+                    mbar_wait(&bars->a_full[it % L::A_STAGES], (uint32_t)((it / L::A_STAGES) & 1), abort_flag, 6);
+                mbar_wait(&bars->drain, 0, abort_flag, 7);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- epilogue: a thread a slot
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        const int group = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const int jj = IG == 1 ? group : 0, j = j0 + jj;
+        const int g = IG == 1 ? 0 : group;
+        int mine = 0;
+#pragma unroll
+        for (int x = 0; x < IG; ++x)
+            if (x == g) mine = tiles[x];
+        if (jj < steps && mine > 0) {
+            const int me = me0 + g;
+            Cursor cur;
+            cur.start(work, lists, total, workers, me, lane);
+            const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * 2 * BR_HD);
+            float* q_sh = reinterpret_cast<float*>(sm + L::Q) + warp * 64;            // a copy a warp: the warps of a group never meet
+            const uint32_t q_at = smem_u32(q_sh);
+            const uint32_t e_row = smem_u32(sm) + L::EK + row * 128;
+            const uint32_t flip = (uint32_t)(row & 7) << 4;
+            float m = -INFINITY, l = 0.f, o[64];
+            int staged = -1;
+            const uint32_t* bits = nullptr;
+            bool fresh = true, go = true;
+            for (int r = 0; r < mine && go; ++r) {
+                if (fresh) {                                      // a new list: its row's q, scaled to base-2 scores
+                    const int64_t branch = a.row_branch(cur.list);
+                    const bool prefix = a.row_is_prefix(cur.list);
+                    const uint32_t x = reinterpret_cast<const uint32_t*>(a.q)[((((size_t)branch * a.n + j) * a.H + h) * BR_HD) / 2 + lane];
+                    __syncwarp();
+                    *reinterpret_cast<float2*>(q_sh + 2 * lane) = make_float2(bf16_lo(x) * BR_SCORE_LOG2, bf16_hi(x) * BR_SCORE_LOG2);
+                    __syncwarp();
+                    staged = lane < j ? (prefix ? br.st_pos : br.st_own)[br_index(br, branch, lane)] : -1;
+                    bits = prefix ? br.touched + (size_t)branch * ((br.Kcap + 31) / 32) : nullptr;
+                    m = -INFINITY;
+                    l = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) o[i] = 0.f;
+                    fresh = false;
+                }
+                int it = 0;                                       // number of this tile among the CTA's
+#pragma unroll
+                for (int x = 0; x < IG; ++x) it += min(x < g ? r + 1 : r, tiles[x]);
+                const int st = it % L::E_STAGES;
+                const int k_w = cur.k + quarter * 32;             // this warp's 32 slots
+                unsigned hide = 0u;
+                if (bits && k_w < br.Kcap) hide = bits[k_w >> 5];
+                if (j > 0) {
+                    const unsigned d = (unsigned)(staged - k_w);
+                    hide |= __reduce_or_sync(0xffffffffu, d < 32u ? 1u << d : 0u);
+                }
+                const bool hidden = ((hide >> lane) & 1u) || k_w + lane >= cur.count;
+                const uint32_t e_at = e_row + st * L::E_STAGE, t_at = taddr + (uint32_t)((r & 1) * BR_HD);
+                go = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[group][r & 1], (uint32_t)((r >> 1) & 1), abort_flag, 8));
+                if (go) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_full[st], (uint32_t)((it / L::E_STAGES) & 1), abort_flag, 9));
+                if (!go) break;
+                tc_fence_after_sync();
+                float s0 = 0.f, s1 = 0.f, v[2][16];               // 16 channels at a time, the next ones on their way
+                tmem_ld16_nb(t_at, v[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float (&g16)[16] = v[c & 1];
+                    const uint4 e0 = lds128(e_at + (((c * 2) << 4) ^ flip)), e1 = lds128(e_at + (((c * 2 + 1) << 4) ^ flip));
+                    const uint32_t e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
+                    tmem_wait_ld16(g16);
+                    if (c < 3) tmem_ld16_nb(t_at + (uint32_t)((c + 1) * 16), v[(c + 1) & 1]);
+                    if (SILU) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) g16[i] = fmaf(g16[i], tanh_approx(g16[i]), g16[i]);
+                        tmem_st_32x32b_x16(t_at + (uint32_t)(c * 16), g16);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 q = lds_f4(q_at + c * 64 + i * 16);
+                        s0 = fmaf(bf16_lo(e[2 * i]) * q.x, g16[4 * i], s0);
+                        s1 = fmaf(bf16_hi(e[2 * i]) * q.y, g16[4 * i + 1], s1);
+                        s0 = fmaf(bf16_lo(e[2 * i + 1]) * q.z, g16[4 * i + 2], s0);
+                        s1 = fmaf(bf16_hi(e[2 * i + 1]) * q.w, g16[4 * i + 3], s1);
+                    }
+                }
+                const float x = s0 + s1;
+                const bool grow = !hidden && x > m + 8.0f;        // o is scaled again only where the maximum moves by more than 2^8
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float alpha = grow ? ex2_approx(m - x) : 1.0f;
+                    if (grow) m = x;
+                    l *= alpha;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) o[i] *= alpha;
+                }
+                const float p = hidden ? 0.f : ex2_approx(x - m);
+                l += p;
+                if (SILU) tmem_wait_st();
+                tmem_ld16_nb(t_at, v[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float (&g16)[16] = v[c & 1];
+                    const uint4 e0 = lds128(e_at + 16384 + (((c * 2) << 4) ^ flip)), e1 = lds128(e_at + 16384 + (((c * 2 + 1) << 4) ^ flip));
+                    const uint32_t e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
+                    tmem_wait_ld16(g16);
+                    if (c < 3) tmem_ld16_nb(t_at + (uint32_t)((c + 1) * 16), v[(c + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {                 // (a hidden slot's value that is not finite: the row lists the same slot as its own)
+                        o[c * 16 + 2 * i] = fmaf(p * g16[2 * i], bf16_lo(e[i]), o[c * 16 + 2 * i]);
+                        o[c * 16 + 2 * i + 1] = fmaf(p * g16[2 * i + 1], bf16_hi(e[i]), o[c * 16 + 2 * i + 1]);
+                    }
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&bars->acc_empty[group][r & 1]);
+                    mbar_arrive(&bars->e_empty[st]);
+                }
+                const int list = cur.list;
+                const bool more = cur.next(work);
+                if (!more || cur.list != list) {                  // the list or the stretch ends: join the lanes, two channels each
+                    float M = m;
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                    const float w = m == -INFINITY ? (l == 0.f ? 0.f : l) : ex2_approx(m - M);      // (l NaN without a maximum: keep it)
+                    l = warp_sum(l == 0.f ? 0.f : l * w);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) o[i] *= w;
+#pragma unroll
+                    for (int d = 16, c = 32; d; d >>= 1, c >>= 1) {
+                        const bool up = lane & d;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i < c) {
+                                const float send = up ? o[i] : o[i + c], keep = up ? o[i + c] : o[i];
+                                o[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+                            }
+                        }
+                    }
+                    const size_t at = ((((size_t)(list + me)) * 4 + quarter) * a.n + j) * a.H + h + a.row_part0;
+                    *reinterpret_cast<float2*>(a.po + at * BR_HD + 2 * lane) = make_float2(o[0], o[1]);
+                    if (lane == 0) a.ml[at] = make_float2(M, l);
+                    fresh = true;
+                }
+            }
+        }
+    }
+    if (tid == 0) br_wait_for_kernel_before();                    // the merge waits for this kernel alone
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+    if (tid == 0 && *abort_flag) atomicOr(br.status, *abort_flag);
+}
+
+template <int ATOMS, int IG, bool SILU>
+static int launch(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st) {
+    static std::atomic<unsigned long long> done{0};
+    auto* kernel = k_branch_rows<ATOMS, IG, SILU>;
+    MBEMA_CUDA_TRY(allow_smem(kernel, Smem<ATOMS>::BYTES, done));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Smem<ATOMS>::BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 1 : 0;
+    MBEMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, p.JW));
+    return check_launch();
+}
+
+template <int ATOMS>
+static int launch_silu(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st) {
+    if (p.IG == 1) return a.silu ? launch<ATOMS, 1, true>(a, p, early, st) : launch<ATOMS, 1, false>(a, p, early, st);
+    return a.silu ? launch<ATOMS, 3, true>(a, p, early, st) : launch<ATOMS, 3, false>(a, p, early, st);
+}
+
+}  // namespace brows
+
+// One step: three workers a CTA.  More: up to three steps a worker, whichever leaves the fewest groups idle.
+BranchRows branch_rows(int64_t n, int64_t H) {
+    BranchRows p;
+    p.JW = n == 1 ? 1 : n == 2 || n == 4 ? 2 : 3;
+    p.IG = p.JW == 1 ? 3 : 1;
+    p.zb = (int)((n + p.JW - 1) / p.JW);
+    p.ctas = (int)std::max<int64_t>(1, 148 / (H * p.zb));
+    return p;
+}
+
+// early: the kernel before (the prefixes, for more than one branch) is this call's too
+int launch_branch_rows(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st) {
+    if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
+    return a.br.N == 64 ? brows::launch_silu<1>(a, p, early, st) : brows::launch_silu<2>(a, p, early, st);
+}
+
+}  // namespace mbema

@@ -144,19 +144,18 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
 }
 
 // Operand copies of all listed slots at the first staged step, state * rho^(t0 + len - last) / 64 in fp16 (11 significant bits; a
-// state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head.  grid: x = shares of a list,
-// y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sum of
-// the lists' units that the attention deals its work by.
-__device__ void running_sum(const mbema_branches& br) {
+// state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head, in the layouts that branches.cuh gives.
+// grid: x = shares of a list, y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sums of the
+// lists' units that the attention deals its work by.
+__device__ int running_sum(const mbema_branches& br, int2* out, int lists, int unit, bool prefixes, int blocks) {
     __shared__ int s_warp[8];
     const int tid = threadIdx.x, lane = tid & 31;
-    const int blocks = br.S == 1 ? 1 : (int)((br.S + BR_BLOCK - 1) / BR_BLOCK);
-    const int n_pre = (int)br.B * blocks, lists = n_pre + (int)(br.B * br.S);
+    const int n_pre = prefixes ? (int)br.B * blocks : 0;
     int base = 0;
     for (int x0 = 0; x0 < lists; x0 += 256) {
         const int x = x0 + tid;
-        const int count = x < n_pre ? min(br.n_active[x / blocks], (int)br.Kcap) : x < lists ? br.own_n[x - n_pre] : 0;
-        const int c = (count + 15) / 16 * (x >= n_pre ? BR_COST_OWN : br.S == 1 ? BR_COST_ONE : BR_COST_BLOCK);
+        const int count = x >= lists ? 0 : x < n_pre ? min(br.n_active[x / blocks], (int)br.Kcap) : br.own_n[x - n_pre];
+        const int c = (count + unit - 1) / unit;
         int sum = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -170,62 +169,90 @@ __device__ void running_sum(const mbema_branches& br) {
             if (w < (tid >> 5)) sum += s_warp[w];
             all += s_warp[w];
         }
-        if (x < lists) reinterpret_cast<int2*>(br.work)[x] = make_int2(base + sum - c, count);
+        if (x < lists) out[x] = make_int2(base + sum - c, count);
         base += all;
         __syncthreads();
     }
-    if (tid == 0) reinterpret_cast<int2*>(br.work)[lists] = make_int2(base, 0);
+    if (tid == 0) out[lists] = make_int2(base, 0);
+    return base;
+}
+
+__device__ __forceinline__ void decayed(float (&f)[8], const float* src, float dt, const float (&l2r)[8]) {
+    const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
+    const float in[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fminf(in[e] * exp2f(dt * l2r[e]) * BR_OP_SCALE, 65504.f);
+}
+__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
+    const __half2 o = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&o);
 }
 
 __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
     br_wait_for_kernel_before();
     if (blockIdx.y == br.B) {
-        if (blockIdx.x == 0 && blockIdx.z == 0) running_sum(br);
+        const int blocks = (int)((br.S + BR_BLOCK - 1) / BR_BLOCK), n_pre = br.S > 1 ? (int)br.B * blocks : 0;
+        int2* work = reinterpret_cast<int2*>(br.work);
+        if (blockIdx.x == 0 && blockIdx.z == 0) {
+            running_sum(br, work, n_pre, 16, true, blocks);
+            running_sum(br, work + n_pre + 1, (int)(br.B * br.S + (br.S == 1 ? br.B : 0)), BR_TILE, br.S == 1, 1);
+        }
         return;
     }
     const int b = blockIdx.y, z = blockIdx.z;
-    const int N = (int)br.N, half = N / 32;             // pairs of fragments: a warp makes one of sixteen slots
+    const int N = (int)br.N;
     const int64_t r = (int64_t)b * br.S + (z ? z - 1 : 0);
     const int count = z ? br.own_n[r] : min(br.n_active[b], (int)br.Kcap);
     const int now = br.t0[0] + br.len[r];
-    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int i = warp % half, c = 32 * i + 8 * (lane & 3);
-    char* out = reinterpret_cast<char*>(z ? br.own_op : br.pre_op) + (z ? (size_t)r * br_operand_bytes(br.cap, N) : (size_t)b * br_operand_bytes(br.Kcap, N));
+    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5), warps = gridDim.x * 8;
+    char* out = z ? reinterpret_cast<char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, N)
+                  : reinterpret_cast<char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, N);
+    auto source = [&](int slot, float& dt) {
+        if (z) {
+            dt = (float)(now - br.own_t[(size_t)r * br.cap + slot]);
+            return (const float*)br.own_state + ((size_t)r * br.cap + slot) * N;
+        }
+        const int v = br.active[(size_t)b * br.Kcap + slot];
+        dt = (float)(now - br.last_t[(size_t)b * br.V + v]);
+        return (const float*)br.state + ((size_t)b * br.V + v) * N;
+    };
+    float l2r[8];
+    if (z || br.S == 1) {                               // rows of 64 channels: eight lanes a row, four rows a warp
+        const int atoms = N / 64, atom = warp % atoms, c = 64 * atom + 8 * (lane & 7);
+        const int past = (count + BR_TILE - 1) / BR_TILE * BR_TILE;
+        int k = warp / atoms * 4 + (lane >> 3);
+        if (k - (lane >> 3) >= past) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l2r[e] = log2f(br.rhos[c + e]);
+        for (; k - (lane >> 3) < past; k += warps / atoms * 4) {
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, dt;
+            if (k < count) {
+                const float* src = source(k, dt);
+                decayed(f, src + c, dt, l2r);
+            }
+            const int row = k % BR_TILE;
+            *reinterpret_cast<uint4*>(out + ((size_t)(k / BR_TILE) * atoms + atom) * 16384 + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) =
+                make_uint4(half_pair(f[0], f[1]), half_pair(f[2], f[3]), half_pair(f[4], f[5]), half_pair(f[6], f[7]));
+        }
+        return;
+    }
+    // fragments: a warp makes a pair of them, for sixteen slots
+    const int half = N / 32, i = warp % half, c = 32 * i + 8 * (lane & 3);
     int k = warp / half * 16 + (lane >> 2);
     if (k - (lane >> 2) >= count) return;
-    float l2r[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) l2r[e] = log2f(br.rhos[c + e]);
-    for (; k - (lane >> 2) < count; k += gridDim.x * 8 / half * 16) {
+    for (; k - (lane >> 2) < count; k += warps / half * 16) {
         uint32_t w[2][4];                               // slots k, k + 8
 #pragma unroll
         for (int hi = 0; hi < 2; ++hi) {
-            const int slot = k + 8 * hi;
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = 0.f;
-            if (slot < count) {
-                const float* src;
-                int last;
-                if (z) {
-                    src = br.own_state + ((size_t)r * br.cap + slot) * N;
-                    last = br.own_t[(size_t)r * br.cap + slot];
-                } else {
-                    const int v = br.active[(size_t)b * br.Kcap + slot];
-                    src = br.state + ((size_t)b * br.V + v) * N;
-                    last = br.last_t[(size_t)b * br.V + v];
-                }
-                const float dt = (float)(now - last);
-                const float4 x = *reinterpret_cast<const float4*>(src + c), y = *reinterpret_cast<const float4*>(src + c + 4);
-                const float in[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = fminf(in[e] * exp2f(dt * l2r[e]) * BR_OP_SCALE, 65504.f);
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, dt;
+            if (k + 8 * hi < count) {
+                const float* src = source(k + 8 * hi, dt);
+                decayed(f, src + c, dt, l2r);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const __half2 o = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
-                w[hi][e] = *reinterpret_cast<const uint32_t*>(&o);
-            }
+            for (int e = 0; e < 4; ++e) w[hi][e] = half_pair(f[2 * e], f[2 * e + 1]);
         }
         char* dst = out + (size_t)(k >> 4) * N * 32 + (2 * i) * 512 + lane * 16;
         *reinterpret_cast<uint4*>(dst) = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
@@ -280,12 +307,12 @@ static int check_branches(const mbema_branches* br) {
                           br->st_new, br->st_state, br->overflow};
     for (const void* p : need)
         if (!p) return MBEMA_ERR_NULL;
-    if (br->pre_op || br->own_op || br->work) {              // all three or none
+    if (br->pre_op || br->own_op || br->work || br->status) {              // all four or none
         if (!branch_tc_supported(br->N) || br->S >= 65535 || br->B >= 65535) return MBEMA_ERR_UNSUPPORTED;
-        if (!br->pre_op || !br->own_op || !br->work) return MBEMA_ERR_NULL;
-        const int64_t blocks = (br->S + BR_BLOCK - 1) / BR_BLOCK;                   // the running sum stays below 2^30
-        if (br->B * blocks * (br->Kcap / 16 + 1) * BR_COST_BLOCK + br->B * br->S * (br->cap / 16 + 1) * BR_COST_OWN >= 1ll << 30)
-            return MBEMA_ERR_UNSUPPORTED;
+        if (!br->pre_op || !br->own_op || !br->work || !br->status) return MBEMA_ERR_NULL;
+        if (((uintptr_t)br->pre_op | (uintptr_t)br->own_op | (uintptr_t)br->state | (uintptr_t)br->own_state) & 15) return MBEMA_ERR_ALIGN;
+        const int64_t blocks = (br->S + BR_BLOCK - 1) / BR_BLOCK;                   // the running sums stay below 2^30
+        if (br->B * blocks * (br->Kcap / 16 + 1) + br->B * br->S * (br->cap / 16 + 1) >= 1ll << 30) return MBEMA_ERR_UNSUPPORTED;
     }
     return MBEMA_OK;
 }
@@ -313,8 +340,8 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
                                                                                    (int)n_pending, C_q);
     rc = check_launch();
     if (rc != MBEMA_OK || !br->pre_op) return rc;
-    // shares of a list: eight CTAs an SM over all lists, one for every 64 or 32 slots where that is enough
-    const int64_t items = 16 * 8 / (br->N / 32), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
+    // shares of a list: eight CTAs an SM over all lists, one for every 32 or 16 slots where that is enough
+    const int64_t items = 32 / (br->N / 64), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
     const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
     MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, (cudaStream_t)stream, *br));
     return check_launch();

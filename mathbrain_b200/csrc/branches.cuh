@@ -14,9 +14,6 @@ static constexpr float BR_OP_SCALE = 1.0f / 64.0f;  // operand copies hold state
 static constexpr float BR_SCORE_LOG2 = 0.125f * 1.4426950408889634f;   // 1 / sqrt(64), in powers of two
 
 static constexpr int BR_BLOCK = 16;                // branches that read a prefix together on the tensor cores
-// Cost of a unit (16 slots) of a list, in the running sum that mbema_branches_extend leaves: own slots, a prefix read by one branch,
-// a prefix read by sixteen.
-static constexpr int BR_COST_OWN = 2, BR_COST_ONE = 2, BR_COST_BLOCK = 3;
 
 // fp32 arithmetic: how the slot lists are cut into chunks.  A chunk of a sequence's prefix for all its branches, or one of a
 // branch's own slots, leaves one partial (m, l, o[64]) for each of its rows, heads and steps, which k_branch_merge joins.
@@ -26,10 +23,17 @@ struct BranchPlan {
     int steps, JP;     // steps a job of a prefix, blocks of steps
 };
 
-// Tensor cores: workers, and the lists in the running sum: prefixes (as blocks of branches read them), then the branches' own.
+// Prefixes that several branches read, in units of 16 slots.
 struct BranchShape {
-    int rows, blocks;      // branches that read a prefix together; such blocks a sequence
-    int warps, JW, IG;     // of a CTA: warps, steps a worker, workers
+    int blocks;            // of sixteen branches, a sequence
+    int JW, IG;            // of a CTA: steps a worker, workers
+    int zb, ctas;          // blocks of steps; CTAs a head and block of steps
+};
+
+// Rows walked alone on tcgen05 (own lists; the prefix of a sequence with one branch), in tiles of 128 slots.
+static constexpr int BR_TILE = 128;
+struct BranchRows {
+    int JW, IG;            // steps a worker, workers a CTA
     int zb, ctas;          // blocks of steps; CTAs a head and block of steps
 };
 
@@ -48,23 +52,51 @@ struct BranchArgs {
     int silu, listed_only;
     // fp32 arithmetic: partials [rows, H, SP + SO]
     BranchPlan plan;
-    // tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order; partials of the prefixes
-    // [piece, BR_BLOCK or 1, n, H], of the own lists [own_piece0 + piece, n, H]
-    int64_t n_pre, own_piece0, max_workers;
-    int rows, blocks, cost_pre, ring_bytes, w_offset;
+    // tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order.  Prefixes of several
+    // branches: lists (sequence, block of sixteen), partials [piece, BR_BLOCK, n, H].
+    int n_pre, blocks, pre_workers, ring_bytes, w_offset;
+    // Single rows: lists (the sequences' prefixes, for one branch), the branches' own; partials from row_part0 on, [piece, 4 warps, n, H]
+    int row_lists, row_work, row_workers;      // their number, where their running sum begins in `work`, workers
+    int64_t row_part0;
+    __device__ __forceinline__ bool row_is_prefix(int list) const { return br.S == 1 && list < (int)br.B; }
+    __device__ __forceinline__ int row_branch(int list) const { return br.S == 1 && list >= (int)br.B ? list - (int)br.B : list; }
+    __device__ __forceinline__ const int* row_slots(int list) const {
+        return row_is_prefix(list) ? br.active + (size_t)list * br.Kcap : br.own_slot + (size_t)row_branch(list) * br.cap;
+    }
+    __device__ __forceinline__ const char* row_operands(int list) const;
 };
 
-// The workers that a running sum of `total` occupies, each with two units or more, and where their stretches begin.
-__device__ __forceinline__ int branch_workers(int total, int most) { return max(1, min(most, total / (2 * BR_COST_BLOCK))); }
+// The workers that a running sum of `total` units (tiles) occupies, and where their stretches begin.
+__device__ __forceinline__ int branch_workers(int total, int most, int least) { return max(1, min(most, total / least)); }
+static constexpr int BR_LEAST_UNITS = 2;           // a worker's
 __device__ __forceinline__ int branch_cut(int total, int workers, int w) { return (int)((long long)total * w / workers); }
-// the worker whose stretch holds cost c < total
+// the worker whose stretch holds unit c < total
 __device__ __forceinline__ int branch_worker_of(int total, int workers, int c) {
     return (int)((((long long)c + 1) * workers - 1) / total);
 }
+// Where a stretch begins: the list that holds unit c, by 32 samples of the running sum at a time.
+__device__ __forceinline__ int find_list(const int2* work, int lists, int c, int lane) {
+    int lo = 0, hi = lists;                       // work[lo].x <= c < work[hi].x
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int at = lo + (lane + 1) * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at].x <= c);
+        lo += __popc(below) * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
 
-// Operands of a list: fp16 fragments of the gate product, 16 slots after 16 slots.  Slot k, channel c = 32 i + 8 t + 4 u + 2 p + e is half e
+// Operands of a list, state / 64 in fp16, tile after tile of 128 slots (the last one's other slots zero); N * 256 bytes each.
+// Lists of single rows: what tcgen05 reads from shared memory, N / 64 blocks of 128 rows of 64 channels, 128 bytes a row, the 16-byte
+// pieces of row k in order piece ^ (k % 8).
+// Prefixes of several branches: fragments of mma.sync, 16 slots after 16 slots.  Slot k, channel c = 32 i + 8 t + 4 u + 2 p + e is half e
 // of word (row / 8) + 2 p (row = k % 16) of lane 4 (row % 8) + t in fragment 2 i + u of its sixteen (512 bytes each).
-__host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + 15) / 16) * N * 32; }
+__host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + BR_TILE - 1) / BR_TILE) * N * (2 * BR_TILE); }
+__device__ __forceinline__ const char* BranchArgs::row_operands(int list) const {
+    return row_is_prefix(list) ? reinterpret_cast<const char*>(br.pre_op) + (size_t)list * br_operand_bytes(br.Kcap, br.N)
+                               : reinterpret_cast<const char*>(br.own_op) + (size_t)row_branch(list) * br_operand_bytes(br.cap, br.N);
+}
 
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
 
@@ -99,7 +131,9 @@ __device__ __forceinline__ void br_wait_for_kernel_before() { asm volatile("grid
 __device__ __forceinline__ void br_let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 bool branch_tc_supported(int64_t N);
-BranchShape branch_shape(int64_t B, int64_t S, int64_t N, int64_t n, int64_t H);
+BranchShape branch_shape(int64_t S, int64_t n, int64_t H);
+BranchRows branch_rows(int64_t n, int64_t H);
+int launch_branch_rows(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st);
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st);
 int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st);
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st);

@@ -54,8 +54,8 @@ def test_branch_argument_errors(lib):
     assert attend(br=None) == 1 and attend(n=0) == 2 and attend(n=9) == 2 and attend(H=0) == 2 and attend(hd=32) == 3
     assert attend(q=None) == 1 and attend(qd=2) == 6 and attend(ed=7) == 6 and attend(q=addr + 4) == 7 and attend(O=addr + 2) == 7
     assert attend(nbytes=64) == 4 and attend(ws=None) == 1
-    assert lib.mbema_branches_attend_workspace_bytes(0, 1, 64, 1, 8, 40, 20, 0) > 0
-    for bad in ((-1, 1, 64, 1, 8, 40, 20), (1, 0, 64, 1, 8, 40, 20), (1, 1, 64, 33, 8, 40, 20), (1, 1, 64, 1, 0, 40, 20), (1, 1, 64, 1, 8, 0, 20)):
+    assert lib.mbema_branches_attend_workspace_bytes(0, 1, 1, 8, 40, 20, 0) > 0
+    for bad in ((-1, 1, 1, 8, 40, 20), (1, 0, 1, 8, 40, 20), (1, 1, 33, 8, 40, 20), (1, 1, 1, 0, 40, 20), (1, 1, 1, 8, 0, 20)):
         assert lib.mbema_branches_attend_workspace_bytes(*bad, 0) == 0
     empty, _, _ = _branches(B=0, state=None, overflow=None)
     assert lib.mbema_branches_init(ctypes.byref(empty), 0, None, None) == 0
