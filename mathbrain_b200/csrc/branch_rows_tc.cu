@@ -12,6 +12,7 @@
 // two or three steps they take the same tile, a step each.
 // Bound by the FMA and ALU instructions of the two passes (eight a slot, channel and step, one MUFU among them).
 #include <algorithm>
+#include <type_traits>
 
 #include "branches.cuh"
 #include "sm100_ptx.cuh"
@@ -23,14 +24,14 @@ using namespace ptx;
 
 static constexpr int TILE = BR_TILE, GROUPS = 3, EPI_WARPS = 4 * GROUPS, THREADS = (EPI_WARPS + 4) * 32;
 static constexpr int WARP_K = EPI_WARPS, WARP_V = EPI_WARPS + 1, WARP_MMA = EPI_WARPS + 2;
-// setmaxnreg: 12 * 32 * 152 (epilogue) + 4 * 32 * 56 (producers) = the launch allocation 512 * 128
+// setmaxnreg: 12 * 32 * 144 (epilogue) + 4 * 32 * 80 (producers) = the launch allocation 512 * 128
 static constexpr float W_SCALE = 64.0f;           // undoes BR_OP_SCALE
 
 template <int ATOMS>                               // of 64 state channels
 struct Smem {
     static constexpr int A_STAGES = 2, E_STAGES = ATOMS == 1 ? 5 : 3, OP_BYTES = ATOMS * 16384;
     static constexpr int EK = A_STAGES * OP_BYTES, EV = EK + 16384, E_STAGE = 32768;
-    static constexpr int B = EK + E_STAGES * E_STAGE, B_STEP = ATOMS * 8192, Q = B + GROUPS * B_STEP, BARS = Q + EPI_WARPS * 256, BYTES = BARS + 256 + 1024;
+    static constexpr int B = EK + E_STAGES * E_STAGE, B_STEP = ATOMS * 8192, Q = B + GROUPS * B_STEP, BARS = Q + EPI_WARPS * 128, BYTES = BARS + 256 + 1024;
 };
 
 struct Bars {
@@ -40,6 +41,7 @@ struct Bars {
     uint64_t e_empty[5];           // every epilogue warp of the tile has read them            (4 a step)
     uint64_t acc_full[GROUPS][2];  // gate product of a group's tile done                      (1 commit)
     uint64_t acc_empty[GROUPS][2]; // the group's warps have read its accumulators a second time (4)
+    uint64_t w_full;               // W of every step is laid out                              (12: the epilogue warps)
     uint64_t drain;                // every product has completed (teardown)                   (1 commit)
     uint32_t tmem_base;
     int abort_flag;
@@ -48,23 +50,28 @@ static_assert(sizeof(Bars) <= 256, "barrier block");
 
 struct Cursor {                    // a worker's place in the lists
     int list, left, k, count, end; // left tiles of this list from slot k on; end: of the stretch, in tiles
+    int2 n1, n2;                   // (running sum, length) of the next two lists, read ahead of their use
     __device__ __forceinline__ void start(const int2* work, int lists, int total, int workers, int me, int lane) {
         const int c0 = branch_cut(total, workers, me);
         end = branch_cut(total, workers, me + 1);
         list = find_list(work, lists, c0, lane);
         const int2 at = work[list];
+        n1 = work[list + 1];
+        n2 = work[min(list + 2, lists)];
         count = at.y;
         k = (c0 - at.x) * TILE;
-        left = min(work[list + 1].x, end) - c0;
+        left = min(n1.x, end) - c0;
     }
-    __device__ __forceinline__ bool next(const int2* work) {       // false: the stretch ends
+    __device__ __forceinline__ bool next(const int2* work, int lists) {       // false: the stretch ends
         k += TILE;
         if (--left > 0) return true;
         for (;;) {
-            const int2 at = work[++list];
+            const int2 at = n1;
             if (at.x >= end) return false;
-            const int hi = work[list + 1].x;
-            if (hi > at.x) { left = min(hi, end) - at.x; k = 0; count = at.y; return true; }
+            ++list;
+            n1 = n2;
+            n2 = work[min(list + 2, lists)];
+            if (n1.x > at.x) { left = min(n1.x, end) - at.x; k = 0; count = at.y; return true; }
         }
     }
 };
@@ -75,14 +82,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {        // once this thread's copies so far have landed
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+template <int OFFSET>
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(OFFSET));
     return v;
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -128,6 +131,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 mbar_init(&bars->acc_full[g][i], 1);
                 mbar_init(&bars->acc_empty[g][i], 4);
             }
+        mbar_init(&bars->w_full, EPI_WARPS);
         mbar_init(&bars->drain, 1);
         bars->abort_flag = *reinterpret_cast<volatile int*>(br.status);
         fence_barrier_init();
@@ -136,40 +140,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
         tmem_alloc(&bars->tmem_base, 512);
         tmem_relinquish();
     }
-    {   // W of every step, fp16, K-major rows of 64 state channels, 128-byte swizzle: a thread packs 8 channels of one output column
-        const float scale = SILU ? 0.5f * W_SCALE : W_SCALE;      // SiLU(x) = h + h tanh(h), h = x / 2
-        for (int i = tid; i < N * 8; i += THREADS) {
-            const int d = i & 63, c = (i >> 6) * 8;
-            float w[8], l2r[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w[e] = a.W[(size_t)(c + e) * D + h * BR_HD + d] * scale;
-                l2r[e] = log2f(br.rhos[c + e]);
-            }
-            unsigned char* dst = sm + L::B + (c >> 6) * 8192 + d * 128 + ((((c & 63) >> 3) ^ (d & 7)) << 4);
-            for (int s = 0; s < steps; ++s) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = w[e] * exp2f((float)(j0 + s) * l2r[e]);
-                *reinterpret_cast<uint4*>(dst + s * L::B_STEP) = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
-            }
-        }
-    }
-    fence_proxy_async_smem();
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = bars->tmem_base;
     // tiles of this CTA's workers; the CTA's tiles are numbered round by round
-    int tiles[IG], rounds = 0;
-#pragma unroll
-    for (int g = 0; g < IG; ++g) {
-        tiles[g] = me0 + g < workers ? branch_cut(total, workers, me0 + g + 1) - branch_cut(total, workers, me0 + g) : 0;
-        rounds = max(rounds, tiles[g]);
-    }
+    auto count_of = [&](int g) { return me0 + g < workers ? branch_cut(total, workers, me0 + g + 1) - branch_cut(total, workers, me0 + g) : 0; };
+    int rounds = 0;
+    for (int g = 0; g < IG; ++g) rounds = max(rounds, count_of(g));
 
     if (warp >= EPI_WARPS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp <= WARP_V) {
             // ------------------------------------------------------------ gathering warps: E_k or E_v rows, 8 lanes a row
             const char* table = reinterpret_cast<const char*>(warp == WARP_K ? a.Ek : a.Ev) + h * (BR_HD * 2) + (lane & 7) * 16;
@@ -178,95 +159,92 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             const uint32_t base = smem_u32(sm) + (warp == WARP_K ? L::EK : L::EV);
             const uint32_t even = base + sub * 128 + (((lane & 7) ^ sub) << 4), odd = base + (sub + 4) * 128 + (((lane & 7) ^ (sub + 4)) << 4);
             Cursor cur[IG];
+            int ids[IG][4];                                       // of each worker's next tile
+            auto fetch_ids = [&](int g) {
+                const int* slots = a.row_slots(cur[g].list);
 #pragma unroll
+                for (int i = 0; i < 4; ++i) ids[g][i] = slots[min(cur[g].k + 32 * i + lane, cur[g].count - 1)];
+            };
+#pragma unroll 1
             for (int g = 0; g < IG; ++g)
-                if (tiles[g] > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
-            int it = 0;
+                if (count_of(g) > 0) { cur[g].start(work, lists, total, workers, me0 + g, lane); fetch_ids(g); }
+            int st = 0, use = 0;
             bool go = true;
-            for (int r = 0; r < rounds && go; ++r) {
+#pragma unroll 1
+            for (int i = 0; go; ++i) {                            // (loops kept rolled: a launch fetches its code cold)
+                const int r = i / IG, g = i - r * IG;
+                if (r >= rounds) break;
+                if (r >= count_of(g)) continue;
+                if (use > 0) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 1));
+                if (!go) break;
+                uint32_t at = st * L::E_STAGE;
+                int id[4] = {ids[g][0], ids[g][1], ids[g][2], ids[g][3]};
+#pragma unroll 1
+                for (int part = 0; part < 4; ++part) {            // 32 rows at a time: rows 4 x + sub
 #pragma unroll
-                for (int g = 0; g < IG; ++g) {
-                    if (r >= tiles[g] || !go) continue;
-                    const int* slots = a.row_slots(cur[g].list);
-                    int ids[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) ids[i] = slots[min(cur[g].k + 32 * i + lane, cur[g].count - 1)];
-                    const int st = it % L::E_STAGES, use = it / L::E_STAGES;
-                    if (use > 0) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 1));
-                    if (!go) continue;
-                    const uint32_t at = st * L::E_STAGE;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {                // rows 4 i + sub
-                        const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, ids[i >> 3], (i & 7) * 4 + sub);
-                        cp_async16(at + ((i & 1) ? odd : even) + (i >> 1) * 1024, table + (uint64_t)v * D2);
+                    for (int x = 0; x < 8; ++x) {
+                        const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, id[0], x * 4 + sub);
+                        cp_async16(at + ((x & 1) ? odd : even) + (x >> 1) * 1024, table + (uint64_t)v * D2);
                     }
-                    cp_async_arrive(&bars->e_full[st]);
-                    ++it;
-                    cur[g].next(work);
+                    at += 4096;
+                    id[0] = id[1]; id[1] = id[2]; id[2] = id[3];
                 }
+                cp_async_arrive(&bars->e_full[st]);
+                if (++st == L::E_STAGES) { st = 0; ++use; }
+                if (cur[g].next(work, lists)) fetch_ids(g);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         } else if (warp == WARP_MMA) {
             // ------------------------------------------------------------ one lane: operand copies, a stage or more ahead, and all products
             Cursor cur[IG];
-#pragma unroll
+#pragma unroll 1
             for (int g = 0; g < IG; ++g)
-                if (tiles[g] > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
+                if (count_of(g) > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
             if (lane == 0) {
                 int all = 0;
-#pragma unroll
-                for (int g = 0; g < IG; ++g) all += tiles[g];
+                for (int g = 0; g < IG; ++g) all += count_of(g);
                 const uint32_t idesc = umma_idesc_16(TILE, BR_HD, 0, 0, 0, 0);
                 int it = 0, copied = 0, cr = 0, cg = 0;
                 bool go = true;
                 auto copy_next = [&]() {                          // operands of the next tile in order, into a stage that is free
-                    for (;;) {                                    // (cr, cg): the next tile that exists
-                        bool there = false;
-#pragma unroll
-                        for (int g = 0; g < IG; ++g) there |= g == cg && cr < tiles[g];
-                        if (there) break;
+                    while (cr >= count_of(cg))                    // (cr, cg): the next tile that exists
                         if (++cg == IG) { cg = 0; ++cr; }
-                    }
                     const int st = copied % L::A_STAGES;
-#pragma unroll
-                    for (int g = 0; g < IG; ++g) {
-                        if (g != cg) continue;
-                        mbar_expect_tx(&bars->a_full[st], L::OP_BYTES);
-                        bulk_load(sm + st * L::OP_BYTES, a.row_operands(cur[g].list) + (size_t)(cur[g].k / TILE) * L::OP_BYTES, L::OP_BYTES, &bars->a_full[st]);
-                        cur[g].next(work);
-                    }
+                    mbar_expect_tx(&bars->a_full[st], L::OP_BYTES);
+                    bulk_load(sm + st * L::OP_BYTES, a.row_operands(cur[cg].list) + (size_t)(cur[cg].k / TILE) * L::OP_BYTES, L::OP_BYTES, &bars->a_full[st]);
+                    cur[cg].next(work, lists);
                     ++copied;
                     if (++cg == IG) { cg = 0; ++cr; }
                 };
                 while (copied < min(L::A_STAGES, all)) copy_next();
-                for (int r = 0; r < rounds && go; ++r) {
-                    for (int g = 0; g < IG && go; ++g) {
-                        bool there = false;
-#pragma unroll
-                        for (int x = 0; x < IG; ++x) there |= x == g && r < tiles[x];
-                        if (!there) continue;
-                        const int st = it % L::A_STAGES;
-                        go = mbar_wait(&bars->a_full[st], (uint32_t)((it / L::A_STAGES) & 1), abort_flag, 3);
-                        const uint64_t da = umma_desc_k_sw128(smem_u32(sm + st * L::OP_BYTES));
-                        for (int s = 0; s < steps && go; ++s) {
-                            const int w = IG == 1 ? s : g;
-                            if (r >= 2) go = mbar_wait(&bars->acc_empty[w][r & 1], (uint32_t)(((r >> 1) - 1) & 1), abort_flag, 4);
-                            if (!go) break;
-                            tc_fence_after_sync();
-                            const uint64_t db = umma_desc_k_sw128(smem_u32(sm + L::B + s * L::B_STEP));
-#pragma unroll
-                            for (int k16 = 0; k16 < 4 * ATOMS; ++k16)
-                                umma_bf16_ss(tmem + (uint32_t)((w * 2 + (r & 1)) * BR_HD), da + (uint64_t)(((k16 >> 2) * 16384 + (k16 & 3) * 32) >> 4),
-                                             db + (uint64_t)(((k16 >> 2) * 8192 + (k16 & 3) * 32) >> 4), idesc, k16 != 0 ? 1u : 0u);
-                            umma_commit(&bars->acc_full[w][r & 1]);
-                        }
+                go = mbar_wait(&bars->w_full, 0, abort_flag, 5);
+#pragma unroll 1
+                for (int i = 0; go; ++i) {
+                    const int r = i / IG, g = i - r * IG;
+                    if (r >= rounds) break;
+                    if (r >= count_of(g)) continue;
+                    const int st = it % L::A_STAGES;
+                    go = mbar_wait(&bars->a_full[st], (uint32_t)((it / L::A_STAGES) & 1), abort_flag, 3);
+                    const uint64_t da = umma_desc_k_sw128(smem_u32(sm + st * L::OP_BYTES));
+#pragma unroll 1
+                    for (int s = 0; s < steps && go; ++s) {
+                        const int w = IG == 1 ? s : g;
+                        if (r >= 2) go = mbar_wait(&bars->acc_empty[w][r & 1], (uint32_t)(((r >> 1) - 1) & 1), abort_flag, 4);
                         if (!go) break;
-                        umma_commit(&bars->a_empty[st]);
-                        ++it;
-                        if (copied < all) {                       // the stage just read serves tile it + 1 (products take a few hundred cycles)
-                            go = mbar_wait(&bars->a_empty[st], (uint32_t)(((it - 1) / L::A_STAGES) & 1), abort_flag, 2);
-                            if (go) copy_next();
-                        }
+                        tc_fence_after_sync();
+                        const uint64_t db = umma_desc_k_sw128(smem_u32(sm + L::B + s * L::B_STEP));
+#pragma unroll
+                        for (int k16 = 0; k16 < 4 * ATOMS; ++k16)
+                            umma_bf16_ss(tmem + (uint32_t)((w * 2 + (r & 1)) * BR_HD), da + (uint64_t)(((k16 >> 2) * 16384 + (k16 & 3) * 32) >> 4),
+                                         db + (uint64_t)(((k16 >> 2) * 8192 + (k16 & 3) * 32) >> 4), idesc, k16 != 0 ? 1u : 0u);
+                        umma_commit(&bars->acc_full[w][r & 1]);
+                    }
+                    if (!go) break;
+                    umma_commit(&bars->a_empty[st]);
+                    ++it;
+                    if (copied < all) {                           // the stage just read serves tile it + 1 (products take a few hundred cycles)
+                        go = mbar_wait(&bars->a_empty[st], (uint32_t)(((it - 1) / L::A_STAGES) & 1), abort_flag, 2);
+                        if (go) copy_next();
                     }
                 }
                 umma_commit(&bars->drain);
@@ -277,35 +255,72 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
         }
     } else {
         // ---------------------------------------------------------------- epilogue: a thread a slot
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+        {   // W of every step, fp16, K-major rows of 64 state channels, 128-byte swizzle: a thread packs 8 channels of one output column
+            const float scale = SILU ? 0.5f * W_SCALE : W_SCALE;      // SiLU(x) = h + h tanh(h), h = x / 2
+            for (int i = tid; i < N * 8; i += EPI_WARPS * 32) {
+                const int d = i & 63, c = (i >> 6) * 8;
+                float w[8], l2r[8];
+    #pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = a.W[(size_t)(c + e) * D + h * BR_HD + d] * scale;
+                    l2r[e] = log2f(br.rhos[c + e]);
+                }
+                unsigned char* dst = sm + L::B + (c >> 6) * 8192 + d * 128 + ((((c & 63) >> 3) ^ (d & 7)) << 4);
+                for (int s = 0; s < steps; ++s) {
+                    float x[8];
+    #pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = w[e] * exp2f((float)(j0 + s) * l2r[e]);
+                    *reinterpret_cast<uint4*>(dst + s * L::B_STEP) = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
+                }
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->w_full);
         const int group = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const int jj = IG == 1 ? group : 0, j = j0 + jj;
         const int g = IG == 1 ? 0 : group;
-        int mine = 0;
-#pragma unroll
-        for (int x = 0; x < IG; ++x)
-            if (x == g) mine = tiles[x];
+        const int mine = count_of(g);
         if (jj < steps && mine > 0) {
             const int me = me0 + g;
             Cursor cur;
             cur.start(work, lists, total, workers, me, lane);
             const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * 2 * BR_HD);
-            float* q_sh = reinterpret_cast<float*>(sm + L::Q) + warp * 64;            // a copy a warp: the warps of a group never meet
+            uint32_t* q_sh = reinterpret_cast<uint32_t*>(sm + L::Q) + warp * 32;      // bf16; a copy a warp: the warps of a group never meet
             const uint32_t q_at = smem_u32(q_sh);
-            const uint32_t e_row = smem_u32(sm) + L::EK + row * 128;
-            const uint32_t flip = (uint32_t)(row & 7) << 4;
+            const uint32_t e_row = smem_u32(sm) + L::EK + row * 128 + ((uint32_t)(row & 7) << 4);       // piece c of the row: ^ c * 16
+            auto q_of = [&](int list) {
+                return reinterpret_cast<const uint32_t*>(a.q)[((((size_t)a.row_branch(list) * a.n + j) * a.H + h) * BR_HD) / 2 + lane];
+            };
+            int q_list = cur.list;                                // the list whose q has been fetched
+            uint32_t q_next = q_of(q_list);
             float m = -INFINITY, l = 0.f, o[64];
             int staged = -1;
             const uint32_t* bits = nullptr;
             bool fresh = true, go = true;
+            // this tile's number among the CTA's, as a stage and its use: tiles of one round lie one behind another
+            int st = 0, use = 0;
+            auto forward = [&](int by) {
+                st += by;
+                while (st >= L::E_STAGES) { st -= L::E_STAGES; ++use; }
+            };
+            int others[IG];                                       // tiles of the CTA's workers
+#pragma unroll
+            for (int x = 0; x < IG; ++x) others[x] = count_of(x);
+#pragma unroll
+            for (int x = 0; x < IG; ++x) forward(x < g && others[x] > 0 ? 1 : 0);
+#pragma unroll 1
             for (int r = 0; r < mine && go; ++r) {
-                if (fresh) {                                      // a new list: its row's q, scaled to base-2 scores
+                if (fresh) {                                      // a new list: its row's q
                     const int64_t branch = a.row_branch(cur.list);
                     const bool prefix = a.row_is_prefix(cur.list);
-                    const uint32_t x = reinterpret_cast<const uint32_t*>(a.q)[((((size_t)branch * a.n + j) * a.H + h) * BR_HD) / 2 + lane];
+                    const uint32_t x = q_list == cur.list ? q_next : q_of(cur.list);
                     __syncwarp();
-                    *reinterpret_cast<float2*>(q_sh + 2 * lane) = make_float2(bf16_lo(x) * BR_SCORE_LOG2, bf16_hi(x) * BR_SCORE_LOG2);
+                    q_sh[lane] = x;
                     __syncwarp();
+                    q_list = min(cur.list + 1, lists - 1);
+                    q_next = q_of(q_list);
                     staged = lane < j ? (prefix ? br.st_pos : br.st_own)[br_index(br, branch, lane)] : -1;
                     bits = prefix ? br.touched + (size_t)branch * ((br.Kcap + 31) / 32) : nullptr;
                     m = -INFINITY;
@@ -314,10 +329,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     for (int i = 0; i < 64; ++i) o[i] = 0.f;
                     fresh = false;
                 }
-                int it = 0;                                       // number of this tile among the CTA's
-#pragma unroll
-                for (int x = 0; x < IG; ++x) it += min(x < g ? r + 1 : r, tiles[x]);
-                const int st = it % L::E_STAGES;
                 const int k_w = cur.k + quarter * 32;             // this warp's 32 slots
                 unsigned hide = 0u;
                 if (bits && k_w < br.Kcap) hide = bits[k_w >> 5];
@@ -328,33 +339,40 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 const bool hidden = ((hide >> lane) & 1u) || k_w + lane >= cur.count;
                 const uint32_t e_at = e_row + st * L::E_STAGE, t_at = taddr + (uint32_t)((r & 1) * BR_HD);
                 go = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[group][r & 1], (uint32_t)((r >> 1) & 1), abort_flag, 8));
-                if (go) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_full[st], (uint32_t)((it / L::E_STAGES) & 1), abort_flag, 9));
+                if (go) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_full[st], (uint32_t)(use & 1), abort_flag, 9));
                 if (!go) break;
                 tc_fence_after_sync();
-                float s0 = 0.f, s1 = 0.f, v[2][16];               // 16 channels at a time, the next ones on their way
-                tmem_ld16_nb(t_at, v[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float (&g16)[16] = v[c & 1];
-                    const uint4 e0 = lds128(e_at + (((c * 2) << 4) ^ flip)), e1 = lds128(e_at + (((c * 2 + 1) << 4) ^ flip));
+                // 16 channels at a time, the next ones on their way.  The gate of the first 32 goes back to TMEM, the other 32 stay.
+                float s0 = 0.f, s1 = 0.f, v0[16], v1[16];
+                auto score = [&](float (&g16)[16], int c) {
+                    const uint4 e0 = lds128<0>(e_at ^ (c << 5)), e1 = lds128<0>(e_at ^ ((c << 5) | 16));
                     const uint32_t e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
-                    tmem_wait_ld16(g16);
-                    if (c < 3) tmem_ld16_nb(t_at + (uint32_t)((c + 1) * 16), v[(c + 1) & 1]);
                     if (SILU) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) g16[i] = fmaf(g16[i], tanh_approx(g16[i]), g16[i]);
-                        tmem_st_32x32b_x16(t_at + (uint32_t)(c * 16), g16);
+                        if (c < 2) tmem_st_32x32b_x16(t_at + (uint32_t)(c * 16), g16);
                     }
+                    const uint4 qa = lds128<0>(q_at + c * 32), qb = lds128<16>(q_at + c * 32);
+                    const uint32_t q[8] = {qa.x, qa.y, qa.z, qa.w, qb.x, qb.y, qb.z, qb.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 q = lds_f4(q_at + c * 64 + i * 16);
-                        s0 = fmaf(bf16_lo(e[2 * i]) * q.x, g16[4 * i], s0);
-                        s1 = fmaf(bf16_hi(e[2 * i]) * q.y, g16[4 * i + 1], s1);
-                        s0 = fmaf(bf16_lo(e[2 * i + 1]) * q.z, g16[4 * i + 2], s0);
-                        s1 = fmaf(bf16_hi(e[2 * i + 1]) * q.w, g16[4 * i + 3], s1);
+                    for (int i = 0; i < 8; ++i) {                 // (the product of two bf16 is exact in fp32, and needs no unpacking)
+                        float x = 0.f, y = 0.f;
+                        fma_f32_bf16x2(x, y, e[i], q[i]);
+                        s0 = fmaf(x, g16[2 * i], s0);
+                        s1 = fmaf(y, g16[2 * i + 1], s1);
                     }
+                };
+                tmem_ld16_nb(t_at, v0);
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    tmem_wait_ld16(v0);
+                    tmem_ld16_nb(t_at + (uint32_t)((c + 1) * 16), v1);
+                    score(v0, c);
+                    tmem_wait_ld16(v1);
+                    if (c < 2) tmem_ld16_nb(t_at + 32, v0);
+                    score(v1, c + 1);
                 }
-                const float x = s0 + s1;
+                const float x = (s0 + s1) * BR_SCORE_LOG2;
                 const bool grow = !hidden && x > m + 8.0f;        // o is scaled again only where the maximum moves by more than 2^8
                 if (__any_sync(0xffffffffu, grow)) {
                     const float alpha = grow ? ex2_approx(m - x) : 1.0f;
@@ -365,29 +383,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 }
                 const float p = hidden ? 0.f : ex2_approx(x - m);
                 l += p;
-                if (SILU) tmem_wait_st();
-                tmem_ld16_nb(t_at, v[0]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float (&g16)[16] = v[c & 1];
-                    const uint4 e0 = lds128(e_at + 16384 + (((c * 2) << 4) ^ flip)), e1 = lds128(e_at + 16384 + (((c * 2 + 1) << 4) ^ flip));
+                auto values = [&](float (&g16)[16], auto chunk) {
+                    constexpr int c = decltype(chunk)::value;
+                    const uint4 e0 = lds128<16384>(e_at ^ (c << 5)), e1 = lds128<16384>(e_at ^ ((c << 5) | 16));
                     const uint32_t e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
-                    tmem_wait_ld16(g16);
-                    if (c < 3) tmem_ld16_nb(t_at + (uint32_t)((c + 1) * 16), v[(c + 1) & 1]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {                 // (a hidden slot's value that is not finite: the row lists the same slot as its own)
                         o[c * 16 + 2 * i] = fmaf(p * g16[2 * i], bf16_lo(e[i]), o[c * 16 + 2 * i]);
                         o[c * 16 + 2 * i + 1] = fmaf(p * g16[2 * i + 1], bf16_hi(e[i]), o[c * 16 + 2 * i + 1]);
                     }
-                }
+                };
+                values(v0, std::integral_constant<int, 2>());
+                if (SILU) tmem_wait_st();
+                tmem_ld16_nb(t_at, v0);
+                values(v1, std::integral_constant<int, 3>());
+                tmem_wait_ld16(v0);
+                tmem_ld16_nb(t_at + 16, v1);
+                values(v0, std::integral_constant<int, 0>());
+                tmem_wait_ld16(v1);
+                values(v1, std::integral_constant<int, 1>());
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&bars->acc_empty[group][r & 1]);
                     mbar_arrive(&bars->e_empty[st]);
                 }
+                int by = 0;                                       // to this worker's tile of the next round
+#pragma unroll
+                for (int x = 0; x < IG; ++x) by += (x < g ? r + 1 : r) < others[x];
+                forward(by);
                 const int list = cur.list;
-                const bool more = cur.next(work);
+                const bool more = cur.next(work, lists);
                 if (!more || cur.list != list) {                  // the list or the stretch ends: join the lanes, two channels each
                     float M = m;
 #pragma unroll
