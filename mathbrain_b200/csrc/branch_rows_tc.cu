@@ -7,8 +7,8 @@
 // own running maximum, sum and o[64] over the tiles of a list, and only where the list (or the worker's stretch) ends do the 32 lanes of
 // a warp join.  The gate goes back to TMEM between the two passes (q.K; P.V), since 64 of its values beside o[64] do not fit the registers.
 //
-// Roles: three epilogue groups of four warps; two warps gather the E_k and E_v rows (cp.async, mbarrier arrivals), one lane copies the
-// operands and issues the products.  With one step the groups are workers with stretches of their own, a tile each in turn; with
+// Roles: three epilogue groups of four warps; two warps gather the E_k and E_v rows (cp.async, mbarrier arrivals), one lane copies
+// the operands, one issues the products.  With one step the groups are workers with stretches of their own, a tile each in turn; with
 // two or three steps they take the same tile, a step each.
 // Bound by the FMA and ALU instructions of the two passes (eight a slot, channel and step, one MUFU among them).
 #include <algorithm>
@@ -23,30 +23,31 @@ namespace brows {
 using namespace ptx;
 
 static constexpr int TILE = BR_TILE, GROUPS = 3, EPI_WARPS = 4 * GROUPS, THREADS = (EPI_WARPS + 4) * 32;
-static constexpr int WARP_K = EPI_WARPS, WARP_V = EPI_WARPS + 1, WARP_MMA = EPI_WARPS + 2;
+static constexpr int WARP_K = EPI_WARPS, WARP_V = EPI_WARPS + 1, WARP_MMA = EPI_WARPS + 2, WARP_A = EPI_WARPS + 3;
 // setmaxnreg: 12 * 32 * 144 (epilogue) + 4 * 32 * 80 (producers) = the launch allocation 512 * 128
 static constexpr float W_SCALE = 64.0f;           // undoes BR_OP_SCALE
 
 template <int ATOMS>                               // of 64 state channels
 struct Smem {
-    static constexpr int A_STAGES = 2, E_STAGES = ATOMS == 1 ? 5 : 3, OP_BYTES = ATOMS * 16384;
+    static constexpr int A_STAGES = ATOMS == 1 ? 4 : 2, E_STAGES = ATOMS == 1 ? 4 : 3, OP_BYTES = ATOMS * 16384;
     static constexpr int EK = A_STAGES * OP_BYTES, EV = EK + 16384, E_STAGE = 32768;
-    static constexpr int B = EK + E_STAGES * E_STAGE, B_STEP = ATOMS * 8192, Q = B + GROUPS * B_STEP, BARS = Q + EPI_WARPS * 128, BYTES = BARS + 256 + 1024;
+    static constexpr int B = EK + E_STAGES * E_STAGE, B_STEP = ATOMS * 8192, Q = B + GROUPS * B_STEP, BARS = Q + EPI_WARPS * 128, BYTES = BARS + 320 + 1024;
 };
 
 struct Bars {
-    uint64_t a_full[2];            // operands have landed                                     (1 arrival and their bytes)
-    uint64_t a_empty[2];           // every product that reads them has completed              (1 commit)
-    uint64_t e_full[5];            // E rows have landed                                       (64: the lanes of both gathering warps)
-    uint64_t e_empty[5];           // every epilogue warp of the tile has read them            (4 a step)
+    uint64_t a_full[4];            // operands have landed                                     (1 arrival and their bytes)
+    uint64_t a_empty[4];           // every product that reads them has completed              (1 commit)
+    uint64_t e_full[4];            // E rows have landed                                       (64: the lanes of both gathering warps)
+    uint64_t e_empty[4];           // every epilogue warp of the tile has read them            (4 a step)
     uint64_t acc_full[GROUPS][2];  // gate product of a group's tile done                      (1 commit)
     uint64_t acc_empty[GROUPS][2]; // the group's warps have read its accumulators a second time (4)
     uint64_t w_full;               // W of every step is laid out                              (12: the epilogue warps)
     uint64_t drain;                // every product has completed (teardown)                   (1 commit)
     uint32_t tmem_base;
     int abort_flag;
+    int tiles[GROUPS];             // of the CTA's workers
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+static_assert(sizeof(Bars) <= 320, "barrier block");
 
 struct Cursor {                    // a worker's place in the lists
     int list, left, k, count, end; // left tiles of this list from slot k on; end: of the stretch, in tiles
@@ -134,6 +135,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
         mbar_init(&bars->w_full, EPI_WARPS);
         mbar_init(&bars->drain, 1);
         bars->abort_flag = *reinterpret_cast<volatile int*>(br.status);
+        for (int g = 0; g < IG; ++g)
+            bars->tiles[g] = me0 + g < workers ? branch_cut(total, workers, me0 + g + 1) - branch_cut(total, workers, me0 + g) : 0;
         fence_barrier_init();
     }
     if (warp == WARP_MMA) {
@@ -145,9 +148,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
     tc_fence_after_sync();
     const uint32_t tmem = bars->tmem_base;
     // tiles of this CTA's workers; the CTA's tiles are numbered round by round
-    auto count_of = [&](int g) { return me0 + g < workers ? branch_cut(total, workers, me0 + g + 1) - branch_cut(total, workers, me0 + g) : 0; };
     int rounds = 0;
-    for (int g = 0; g < IG; ++g) rounds = max(rounds, count_of(g));
+#pragma unroll
+    for (int g = 0; g < IG; ++g) rounds = max(rounds, bars->tiles[g]);
+    const volatile int* count_of = bars->tiles;
 
     if (warp >= EPI_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -167,14 +171,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             };
 #pragma unroll 1
             for (int g = 0; g < IG; ++g)
-                if (count_of(g) > 0) { cur[g].start(work, lists, total, workers, me0 + g, lane); fetch_ids(g); }
+                if (count_of[g] > 0) { cur[g].start(work, lists, total, workers, me0 + g, lane); fetch_ids(g); }
             int st = 0, use = 0;
             bool go = true;
 #pragma unroll 1
             for (int i = 0; go; ++i) {                            // (loops kept rolled: a launch fetches its code cold)
                 const int r = i / IG, g = i - r * IG;
                 if (r >= rounds) break;
-                if (r >= count_of(g)) continue;
+                if (r >= count_of[g]) continue;
                 if (use > 0) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 1));
                 if (!go) break;
                 uint32_t at = st * L::E_STAGE;
@@ -194,64 +198,64 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 if (cur[g].next(work, lists)) fetch_ids(g);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-        } else if (warp == WARP_MMA) {
-            // ------------------------------------------------------------ one lane: operand copies, a stage or more ahead, and all products
+        } else if (warp == WARP_A) {
+            // ------------------------------------------------------------ operand copies
             Cursor cur[IG];
 #pragma unroll 1
             for (int g = 0; g < IG; ++g)
-                if (count_of(g) > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
+                if (count_of[g] > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
             if (lane == 0) {
-                int all = 0;
-                for (int g = 0; g < IG; ++g) all += count_of(g);
-                const uint32_t idesc = umma_idesc_16(TILE, BR_HD, 0, 0, 0, 0);
-                int it = 0, copied = 0, cr = 0, cg = 0;
+                int st = 0, use = 0;
                 bool go = true;
-                auto copy_next = [&]() {                          // operands of the next tile in order, into a stage that is free
-                    while (cr >= count_of(cg))                    // (cr, cg): the next tile that exists
-                        if (++cg == IG) { cg = 0; ++cr; }
-                    const int st = copied % L::A_STAGES;
-                    mbar_expect_tx(&bars->a_full[st], L::OP_BYTES);
-                    bulk_load(sm + st * L::OP_BYTES, a.row_operands(cur[cg].list) + (size_t)(cur[cg].k / TILE) * L::OP_BYTES, L::OP_BYTES, &bars->a_full[st]);
-                    cur[cg].next(work, lists);
-                    ++copied;
-                    if (++cg == IG) { cg = 0; ++cr; }
-                };
-                while (copied < min(L::A_STAGES, all)) copy_next();
-                go = mbar_wait(&bars->w_full, 0, abort_flag, 5);
 #pragma unroll 1
                 for (int i = 0; go; ++i) {
                     const int r = i / IG, g = i - r * IG;
                     if (r >= rounds) break;
-                    if (r >= count_of(g)) continue;
-                    const int st = it % L::A_STAGES;
-                    go = mbar_wait(&bars->a_full[st], (uint32_t)((it / L::A_STAGES) & 1), abort_flag, 3);
-                    const uint64_t da = umma_desc_k_sw128(smem_u32(sm + st * L::OP_BYTES));
-#pragma unroll 1
-                    for (int s = 0; s < steps && go; ++s) {
-                        const int w = IG == 1 ? s : g;
-                        if (r >= 2) go = mbar_wait(&bars->acc_empty[w][r & 1], (uint32_t)(((r >> 1) - 1) & 1), abort_flag, 4);
-                        if (!go) break;
-                        tc_fence_after_sync();
-                        const uint64_t db = umma_desc_k_sw128(smem_u32(sm + L::B + s * L::B_STEP));
-#pragma unroll
-                        for (int k16 = 0; k16 < 4 * ATOMS; ++k16)
-                            umma_bf16_ss(tmem + (uint32_t)((w * 2 + (r & 1)) * BR_HD), da + (uint64_t)(((k16 >> 2) * 16384 + (k16 & 3) * 32) >> 4),
-                                         db + (uint64_t)(((k16 >> 2) * 8192 + (k16 & 3) * 32) >> 4), idesc, k16 != 0 ? 1u : 0u);
-                        umma_commit(&bars->acc_full[w][r & 1]);
-                    }
+                    if (r >= count_of[g]) continue;
+                    if (use > 0) go = mbar_wait(&bars->a_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 2);
                     if (!go) break;
-                    umma_commit(&bars->a_empty[st]);
-                    ++it;
-                    if (copied < all) {                           // the stage just read serves tile it + 1 (products take a few hundred cycles)
-                        go = mbar_wait(&bars->a_empty[st], (uint32_t)(((it - 1) / L::A_STAGES) & 1), abort_flag, 2);
-                        if (go) copy_next();
-                    }
+                    mbar_expect_tx(&bars->a_full[st], L::OP_BYTES);
+                    bulk_load(sm + st * L::OP_BYTES, a.row_operands(cur[g].list) + (size_t)(cur[g].k / TILE) * L::OP_BYTES, L::OP_BYTES, &bars->a_full[st]);
+                    cur[g].next(work, lists);
+                    if (++st == L::A_STAGES) { st = 0; ++use; }
                 }
-                umma_commit(&bars->drain);
-                for (; !go && it < copied; ++it)                  // given up: operand copies still on their way
-                    mbar_wait(&bars->a_full[it % L::A_STAGES], (uint32_t)((it / L::A_STAGES) & 1), abort_flag, 6);
-                mbar_wait(&bars->drain, 0, abort_flag, 7);
+                // given up: copies that may still be on their way (a wait that gives up returns soon after)
+                for (int i = 0; !go && i < L::A_STAGES; ++i) {
+                    const int uses = use + (i < st);               // times stage i was filled
+                    if (uses > 0) mbar_wait(&bars->a_full[i], (uint32_t)((uses - 1) & 1), abort_flag, 6);
+                }
             }
+        } else if (warp == WARP_MMA && lane == 0) {
+            // ------------------------------------------------------------ all products
+            const uint32_t idesc = umma_idesc_16(TILE, BR_HD, 0, 0, 0, 0);
+            int st = 0, use = 0;
+            bool go = mbar_wait(&bars->w_full, 0, abort_flag, 5);
+#pragma unroll 1
+            for (int i = 0; go; ++i) {
+                const int r = i / IG, g = i - r * IG;
+                if (r >= rounds) break;
+                if (r >= count_of[g]) continue;
+                go = mbar_wait(&bars->a_full[st], (uint32_t)(use & 1), abort_flag, 3);
+                const uint64_t da = umma_desc_k_sw128(smem_u32(sm + st * L::OP_BYTES));
+#pragma unroll 1
+                for (int s = 0; s < steps && go; ++s) {
+                    const int w = IG == 1 ? s : g;
+                    if (r >= 2) go = mbar_wait(&bars->acc_empty[w][r & 1], (uint32_t)(((r >> 1) - 1) & 1), abort_flag, 4);
+                    if (!go) break;
+                    tc_fence_after_sync();
+                    const uint64_t db = umma_desc_k_sw128(smem_u32(sm + L::B + s * L::B_STEP));
+#pragma unroll
+                    for (int k16 = 0; k16 < 4 * ATOMS; ++k16)
+                        umma_bf16_ss(tmem + (uint32_t)((w * 2 + (r & 1)) * BR_HD), da + (uint64_t)(((k16 >> 2) * 16384 + (k16 & 3) * 32) >> 4),
+                                     db + (uint64_t)(((k16 >> 2) * 8192 + (k16 & 3) * 32) >> 4), idesc, k16 != 0 ? 1u : 0u);
+                    umma_commit(&bars->acc_full[w][r & 1]);
+                }
+                if (!go) break;
+                umma_commit(&bars->a_empty[st]);
+                if (++st == L::A_STAGES) { st = 0; ++use; }
+            }
+            umma_commit(&bars->drain);
+            mbar_wait(&bars->drain, 0, abort_flag, 7);
         }
     } else {
         // ---------------------------------------------------------------- epilogue: a thread a slot
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
         const int group = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const int jj = IG == 1 ? group : 0, j = j0 + jj;
         const int g = IG == 1 ? 0 : group;
-        const int mine = count_of(g);
+        const int mine = count_of[g];
         if (jj < steps && mine > 0) {
             const int me = me0 + g;
             Cursor cur;
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             };
             int others[IG];                                       // tiles of the CTA's workers
 #pragma unroll
-            for (int x = 0; x < IG; ++x) others[x] = count_of(x);
+            for (int x = 0; x < IG; ++x) others[x] = count_of[x];
 #pragma unroll
             for (int x = 0; x < IG; ++x) forward(x < g && others[x] > 0 ? 1 : 0);
 #pragma unroll 1
