@@ -367,16 +367,16 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
         };
         int first;
         if (br.S == 1) {
-            np = 4 * pieces(work + a.row_work, a.row_lists, b, a.row_workers, 1, first);
+            np = 4 * pieces(work + a.row_work, a.row_lists, 2 * b, a.row_workers, 1, first);
             p_step = each;
-            p0 = (size_t)a.row_part0 + (size_t)(b + first) * 4 * each + at;
+            p0 = (size_t)a.row_part0 + (size_t)(2 * b + first) * 4 * each + at;
         } else {
             const int list = b * a.blocks + s / BR_BLOCK;
             np = pieces(work, a.n_pre, list, a.pre_workers, BR_LEAST_UNITS, first);
             p_step = BR_BLOCK * each;
             p0 = ((size_t)(list + first) * BR_BLOCK + s % BR_BLOCK) * each + at;
         }
-        const int list = (br.S == 1 ? (int)br.B : 0) + (int)r;
+        const int list = br.S == 1 ? 2 * b + 1 : (int)r;
         nq = 4 * pieces(work + a.row_work, a.row_lists, list, a.row_workers, 1, first);
         q_step = each;
         q0 = (size_t)a.row_part0 + (size_t)(list + first) * 4 * each + at;

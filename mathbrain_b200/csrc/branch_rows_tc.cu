@@ -95,7 +95,6 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     return r;
 }
 
-// lists: [B prefixes (S = 1)] [B S own]
 template <int ATOMS, int IG, bool SILU>
 __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW) {
     using L = Smem<ATOMS>;
@@ -169,33 +168,34 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
 #pragma unroll
                 for (int i = 0; i < 4; ++i) ids[g][i] = slots[min(cur[g].k + 32 * i + lane, cur[g].count - 1)];
             };
-#pragma unroll 1
+#pragma unroll
             for (int g = 0; g < IG; ++g)
                 if (count_of[g] > 0) { cur[g].start(work, lists, total, workers, me0 + g, lane); fetch_ids(g); }
             int st = 0, use = 0;
             bool go = true;
 #pragma unroll 1
-            for (int i = 0; go; ++i) {                            // (loops kept rolled: a launch fetches its code cold)
-                const int r = i / IG, g = i - r * IG;
-                if (r >= rounds) break;
-                if (r >= count_of[g]) continue;
-                if (use > 0) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 1));
-                if (!go) break;
-                uint32_t at = st * L::E_STAGE;
-                int id[4] = {ids[g][0], ids[g][1], ids[g][2], ids[g][3]};
-#pragma unroll 1
-                for (int part = 0; part < 4; ++part) {            // 32 rows at a time: rows 4 x + sub
+            for (int r = 0; r < rounds && go; ++r) {
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, id[0], x * 4 + sub);
-                        cp_async16(at + ((x & 1) ? odd : even) + (x >> 1) * 1024, table + (uint64_t)v * D2);
+                for (int g = 0; g < IG; ++g) {
+                    if (!go || r >= count_of[g]) continue;
+                    if (use > 0) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_empty[st], (uint32_t)((use - 1) & 1), abort_flag, 1));
+                    if (!go) continue;
+                    uint32_t at = st * L::E_STAGE;
+                    int id[4] = {ids[g][0], ids[g][1], ids[g][2], ids[g][3]};
+#pragma unroll 1
+                    for (int part = 0; part < 4; ++part) {        // 32 rows at a time: rows 4 x + sub
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const uint32_t v = (uint32_t)__shfl_sync(0xffffffffu, id[0], x * 4 + sub);
+                            cp_async16(at + ((x & 1) ? odd : even) + (x >> 1) * 1024, table + (uint64_t)v * D2);
+                        }
+                        at += 4096;
+                        id[0] = id[1]; id[1] = id[2]; id[2] = id[3];
                     }
-                    at += 4096;
-                    id[0] = id[1]; id[1] = id[2]; id[2] = id[3];
+                    cp_async_arrive(&bars->e_full[st]);
+                    if (++st == L::E_STAGES) { st = 0; ++use; }
+                    if (cur[g].next(work, lists)) fetch_ids(g);
                 }
-                cp_async_arrive(&bars->e_full[st]);
-                if (++st == L::E_STAGES) { st = 0; ++use; }
-                if (cur[g].next(work, lists)) fetch_ids(g);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         } else if (warp == WARP_A) {
@@ -334,13 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     fresh = false;
                 }
                 const int k_w = cur.k + quarter * 32;             // this warp's 32 slots
-                unsigned hide = 0u;
-                if (bits && k_w < br.Kcap) hide = bits[k_w >> 5];
-                if (j > 0) {
-                    const unsigned d = (unsigned)(staged - k_w);
-                    hide |= __reduce_or_sync(0xffffffffu, d < 32u ? 1u << d : 0u);
-                }
-                const bool hidden = ((hide >> lane) & 1u) || k_w + lane >= cur.count;
+                const unsigned touched = bits && k_w < br.Kcap ? bits[k_w >> 5] : 0u;
                 const uint32_t e_at = e_row + st * L::E_STAGE, t_at = taddr + (uint32_t)((r & 1) * BR_HD);
                 go = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[group][r & 1], (uint32_t)((r >> 1) & 1), abort_flag, 8));
                 if (go) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_full[st], (uint32_t)(use & 1), abort_flag, 9));
@@ -376,6 +370,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     if (c < 2) tmem_ld16_nb(t_at + 32, v0);
                     score(v1, c + 1);
                 }
+                unsigned hide = touched;
+                if (j > 0) {
+                    const unsigned d = (unsigned)(staged - k_w);
+                    hide |= __reduce_or_sync(0xffffffffu, d < 32u ? 1u << d : 0u);
+                }
+                const bool hidden = ((hide >> lane) & 1u) || k_w + lane >= cur.count;
                 const float x = (s0 + s1) * BR_SCORE_LOG2;
                 const bool grow = !hidden && x > m + 8.0f;        // o is scaled again only where the maximum moves by more than 2^8
                 if (__any_sync(0xffffffffu, grow)) {

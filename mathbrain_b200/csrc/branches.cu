@@ -147,14 +147,14 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
 // state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head, in the layouts that branches.cuh gives.
 // grid: x = shares of a list, y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sums of the
 // lists' units that the attention deals its work by.
-__device__ int running_sum(const mbema_branches& br, int2* out, int lists, int unit, bool prefixes, int blocks) {
+template <typename Count>
+__device__ void running_sum(int2* out, int lists, int unit, Count count_of) {
     __shared__ int s_warp[8];
     const int tid = threadIdx.x, lane = tid & 31;
-    const int n_pre = prefixes ? (int)br.B * blocks : 0;
     int base = 0;
     for (int x0 = 0; x0 < lists; x0 += 256) {
         const int x = x0 + tid;
-        const int count = x >= lists ? 0 : x < n_pre ? min(br.n_active[x / blocks], (int)br.Kcap) : br.own_n[x - n_pre];
+        const int count = x < lists ? count_of(x) : 0;
         const int c = (count + unit - 1) / unit;
         int sum = c;
 #pragma unroll
@@ -174,7 +174,6 @@ __device__ int running_sum(const mbema_branches& br, int2* out, int lists, int u
         __syncthreads();
     }
     if (tid == 0) out[lists] = make_int2(base, 0);
-    return base;
 }
 
 __device__ __forceinline__ void decayed(float (&f)[8], const float* src, float dt, const float (&l2r)[8]) {
@@ -194,8 +193,10 @@ __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
         const int blocks = (int)((br.S + BR_BLOCK - 1) / BR_BLOCK), n_pre = br.S > 1 ? (int)br.B * blocks : 0;
         int2* work = reinterpret_cast<int2*>(br.work);
         if (blockIdx.x == 0 && blockIdx.z == 0) {
-            running_sum(br, work, n_pre, 16, true, blocks);
-            running_sum(br, work + n_pre + 1, (int)(br.B * br.S + (br.S == 1 ? br.B : 0)), BR_TILE, br.S == 1, 1);
+            auto prefix = [&](int b) { return min(br.n_active[b], (int)br.Kcap); };
+            running_sum(work, n_pre, 16, [&](int x) { return prefix(x / blocks); });
+            if (br.S == 1) running_sum(work + 1, (int)(2 * br.B), BR_TILE, [&](int x) { return x & 1 ? br.own_n[x >> 1] : prefix(x >> 1); });
+            else running_sum(work + n_pre + 1, (int)(br.B * br.S), BR_TILE, [&](int x) { return br.own_n[x]; });
         }
         return;
     }

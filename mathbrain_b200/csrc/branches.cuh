@@ -55,13 +55,15 @@ struct BranchArgs {
     // tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order.  Prefixes of several
     // branches: lists (sequence, block of sixteen), partials [piece, BR_BLOCK, n, H].
     int n_pre, blocks, pre_workers, ring_bytes, w_offset;
-    // Single rows: lists (the sequences' prefixes, for one branch), the branches' own; partials from row_part0 on, [piece, 4 warps, n, H]
+    // Single rows: the branches' own lists, or, for one branch, prefix and own list of every sequence in turn (a stretch then holds
+    // long and short ones as the others do: a list's start and end cost as much as half a tile); partials from row_part0 on,
+    // [piece, 4 warps, n, H]
     int row_lists, row_work, row_workers;      // their number, where their running sum begins in `work`, workers
     int64_t row_part0;
-    __device__ __forceinline__ bool row_is_prefix(int list) const { return br.S == 1 && list < (int)br.B; }
-    __device__ __forceinline__ int row_branch(int list) const { return br.S == 1 && list >= (int)br.B ? list - (int)br.B : list; }
+    __device__ __forceinline__ bool row_is_prefix(int list) const { return br.S == 1 && !(list & 1); }
+    __device__ __forceinline__ int row_branch(int list) const { return br.S == 1 ? list >> 1 : list; }
     __device__ __forceinline__ const int* row_slots(int list) const {
-        return row_is_prefix(list) ? br.active + (size_t)list * br.Kcap : br.own_slot + (size_t)row_branch(list) * br.cap;
+        return row_is_prefix(list) ? br.active + (size_t)row_branch(list) * br.Kcap : br.own_slot + (size_t)row_branch(list) * br.cap;
     }
     __device__ __forceinline__ const char* row_operands(int list) const;
 };
@@ -69,7 +71,11 @@ struct BranchArgs {
 // The workers that a running sum of `total` units (tiles) occupies, and where their stretches begin.
 __device__ __forceinline__ int branch_workers(int total, int most, int least) { return max(1, min(most, total / least)); }
 static constexpr int BR_LEAST_UNITS = 2;           // a worker's
-__device__ __forceinline__ int branch_cut(int total, int workers, int w) { return (int)((long long)total * w / workers); }
+// total * w / workers in 32 bits (workers below 2^15)
+__device__ __forceinline__ int branch_cut(int total, int workers, int w) {
+    const int q = total / workers, r = total - q * workers;
+    return q * w + r * w / workers;
+}
 // the worker whose stretch holds unit c < total
 __device__ __forceinline__ int branch_worker_of(int total, int workers, int c) {
     return (int)((((long long)c + 1) * workers - 1) / total);
@@ -94,7 +100,7 @@ __device__ __forceinline__ int find_list(const int2* work, int lists, int c, int
 // of word (row / 8) + 2 p (row = k % 16) of lane 4 (row % 8) + t in fragment 2 i + u of its sixteen (512 bytes each).
 __host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + BR_TILE - 1) / BR_TILE) * N * (2 * BR_TILE); }
 __device__ __forceinline__ const char* BranchArgs::row_operands(int list) const {
-    return row_is_prefix(list) ? reinterpret_cast<const char*>(br.pre_op) + (size_t)list * br_operand_bytes(br.Kcap, br.N)
+    return row_is_prefix(list) ? reinterpret_cast<const char*>(br.pre_op) + (size_t)row_branch(list) * br_operand_bytes(br.Kcap, br.N)
                                : reinterpret_cast<const char*>(br.own_op) + (size_t)row_branch(list) * br_operand_bytes(br.cap, br.N);
 }
 
