@@ -383,7 +383,7 @@ typedef struct mbema_branches {
     float* st_state;        /* [B,S,max_new,N] C_q of the staged tokens */
     void* pre_op;           /* [B,ceil128(Kcap),N] fp16 or NULL (with the next three): prefix states at the first staged step, */
     void* own_op;           /* [B,S,ceil128(cap),N] fp16 or NULL: the same of the own slots; operands of the tensor cores, 16-byte aligned */
-    int32_t* work;          /* [B (ceil(S/16) + S) + 2, 2] or NULL: running sums of the lists' units, by which the work is dealt, and lengths */
+    int32_t* work;          /* [B (ceil(S/16) + S) + 1, 2] or NULL: running sum of the lists' units, by which the work is dealt, and lengths */
     int32_t* status;        /* [1] or NULL: status word of the tensor-core attends (see the conventions above) */
     int32_t* overflow;      /* [1] */
     int64_t B, S, V, N, Kcap, cap, max_new;

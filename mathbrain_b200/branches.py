@@ -60,7 +60,7 @@ class Branches:
         if self._tensor_cores:
             self._hold.update(pre_op=torch.empty(B, (Kcap + 127) // 128 * 128, N, dtype=torch.float16, device=dev),
                               own_op=torch.empty(B, S, (cap + 127) // 128 * 128, N, dtype=torch.float16, device=dev),
-                              work=torch.empty(B * ((S + 15) // 16 + S) + 2, 2, **i32), status=torch.zeros(1, **i32))
+                              work=torch.empty(B * ((S + 15) // 16 + S) + 1, 2, **i32), status=torch.zeros(1, **i32))
         self._c = _lib.BranchesStruct(**{k: _ptr(t) for k, t in self._hold.items()}, B=B, S=S, V=V, N=N, Kcap=Kcap, cap=cap,
                                       max_new=max_new)
         self._ref = ctypes.byref(self._c)

@@ -357,29 +357,31 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     if constexpr (PIECES) {
         const int2* work = reinterpret_cast<const int2*>(br.work);
         const size_t each = (size_t)n * H, at = (size_t)j * H + h;
-        auto pieces = [&](const int2* sum, int lists, int list, int most, int least, int& first) {
-            const int lo = sum[list].x, hi = sum[list + 1].x, total = sum[lists].x;
+        const bool one = br.S == 1;
+        const int total = work[a.lists].x, workers = branch_workers(total, a.max_workers, one ? 1 : BR_LEAST_COST);
+        auto pieces = [&](int list, int unit, int& first) {
+            const int lo = work[list].x, hi = work[list + 1].x;
             first = 0;
             if (hi == lo) return 0;
-            const int workers = branch_workers(total, most, least);
             first = branch_worker_of(total, workers, lo);
-            return branch_worker_of(total, workers, hi - 1) - first + 1;
+            return branch_worker_of(total, workers, hi - unit) - first + 1;
         };
-        int first;
-        if (br.S == 1) {
-            np = 4 * pieces(work + a.row_work, a.row_lists, 2 * b, a.row_workers, 1, first);
-            p_step = each;
-            p0 = (size_t)a.row_part0 + (size_t)(2 * b + first) * 4 * each + at;
-        } else {
-            const int list = b * a.blocks + s / BR_BLOCK;
-            np = pieces(work, a.n_pre, list, a.pre_workers, BR_LEAST_UNITS, first);
-            p_step = BR_BLOCK * each;
-            p0 = ((size_t)(list + first) * BR_BLOCK + s % BR_BLOCK) * each + at;
-        }
-        const int list = br.S == 1 ? 2 * b + 1 : (int)r;
-        nq = 4 * pieces(work + a.row_work, a.row_lists, list, a.row_workers, 1, first);
+        const int pre = one ? 2 * b : b * a.blocks + s / BR_BLOCK, own = one ? 2 * b + 1 : a.n_pre + (int)r;
+        int wp, wq;
+        np = pieces(pre, one ? 1 : BR_COST_BLOCK, wp);
+        nq = pieces(own, one ? 1 : BR_COST_OWN, wq);
         q_step = each;
-        q0 = (size_t)a.row_part0 + (size_t)(list + first) * 4 * each + at;
+        if (one) {
+            np *= 4;
+            nq *= 4;
+            p_step = each;
+            p0 = (size_t)(pre + wp) * 4 * each + at;
+            q0 = (size_t)(own + wq) * 4 * each + at;
+        } else {
+            p_step = BR_BLOCK * each;
+            p0 = ((size_t)(pre + wp) * BR_BLOCK + s % BR_BLOCK) * each + at;
+            q0 = (size_t)(a.own_piece0 + r + wq) * each + at;
+        }
     } else {
         const int SP = a.plan.SP, SO = a.plan.SO;
         np = (na + a.plan.chp - 1) / a.plan.chp;
@@ -485,21 +487,24 @@ static int64_t partials(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap
         if (a) a->plan = p;
         return B * S * n * H * (p.SP + p.SO);
     }
+    if (S == 1) {
+        const BranchRows p = branch_rows(n, H);
+        if (a) {
+            a->lists = (int)(2 * B);
+            a->max_workers = p.ctas * p.IG;
+        }
+        return (2 * B + p.ctas * p.IG) * 4 * n * H;
+    }
     const BranchShape p = branch_shape(S, n, H);
-    const BranchRows q = branch_rows(n, H);
-    const int64_t n_pre = S > 1 ? B * p.blocks : 0, pre_workers = (int64_t)p.ctas * p.IG;
-    const int64_t rows = (S == 1 ? B : 0) + B * S, row_workers = (int64_t)q.ctas * q.IG;
-    const int64_t part0 = n_pre ? (n_pre + pre_workers) * BR_BLOCK * n * H : 0;
+    const int64_t n_pre = B * p.blocks, workers = (int64_t)p.ctas * p.IG, own0 = (n_pre + workers) * BR_BLOCK;
     if (a) {
+        a->lists = (int)(n_pre + B * S);
         a->n_pre = (int)n_pre;
         a->blocks = p.blocks;
-        a->pre_workers = (int)pre_workers;
-        a->row_lists = (int)rows;
-        a->row_work = (int)n_pre + 1;
-        a->row_workers = (int)row_workers;
-        a->row_part0 = part0;
+        a->max_workers = (int)workers;
+        a->own_piece0 = own0;
     }
-    return part0 + (rows + row_workers) * 4 * n * H;
+    return (own0 + B * S + workers) * n * H;
 }
 
 extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, int64_t n, int64_t H, int64_t Kcap, int64_t cap, int mode) {
@@ -532,12 +537,7 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     a.ml = reinterpret_cast<float2*>(a.po + (size_t)parts * BR_HD);
     cudaStream_t st = (cudaStream_t)stream;
     const bool tc = mode == MBEMA_MODE_TC_BF16;
-    int rc = MBEMA_OK;
-    if (tc) {
-        if (br->S > 1) rc = launch_branch_attend_tc(a, branch_shape(br->S, n, H), st);
-        if (rc == MBEMA_OK) rc = launch_branch_rows(a, branch_rows(n, H), br->S > 1, st);
-    } else {
-        rc = launch_branch_attend_fp32(a, st);
-    }
+    int rc = !tc ? launch_branch_attend_fp32(a, st)
+             : br->S == 1 ? launch_branch_rows(a, branch_rows(n, H), st) : launch_branch_attend_tc(a, branch_shape(br->S, n, H), st);
     return rc != MBEMA_OK ? rc : launch_branch_merge(a, tc, st);
 }

@@ -1,18 +1,20 @@
-// Attention over the prefix of sequences that several branches share, on the tensor cores (mbema_branches_attend,
-// MBEMA_MODE_TC_BF16).  (The branches' own slots, and the prefix of a single branch: branch_rows_tc.cu.)
+// Attention of branches that share prefixes, on the tensor cores (mbema_branches_attend, MBEMA_MODE_TC_BF16, more than one branch a
+// sequence; a single branch: branch_rows_tc.cu).
 //
 // The states that the rows of one call see differ from the ones at the call's first step by rho^j alone, so the operand copies
 // (fp16, made once by mbema_branches_extend for all layers and steps) are the A operands of every step and rho^j goes into W:
 //     gate(j) = SiLU(A . (rho^j * W)),   16 slots x 64 channels of a head to a warp (mma.sync m16n8k16, fp32 accumulators).
-// The accumulators, K = E_k gate and V = E_v gate stay in registers: the layout of the gate's accumulators is the layout of K as the
-// operand of q.K for sixteen branches, V's 8 x 8 blocks are transposed in registers for P.V, and a thread holds the same 16 channels
-// of slots g and g + 8 in the gate, in the 16-byte pieces that it reads of the E rows, and in q and O.
+// A warp keeps its step's W in registers and its accumulators in the layout that the next operand needs: a thread holds the same
+// 16 channels of slots g and g + 8 in the gate, in the 16-byte pieces that it reads of the E rows, and in q and O.
+// A prefix is walked for sixteen branches at a time (q.K and P.V as products too), a branch's own slots for its row alone.
 //
 // Work is dealt in units of 16 slots: mbema_branches_extend leaves the running sum of all lists' units, every worker (one warp, or
 // the warps of several steps together) takes an equal stretch of it and walks it without a stop; a list is cut where a stretch
 // ends, and each piece leaves a partial (m, l, o[64]) a row.  The operand and E rows of a unit come by cp.async into a ring of
 // shared memory, some units ahead across the ends of lists: they are gathered rows that mostly come from DRAM, and with them loaded
 // a unit ahead into registers half of all cycles were spent waiting.
+// Own slots go through tcgen05 in branch_rows_tc.cu's tiles of 128 slots too, but not faster: its two gathering warps and a list's start
+// and end (own lists are short) took 4 x 16 branches of 400 own slots from 31 us to 45, 64 branches of 180 from 31 to 39.
 #include <algorithm>
 
 #include "branches.cuh"
@@ -107,7 +109,8 @@ __device__ __forceinline__ void build_W(uint32_t dst, const float* W_sh, const f
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * 512 + lane * 16), "r"(x[0]), "r"(x[1]), "r"(y[0]), "r"(y[1]) : "memory");
     }
 }
-// A warp's copy of them in registers (64 a thread for 64 channels; 128 channels have no room for it).
+// A warp's copy of them in registers (64 a thread for 64 channels; 128 channels have no room for it): in shared memory, with twelve warps,
+// 64 samples of a long prompt took 31 us for 25.
 template <int KS, int I = 0>
 __device__ __forceinline__ void read_W(uint4 (&w)[KS * 4], uint32_t at) {
     if constexpr (I < KS * 4) {
@@ -187,7 +190,7 @@ __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
     }
 }
 
-// The prefix of a sequence as a block of its branches reads it.
+// A list of slots: the prefix of a sequence as 16 of its branches read it, or a branch's own slots.
 struct List {
     const int* slots;
     const char* op;           // operands, 16 slots after 16 slots
@@ -196,9 +199,130 @@ struct List {
 
 __device__ __forceinline__ List get_list(const BranchArgs& a, int x, int count) {
     const mbema_branches& br = a.br;
-    const int b = x / a.blocks;
-    return List{br.active + (size_t)b * br.Kcap, reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N), count};
+    List t;
+    t.count = count;
+    if (x < a.n_pre) {
+        const int b = x / a.blocks;
+        t.slots = br.active + (size_t)b * br.Kcap;
+        t.op = reinterpret_cast<const char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, br.N);
+    } else {
+        const int r = x - a.n_pre;
+        t.slots = br.own_slot + (size_t)r * br.cap;
+        t.op = reinterpret_cast<const char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, br.N);
+    }
+    return t;
 }
+
+// bit i: own slot k0 + i (i < 16) is hidden; staged: lane i holds the list place that staged token i < j hides, or -1
+__device__ __forceinline__ unsigned hidden16(int k0, int staged, bool any_staged, int count) {
+    unsigned m = 0u;
+    if (any_staged) {
+        const unsigned d = (unsigned)(staged - k0);
+        m = __reduce_or_sync(0xffffffffu, d < 16u ? 1u << d : 0u);
+    }
+    if (count - k0 < 16) m |= 0xffffffffu << (count - k0);
+    return m;
+}
+
+// One partial of a warp: the eight quads' (m, l, o[16]) joined.  A lane is left with o of channels 32 (x / 4) + 8 t + 2 (x % 4) + {0, 1},
+// x = g with its bits reversed in place: see quad_columns.
+__device__ __forceinline__ void join_quads(float& m, float& l, float (&o)[16], float2& out) {
+    float M = m;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    const float w = M == -INFINITY ? 0.f : exp2f(m - M);
+    l *= w;
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] *= w;
+    const bool b0 = lane & 4, b1 = lane & 8, b2 = lane & 16;
+    float x[8], y[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {          // keep the half that bit 0 of g names
+        const float send = b0 ? o[i] : o[8 + i], keep = b0 ? o[8 + i] : o[i];
+        x[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float send = b1 ? x[i] : x[4 + i], keep = b1 ? x[4 + i] : x[i];
+        y[i] = keep + __shfl_xor_sync(0xffffffffu, send, 8);
+    }
+    const float s0 = b2 ? y[0] : y[2], s1 = b2 ? y[1] : y[3], k0 = b2 ? y[2] : y[0], k1 = b2 ? y[3] : y[1];
+    out.x = k0 + __shfl_xor_sync(0xffffffffu, s0, 16);
+    out.y = k1 + __shfl_xor_sync(0xffffffffu, s1, 16);
+    m = M;
+}
+// first of the two head channels that join_quads leaves in this lane
+__device__ __forceinline__ int quad_columns(int lane) {
+    const int t = lane & 3, i = ((lane >> 2) & 1) * 8 + ((lane >> 3) & 1) * 4 + ((lane >> 4) & 1) * 2;    // index into o[16]
+    return 32 * (i >> 3) + 8 * t + (i & 7);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// One row: q.K and P.V on the CUDA cores, in fp32, straight from the gate's accumulators.  A quad of lanes has its own running
+// maximum and sums, joined at the end of the piece.
+// ---------------------------------------------------------------------------------------------------------------------------
+struct OneRow {
+    float m, l, o[16], q[16];
+    int staged;
+    __device__ __forceinline__ void start(const BranchArgs& a, int64_t r, int j, int h, int lane) {
+        uint32_t x[8];
+        load_q(x, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { q[2 * i] = bf_lo(x[i]) * BR_SCORE_LOG2; q[2 * i + 1] = bf_hi(x[i]) * BR_SCORE_LOG2; }
+        staged = -1;
+        if (lane < j) staged = a.br.st_own[br_index(a.br, r, lane)];
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    }
+    __device__ __forceinline__ void unit(float (&acc)[8][4], uint32_t at_lo, uint32_t at_hi, unsigned hide, int g) {
+        uint32_t e0[8], e1[8];
+        load_E<0>(e0, e1, at_lo, at_hi);
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+            s0 = fmaf(bf_lo(e0[nt]) * q[2 * nt], acc[nt][0], s0);
+            s1 = fmaf(bf_hi(e0[nt]) * q[2 * nt + 1], acc[nt][1], s1);
+            s2 = fmaf(bf_lo(e1[nt]) * q[2 * nt], acc[nt][2], s2);
+            s3 = fmaf(bf_hi(e1[nt]) * q[2 * nt + 1], acc[nt][3], s3);
+        }
+        load_E<2048>(e0, e1, at_lo, at_hi);
+        s0 += s1;
+        s2 += s3;
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
+        const float x0 = (hide >> g) & 1u ? -INFINITY : s0, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2;
+        const float m_new = fmaxf(m, fmaxf(x0, x1));
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float p0 = ex2(x0 - ref), p1 = ex2(x1 - ref);
+        if (__any_sync(0xffffffffu, m_new > m)) {
+            const float alpha = ex2(m - ref);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= alpha;
+        }
+        m = m_new;
+        l += p0 + p1;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {      // (a value that is not finite stays in a row that hides it: the same slot is listed as the branch's own)
+            o[2 * nt] = fmaf(p0 * acc[nt][0], bf_lo(e0[nt]), fmaf(p1 * acc[nt][2], bf_lo(e1[nt]), o[2 * nt]));
+            o[2 * nt + 1] = fmaf(p0 * acc[nt][1], bf_hi(e0[nt]), fmaf(p1 * acc[nt][3], bf_hi(e1[nt]), o[2 * nt + 1]));
+        }
+    }
+    __device__ __forceinline__ void leave(const BranchArgs& a, int64_t piece, int j, int h, int lane) {
+        float2 out;
+        join_quads(m, l, o, out);
+        const size_t at = ((size_t)piece * a.n + j) * a.H + h;
+        *reinterpret_cast<float2*>(a.po + at * BR_HD + quad_columns(lane)) = out;
+        if (lane == 0) a.ml[at] = make_float2(m, l);
+    }
+};
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Sixteen branches at a time: q.K and P.V as products too.  K goes in as two bf16 terms (its rounding would come back
@@ -341,7 +465,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.H * BR_HD;
     br_let_next_kernel_start();
-    const int lists = a.n_pre;
+    const int lists = a.n_pre + (int)(br.B * br.S), n_pre = a.n_pre;
     const int2* work = reinterpret_cast<const int2*>(br.work);
     const int total = work[lists].x;
     // behind the ring the steps' fragments of W, then (or in the ring, where there is no room) the staged slice of W
@@ -354,7 +478,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         dst[1] = make_float2(x.z, x.w);
     }
     for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = log2f(br.rhos[i]);
-    const int workers = branch_workers(total, (int)gridDim.x * IG, BR_LEAST_UNITS);
+    const int workers = branch_workers(total, (int)gridDim.x * IG, BR_LEAST_COST);
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;
     const int steps = min(JW, a.n - (int)blockIdx.z * JW);       // of this CTA
@@ -368,22 +492,27 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     // producer: `left` units of list px from slot pk on; the ids of its next unit are a unit ahead
     int px = 0, pk = 0, left = 0;
     List pl = {nullptr, nullptr, 0};
+    auto units_to = [&](int from, int to, int cost) { return (min(to, c_end) - from + cost - 1) / cost; };
+    auto cost_of = [&](int list) { return list < n_pre ? BR_COST_BLOCK : BR_COST_OWN; };
     auto next_list = [&](int& list, int& count) {                // the next list with units in this stretch: their number, or 0
         for (;;) {
             const int2 at = work[++list];
             if (at.x >= c_end) return 0;
             const int hi = work[list + 1].x;
             count = at.y;
-            if (hi > at.x) return min(hi, c_end) - at.x;
+            if (hi > at.x) return units_to(at.x, hi, cost_of(list));
         }
     };
     if (works) {
         const int c0 = branch_cut(total, workers, me);
         px = find_list(work, lists, c0, lane);
         const int2 lo = work[px];
-        pk = (c0 - lo.x) * 16;
-        left = min(work[px + 1].x, c_end) - c0;
-        pl = get_list(a, px, lo.y);
+        const int hi = work[px + 1].x, cost = cost_of(px), skip = (c0 - lo.x + cost - 1) / cost;     // units of the list before this stretch
+        int count = lo.y;
+        pk = skip * 16;
+        left = max(units_to(lo.x + skip * cost, hi, cost), 0);
+        if (left == 0) { pk = 0; left = next_list(px, count); }
+        pl = get_list(a, px, count);
     }
     int x = px;                                                  // consumer: c_left units of list x from slot k0 on
     int k0 = pk, c_left = left, count = pl.count;
@@ -440,19 +569,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     constexpr bool W_REGS = KS == 4;
     uint4 w[KS * 4];
     if constexpr (W_REGS) read_W<KS>(w, w_at);
+    OneRow one;
     SixteenRows many;
-    bool fresh = true;
+    bool fresh = true, own = false;
     int rows = 1;
     uint32_t at = ring;
     const uint32_t lane_lo = g * 128 + ((t ^ ((g & 1) << 2)) << 4), lane_hi = lane_lo ^ 64u;
     for (;;) {
         if (fresh) {
-            const int b = x / a.blocks, s0 = (x - b * a.blocks) * BR_BLOCK;
-            rows = min(BR_BLOCK, (int)br.S - s0);
-            many.start(a, (int64_t)b * br.S + s0, rows, j, h, lane);
+            own = x >= n_pre;
+            if (own) {
+                one.start(a, x - n_pre, j, h, lane);
+            } else {
+                const int b = x / a.blocks, s0 = (x - b * a.blocks) * BR_BLOCK;
+                rows = min(BR_BLOCK, (int)br.S - s0);
+                many.start(a, (int64_t)b * br.S + s0, rows, j, h, lane);
+            }
             fresh = false;
         }
-        const unsigned touched0 = many.hid0[k0 >> 5], touched1 = many.hid1[k0 >> 5];
+        unsigned touched0 = 0u, touched1 = 0u;
+        if (!own) { touched0 = many.hid0[k0 >> 5]; touched1 = many.hid1[k0 >> 5]; }
         cp_wait<STAGES - 2>();
         if (steps == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(ig + 1), "r"(steps * 32) : "memory");
@@ -465,12 +601,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
             else gate<KS>(acc, A, w_at);
         }
         apply_gate(acc, a.silu);
-        many.unit(a, acc, at + lane_lo, at + lane_hi, k0, count, touched0, touched1, j, t);
+        if (own) one.unit(acc, at + lane_lo, at + lane_hi, hidden16(k0, one.staged, j > 0, count), g);
+        else many.unit(a, acc, at + lane_lo, at + lane_hi, k0, count, touched0, touched1, j, t);
         at += Unit::BYTES;
         if (at == ring_end) at = ring;
         k0 += 16;
         if (--c_left == 0) {                                     // end of the list or of the stretch
-            many.leave(a, (int64_t)x + me, rows, j, h, lane);
+            if (own) one.leave(a, a.own_piece0 + (x - n_pre) + me, j, h, lane);
+            else many.leave(a, (int64_t)x + me, rows, j, h, lane);
             c_left = next_list(x, count);
             if (c_left == 0) break;
             k0 = 0;

@@ -1,5 +1,5 @@
-// Attention of single rows over lists of slots on tcgen05 (mbema_branches_attend, MBEMA_MODE_TC_BF16): the branches' own slots, and the
-// prefix of a sequence with one branch.
+// Attention of a single branch a sequence on tcgen05 (mbema_branches_attend, MBEMA_MODE_TC_BF16): drafted rows, or one row as in a
+// decode step, over the prefix and the branch's own slots.
 //
 // A tile is 128 slots of a list; its operands lie in memory as the gate product wants them in shared memory (mbema_branches_extend),
 // so one bulk copy fetches them, and rho^j of staged step j is in that step's W:  gate(j) = SiLU(A (rho^j W)),  M = 128 slots, N = 64
@@ -108,15 +108,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = a.H * BR_HD;
     const int steps = min(JW, a.n - (int)blockIdx.z * JW), j0 = blockIdx.z * JW;
-    const int lists = a.row_lists;
-    const int2* work = reinterpret_cast<const int2*>(br.work) + a.row_work;
+    const int lists = a.lists;
+    const int2* work = reinterpret_cast<const int2*>(br.work);
     const int total = work[lists].x;
     const int workers = max(1, min((int)gridDim.x * IG, total));
     const int me0 = blockIdx.x * IG;
-    if (total == 0 || me0 >= workers) {                           // nothing to do (the same for all threads)
-        if (tid == 0) br_wait_for_kernel_before();                // the merge waits for this kernel alone
-        return;
-    }
+    if (total == 0 || me0 >= workers) return;                     // nothing to do (the same for all threads)
     if (tid == 0) {
         for (int i = 0; i < L::A_STAGES; ++i) {
             mbar_init(&bars->a_full[i], 1);
@@ -437,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                             }
                         }
                     }
-                    const size_t at = ((((size_t)(list + me)) * 4 + quarter) * a.n + j) * a.H + h + a.row_part0;
+                    const size_t at = ((((size_t)(list + me)) * 4 + quarter) * a.n + j) * a.H + h;
                     *reinterpret_cast<float2*>(a.po + at * BR_HD + 2 * lane) = make_float2(o[0], o[1]);
                     if (lane == 0) a.ml[at] = make_float2(M, l);
                     fresh = true;
@@ -445,7 +442,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             }
         }
     }
-    if (tid == 0) br_wait_for_kernel_before();                    // the merge waits for this kernel alone
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -454,28 +450,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
 }
 
 template <int ATOMS, int IG, bool SILU>
-static int launch(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st) {
+static int launch(const BranchArgs& a, const BranchRows& p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    auto* kernel = k_branch_rows<ATOMS, IG, SILU>;
-    MBEMA_CUDA_TRY(allow_smem(kernel, Smem<ATOMS>::BYTES, done));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Smem<ATOMS>::BYTES;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = early ? 1 : 0;
-    MBEMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, p.JW));
+    MBEMA_CUDA_TRY(allow_smem(k_branch_rows<ATOMS, IG, SILU>, Smem<ATOMS>::BYTES, done));
+    k_branch_rows<ATOMS, IG, SILU><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), THREADS, Smem<ATOMS>::BYTES, st>>>(a, p.JW);
     return check_launch();
 }
 
 template <int ATOMS>
-static int launch_silu(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st) {
-    if (p.IG == 1) return a.silu ? launch<ATOMS, 1, true>(a, p, early, st) : launch<ATOMS, 1, false>(a, p, early, st);
-    return a.silu ? launch<ATOMS, 3, true>(a, p, early, st) : launch<ATOMS, 3, false>(a, p, early, st);
+static int launch_silu(const BranchArgs& a, const BranchRows& p, cudaStream_t st) {
+    if (p.IG == 1) return a.silu ? launch<ATOMS, 1, true>(a, p, st) : launch<ATOMS, 1, false>(a, p, st);
+    return a.silu ? launch<ATOMS, 3, true>(a, p, st) : launch<ATOMS, 3, false>(a, p, st);
 }
 
 }  // namespace brows
@@ -490,10 +475,9 @@ BranchRows branch_rows(int64_t n, int64_t H) {
     return p;
 }
 
-// early: the kernel before (the prefixes, for more than one branch) is this call's too
-int launch_branch_rows(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st) {
+int launch_branch_rows(const BranchArgs& a, const BranchRows& p, cudaStream_t st) {
     if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
-    return a.br.N == 64 ? brows::launch_silu<1>(a, p, early, st) : brows::launch_silu<2>(a, p, early, st);
+    return a.br.N == 64 ? brows::launch_silu<1>(a, p, st) : brows::launch_silu<2>(a, p, st);
 }
 
 }  // namespace mbema

@@ -145,17 +145,17 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
 
 // Operand copies of all listed slots at the first staged step, state * rho^(t0 + len - last) / 64 in fp16 (11 significant bits; a
 // state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head, in the layouts that branches.cuh gives.
-// grid: x = shares of a list, y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sums of the
+// grid: x = shares of a list, y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sum of the
 // lists' units that the attention deals its work by.
 template <typename Count>
-__device__ void running_sum(int2* out, int lists, int unit, Count count_of) {
+__device__ void running_sum(int2* out, int lists, Count count_of) {
     __shared__ int s_warp[8];
     const int tid = threadIdx.x, lane = tid & 31;
     int base = 0;
     for (int x0 = 0; x0 < lists; x0 += 256) {
         const int x = x0 + tid;
-        const int count = x < lists ? count_of(x) : 0;
-        const int c = (count + unit - 1) / unit;
+        int c = 0;
+        const int count = x < lists ? count_of(x, c) : 0;
         int sum = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -190,14 +190,22 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
 __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
     br_wait_for_kernel_before();
     if (blockIdx.y == br.B) {
-        const int blocks = (int)((br.S + BR_BLOCK - 1) / BR_BLOCK), n_pre = br.S > 1 ? (int)br.B * blocks : 0;
         int2* work = reinterpret_cast<int2*>(br.work);
-        if (blockIdx.x == 0 && blockIdx.z == 0) {
-            auto prefix = [&](int b) { return min(br.n_active[b], (int)br.Kcap); };
-            running_sum(work, n_pre, 16, [&](int x) { return prefix(x / blocks); });
-            if (br.S == 1) running_sum(work + 1, (int)(2 * br.B), BR_TILE, [&](int x) { return x & 1 ? br.own_n[x >> 1] : prefix(x >> 1); });
-            else running_sum(work + n_pre + 1, (int)(br.B * br.S), BR_TILE, [&](int x) { return br.own_n[x]; });
-        }
+        const int blocks = (int)((br.S + BR_BLOCK - 1) / BR_BLOCK), n_pre = (int)br.B * blocks;
+        auto prefix = [&](int b) { return min(br.n_active[b], (int)br.Kcap); };
+        if (blockIdx.x > 0 || blockIdx.z > 0) return;
+        if (br.S == 1)
+            running_sum(work, (int)(2 * br.B), [&](int x, int& cost) {
+                const int count = x & 1 ? br.own_n[x >> 1] : prefix(x >> 1);
+                cost = (count + BR_TILE - 1) / BR_TILE;
+                return count;
+            });
+        else
+            running_sum(work, n_pre + (int)(br.B * br.S), [&](int x, int& cost) {
+                const int count = x < n_pre ? prefix(x / blocks) : br.own_n[x - n_pre];
+                cost = (count + 15) / 16 * (x < n_pre ? BR_COST_BLOCK : BR_COST_OWN);
+                return count;
+            });
         return;
     }
     const int b = blockIdx.y, z = blockIdx.z;
@@ -218,7 +226,7 @@ __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
         return (const float*)br.state + ((size_t)b * br.V + v) * N;
     };
     float l2r[8];
-    if (z || br.S == 1) {                               // rows of 64 channels: eight lanes a row, four rows a warp
+    if (br.S == 1) {                                    // rows of 64 channels: eight lanes a row, four rows a warp
         const int atoms = N / 64, atom = warp % atoms, c = 64 * atom + 8 * (lane & 7);
         const int past = (count + BR_TILE - 1) / BR_TILE * BR_TILE;
         int k = warp / atoms * 4 + (lane >> 3);
@@ -313,7 +321,7 @@ static int check_branches(const mbema_branches* br) {
         if (!br->pre_op || !br->own_op || !br->work || !br->status) return MBEMA_ERR_NULL;
         if (((uintptr_t)br->pre_op | (uintptr_t)br->own_op | (uintptr_t)br->state | (uintptr_t)br->own_state) & 15) return MBEMA_ERR_ALIGN;
         const int64_t blocks = (br->S + BR_BLOCK - 1) / BR_BLOCK;                   // the running sums stay below 2^30
-        if (br->B * blocks * (br->Kcap / 16 + 1) + br->B * br->S * (br->cap / 16 + 1) >= 1ll << 30) return MBEMA_ERR_UNSUPPORTED;
+        if (br->B * blocks * (br->Kcap / 16 + 1) * BR_COST_BLOCK + br->B * br->S * (br->cap / 16 + 1) * BR_COST_OWN >= 1ll << 30) return MBEMA_ERR_UNSUPPORTED;
     }
     return MBEMA_OK;
 }

@@ -23,14 +23,16 @@ struct BranchPlan {
     int steps, JP;     // steps a job of a prefix, blocks of steps
 };
 
-// Prefixes that several branches read, in units of 16 slots.
+// Several branches: units of 16 slots.  Cost of one in the running sum that mbema_branches_extend leaves: of a branch's own slots, of a
+// prefix for sixteen branches; a worker's least.
+static constexpr int BR_COST_OWN = 2, BR_COST_BLOCK = 3, BR_LEAST_COST = 2 * BR_COST_BLOCK;
 struct BranchShape {
     int blocks;            // of sixteen branches, a sequence
     int JW, IG;            // of a CTA: steps a worker, workers
     int zb, ctas;          // blocks of steps; CTAs a head and block of steps
 };
 
-// Rows walked alone on tcgen05 (own lists; the prefix of a sequence with one branch), in tiles of 128 slots.
+// One branch: tiles of 128 slots.
 static constexpr int BR_TILE = 128;
 struct BranchRows {
     int JW, IG;            // steps a worker, workers a CTA
@@ -52,25 +54,22 @@ struct BranchArgs {
     int silu, listed_only;
     // fp32 arithmetic: partials [rows, H, SP + SO]
     BranchPlan plan;
-    // tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order.  Prefixes of several
-    // branches: lists (sequence, block of sixteen), partials [piece, BR_BLOCK, n, H].
-    int n_pre, blocks, pre_workers, ring_bytes, w_offset;
-    // Single rows: the branches' own lists, or, for one branch, prefix and own list of every sequence in turn (a stretch then holds
-    // long and short ones as the others do: a list's start and end cost as much as half a tile); partials from row_part0 on,
-    // [piece, 4 warps, n, H]
-    int row_lists, row_work, row_workers;      // their number, where their running sum begins in `work`, workers
-    int64_t row_part0;
-    __device__ __forceinline__ bool row_is_prefix(int list) const { return br.S == 1 && !(list & 1); }
-    __device__ __forceinline__ int row_branch(int list) const { return br.S == 1 ? list >> 1 : list; }
+    // Tensor cores: a list's piece in worker w is number list + w, as lists and workers come in the same order.
+    // Several branches: n_pre lists (sequence, block of sixteen), then the branches' own; partials [piece, BR_BLOCK, n, H] and
+    // [own_piece0 + piece, n, H].  One branch: prefix and own list of every sequence in turn (a stretch then holds long and short ones as
+    // the others do: a list's start and end cost as much as half a tile); partials [piece, 4 warps, n, H].
+    int lists, n_pre, blocks, max_workers, ring_bytes, w_offset;
+    int64_t own_piece0;
+    __device__ __forceinline__ bool row_is_prefix(int list) const { return !(list & 1); }
+    __device__ __forceinline__ int row_branch(int list) const { return list >> 1; }
     __device__ __forceinline__ const int* row_slots(int list) const {
-        return row_is_prefix(list) ? br.active + (size_t)row_branch(list) * br.Kcap : br.own_slot + (size_t)row_branch(list) * br.cap;
+        return list & 1 ? br.own_slot + (size_t)(list >> 1) * br.cap : br.active + (size_t)(list >> 1) * br.Kcap;
     }
     __device__ __forceinline__ const char* row_operands(int list) const;
 };
 
 // The workers that a running sum of `total` units (tiles) occupies, and where their stretches begin.
 __device__ __forceinline__ int branch_workers(int total, int most, int least) { return max(1, min(most, total / least)); }
-static constexpr int BR_LEAST_UNITS = 2;           // a worker's
 // total * w / workers in 32 bits (workers below 2^15)
 __device__ __forceinline__ int branch_cut(int total, int workers, int w) {
     const int q = total / workers, r = total - q * workers;
@@ -94,14 +93,14 @@ __device__ __forceinline__ int find_list(const int2* work, int lists, int c, int
 }
 
 // Operands of a list, state / 64 in fp16, tile after tile of 128 slots (the last one's other slots zero); N * 256 bytes each.
-// Lists of single rows: what tcgen05 reads from shared memory, N / 64 blocks of 128 rows of 64 channels, 128 bytes a row, the 16-byte
+// One branch: what tcgen05 reads from shared memory, N / 64 blocks of 128 rows of 64 channels, 128 bytes a row, the 16-byte
 // pieces of row k in order piece ^ (k % 8).
-// Prefixes of several branches: fragments of mma.sync, 16 slots after 16 slots.  Slot k, channel c = 32 i + 8 t + 4 u + 2 p + e is half e
+// Several branches: fragments of mma.sync, 16 slots after 16 slots.  Slot k, channel c = 32 i + 8 t + 4 u + 2 p + e is half e
 // of word (row / 8) + 2 p (row = k % 16) of lane 4 (row % 8) + t in fragment 2 i + u of its sixteen (512 bytes each).
 __host__ __device__ inline size_t br_operand_bytes(int64_t slots, int64_t N) { return (size_t)((slots + BR_TILE - 1) / BR_TILE) * N * (2 * BR_TILE); }
 __device__ __forceinline__ const char* BranchArgs::row_operands(int list) const {
-    return row_is_prefix(list) ? reinterpret_cast<const char*>(br.pre_op) + (size_t)row_branch(list) * br_operand_bytes(br.Kcap, br.N)
-                               : reinterpret_cast<const char*>(br.own_op) + (size_t)row_branch(list) * br_operand_bytes(br.cap, br.N);
+    return list & 1 ? reinterpret_cast<const char*>(br.own_op) + (size_t)(list >> 1) * br_operand_bytes(br.cap, br.N)
+                    : reinterpret_cast<const char*>(br.pre_op) + (size_t)(list >> 1) * br_operand_bytes(br.Kcap, br.N);
 }
 
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
@@ -139,7 +138,7 @@ __device__ __forceinline__ void br_let_next_kernel_start() { asm volatile("gridd
 bool branch_tc_supported(int64_t N);
 BranchShape branch_shape(int64_t S, int64_t n, int64_t H);
 BranchRows branch_rows(int64_t n, int64_t H);
-int launch_branch_rows(const BranchArgs& a, const BranchRows& p, bool early, cudaStream_t st);
+int launch_branch_rows(const BranchArgs& a, const BranchRows& p, cudaStream_t st);
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st);
 int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st);
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st);
