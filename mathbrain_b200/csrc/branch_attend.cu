@@ -18,7 +18,7 @@ static constexpr int BA_TILE = 64;       // slots a tile
 static constexpr int BA_ROWS = 32;       // branches a CTA
 static constexpr int BA_LD = 68;         // floats a row of 64 in shared memory: 16-byte pieces of eight rows lie in different banks
 static constexpr int BM_WARPS = 4;
-static constexpr int BM_STAGED = 8;      // staged tokens at a time
+static constexpr int BM_STAGED = 2 * BM_WARPS;      // staged tokens at a time: two a warp
 
 static size_t ba_smem(int N) {
     return ((size_t)N * BR_HD + (size_t)N * BA_LD + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * (2 * BR_HD + BA_LD) + 2 * ((N + 3) & ~3) + 3 * BA_ROWS +
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
 // PIECES: partials of the tensor-core kernel (a list's pieces, one a worker), else of the fp32 kernel (its chunks).
 template <bool PIECES>
 __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
-    __shared__ float s_c[BM_STAGED][128];                       // states of the staged tokens at this row
+    __shared__ __align__(16) float s_c[128][BM_STAGED];         // states of the staged tokens at this row
     __shared__ float2 s_x[BM_WARPS][BM_STAGED][32];             // partial pre-activations
     __shared__ float s_m[BM_WARPS], s_l[BM_WARPS];
     __shared__ float2 s_o[BM_WARPS][32];
@@ -301,24 +301,52 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
     // the staged tokens do not wait for the kernel before, which has seen the calls before it end
     for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
         const int cnt = min(BM_STAGED, j - i0);
+        // a warp's two tokens: their E rows are on their way while the states are made
+        float2 ek[2], ev[2], q = make_float2(0.f, 0.f);
+        bool see[2];
+        const size_t qoff = (size_t)wid * BR_HD + 2 * lane;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int place = i0 + warp + e * BM_WARPS;
+            see[e] = place < j;
+            const size_t at = br_index(br, r, see[e] ? place : 0);
+            const int v = br.st_tok[at];
+            // none, or repeated before this row (j <= 31)
+            see[e] = see[e] && v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
+            ek[e] = ev[e] = make_float2(0.f, 0.f);
+            if (see[e]) {
+                const size_t off = (size_t)v * D + h * BR_HD + 2 * lane;
+                ek[e] = make_float2(ld_dyn_f32(a.Ek, a.e_dt, off), ld_dyn_f32(a.Ek, a.e_dt, off + 1));
+                ev[e] = make_float2(ld_dyn_f32(a.Ev, a.e_dt, off), ld_dyn_f32(a.Ev, a.e_dt, off + 1));
+                q = make_float2(ld_dyn_f32(a.q, a.q_dt, qoff), ld_dyn_f32(a.q, a.q_dt, qoff + 1));
+            }
+        }
         __syncthreads();
         for (int e = threadIdx.x; e < cnt * N; e += BM_WARPS * 32) {
             const int i = e / N, c = e - i * N;
-            s_c[i][c] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * log2f(br.rhos[c]));
+            s_c[c][i] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * log2f(br.rhos[c]));
         }
         __syncthreads();
         const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
         float x0[BM_STAGED], x1[BM_STAGED];
 #pragma unroll
         for (int i = 0; i < BM_STAGED; ++i) x0[i] = x1[i] = 0.f;
-#pragma unroll 4
-        for (int c = warp; c < N; c += BM_WARPS) {
-            const float2 w = Wc[(size_t)c * (D / 2)];
+        for (int c0 = warp; c0 < N; c0 += BM_WARPS * 8) {         // eight rows of W in flight
+            float2 w[8];
 #pragma unroll
-            for (int i = 0; i < BM_STAGED; ++i) {
-                if (i < cnt) {
-                    x0[i] = fmaf(s_c[i][c], w.x, x0[i]);
-                    x1[i] = fmaf(s_c[i][c], w.y, x1[i]);
+            for (int u = 0; u < 8; ++u) {
+                const int c = c0 + u * BM_WARPS;
+                w[u] = c < N ? Wc[(size_t)c * (D / 2)] : make_float2(0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int c = min(c0 + u * BM_WARPS, N - 1);
+                const float4 m0 = *reinterpret_cast<const float4*>(&s_c[c][0]), m1 = *reinterpret_cast<const float4*>(&s_c[c][4]);
+                const float m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+#pragma unroll
+                for (int i = 0; i < BM_STAGED; ++i) {             // (places past the last token hold whatever: their sums are not read)
+                    x0[i] = fmaf(m[i], w[u].x, x0[i]);
+                    x1[i] = fmaf(m[i], w[u].y, x1[i]);
                 }
             }
         }
@@ -326,26 +354,20 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
         for (int i = 0; i < BM_STAGED; ++i)
             if (i < cnt) s_x[warp][i][lane] = make_float2(x0[i], x1[i]);
         __syncthreads();
-        for (int i = warp; i < cnt; i += BM_WARPS) {             // a staged token each
-            const int place = i0 + i;
-            const size_t at = br_index(br, r, place);
-            const int v = br.st_tok[at];
-            // none, or repeated before this row (j <= 31)
-            const bool see = v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
-            if (see) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = warp + e * BM_WARPS;
+            if (see[e]) {
                 float y0 = 0.f, y1 = 0.f;
 #pragma unroll
                 for (int w = 0; w < BM_WARPS; ++w) { const float2 y = s_x[w][i][lane]; y0 += y.x; y1 += y.y; }
                 const float g0 = a.silu ? y0 / (1.0f + expf(-y0)) : y0, g1 = a.silu ? y1 / (1.0f + expf(-y1)) : y1;
-                const size_t e = (size_t)v * D + h * BR_HD + 2 * lane, qoff = (size_t)wid * BR_HD + 2 * lane;
-                const float score = warp_sum(ld_dyn_f32(a.q, a.q_dt, qoff) * (ld_dyn_f32(a.Ek, a.e_dt, e) * g0) +
-                             ld_dyn_f32(a.q, a.q_dt, qoff + 1) * (ld_dyn_f32(a.Ek, a.e_dt, e + 1) * g1)) * BR_SCORE_LOG2;
-                const float2 val = make_float2(ld_dyn_f32(a.Ev, a.e_dt, e) * g0, ld_dyn_f32(a.Ev, a.e_dt, e + 1) * g1);
+                const float score = warp_sum(q.x * (ek[e].x * g0) + q.y * (ek[e].y * g1)) * BR_SCORE_LOG2;
                 const float m_new = fmaxf(M, score);
                 const float keep = exp2f(M - m_new), w = exp2f(score - m_new);
                 L = fmaf(L, keep, w);
-                o.x = fmaf(val.x, w, o.x * keep);
-                o.y = fmaf(val.y, w, o.y * keep);
+                o.x = fmaf(ev[e].x * g0, w, o.x * keep);
+                o.y = fmaf(ev[e].y * g1, w, o.y * keep);
                 M = m_new;
             }
         }
