@@ -181,6 +181,15 @@ __device__ __forceinline__ void load_q(uint32_t (&E)[8], const char* row) {
     }
 }
 
+__device__ __forceinline__ void mul_bf16x2(float& x, float& y, uint32_t a, uint32_t b) {
+    asm("{\n\t.reg .b16 al, ah, bl, bh;\n\t"
+        "mov.b32 {al, ah}, %2;\n\t"
+        "mov.b32 {bl, bh}, %3;\n\t"
+        "fma.rn.f32.bf16 %0, al, bl, 0f00000000;\n\t"
+        "fma.rn.f32.bf16 %1, ah, bh, 0f00000000;\n\t}"
+        : "=f"(x), "=f"(y) : "r"(a), "r"(b));
+}
+
 __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
     if (silu) {              // W carries 1/2: SiLU(x) = h + h tanh(h), h = x / 2
 #pragma unroll
@@ -265,13 +274,11 @@ __device__ __forceinline__ int quad_columns(int lane) {
 // maximum and sums, joined at the end of the piece.
 // ---------------------------------------------------------------------------------------------------------------------------
 struct OneRow {
-    float m, l, o[16], q[16];
+    float m, l, o[16];
+    uint32_t q[8];
     int staged;
     __device__ __forceinline__ void start(const BranchArgs& a, int64_t r, int j, int h, int lane) {
-        uint32_t x[8];
-        load_q(x, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { q[2 * i] = bf_lo(x[i]) * BR_SCORE_LOG2; q[2 * i + 1] = bf_hi(x[i]) * BR_SCORE_LOG2; }
+        load_q(q, reinterpret_cast<const char*>(a.q) + (((size_t)r * a.n + j) * a.H + h) * (BR_HD * 2) + 16 * (lane & 3));
         staged = -1;
         if (lane < j) staged = a.br.st_own[br_index(a.br, r, lane)];
         m = -INFINITY;
@@ -285,10 +292,13 @@ struct OneRow {
         float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            s0 = fmaf(bf_lo(e0[nt]) * q[2 * nt], acc[nt][0], s0);
-            s1 = fmaf(bf_hi(e0[nt]) * q[2 * nt + 1], acc[nt][1], s1);
-            s2 = fmaf(bf_lo(e1[nt]) * q[2 * nt], acc[nt][2], s2);
-            s3 = fmaf(bf_hi(e1[nt]) * q[2 * nt + 1], acc[nt][3], s3);
+            float x, y;                                          // (the product of two bf16 is exact in fp32, and needs no unpacking)
+            mul_bf16x2(x, y, e0[nt], q[nt]);
+            s0 = fmaf(x, acc[nt][0], s0);
+            s1 = fmaf(y, acc[nt][1], s1);
+            mul_bf16x2(x, y, e1[nt], q[nt]);
+            s2 = fmaf(x, acc[nt][2], s2);
+            s3 = fmaf(y, acc[nt][3], s3);
         }
         load_E<2048>(e0, e1, at_lo, at_hi);
         s0 += s1;
@@ -297,7 +307,7 @@ struct OneRow {
         s2 += __shfl_xor_sync(0xffffffffu, s2, 1);
         s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
         s2 += __shfl_xor_sync(0xffffffffu, s2, 2);
-        const float x0 = (hide >> g) & 1u ? -INFINITY : s0, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2;
+        const float x0 = (hide >> g) & 1u ? -INFINITY : s0 * BR_SCORE_LOG2, x1 = (hide >> (g + 8)) & 1u ? -INFINITY : s2 * BR_SCORE_LOG2;
         const float m_new = fmaxf(m, fmaxf(x0, x1));
         const float ref = m_new == -INFINITY ? 0.f : m_new;
         const float p0 = ex2(x0 - ref), p1 = ex2(x1 - ref);
@@ -467,6 +477,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     br_let_next_kernel_start();
     const int lists = a.n_pre + (int)(br.B * br.S), n_pre = a.n_pre;
     const int2* work = reinterpret_cast<const int2*>(br.work);
+    ListSearch search;
+    search.begin(work, lists, lane);
     const int total = work[lists].x;
     // behind the ring the steps' fragments of W, then (or in the ring, where there is no room) the staged slice of W
     const uint32_t w_all = (uint32_t)__cvta_generic_to_shared(smem) + a.ring_bytes;
@@ -505,12 +517,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     };
     if (works) {
         const int c0 = branch_cut(total, workers, me);
-        px = find_list(work, lists, c0, lane);
-        const int2 lo = work[px];
-        const int hi = work[px + 1].x, cost = cost_of(px), skip = (c0 - lo.x + cost - 1) / cost;     // units of the list before this stretch
+        int2 lo, hi;
+        px = search.find(work, lists, c0, lane, lo, hi);
+        const int cost = cost_of(px), skip = (c0 - lo.x + cost - 1) / cost;     // units of the list before this stretch
         int count = lo.y;
         pk = skip * 16;
-        left = max(units_to(lo.x + skip * cost, hi, cost), 0);
+        left = max(units_to(lo.x + skip * cost, hi.x, cost), 0);
         if (left == 0) { pk = 0; left = next_list(px, count); }
         pl = get_list(a, px, count);
     }

@@ -52,12 +52,11 @@ static_assert(sizeof(Bars) <= 320, "barrier block");
 struct Cursor {                    // a worker's place in the lists
     int list, left, k, count, end; // left tiles of this list from slot k on; end: of the stretch, in tiles
     int2 n1, n2;                   // (running sum, length) of the next two lists, read ahead of their use
-    __device__ __forceinline__ void start(const int2* work, int lists, int total, int workers, int me, int lane) {
+    __device__ __forceinline__ void start(const ListSearch& search, const int2* work, int lists, int total, int workers, int me, int lane) {
         const int c0 = branch_cut(total, workers, me);
         end = branch_cut(total, workers, me + 1);
-        list = find_list(work, lists, c0, lane);
-        const int2 at = work[list];
-        n1 = work[list + 1];
+        int2 at;
+        list = search.find(work, lists, c0, lane, at, n1);
         n2 = work[min(list + 2, lists)];
         count = at.y;
         k = (c0 - at.x) * TILE;
@@ -110,6 +109,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
     const int steps = min(JW, a.n - (int)blockIdx.z * JW), j0 = blockIdx.z * JW;
     const int lists = a.lists;
     const int2* work = reinterpret_cast<const int2*>(br.work);
+    ListSearch search;
+    search.begin(work, lists, tid & 31);
     const int total = work[lists].x;
     const int workers = max(1, min((int)gridDim.x * IG, total));
     const int me0 = blockIdx.x * IG;
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             };
 #pragma unroll
             for (int g = 0; g < IG; ++g)
-                if (count_of[g] > 0) { cur[g].start(work, lists, total, workers, me0 + g, lane); fetch_ids(g); }
+                if (count_of[g] > 0) { cur[g].start(search, work, lists, total, workers, me0 + g, lane); fetch_ids(g); }
             int st = 0, use = 0;
             bool go = true;
 #pragma unroll 1
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             Cursor cur[IG];
 #pragma unroll 1
             for (int g = 0; g < IG; ++g)
-                if (count_of[g] > 0) cur[g].start(work, lists, total, workers, me0 + g, lane);
+                if (count_of[g] > 0) cur[g].start(search, work, lists, total, workers, me0 + g, lane);
             if (lane == 0) {
                 int st = 0, use = 0;
                 bool go = true;
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
         if (jj < steps && mine > 0) {
             const int me = me0 + g;
             Cursor cur;
-            cur.start(work, lists, total, workers, me, lane);
+            cur.start(search, work, lists, total, workers, me, lane);
             const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * 2 * BR_HD);
             uint32_t* q_sh = reinterpret_cast<uint32_t*>(sm + L::Q) + warp * 32;      // bf16; a copy a warp: the warps of a group never meet
             const uint32_t q_at = smem_u32(q_sh);

@@ -79,18 +79,35 @@ __device__ __forceinline__ int branch_cut(int total, int workers, int w) {
 __device__ __forceinline__ int branch_worker_of(int total, int workers, int c) {
     return (int)((((long long)c + 1) * workers - 1) / total);
 }
-// Where a stretch begins: the list that holds unit c, by 32 samples of the running sum at a time.
-__device__ __forceinline__ int find_list(const int2* work, int lists, int c, int lane) {
-    int lo = 0, hi = lists;                       // work[lo].x <= c < work[hi].x
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
-        const int at = lo + (lane + 1) * step;
-        const unsigned below = __ballot_sync(0xffffffffu, at < hi && work[at].x <= c);
-        lo += __popc(below) * step;
-        hi = min(hi, lo + step);
+// Where a stretch begins: the list that holds unit c, with its (running sum, length) and the next one's, by 32 samples of the running
+// sum at a time.  The first samples depend on nothing but the number of lists: they are read with the total that c comes from.
+struct ListSearch {
+    int2 base, mine;                              // entries lo and min(lo + (lane + 1) step, hi)
+    __device__ __forceinline__ void begin(const int2* work, int lists, int lane) {
+        base = work[0];
+        mine = work[min((lane + 1) * ((lists + 31) / 32), lists)];
     }
-    return lo;
-}
+    __device__ __forceinline__ int find(const int2* work, int lists, int c, int lane, int2& at, int2& next) const {
+        int2 first = base, s = mine;
+        int lo = 0, hi = lists, step = (lists + 31) / 32;
+        for (;;) {
+            const unsigned below = __ballot_sync(0xffffffffu, lo + (lane + 1) * step < hi && s.x <= c);
+            const int k = __popc(below);
+            lo += k * step;
+            if (step == 1) {
+                const int before = max(k - 1, 0);
+                const int2 p = make_int2(__shfl_sync(0xffffffffu, s.x, before), __shfl_sync(0xffffffffu, s.y, before));
+                at = k ? p : first;
+                next = make_int2(__shfl_sync(0xffffffffu, s.x, k), __shfl_sync(0xffffffffu, s.y, k));
+                return lo;
+            }
+            hi = min(hi, lo + step);
+            step = (hi - lo + 31) / 32;
+            first = work[lo];
+            s = work[min(lo + (lane + 1) * step, hi)];
+        }
+    }
+};
 
 // Operands of a list, state / 64 in fp16, tile after tile of 128 slots (the last one's other slots zero); N * 256 bytes each.
 // One branch: what tcgen05 reads from shared memory, N / 64 blocks of 128 rows of 64 channels, 128 bytes a row, the 16-byte

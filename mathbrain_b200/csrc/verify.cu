@@ -34,6 +34,12 @@ __device__ __forceinline__ double vd_weight(double w) { return w > 0.0 && w <= 3
 
 // s + e += weight of (p - q), as a lane's sum of a few dozen of them: the difference and every sum with its rounding error kept (Knuth's
 // two-sum; relative error about 2^-47).  In double, the conversions and the compares of a whole row took longer than its bytes.
+__device__ __forceinline__ void add_weight(float& s, float& e, float w) {
+    const float d = w > 0.f && w <= 3.402823466e38f ? w : 0.f;
+    const float t = __fadd_rn(s, d), c = __fsub_rn(t, s);
+    e = __fadd_rn(e, __fadd_rn(__fsub_rn(s, __fsub_rn(t, c)), __fsub_rn(d, c)));
+    s = t;
+}
 __device__ __forceinline__ void add_weight(float& s, float& e, float p, float q) {
     float d = __fsub_rn(p, q);
     const float b = __fsub_rn(d, p);
@@ -138,13 +144,16 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
         for (int i0 = lo + lane; i0 < hi; i0 += 32 * VD_BATCH) {         // a batch of loads is in flight, the last one too
             float x[VD_BATCH], y[VD_BATCH];
 #pragma unroll
-            for (int k = 0; k < VD_BATCH; ++k) {
-                const int i = i0 + 32 * k;
-                x[k] = i < hi ? ld_as_f32<DT>(a.p, po + i) : 0.f;
-                y[k] = i < hi && from_q ? ld_as_f32<DT>(a.q, qo + i) : (i == spike ? 1.f : 0.f);
-            }
+            for (int k = 0; k < VD_BATCH; ++k) x[k] = i0 + 32 * k < hi ? ld_as_f32<DT>(a.p, po + i0 + 32 * k) : 0.f;
+            if (from_q) {
 #pragma unroll
-            for (int k = 0; k < VD_BATCH; ++k) add_weight(s, e, x[k], y[k]);
+                for (int k = 0; k < VD_BATCH; ++k) y[k] = i0 + 32 * k < hi ? ld_as_f32<DT>(a.q, qo + i0 + 32 * k) : 0.f;
+#pragma unroll
+                for (int k = 0; k < VD_BATCH; ++k) add_weight(s, e, x[k], y[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VD_BATCH; ++k) add_weight(s, e, i0 + 32 * k == spike ? x[k] - 1.0f : x[k]);
+            }
         }
         const double sum = warp_sum_d((double)s + (double)e);
         if (lane < VD_CTAS) cluster.map_shared_rank(s_sum, lane)[w_id] = sum;
@@ -231,10 +240,10 @@ extern "C" int mbema_verify_drafts(const void* p, int64_t p_row, int64_t p_pos, 
     if (R == 0) return MBEMA_OK;
     if (!p || (G > 0 && !drafted) || !uniforms || !n_accepted || !tokens) return MBEMA_ERR_NULL;
     VerifyArgs a{p, q, p_row, p_pos, q_row, q_pos, (const long long*)drafted, uniforms, (long long*)n_accepted, (long long*)tokens, (int)G, (int)V};
-    // the largest cluster with which all rows are resident at once, two CTAs an SM (one sequence and 20: 8 or 2 make no difference; 64: 8 17 us,
-    // 4 12.7, 2 14.5; 256: 8 48 us, 4 37, 2 34)
+    // the largest cluster with which all rows are resident at once, three CTAs an SM (one sequence and 20: 8 or 2 make no difference; 64:
+    // 8 17 us, 4 13, 2 15; 100 without q, bf16: 4 14, 2 16; 256: 8 48, 4 37, 2 34)
     int64_t ctas = 8;
-    while (ctas > 2 && R * ctas > 2 * 148) ctas >>= 1;
+    while (ctas > 2 && R * ctas > 3 * 148) ctas >>= 1;
     if (dtype == MBEMA_F32) return ctas == 8 ? launch<MBEMA_F32, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_F32, 4>(a, R, stream) : launch<MBEMA_F32, 2>(a, R, stream);
     return ctas == 8 ? launch<MBEMA_BF16, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_BF16, 4>(a, R, stream) : launch<MBEMA_BF16, 2>(a, R, stream);
 }
