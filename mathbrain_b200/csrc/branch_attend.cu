@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     if (tid < BA_TILE) slots_of(k_lo);
     for (int i = tid; i < N * (BR_HD / 4); i += BA_THREADS)
         *reinterpret_cast<float4*>(W_sh + i * 4) = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
-    for (int i = tid; i < N; i += BA_THREADS) l2r_sh[i] = log2f(br.rhos[i]);
+    for (int i = tid; i < N; i += BA_THREADS) l2r_sh[i] = br_log2(br.rhos[i]);
     for (int i = tid; i < rows * BR_HD; i += BA_THREADS) {
         const int row = i >> 6, st = row / branches;
         q_sh[i] = ld_dyn_f32(a.q, a.q_dt, ((((size_t)(r0 + row - st * branches)) * n + j0 + st) * H + h) * BR_HD + (i & 63)) * BR_SCORE_LOG2;
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
         __syncthreads();
         for (int e = threadIdx.x; e < cnt * N; e += BM_WARPS * 32) {
             const int i = e / N, c = e - i * N;
-            s_c[c][i] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * log2f(br.rhos[c]));
+            s_c[c][i] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * br_log2(br.rhos[c]));
         }
         __syncthreads();
         const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
                 for (int w = 0; w < BM_WARPS; ++w) { const float2 y = s_x[w][i][lane]; y0 += y.x; y1 += y.y; }
                 const float g0 = a.silu ? y0 / (1.0f + expf(-y0)) : y0, g1 = a.silu ? y1 / (1.0f + expf(-y1)) : y1;
                 const float score = warp_sum(q.x * (ek[e].x * g0) + q.y * (ek[e].y * g1)) * BR_SCORE_LOG2;
+                if (score == -INFINITY) continue;                 // beyond fp32: no weight
                 const float m_new = fmaxf(M, score);
                 const float keep = exp2f(M - m_new), w = exp2f(score - m_new);
                 L = fmaf(L, keep, w);

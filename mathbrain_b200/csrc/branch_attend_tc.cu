@@ -362,9 +362,9 @@ struct SixteenRows {
                                          unsigned touched0, unsigned touched1, int j, int t) {
         uint32_t e0[8], e1[8];
         load_E<0>(e0, e1, at_lo, at_hi);
-        float sc[2][4];
+        float sc[2][4], sl[2][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[0][i] = sc[1][i] = 0.f;
+        for (int i = 0; i < 4; ++i) sc[0][i] = sc[1][i] = sl[0][i] = sl[1][i] = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const uint32_t Q[4] = {q0[2 * c], q1[2 * c], q0[2 * c + 1], q1[2 * c + 1]};
@@ -382,10 +382,15 @@ struct SixteenRows {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 mma_bf16(sc[x], Q, hi[x][0], hi[x][1]);
-                mma_bf16(sc[x], Q, lo[x][0], lo[x][1]);
+                mma_bf16(sl[x], Q, lo[x][0], lo[x][1]);
             }
         }
         load_E<2048>(e0, e1, at_lo, at_hi);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                           // (a product beyond fp32 stays infinite: its second term may have the other sign)
+            sc[0][i] = fabsf(sc[0][i]) == INFINITY ? sc[0][i] : sc[0][i] + sl[0][i];
+            sc[1][i] = fabsf(sc[1][i]) == INFINITY ? sc[1][i] : sc[1][i] + sl[1][i];
+        }
         unsigned hide0 = (touched0 >> (k0 & 31)) & 0xffffu, hide1 = (touched1 >> (k0 & 31)) & 0xffffu;
         if (j > 0) {
             unsigned x = 0u, y = 0u;
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
         dst[0] = make_float2(x.x, x.y);
         dst[1] = make_float2(x.z, x.w);
     }
-    for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = log2f(br.rhos[i]);
+    for (int i = tid; i < N; i += WARPS * 32) s_l2r[i] = br_log2(br.rhos[i]);
     const int workers = branch_workers(total, (int)gridDim.x * IG, BR_LEAST_COST);
     const int jj = warp % JW, ig = warp / JW;
     const int j = blockIdx.z * JW + jj;

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
     #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     w[e] = a.W[(size_t)(c + e) * D + h * BR_HD + d] * scale;
-                    l2r[e] = log2f(br.rhos[c + e]);
+                    l2r[e] = br_log2(br.rhos[c + e]);
                 }
                 unsigned char* dst = sm + L::B + (c >> 6) * 8192 + d * 128 + ((((c & 63) >> 3) ^ (d & 7)) << 4);
                 for (int s = 0; s < steps; ++s) {
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
 #pragma unroll
                     for (int i = 0; i < 64; ++i) o[i] *= alpha;
                 }
-                const float p = hidden ? 0.f : ex2_approx(x - m);
+                const float p = hidden || x == -INFINITY ? 0.f : ex2_approx(x - m);      // (below fp32: no weight, before any maximum too)
                 l += p;
                 auto values = [&](float (&g16)[16], auto chunk) {
                     constexpr int c = decltype(chunk)::value;

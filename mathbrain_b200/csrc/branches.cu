@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
         const int v = s_tok[i], own = s_own[i];
         double x = 0.0;
         if (v >= 0) {
-            const double l2 = log2((double)br.rhos[c]);
+            const double l2 = fmax(log2((double)br.rhos[c]), -1e30);
             const int last = own >= 0 ? br.own_t[(size_t)r * cap + own] : br.last_t[(size_t)b * br.V + v];
             if (own >= 0 || last >= 0) {
                 const float base = own >= 0 ? br.own_state[((size_t)r * cap + own) * N + c] : br.state[((size_t)b * br.V + v) * N + c];
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
         int k = warp / atoms * 4 + (lane >> 3);
         if (k - (lane >> 3) >= past) return;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) l2r[e] = log2f(br.rhos[c + e]);
+        for (int e = 0; e < 8; ++e) l2r[e] = br_log2(br.rhos[c + e]);
         for (; k - (lane >> 3) < past; k += warps / atoms * 4) {
             float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, dt;
             if (k < count) {
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
     int k = warp / half * 16 + (lane >> 2);
     if (k - (lane >> 2) >= count) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) l2r[e] = log2f(br.rhos[c + e]);
+    for (int e = 0; e < 8; ++e) l2r[e] = br_log2(br.rhos[c + e]);
     for (; k - (lane >> 2) < count; k += warps / half * 16) {
         uint32_t w[2][4];                               // slots k, k + 8
 #pragma unroll

@@ -120,6 +120,9 @@ __device__ __forceinline__ const char* BranchArgs::row_operands(int list) const 
                     : reinterpret_cast<const char*>(br.pre_op) + (size_t)(list >> 1) * br_operand_bytes(br.Kcap, br.N);
 }
 
+// log2(rho) as a factor of a step count: rho = 0 (a half-life too short for fp32) keeps 0 * log2(rho) = 0
+__device__ __forceinline__ float br_log2(float rho) { return fmaxf(log2f(rho), -1e30f); }
+
 __host__ __device__ inline size_t br_index(const mbema_branches& br, int64_t r, int i) { return (size_t)r * br.max_new + i; }
 
 // cudaFuncAttributeMaxDynamicSharedMemorySize raised to what every later call needs, once a device (the call costs the host as much
