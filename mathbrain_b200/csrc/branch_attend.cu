@@ -19,6 +19,8 @@ static constexpr int BA_ROWS = 32;       // branches a CTA
 static constexpr int BA_LD = 68;         // floats a row of 64 in shared memory: 16-byte pieces of eight rows lie in different banks
 static constexpr int BM_WARPS = 4;
 static constexpr int BM_STAGED = 2 * BM_WARPS;      // staged tokens at a time: two a warp
+static constexpr int BM_ROWS = 8;                   // steps a CTA, at most
+static constexpr int BM_BATCH = 8;                  // partials in flight
 
 static size_t ba_smem(int N) {
     return ((size_t)N * BR_HD + (size_t)N * BA_LD + 2 * BA_TILE * BA_LD + (size_t)BA_ROWS * (2 * BR_HD + BA_LD) + 2 * ((N + 3) & ~3) + 3 * BA_ROWS +
@@ -278,108 +280,119 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     }
 }
 
-// A CTA per (row, head): its four warps share the partials and, for the staged tokens, the state channels; a lane holds two output
-// columns.
-// PIECES: partials of the tensor-core kernel (a list's pieces, one a worker), else of the fp32 kernel (its chunks).
+// A CTA takes up to RJ steps of a (branch, head): for the staged tokens its four warps share the state channels (W, 4 N * 64 bytes, is read
+// once a CTA from L2, then from L1), a lane holds two output columns.  One step: the warps share its partials.  More: a step's
+// partials are one warp's.
+// Bound by latency: three dependent loads of staged tokens, two of partials.
+// PIECES: partials of a tensor-core kernel (a list's pieces, one a worker), else of the fp32 kernel (its chunks).
 template <bool PIECES>
-__global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
+__global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a, int RJ) {
     __shared__ __align__(16) float s_c[128][BM_STAGED];         // states of the staged tokens at this row
     __shared__ float2 s_x[BM_WARPS][BM_STAGED][32];             // partial pre-activations
-    __shared__ float s_m[BM_WARPS], s_l[BM_WARPS];
-    __shared__ float2 s_o[BM_WARPS][32];
+    __shared__ float2 s_ml[BM_ROWS][BM_WARPS];                  // a warp's maximum and sum, and
+    __shared__ float2 s_o[BM_ROWS][BM_WARPS][32];               // its o
     const mbema_branches& br = a.br;
     const int N = (int)br.N, n = a.n, H = a.H, D = H * BR_HD;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t wid = blockIdx.x;
-    const int h = (int)(wid % H);
-    const int64_t row = wid / H;
-    const int j = (int)(row % n);
-    const int64_t r = row / n;
+    const int h = (int)(blockIdx.x % H), JB = (n + RJ - 1) / RJ;
+    const int64_t rest_id = blockIdx.x / H, r = rest_id / JB;
+    const int j_first = (int)(rest_id - r * JB) * RJ, rows = min(RJ, n - j_first);
     const int b = (int)(r / br.S), s = (int)(r - (int64_t)b * br.S);
-    float M = -INFINITY, L = 0.f;
-    float2 o = make_float2(0.f, 0.f);
+    const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
     // the staged tokens do not wait for the kernel before, which has seen the calls before it end
-    for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
-        const int cnt = min(BM_STAGED, j - i0);
-        // a warp's two tokens: their E rows are on their way while the states are made
-        float2 ek[2], ev[2], q = make_float2(0.f, 0.f);
-        bool see[2];
-        const size_t qoff = (size_t)wid * BR_HD + 2 * lane;
+    for (int jj = 0; jj < rows; ++jj) {
+        const int j = j_first + jj;
+        float M = -INFINITY, L = 0.f;
+        float2 o = make_float2(0.f, 0.f);
+        for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
+            const int cnt = min(BM_STAGED, j - i0);
+            // loads that depend on no other first: eight rows of W, the states; a warp's two tokens' E rows are on their way while the
+            // states are made
+            auto W_rows = [&](float2 (&w)[8], int c0) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int place = i0 + warp + e * BM_WARPS;
-            see[e] = place < j;
-            const size_t at = br_index(br, r, see[e] ? place : 0);
-            const int v = br.st_tok[at];
-            // none, or repeated before this row (j <= 31)
-            see[e] = see[e] && v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
-            ek[e] = ev[e] = make_float2(0.f, 0.f);
-            if (see[e]) {
-                const size_t off = (size_t)v * D + h * BR_HD + 2 * lane;
-                ek[e] = make_float2(ld_dyn_f32(a.Ek, a.e_dt, off), ld_dyn_f32(a.Ek, a.e_dt, off + 1));
-                ev[e] = make_float2(ld_dyn_f32(a.Ev, a.e_dt, off), ld_dyn_f32(a.Ev, a.e_dt, off + 1));
-                q = make_float2(ld_dyn_f32(a.q, a.q_dt, qoff), ld_dyn_f32(a.q, a.q_dt, qoff + 1));
-            }
-        }
-        __syncthreads();
-        for (int e = threadIdx.x; e < cnt * N; e += BM_WARPS * 32) {
-            const int i = e / N, c = e - i * N;
-            s_c[c][i] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * br_log2(br.rhos[c]));
-        }
-        __syncthreads();
-        const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
-        float x0[BM_STAGED], x1[BM_STAGED];
-#pragma unroll
-        for (int i = 0; i < BM_STAGED; ++i) x0[i] = x1[i] = 0.f;
-        for (int c0 = warp; c0 < N; c0 += BM_WARPS * 8) {         // eight rows of W in flight
+                for (int u = 0; u < 8; ++u) {
+                    const int c = c0 + u * BM_WARPS;
+                    w[u] = c < N ? Wc[(size_t)c * (D / 2)] : make_float2(0.f, 0.f);
+                }
+            };
             float2 w[8];
+            W_rows(w, warp);
+            float2 ek[2], ev[2], q = make_float2(0.f, 0.f);
+            bool see[2];
+            const size_t qoff = (((size_t)r * n + j) * H + h) * BR_HD + 2 * lane;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int c = c0 + u * BM_WARPS;
-                w[u] = c < N ? Wc[(size_t)c * (D / 2)] : make_float2(0.f, 0.f);
+            for (int e = 0; e < 2; ++e) {
+                const int place = i0 + warp + e * BM_WARPS;
+                see[e] = place < j;
+                const size_t at = br_index(br, r, see[e] ? place : 0);
+                const int v = br.st_tok[at];
+                // none, or repeated before this row (j <= 31)
+                see[e] = see[e] && v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
+                ek[e] = ev[e] = make_float2(0.f, 0.f);
+                if (see[e]) {
+                    const size_t off = (size_t)v * D + h * BR_HD + 2 * lane;
+                    ek[e] = make_float2(ld_dyn_f32(a.Ek, a.e_dt, off), ld_dyn_f32(a.Ek, a.e_dt, off + 1));
+                    ev[e] = make_float2(ld_dyn_f32(a.Ev, a.e_dt, off), ld_dyn_f32(a.Ev, a.e_dt, off + 1));
+                    q = make_float2(ld_dyn_f32(a.q, a.q_dt, qoff), ld_dyn_f32(a.q, a.q_dt, qoff + 1));
+                }
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < cnt * N; e += BM_WARPS * 32) {
+                const int i = e / N, c = e - i * N;
+                s_c[c][i] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * br_log2(br.rhos[c]));
+            }
+            __syncthreads();
+            float x0[BM_STAGED], x1[BM_STAGED];
+#pragma unroll
+            for (int i = 0; i < BM_STAGED; ++i) x0[i] = x1[i] = 0.f;
+            for (int c0 = warp; c0 < N; c0 += BM_WARPS * 8) {     // eight rows of W in flight
+                if (c0 != warp) W_rows(w, c0);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int c = min(c0 + u * BM_WARPS, N - 1);
+                    const float4 m0 = *reinterpret_cast<const float4*>(&s_c[c][0]), m1 = *reinterpret_cast<const float4*>(&s_c[c][4]);
+                    const float m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+#pragma unroll
+                    for (int i = 0; i < BM_STAGED; ++i) {         // (places past the last token hold whatever: their sums are not read)
+                        x0[i] = fmaf(m[i], w[u].x, x0[i]);
+                        x1[i] = fmaf(m[i], w[u].y, x1[i]);
+                    }
+                }
             }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int c = min(c0 + u * BM_WARPS, N - 1);
-                const float4 m0 = *reinterpret_cast<const float4*>(&s_c[c][0]), m1 = *reinterpret_cast<const float4*>(&s_c[c][4]);
-                const float m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+            for (int i = 0; i < BM_STAGED; ++i)
+                if (i < cnt) s_x[warp][i][lane] = make_float2(x0[i], x1[i]);
+            __syncthreads();
 #pragma unroll
-                for (int i = 0; i < BM_STAGED; ++i) {             // (places past the last token hold whatever: their sums are not read)
-                    x0[i] = fmaf(m[i], w[u].x, x0[i]);
-                    x1[i] = fmaf(m[i], w[u].y, x1[i]);
+            for (int e = 0; e < 2; ++e) {
+                const int i = warp + e * BM_WARPS;
+                if (see[e]) {
+                    float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+                    for (int u = 0; u < BM_WARPS; ++u) { const float2 y = s_x[u][i][lane]; y0 += y.x; y1 += y.y; }
+                    const float g0 = a.silu ? y0 / (1.0f + expf(-y0)) : y0, g1 = a.silu ? y1 / (1.0f + expf(-y1)) : y1;
+                    const float score = warp_sum(q.x * (ek[e].x * g0) + q.y * (ek[e].y * g1)) * BR_SCORE_LOG2;
+                    if (score == -INFINITY) continue;             // beyond fp32: no weight
+                    const float m_new = fmaxf(M, score);
+                    const float keep = exp2f(M - m_new), p = exp2f(score - m_new);
+                    L = fmaf(L, keep, p);
+                    o.x = fmaf(ev[e].x * g0, p, o.x * keep);
+                    o.y = fmaf(ev[e].y * g1, p, o.y * keep);
+                    M = m_new;
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < BM_STAGED; ++i)
-            if (i < cnt) s_x[warp][i][lane] = make_float2(x0[i], x1[i]);
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = warp + e * BM_WARPS;
-            if (see[e]) {
-                float y0 = 0.f, y1 = 0.f;
-#pragma unroll
-                for (int w = 0; w < BM_WARPS; ++w) { const float2 y = s_x[w][i][lane]; y0 += y.x; y1 += y.y; }
-                const float g0 = a.silu ? y0 / (1.0f + expf(-y0)) : y0, g1 = a.silu ? y1 / (1.0f + expf(-y1)) : y1;
-                const float score = warp_sum(q.x * (ek[e].x * g0) + q.y * (ek[e].y * g1)) * BR_SCORE_LOG2;
-                if (score == -INFINITY) continue;                 // beyond fp32: no weight
-                const float m_new = fmaxf(M, score);
-                const float keep = exp2f(M - m_new), w = exp2f(score - m_new);
-                L = fmaf(L, keep, w);
-                o.x = fmaf(ev[e].x * g0, w, o.x * keep);
-                o.y = fmaf(ev[e].y * g1, w, o.y * keep);
-                M = m_new;
-            }
-        }
+        if (lane == 0) s_ml[jj][warp] = make_float2(M, L);
+        s_o[jj][warp][lane] = o;
     }
     const int na = min(br.n_active[b], (int)br.Kcap);
-    // partials: np of the prefix from p0 on, then nq of the own slots from q0 on, p_step and q_step apart
+    // partials of step j_first: np of the prefix from p0 on, then nq of the own slots from q0 on, p_step and q_step apart; of the next step
+    // j_step further
     int np, nq;
-    size_t p0, q0, p_step, q_step;
+    size_t p0, q0, p_step, q_step, j_step;
     if constexpr (PIECES) {
         const int2* work = reinterpret_cast<const int2*>(br.work);
-        const size_t each = (size_t)n * H, at = (size_t)j * H + h;
+        const size_t each = (size_t)n * H, at = (size_t)j_first * H + h;
         const bool one = br.S == 1;
         const int total = work[a.lists].x, workers = branch_workers(total, a.max_workers, one ? 1 : BR_LEAST_COST);
         auto pieces = [&](int list, int unit, int& first) {
@@ -394,6 +407,7 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
         np = pieces(pre, one ? 1 : BR_COST_BLOCK, wp);
         nq = pieces(own, one ? 1 : BR_COST_OWN, wq);
         q_step = each;
+        j_step = H;
         if (one) {
             np *= 4;
             nq *= 4;
@@ -410,53 +424,86 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a) {
         np = (na + a.plan.chp - 1) / a.plan.chp;
         nq = (br.own_n[r] + a.plan.cho - 1) / a.plan.cho;
         p_step = q_step = 1;
-        p0 = (size_t)wid * (SP + SO);
+        j_step = (size_t)H * (SP + SO);
+        p0 = (((size_t)r * n + j_first) * H + h) * (SP + SO);
         q0 = p0 + SP;
     }
+    const int own_new = br.own_new[r];
     br_wait_for_kernel_before();
-#pragma unroll 4
-    for (int p = warp; p < np + nq; p += BM_WARPS) {
-        const size_t at = p < np ? p0 + p * p_step : q0 + (p - np) * q_step;
-        const float2 ml = a.ml[at];
-        const float2 x = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
-        if (ml.y == 0.f) continue;                              // every slot of it is hidden
-        const float m_new = fmaxf(M, ml.x);
-        const float keep = exp2f(M - m_new), w = exp2f(ml.x - m_new);
-        L = fmaf(ml.y, w, L * keep);
-        o.x = fmaf(x.x, w, o.x * keep);
-        o.y = fmaf(x.y, w, o.y * keep);
-        M = m_new;
+    // joins the warp's share of a step's partials (every share-th) to (M, L, o)
+    auto join = [&](int jj, int first, int share, float& M, float& L, float2& o) {
+        const size_t off = (size_t)jj * j_step;
+        for (int p = first; p < np + nq; p += BM_BATCH * share) {
+            float2 ml[BM_BATCH], x[BM_BATCH];
+#pragma unroll
+            for (int u = 0; u < BM_BATCH; ++u) {
+                const int i = p + u * share;
+                ml[u] = x[u] = make_float2(0.f, 0.f);
+                if (i < np + nq) {
+                    const size_t at = off + (i < np ? p0 + i * p_step : q0 + (i - np) * q_step);
+                    ml[u] = a.ml[at];
+                    x[u] = *reinterpret_cast<const float2*>(a.po + at * BR_HD + 2 * lane);
+                }
+            }
+            float m_new = M;
+#pragma unroll
+            for (int u = 0; u < BM_BATCH; ++u) m_new = ml[u].y == 0.f ? m_new : fmaxf(m_new, ml[u].x);      // (0: every slot of it is hidden)
+            const float keep = L == 0.f ? 0.f : exp2f(M - m_new);
+            L *= keep;
+            o.x *= keep;
+            o.y *= keep;
+#pragma unroll
+            for (int u = 0; u < BM_BATCH; ++u) {
+                if (ml[u].y == 0.f) continue;
+                const float w = exp2f(ml[u].x - m_new);
+                L = fmaf(ml[u].y, w, L);
+                o.x = fmaf(x[u].x, w, o.x);
+                o.y = fmaf(x[u].y, w, o.y);
+            }
+            M = m_new;
+        }
+    };
+    if (rows == 1) {
+        __syncwarp();
+        float2 ml = s_ml[0][warp], o = s_o[0][warp][lane];
+        join(0, warp, BM_WARPS, ml.x, ml.y, o);
+        __syncwarp();
+        if (lane == 0) s_ml[0][warp] = ml;
+        s_o[0][warp][lane] = o;
     }
-    if (lane == 0) { s_m[warp] = M; s_l[warp] = L; }
-    s_o[warp][lane] = o;
     __syncthreads();
-    if (warp != 0) return;
-    float rest = 0.f;
-    if (!a.listed_only) {
-        int listed = na + br.own_new[r];
-        for (int i = 0; i < j; ++i) listed += br.st_new[br_index(br, r, i)];
-        rest = fmaxf(a.v_total - (float)listed, 0.f);
-    }
-    M = rest > 0.f ? 0.f : -INFINITY;
+    for (int jj = warp; jj < rows; jj += BM_WARPS) {
+        const int j = j_first + jj;
+        float rest = 0.f;                                       // slots that the row does not list: score 0, value 0
+        if (!a.listed_only) {
+            const int add = lane < j ? br.st_new[br_index(br, r, lane)] : 0;
+            rest = fmaxf(a.v_total - (float)(na + own_new + __reduce_add_sync(0xffffffffu, add)), 0.f);
+        }
+        float M = rest > 0.f ? 0.f : -INFINITY, L = rest;
+        float2 o = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < BM_WARPS; ++w) M = fmaxf(M, s_m[w]);
-    L = rest > 0.f ? rest * exp2f(-M) : 0.f;
-    o = make_float2(0.f, 0.f);
+        for (int u = 0; u < BM_WARPS; ++u) {
+            const float2 ml = s_ml[jj][u];
+            if (ml.y != 0.f) M = fmaxf(M, ml.x);
+        }
+        L = rest > 0.f ? rest * exp2f(-M) : 0.f;
 #pragma unroll
-    for (int w = 0; w < BM_WARPS; ++w) {
-        if (s_l[w] == 0.f) continue;
-        const float e = exp2f(s_m[w] - M);
-        const float2 x = s_o[w][lane];
-        L = fmaf(s_l[w], e, L);
-        o.x = fmaf(x.x, e, o.x);
-        o.y = fmaf(x.y, e, o.y);
-    }
-    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);      // no slot at all: zero; a NaN stays one
-    const size_t at = (size_t)wid * BR_HD + 2 * lane;
-    if (a.q_dt == MBEMA_F32) {
-        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.O) + at) = make_float2(o.x * inv, o.y * inv);
-    } else {
-        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.O) + at) = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+        for (int u = 0; u < BM_WARPS; ++u) {
+            const float2 ml = s_ml[jj][u], x = s_o[jj][u][lane];
+            if (ml.y == 0.f) continue;
+            const float e = exp2f(ml.x - M);
+            L = fmaf(ml.y, e, L);
+            o.x = fmaf(x.x, e, o.x);
+            o.y = fmaf(x.y, e, o.y);
+        }
+        if (rows > 1) join(jj, 0, 1, M, L, o);
+        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);      // no slot at all: zero; a NaN stays one
+        const size_t at = (((size_t)r * n + j) * H + h) * BR_HD + 2 * lane;
+        if (a.q_dt == MBEMA_F32) {
+            *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.O) + at) = make_float2(o.x * inv, o.y * inv);
+        } else {
+            *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.O) + at) = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+        }
     }
 }
 
@@ -489,9 +536,13 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
 }
 
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st) {
-    const int64_t ctas = a.br.B * a.br.S * a.n * a.H;
+    // eight steps a CTA where three CTAs an SM are left: W then crosses L2 less often (64 sequences of 6 drafted rows: 399 us, with a step
+    // a CTA 408); a step a CTA otherwise, as its loads then do not wait for one another (8 drafted rows of one sequence: 19 us, with eight 31)
+    const int64_t heads = a.br.B * a.br.S * a.H;
+    const int RJ = heads * ((a.n + BM_ROWS - 1) / BM_ROWS) >= 3 * 148 ? std::min(a.n, BM_ROWS) : 1;
+    const int64_t ctas = heads * ((a.n + RJ - 1) / RJ);
     if (ctas > 0x7fffffff) return MBEMA_ERR_UNSUPPORTED;
-    MBEMA_CUDA_TRY(launch_early(pieces ? k_branch_merge<true> : k_branch_merge<false>, dim3((unsigned)ctas), BM_WARPS * 32, st, a));
+    MBEMA_CUDA_TRY(launch_early(pieces ? k_branch_merge<true> : k_branch_merge<false>, dim3((unsigned)ctas), BM_WARPS * 32, st, a, RJ));
     return check_launch();
 }
 

@@ -77,6 +77,7 @@ __device__ __forceinline__ int branch_cut(int total, int workers, int w) {
 }
 // the worker whose stretch holds unit c < total
 __device__ __forceinline__ int branch_worker_of(int total, int workers, int c) {
+    if ((unsigned)total <= 0xffffffffu / (unsigned)workers) return (int)(((unsigned)(c + 1) * (unsigned)workers - 1u) / (unsigned)total);
     return (int)((((long long)c + 1) * workers - 1) / total);
 }
 // Where a stretch begins: the list that holds unit c, with its (running sum, length) and the next one's, by 32 samples of the running

@@ -47,6 +47,9 @@ LONG = [  # B, S, n, V, N, H, listed slots, own rounds (of 32 tokens), dtype
     (1, 2, 32, 600, 64, 1, [500], 2, torch.bfloat16),
     (3, 2, 4, 900, 24, 2, [700, 0, 65], 3, torch.float32),
     (1, 1, 32, 1500, 64, 1, [1400], 4, torch.float32),
+    (230, 1, 9, 60, 64, 2, [i % 61 for i in range(230)], 0, torch.bfloat16),     # many rows: several steps to a merging CTA
+    (80, 3, 3, 50, 64, 2, [i % 51 for i in range(80)], 1, torch.bfloat16),
+    (80, 3, 10, 40, 16, 2, [i % 41 for i in range(80)], 1, torch.float32),
 ]
 
 
