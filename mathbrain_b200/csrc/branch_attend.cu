@@ -33,6 +33,7 @@ static size_t ba_smem(int N) {
 // channels take nine).  Bound by latency at small sizes: nine meetings of the CTA a tile and step.
 __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     extern __shared__ __align__(16) float smem[];
+    br_wait_for_kernel_before();
     br_let_next_kernel_start();
     const mbema_branches& br = a.br;
     const int N = (int)br.N;
@@ -531,7 +532,7 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
     const size_t smem = ba_smem((int)br.N);
     static std::atomic<unsigned long long> done{0};
     MBEMA_CUDA_TRY(allow_smem(k_branch_attend, ba_smem(128), done));
-    k_branch_attend<<<dim3((unsigned)jobs, (unsigned)a.H), BA_THREADS, smem, st>>>(a);
+    MBEMA_CUDA_TRY(launch_early(k_branch_attend, dim3((unsigned)jobs, (unsigned)a.H), BA_THREADS, smem, st, a));
     return check_launch();
 }
 
@@ -542,7 +543,7 @@ int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st) {
     const int RJ = heads * ((a.n + BM_ROWS - 1) / BM_ROWS) >= 3 * 148 ? std::min(a.n, BM_ROWS) : 1;
     const int64_t ctas = heads * ((a.n + RJ - 1) / RJ);
     if (ctas > 0x7fffffff) return MBEMA_ERR_UNSUPPORTED;
-    MBEMA_CUDA_TRY(launch_early(pieces ? k_branch_merge<true> : k_branch_merge<false>, dim3((unsigned)ctas), BM_WARPS * 32, st, a, RJ));
+    MBEMA_CUDA_TRY(launch_early(pieces ? k_branch_merge<true> : k_branch_merge<false>, dim3((unsigned)ctas), BM_WARPS * 32, 0, st, a, RJ));
     return check_launch();
 }
 

@@ -479,6 +479,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k_branch_tc(BranchArgs a, int J
     constexpr int N = 16 * KS;
     const int h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.H * BR_HD;
+    br_wait_for_kernel_before();
     br_let_next_kernel_start();
     const int lists = a.n_pre + (int)(br.B * br.S), n_pre = a.n_pre;
     const int2* work = reinterpret_cast<const int2*>(br.work);
@@ -668,7 +669,7 @@ static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
     const size_t smem = a.ring_bytes + w_all + (in_ring ? 0 : w_sh);
     static std::atomic<unsigned long long> done{0};
     MBEMA_CUDA_TRY(allow_smem(k_branch_tc<KS, STAGES>, most, done));
-    k_branch_tc<KS, STAGES><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st>>>(a, p.JW, p.IG);
+    MBEMA_CUDA_TRY(launch_early(k_branch_tc<KS, STAGES>, dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), WARPS * 32, smem, st, a, p.JW, p.IG));
     return check_launch();
 }
 

@@ -98,6 +98,7 @@ template <int ATOMS, int IG, bool SILU>
 __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW) {
     using L = Smem<ATOMS>;
     extern __shared__ unsigned char smem_raw[];
+    br_wait_for_kernel_before();
     br_let_next_kernel_start();
     unsigned char* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Bars* bars = reinterpret_cast<Bars*>(sm + L::BARS);
@@ -454,7 +455,7 @@ template <int ATOMS, int IG, bool SILU>
 static int launch(const BranchArgs& a, const BranchRows& p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     MBEMA_CUDA_TRY(allow_smem(k_branch_rows<ATOMS, IG, SILU>, Smem<ATOMS>::BYTES, done));
-    k_branch_rows<ATOMS, IG, SILU><<<dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), THREADS, Smem<ATOMS>::BYTES, st>>>(a, p.JW);
+    MBEMA_CUDA_TRY(launch_early(k_branch_rows<ATOMS, IG, SILU>, dim3((unsigned)p.ctas, (unsigned)a.H, (unsigned)p.zb), THREADS, Smem<ATOMS>::BYTES, st, a, p.JW));
     return check_launch();
 }
 

@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
     __shared__ int s_tok[BR_MAX_NEW], s_own[BR_MAX_NEW], s_dst[BR_MAX_NEW];
     __shared__ unsigned s_same[BR_MAX_NEW];
     __shared__ int s_n, s_len;
+    br_wait_for_kernel_before();
     br_let_next_kernel_start();
     const int64_t r = blockIdx.x;
     const int b = (int)(r / br.S);
@@ -345,14 +346,13 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
     if (n < 1 || n > br->max_new || n_pending < 0 || n_pending > br->max_new) return MBEMA_ERR_SHAPE;
     if (br->B == 0) return MBEMA_OK;
     if (!tok || !C_q) return MBEMA_ERR_NULL;
-    k_branch_stage<<<(unsigned)(br->B * br->S), BS_THREADS, 0, (cudaStream_t)stream>>>(*br, (const long long*)tok, (int)n, nullptr,
-                                                                                   (int)n_pending, C_q);
+    MBEMA_CUDA_TRY(launch_early(k_branch_stage, dim3((unsigned)(br->B * br->S)), BS_THREADS, 0, (cudaStream_t)stream, *br, (const long long*)tok, (int)n, nullptr, (int)n_pending, C_q));
     rc = check_launch();
     if (rc != MBEMA_OK || !br->pre_op) return rc;
     // shares of a list: eight CTAs an SM over all lists, one for every 32 or 16 slots where that is enough
     const int64_t items = 32 / (br->N / 64), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
     const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
-    MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, (cudaStream_t)stream, *br));
+    MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream, *br));
     return check_launch();
 }
 
@@ -362,8 +362,7 @@ extern "C" int mbema_branches_keep(const mbema_branches* br, const int64_t* coun
     if (n_pending < 0 || n_pending > br->max_new) return MBEMA_ERR_SHAPE;
     if (br->B == 0 || n_pending == 0) return MBEMA_OK;
     if (!counts) return MBEMA_ERR_NULL;
-    k_branch_stage<<<(unsigned)(br->B * br->S), BS_THREADS, 0, (cudaStream_t)stream>>>(*br, nullptr, 0, (const long long*)counts,
-                                                                                   (int)n_pending, nullptr);
+    MBEMA_CUDA_TRY(launch_early(k_branch_stage, dim3((unsigned)(br->B * br->S)), BS_THREADS, 0, (cudaStream_t)stream, *br, nullptr, 0, (const long long*)counts, (int)n_pending, nullptr));
     return check_launch();
 }
 

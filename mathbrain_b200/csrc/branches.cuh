@@ -141,10 +141,11 @@ inline cudaError_t allow_smem(Kernel kernel, size_t most, std::atomic<unsigned l
 
 // A kernel whose CTAs may start while the kernel before it still runs (it waits for it with br_wait_for_kernel_before).
 template <typename... Params, typename... Args>
-inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -97,7 +97,9 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
     __shared__ double s_sum[VD_CTAS * VD_WARPS];         // sums of all stretches of the row, in vocabulary order
     __shared__ double s_sub[32];
     __shared__ int s_acc[2];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // (waited for before the first write to another CTA: it has started)
     const int rank = (int)cluster.block_rank();
     const int64_t r = blockIdx.x / VD_CTAS;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -156,9 +158,10 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
             }
         }
         const double sum = warp_sum_d((double)s + (double)e);
+        if (pass == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         if (lane < VD_CTAS) cluster.map_shared_rank(s_sum, lane)[w_id] = sum;
         cluster.sync();
-        total = 0.0;                                     // a lane holds four stretches; the same sums in every thread
+        total = 0.0;                                     // (VD_LANE stretches a lane; the same sums in every thread)
 #pragma unroll
         for (int i = 0; i < VD_LANE; ++i) total += s_sum[lane * VD_LANE + i];
         total = warp_sum_d(total);
@@ -217,12 +220,14 @@ static int launch(const VerifyArgs& a, int64_t R, void* stream) {
     cfg.gridDim = dim3((unsigned)(R * CTAS));
     cfg.blockDim = dim3(VD_THREADS);
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];                         // (the launch overlaps the end of the kernel before)
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = CTAS;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     MBEMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_verify<DT, CTAS>, a));
     return check_launch();
 }
