@@ -357,3 +357,52 @@ def test_no_sequences():
     assert C.shape == (0, 2, 1, 64) and O.shape == (0, 2, 1, 1, 64)
     n, out = verify_drafts(torch.zeros(0, 3, 30).cuda(), torch.zeros(0, 2, dtype=torch.int64).cuda(), torch.zeros(0, 3).cuda())
     assert n.shape == (0,) and out.shape == (0, 3)
+
+
+@pytest.mark.parametrize("S,dt", [(1, torch.bfloat16), (3, torch.bfloat16), (2, torch.float32)])
+def test_captured_behind_copies_and_joined_streams(S, dt):
+    """A graph in which copies, another stream's work and library kernels stand between the calls; replayed back to back."""
+    from mathbrain_b200.verify import verify_drafts
+    B, V, N, H, n, rounds = 2, 400, 64, 2, 3, 5
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [350, 40], dt, 71)
+    tabs = E_k.cuda(), E_v.cuda(), W.cuda()
+    toks = torch.randint(0, V, (rounds, B, S, n), generator=g).cuda()
+    qs = torch.randn(rounds, B, S, n, H, 64, generator=g).to(dt).cuda()
+    us = torch.rand(rounds, B * S, n, generator=g).cuda()
+    head = torch.randn(H * 64, V, generator=g).cuda()
+    br, ref = (st.fork(S, t0, capacity=rounds * n + n, max_new=n) for _ in range(2))
+    side = torch.cuda.Stream()
+
+    def round_(which, tok, q, u, other=None):
+        held = torch.empty_like(tok)
+        held.copy_(tok)
+        if other is not None:                                        # the query comes from another stream
+            other.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(other):
+                q2 = q * 1.0
+        C = which.extend(held)
+        if other is not None:
+            torch.cuda.current_stream().wait_stream(other)
+        O = which.attend(q2 if other is not None else q * 1.0, *tabs)
+        p = torch.softmax(O.float().view(B * S, n, H * 64) @ head, -1)
+        n_acc, out = verify_drafts(p, held.view(B * S, n)[:, 1:], u)
+        which.keep(n_acc.view(B, S).min(1).values + 1)
+        return C, O, n_acc, out
+
+    tok, q, u = toks[0].clone(), qs[0].clone(), us[0].clone()
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        spare = st.fork(S, t0, capacity=8, max_new=n)
+        round_(spare, tok, q, u)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = round_(br, tok, q, u, side)
+    for i in range(rounds):
+        tok.copy_(toks[i]); q.copy_(qs[i]); u.copy_(us[i])
+        graph.replay()
+        want = round_(ref, toks[i], qs[i], us[i])
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
+    assert torch.equal(br.lengths, ref.lengths)
+    br.check_overflow()
