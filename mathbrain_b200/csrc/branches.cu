@@ -188,8 +188,7 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&o);
 }
 
-__global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
-    br_wait_for_kernel_before();
+__device__ __forceinline__ void make_operands(const mbema_branches& br) {
     if (blockIdx.y == br.B) {
         int2* work = reinterpret_cast<int2*>(br.work);
         const int blocks = (int)((br.S + BR_BLOCK - 1) / BR_BLOCK), n_pre = (int)br.B * blocks;
@@ -268,6 +267,14 @@ __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br) {
         *reinterpret_cast<uint4*>(dst) = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
         *reinterpret_cast<uint4*>(dst + 512) = make_uint4(w[0][2], w[1][2], w[0][3], w[1][3]);
     }
+}
+
+// Without tokens to keep, the staging kernel leaves lists and lengths alone, and the operands need not wait for it; it starts this one only
+// after its own wait, so that all calls before it have ended.
+__global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br, int pending) {
+    if (pending) br_wait_for_kernel_before();
+    make_operands(br);
+    if (!pending) br_wait_for_kernel_before();      // the kernels behind this one wait for it alone
 }
 
 // One branch of every sequence moves into the prefix; step numbers move with it.
@@ -352,7 +359,7 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
     // shares of a list: eight CTAs an SM over all lists, one for every 32 or 16 slots where that is enough
     const int64_t items = 32 / (br->N / 64), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
     const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
-    MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream, *br));
+    MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream, *br, (int)n_pending));
     return check_launch();
 }
 
