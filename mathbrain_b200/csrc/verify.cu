@@ -11,13 +11,15 @@
 // stretch holds the threshold deals it to its warps once more, so that no warp walks more than a hundred tokens one after another.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace mbema {
 
-static constexpr int VD_THREADS = 512;
+static constexpr int VD_THREADS = 384;
 static constexpr int VD_WARPS = VD_THREADS / 32;
 static constexpr int VD_BATCH = 8;         // loads of p and of q that a lane has in flight
 
@@ -93,8 +95,8 @@ __device__ __forceinline__ int pick(const double* sums, double thr, double& befo
 // CTAS: of a cluster, 2 to 8
 template <int DT, int VD_CTAS>
 __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
-    constexpr int VD_LANE = VD_CTAS * VD_WARPS / 32;     // stretches a lane holds
-    __shared__ double s_sum[VD_CTAS * VD_WARPS];         // sums of all stretches of the row, in vocabulary order
+    constexpr int VD_LANE = (VD_CTAS * VD_WARPS + 31) / 32;      // stretches a lane holds
+    __shared__ double s_sum[VD_LANE * 32];         // sums of all stretches of the row, in vocabulary order, then zeros
     __shared__ double s_sub[32];
     __shared__ int s_acc[2];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -103,6 +105,7 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
     const int rank = (int)cluster.block_rank();
     const int64_t r = blockIdx.x / VD_CTAS;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (VD_CTAS * VD_WARPS + tid < VD_LANE * 32) s_sum[VD_CTAS * VD_WARPS + tid] = 0.0;
     const int G = a.G, V = a.V;
     if (warp == 0) {                                     // every CTA of the cluster finds the row by itself
         int stop = G, rejected = 0;
@@ -143,20 +146,24 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
     double total = 0.0;
     for (int pass = 0; pass < 2; ++pass) {
         float s = 0.f, e = 0.f;
-        for (int i0 = lo + lane; i0 < hi; i0 += 32 * VD_BATCH) {         // a batch of loads is in flight, the last one too
+        auto batch = [&](int i0, auto whole) {            // a batch of loads is in flight, the last one (not whole) too
             float x[VD_BATCH], y[VD_BATCH];
+            auto in = [&](int k) { return decltype(whole)::value || i0 + 32 * k < hi; };
 #pragma unroll
-            for (int k = 0; k < VD_BATCH; ++k) x[k] = i0 + 32 * k < hi ? ld_as_f32<DT>(a.p, po + i0 + 32 * k) : 0.f;
+            for (int k = 0; k < VD_BATCH; ++k) x[k] = in(k) ? ld_as_f32<DT>(a.p, po + i0 + 32 * k) : 0.f;
             if (from_q) {
 #pragma unroll
-                for (int k = 0; k < VD_BATCH; ++k) y[k] = i0 + 32 * k < hi ? ld_as_f32<DT>(a.q, qo + i0 + 32 * k) : 0.f;
+                for (int k = 0; k < VD_BATCH; ++k) y[k] = in(k) ? ld_as_f32<DT>(a.q, qo + i0 + 32 * k) : 0.f;
 #pragma unroll
                 for (int k = 0; k < VD_BATCH; ++k) add_weight(s, e, x[k], y[k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < VD_BATCH; ++k) add_weight(s, e, i0 + 32 * k == spike ? x[k] - 1.0f : x[k]);
             }
-        }
+        };
+        int i0 = lo + lane;
+        for (; i0 + 32 * (VD_BATCH - 1) < hi; i0 += 32 * VD_BATCH) batch(i0, std::true_type());
+        if (i0 < hi) batch(i0, std::false_type());
         const double sum = warp_sum_d((double)s + (double)e);
         if (pass == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         if (lane < VD_CTAS) cluster.map_shared_rank(s_sum, lane)[w_id] = sum;
@@ -245,8 +252,8 @@ extern "C" int mbema_verify_drafts(const void* p, int64_t p_row, int64_t p_pos, 
     if (R == 0) return MBEMA_OK;
     if (!p || (G > 0 && !drafted) || !uniforms || !n_accepted || !tokens) return MBEMA_ERR_NULL;
     VerifyArgs a{p, q, p_row, p_pos, q_row, q_pos, (const long long*)drafted, uniforms, (long long*)n_accepted, (long long*)tokens, (int)G, (int)V};
-    // the largest cluster with which all rows are resident at once, three CTAs an SM (one sequence and 20: 8 or 2 make no difference; 64:
-    // 8 17 us, 4 13, 2 15; 100 without q, bf16: 4 14, 2 16; 256: 8 48, 4 37, 2 34)
+    // the largest cluster with which all rows' CTAs are three an SM (four fit), V = 50257, a row and its q rejected now and then: one sequence
+    // 8 5.8 us, 4 6.6, 2 9.1; 64: 8 10.5, 4 9.6, 2 12.4; 128: 8 20.3, 4 16.2, 2 16.4; 256: 8 36, 4 27.5, 2 26.4
     int64_t ctas = 8;
     while (ctas > 2 && R * ctas > 3 * 148) ctas >>= 1;
     if (dtype == MBEMA_F32) return ctas == 8 ? launch<MBEMA_F32, 8>(a, R, stream) : ctas == 4 ? launch<MBEMA_F32, 4>(a, R, stream) : launch<MBEMA_F32, 2>(a, R, stream);
