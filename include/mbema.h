@@ -14,7 +14,8 @@
  *     may run concurrently as long as their buffers differ (one exception: mbema_query_scan_static, whose
  *     scratch is a device array inside the library; see there);
  *   - STATUS WORD of the tensor-core entry points (mbema_flash_fwd / _bwd / _rows in MBEMA_MODE_TC_BF16,
- *     mbema_decode_attend_tc): the int32 at the start of `workspace` (the workspace must be 256-byte aligned).
+ *     mbema_decode_attend_tc): the int32 at the start of `workspace` (the workspace must be 256-byte aligned);
+ *     of mbema_branches_attend: the one that mbema_branches names.
  *     The kernels only ever OR into it and the library never clears it: zero it once, keep passing the same
  *     buffer, and read it at a synchronisation point of your choice.  Non-zero means a bounded wait inside a
  *     kernel gave up (bit 0; bits 8.. name the wait): the outputs of that call and of every later call that
@@ -348,13 +349,16 @@ int mbema_decode_advance(int32_t* t_now_dev, void* stream);
  * The prefix (state, last_t, active, n_active: the layout above) is read and left alone until mbema_branches_adopt; the other
  * buffers belong to the branches and are filled by the calls below (no initial values needed).
  *   mbema_branches_init    empty branches at step t_now (or *t_now_dev)
- *   mbema_branches_extend  keeps the n_pending tokens staged by the call before (0 after mbema_branches_keep), then stages
+ *   mbema_branches_extend  keeps the n_pending tokens staged by the call before (0 after mbema_branches_keep; a captured call
+ *                          repeats the number that it was given), then stages
  *                          tok [B,S,n] i64 (-1: none; the step passes all the same): C_q [B,S,n,N] f32 = state of every token
  *                          just before its own step
  *   mbema_branches_keep    keeps the first counts[b] (i64, clamped to 0..n_pending) staged tokens of sequence b, drops the others
  *   mbema_branches_attend  O[b,s,j,h,:] = softmax over all V_total slots of q.K/sqrt(hd) times V with the slot states that row
  *                          sees; q, O [B,S,n,H,64] of q_dtype, E_k/E_v [V,H*64], n = the staged count.  mode
- *                          MBEMA_MODE_TC_BF16: tensor cores (bf16 q and tables, N = 64 or 128), MBEMA_MODE_FP32: fp32 arithmetic
+ *                          MBEMA_MODE_TC_BF16: tensor cores (bf16 q and tables, N = 64 or 128; states above 4.19 million and
+ *                          |W_pe| above 1023 are taken as that), MBEMA_MODE_FP32: fp32 arithmetic.  Calls on different streams
+ *                          with workspaces of their own may run at once
  *   mbema_branches_adopt   moves branch[b] (i64) of every sequence into its prefix; step numbers move so that the next step of
  *                          every sequence is t_next (>= t0 + len)
  * *overflow: 1 an own or active list is full, 2 a token is outside [0, V) (and not -1), 3 branch[b] is outside [0, S),

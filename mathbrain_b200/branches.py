@@ -14,6 +14,9 @@ Sampling: S continuations of a prompt, `extend` with one token each; the tokens 
 Drafts:   S = 1, `extend` with the last token and G drafted ones; `verify_drafts` (mathbrain_b200/verify.py) says how many stand,
           `keep(n_accepted + 1)` drops the others.
 Scoring candidates: `extend`, `attend`, `keep` of zeros.
+
+The calls can be captured in CUDA graphs.  A captured `extend` keeps as many tokens at every replay as were staged when it was captured:
+capture a sampling step after one eager `extend`, a drafting round from `extend` to `keep`.
 """
 import ctypes
 
@@ -131,7 +134,7 @@ class Branches:
         """O [B, S, n, H, 64] of q's dtype for the n staged rows of every branch.  q [B, S, n, H, 64] float32 or bfloat16;
         E_k, E_v [V, H*64] projected slot embeddings; W_pe [N, H*64].  Softmax over all V_total slots (the vocabulary by
         default), those that a row does not see with score 0 and value 0; listed_only: over the seen ones alone (a row that
-        has seen none gets 0).  mode: "fp32", "tc_bf16" or "auto" (the package option `mode` by default): the tensor cores
+        has seen none gets 0).  E_v is taken in E_k's type.  mode: "fp32", "tc_bf16" or "auto" (the package option `mode` by default): the tensor cores
         take bfloat16 q and tables with 64 or 128 channels, "auto" runs anything else in fp32 arithmetic."""
         self._alive()
         dev = self._dev

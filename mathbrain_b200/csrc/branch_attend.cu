@@ -537,8 +537,9 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
 }
 
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st) {
-    // eight steps a CTA where three CTAs an SM are left: W then crosses L2 less often (64 sequences of 6 drafted rows: 399 us, with a step
-    // a CTA 408); a step a CTA otherwise, as its loads then do not wait for one another (8 drafted rows of one sequence: 19 us, with eight 31)
+    // eight steps a CTA where three CTAs an SM are left: W then crosses L2 less often (64 sequences of 6 drafted rows with their attention: 394 us,
+    // with a step a CTA 9 more); a step a CTA otherwise, as its loads then do not wait for one another (8 drafted rows of one sequence: 17 us,
+    // with eight 12 more)
     const int64_t heads = a.br.B * a.br.S * a.H;
     const int RJ = heads * ((a.n + BM_ROWS - 1) / BM_ROWS) >= 3 * 148 ? std::min(a.n, BM_ROWS) : 1;
     const int64_t ctas = heads * ((a.n + RJ - 1) / RJ);

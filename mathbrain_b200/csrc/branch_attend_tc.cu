@@ -13,8 +13,11 @@
 // ends, and each piece leaves a partial (m, l, o[64]) a row.  The operand and E rows of a unit come by cp.async into a ring of
 // shared memory, some units ahead across the ends of lists: they are gathered rows that mostly come from DRAM, and with them loaded
 // a unit ahead into registers half of all cycles were spent waiting.
-// Own slots go through tcgen05 in branch_rows_tc.cu's tiles of 128 slots too, but not faster: its two gathering warps and a list's start
-// and end (own lists are short) took 4 x 16 branches of 400 own slots from 31 us to 45, 64 branches of 180 from 31 to 39.
+// Own slots go through tcgen05 in branch_rows_tc.cu's tiles of 128 slots too, but not faster: with its two gathering warps and a list's start
+// and end (own lists are short) 4 x 16 branches of 400 own slots took half as long again, 64 branches of 180 a quarter.
+// 64 branches of 180 own slots behind a prefix of 3400, 8 heads, 64 channels: 24 us with 11 units a warp, of which 5 us until the first
+// unit is there, 3 for the ends of lists and 13 for the units' arithmetic (750 instructions each, 39 % of the issue slots: two warps a
+// scheduler, as W and the accumulators leave registers for).
 #include <algorithm>
 
 #include "branches.cuh"

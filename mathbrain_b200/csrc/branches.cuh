@@ -1,4 +1,4 @@
-// Branches of a decode state: what the kernels of branches.cu, branch_attend.cu and branch_attend_tc.cu share.
+// Branches of a decode state: what the kernels of branches.cu, branch_attend.cu, branch_attend_tc.cu and branch_rows_tc.cu share.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -139,7 +139,9 @@ inline cudaError_t allow_smem(Kernel kernel, size_t most, std::atomic<unsigned l
     return e;
 }
 
-// A kernel whose CTAs may start while the kernel before it still runs (it waits for it with br_wait_for_kernel_before).
+// A kernel whose CTAs may start while the kernel before it still runs; it waits for that one's end with br_wait_for_kernel_before.  All
+// kernels here wait before their first access and only then let the next one start (the merge and the operands reach further: see there);
+// so a kernel's end means the end of all before it.  A launch costs about 2 us less.
 template <typename... Params, typename... Args>
 inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
