@@ -30,7 +30,9 @@ static size_t ba_smem(int N) {
 // grid: x = prefix jobs (B, blocks of 32 branches, chunks; then blocks of steps), then own jobs (B * S, chunks; all steps); y = head.
 // A job's rows are (step, branch) pairs, 32 at most: the tile's states and E rows, loaded once, serve as many steps as that allows.
 // The gate product is tiled 4 slots x 4 channels to a thread (three wavefronts of shared memory for 16 FMAs a warp; one slot and 16
-// channels take nine).  Bound by latency at small sizes: nine meetings of the CTA a tile and step.
+// channels take nine); from step to step the states are multiplied by rho in place, which costs a tenth of a power in front of every row of W.
+// 2 sequences x 5 branches x 3 rows, 701 slots: 30 us, bound by latency (eight meetings of the CTA a tile and step); 8 x 2 x 4, 2000 slots: 260,
+// 64 % of the issue slots and of shared memory's wavefronts.
 __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     extern __shared__ __align__(16) float smem[];
     br_wait_for_kernel_before();
@@ -77,8 +79,8 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     float* o_sh = q_sh + BA_ROWS * BR_HD;                 // [32][64]
     float* P_sh = o_sh + BA_ROWS * BR_HD;                 // [32][68]
     float* l2r_sh = P_sh + BA_ROWS * BA_LD;
-    float* pw_sh = l2r_sh + ((N + 3) & ~3);               // rho^(step - j0)
-    float* m_sh = pw_sh + ((N + 3) & ~3);
+    float* rho_sh = l2r_sh + ((N + 3) & ~3);
+    float* m_sh = rho_sh + ((N + 3) & ~3);
     float* l_sh = m_sh + BA_ROWS;
     float* al_sh = l_sh + BA_ROWS;
     int* v_sh = reinterpret_cast<int*>(al_sh + BA_ROWS);  // the tile's slots, and their ages
@@ -109,7 +111,10 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     if (tid < BA_TILE) slots_of(k_lo);
     for (int i = tid; i < N * (BR_HD / 4); i += BA_THREADS)
         *reinterpret_cast<float4*>(W_sh + i * 4) = *reinterpret_cast<const float4*>(a.W + (size_t)(i >> 4) * D + h * BR_HD + (i & 15) * 4);
-    for (int i = tid; i < N; i += BA_THREADS) l2r_sh[i] = br_log2(br.rhos[i]);
+    for (int i = tid; i < N; i += BA_THREADS) {
+        rho_sh[i] = br.rhos[i];
+        l2r_sh[i] = br_log2(rho_sh[i]);
+    }
     for (int i = tid; i < rows * BR_HD; i += BA_THREADS) {
         const int row = i >> 6, st = row / branches;
         q_sh[i] = ld_dyn_f32(a.q, a.q_dt, ((((size_t)(r0 + row - st * branches)) * n + j0 + st) * H + h) * BR_HD + (i & 63)) * BR_SCORE_LOG2;
@@ -156,17 +161,14 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
         }
         for (int st = 0; st < steps; ++st) {
             const int j = j0 + st, base = st * branches;
-            for (int c = tid; c < N; c += BA_THREADS) pw_sh[c] = exp2f((float)st * l2r_sh[c]);
-            __syncthreads();                              // states and powers are there, the step before has read K, V and P
+            __syncthreads();                              // the states are there, the step before has read K, V and P
             float acc[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll 8
             for (int c = 0; c < N; ++c) {
                 const float4 x = *reinterpret_cast<const float4*>(A_sh + c * BA_LD + 4 * (ty ^ ((c >> 2) & 7)));
-                float4 w = *reinterpret_cast<const float4*>(W_sh + c * BR_HD + 4 * tx);
-                const float pw = pw_sh[c];
-                w.x *= pw; w.y *= pw; w.z *= pw; w.w *= pw;
+                const float4 w = *reinterpret_cast<const float4*>(W_sh + c * BR_HD + 4 * tx);
                 const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -186,6 +188,15 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
                 *reinterpret_cast<float4*>(V_sh + at) = make_float4(ev[i].x * g[0], ev[i].y * g[1], ev[i].z * g[2], ev[i].w * g[3]);
             }
             __syncthreads();
+            if (st + 1 < steps) {                         // the next step's states: every one has been read (at most 31 roundings of 2^-24)
+                for (int i = tid; i < N * (BA_TILE / 4); i += BA_THREADS) {
+                    float4* x = reinterpret_cast<float4*>(A_sh + (i >> 4) * BA_LD + 4 * (i & 15));
+                    const float rho = rho_sh[i >> 4];
+                    float4 y = *x;
+                    y.x *= rho; y.y *= rho; y.z *= rho; y.w *= rho;
+                    *x = y;
+                }
+            }
             if (st + 1 == steps && tid < BA_TILE && k0 + BA_TILE < k_hi) slots_of(k0 + BA_TILE);
             for (int br0 = group; br0 < branches; br0 += 16) {        // branches br0, br0 + 4, + 8, + 12 against one slot's K
                 const float4* kp = reinterpret_cast<const float4*>(K_sh + slot * BA_LD);
