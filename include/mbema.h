@@ -21,6 +21,8 @@
  *     kernel gave up (bit 0; bits 8.. name the wait): the outputs of that call and of every later call that
  *     still sees the non-zero word are undefined (their CTAs skip their work).  Zero it again to go on;
  *   - `stream` is a cudaStream_t passed as void*; work is only enqueued, no entry point synchronises;
+ *     mbema_branches_* and mbema_verify_drafts launch with programmatic stream serialization and wait for the kernel
+ *     before them in the stream; if the caller launches that one so too, it has to wait for its own predecessors;
  *   - the return value is 0 on success, otherwise an MBEMA_ERR_* code (see mbema_strerror); argument
  *     errors are detected before anything is launched;
  *   - dtype codes: MBEMA_F32 = 0, MBEMA_BF16 = 1.
