@@ -10,11 +10,11 @@
 // Roles: three epilogue groups of four warps; two warps gather the E_k and E_v rows (cp.async, mbarrier arrivals), one lane copies
 // the operands, one issues the products.  With one step the groups are workers with stretches of their own, a tile each in turn; with
 // two or three steps they take the same tile, a step each.
-// 64 sequences, 3400 + 90 slots, 6 rows, 8 heads, 64 channels: 381 us (0.56e9 tanh of 16 a clock and SM would be 122), about 4200 cycles for a
-// tile of three steps.  Of these the three epilogue warps of a scheduler issue for 2200 (735 instructions a warp and tile: eight a slot,
-// channel and step, one of them MUFU) and have MUFU work for 1540; the rest are waits that three warps, which is what o[64] leaves registers
-// for, do not hide.  V rounded to bf16 with P . V in mixed-precision FMA needs fewer instructions, but they and the conversions run at half
-// to three quarters of the fp32 rate: 433 us.  The next tile's first channels loaded before this one is left: 398 us.
+// 64 sequences, 3400 + 90 slots, 6 rows, 8 heads, 64 channels: 340 us (0.56e9 tanh of 16 a clock and SM would be 122).  Of a tile's 3800 cycles
+// the three epilogue warps of a scheduler have MUFU work for 1540 and instructions for about 1700; the rest are waits that three warps, which
+// is what o[64] leaves registers for, do not hide.  The two passes written out (372 us without), the mask before the waits, two FMA to an
+// instruction (10 us).  V rounded to bf16 with P . V in mixed-precision FMA needs fewer instructions, but they and the conversions run at half
+// to three quarters of the fp32 rate: an eighth slower.  The next tile's first channels loaded before this one is left: 4 % slower.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,7 +28,9 @@ using namespace ptx;
 
 static constexpr int TILE = BR_TILE, GROUPS = 3, EPI_WARPS = 4 * GROUPS, THREADS = (EPI_WARPS + 4) * 32;
 static constexpr int WARP_K = EPI_WARPS, WARP_V = EPI_WARPS + 1, WARP_MMA = EPI_WARPS + 2, WARP_A = EPI_WARPS + 3;
-// setmaxnreg: 12 * 32 * 144 (epilogue) + 4 * 32 * 80 (producers) = the launch allocation 512 * 128
+// setmaxnreg: 12 * 32 * 152 (epilogue) + 4 * 32 * 56 (the other warps) = 12 * 32 * 144 + 4 * 32 * 80 = the launch allocation 512 * 128.  The
+// second with three workers: each copying warp then follows three stretches, and with 56 registers keeps them in memory (64 sequences of
+// one row 177 us for 121); the first otherwise (of six rows 364 us for 373).
 static constexpr float W_SCALE = 64.0f;           // undoes BR_OP_SCALE
 
 template <int ATOMS>                               // of 64 state channels
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
     const volatile int* count_of = bars->tiles;
 
     if (warp >= EPI_WARPS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if constexpr (IG == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp <= WARP_V) {
             // ------------------------------------------------------------ gathering warps: E_k or E_v rows, 8 lanes a row
             const char* table = reinterpret_cast<const char*>(warp == WARP_K ? a.Ek : a.Ev) + h * (BR_HD * 2) + (lane & 7) * 16;
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
         }
     } else {
         // ---------------------------------------------------------------- epilogue: a thread a slot
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+        if constexpr (IG == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;"); else asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         {   // W of every step, fp16, K-major rows of 64 state channels, 128-byte swizzle: a thread packs 8 channels of one output column
             const float scale = SILU ? 0.5f * W_SCALE : W_SCALE;      // SiLU(x) = h + h tanh(h), h = x / 2
             for (int i = tid; i < N * 8; i += EPI_WARPS * 32) {
@@ -337,7 +339,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     fresh = false;
                 }
                 const int k_w = cur.k + quarter * 32;             // this warp's 32 slots
-                const unsigned touched = bits && k_w < br.Kcap ? bits[k_w >> 5] : 0u;
+                unsigned hide = bits && k_w < br.Kcap ? bits[k_w >> 5] : 0u;      // slots that the row does not see
+                if (j > 0) {
+                    const unsigned d = (unsigned)(staged - k_w);
+                    hide |= __reduce_or_sync(0xffffffffu, d < 32u ? 1u << d : 0u);
+                }
+                if (cur.count - k_w < 32) hide |= 0xffffffffu << max(cur.count - k_w, 0);
                 const uint32_t e_at = e_row + st * L::E_STAGE, t_at = taddr + (uint32_t)((r & 1) * BR_HD);
                 go = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[group][r & 1], (uint32_t)((r >> 1) & 1), abort_flag, 8));
                 if (go) go = __all_sync(0xffffffffu, mbar_wait(&bars->e_full[st], (uint32_t)(use & 1), abort_flag, 9));
@@ -350,7 +357,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     const uint32_t e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
                     if (SILU) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) g16[i] = fmaf(g16[i], tanh_approx(g16[i]), g16[i]);
+                        for (int i = 0; i < 16; i += 2) {
+                            const uint64_t x2 = pair2(g16[i], g16[i + 1]);
+                            unpair2(g16[i], g16[i + 1], fma2(x2, pair2(tanh_approx(g16[i]), tanh_approx(g16[i + 1])), x2));
+                        }
                         if (c < 2) tmem_st_32x32b_x16(t_at + (uint32_t)(c * 16), g16);
                     }
                     const uint4 qa = lds128<0>(q_at + c * 32), qb = lds128<16>(q_at + c * 32);
@@ -359,12 +369,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     for (int i = 0; i < 8; ++i) {                 // (the product of two bf16 is exact in fp32, and needs no unpacking)
                         float x = 0.f, y = 0.f;
                         fma_f32_bf16x2(x, y, e[i], q[i]);
-                        s0 = fmaf(x, g16[2 * i], s0);
-                        s1 = fmaf(y, g16[2 * i + 1], s1);
+                        unpair2(s0, s1, fma2(pair2(x, y), pair2(g16[2 * i], g16[2 * i + 1]), pair2(s0, s1)));
                     }
                 };
                 tmem_ld16_nb(t_at, v0);
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < 4; c += 2) {
                     tmem_wait_ld16(v0);
                     tmem_ld16_nb(t_at + (uint32_t)((c + 1) * 16), v1);
@@ -373,12 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     if (c < 2) tmem_ld16_nb(t_at + 32, v0);
                     score(v1, c + 1);
                 }
-                unsigned hide = touched;
-                if (j > 0) {
-                    const unsigned d = (unsigned)(staged - k_w);
-                    hide |= __reduce_or_sync(0xffffffffu, d < 32u ? 1u << d : 0u);
-                }
-                const bool hidden = ((hide >> lane) & 1u) || k_w + lane >= cur.count;
+                const bool hidden = (hide >> lane) & 1u;
                 const float x = (s0 + s1) * BR_SCORE_LOG2;
                 const bool grow = !hidden && x > m + 8.0f;        // o is scaled again only where the maximum moves by more than 2^8
                 if (__any_sync(0xffffffffu, grow)) {
@@ -390,14 +394,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 }
                 const float p = hidden || x == -INFINITY ? 0.f : ex2_approx(x - m);      // (below fp32: no weight, before any maximum too)
                 l += p;
+                const uint64_t p2 = pair2(p, p);
                 auto values = [&](float (&g16)[16], auto chunk) {
                     constexpr int c = decltype(chunk)::value;
                     const uint4 e0 = lds128<16384>(e_at ^ (c << 5)), e1 = lds128<16384>(e_at ^ ((c << 5) | 16));
                     const uint32_t e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {                 // (a hidden slot's value that is not finite: the row lists the same slot as its own)
-                        o[c * 16 + 2 * i] = fmaf(p * g16[2 * i], bf16_lo(e[i]), o[c * 16 + 2 * i]);
-                        o[c * 16 + 2 * i + 1] = fmaf(p * g16[2 * i + 1], bf16_hi(e[i]), o[c * 16 + 2 * i + 1]);
+                        const uint64_t w2 = mul2(p2, pair2(g16[2 * i], g16[2 * i + 1]));
+                        unpair2(o[c * 16 + 2 * i], o[c * 16 + 2 * i + 1], fma2(w2, pair2(bf16_lo(e[i]), bf16_hi(e[i])), pair2(o[c * 16 + 2 * i], o[c * 16 + 2 * i + 1])));
                     }
                 };
                 values(v0, std::integral_constant<int, 2>());

@@ -159,6 +159,24 @@ inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int thread
 __device__ __forceinline__ void br_wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void br_let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Two fp32 values as one operand: one instruction for two FMA, at the same rate (it is issue slots that run short).
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair2(float& a, float& b, uint64_t r) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 bool branch_tc_supported(int64_t N);
 BranchShape branch_shape(int64_t S, int64_t n, int64_t H);
 BranchRows branch_rows(int64_t n, int64_t H);
