@@ -198,7 +198,10 @@ __device__ __forceinline__ void apply_gate(float (&acc)[8][4], int silu) {
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][e] = fmaf(acc[nt][e], tanh_fast(acc[nt][e]), acc[nt][e]);
+            for (int e = 0; e < 4; e += 2) {
+                const uint64_t x = pair2(acc[nt][e], acc[nt][e + 1]);
+                unpair2(acc[nt][e], acc[nt][e + 1], fma2(x, pair2(tanh_fast(acc[nt][e]), tanh_fast(acc[nt][e + 1])), x));
+            }
     }
 }
 
@@ -297,11 +300,9 @@ struct OneRow {
         for (int nt = 0; nt < 8; ++nt) {
             float x, y;                                          // (the product of two bf16 is exact in fp32, and needs no unpacking)
             mul_bf16x2(x, y, e0[nt], q[nt]);
-            s0 = fmaf(x, acc[nt][0], s0);
-            s1 = fmaf(y, acc[nt][1], s1);
+            unpair2(s0, s1, fma2(pair2(x, y), pair2(acc[nt][0], acc[nt][1]), pair2(s0, s1)));
             mul_bf16x2(x, y, e1[nt], q[nt]);
-            s2 = fmaf(x, acc[nt][2], s2);
-            s3 = fmaf(y, acc[nt][3], s3);
+            unpair2(s2, s3, fma2(pair2(x, y), pair2(acc[nt][2], acc[nt][3]), pair2(s2, s3)));
         }
         load_E<2048>(e0, e1, at_lo, at_hi);
         s0 += s1;
@@ -324,8 +325,9 @@ struct OneRow {
         l += p0 + p1;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {      // (a value that is not finite stays in a row that hides it: the same slot is listed as the branch's own)
-            o[2 * nt] = fmaf(p0 * acc[nt][0], bf_lo(e0[nt]), fmaf(p1 * acc[nt][2], bf_lo(e1[nt]), o[2 * nt]));
-            o[2 * nt + 1] = fmaf(p0 * acc[nt][1], bf_hi(e0[nt]), fmaf(p1 * acc[nt][3], bf_hi(e1[nt]), o[2 * nt + 1]));
+            const uint64_t w0 = mul2(pair2(p0, p0), pair2(acc[nt][0], acc[nt][1])), w1 = mul2(pair2(p1, p1), pair2(acc[nt][2], acc[nt][3]));
+            const uint64_t x = fma2(w1, pair2(bf_lo(e1[nt]), bf_hi(e1[nt])), pair2(o[2 * nt], o[2 * nt + 1]));
+            unpair2(o[2 * nt], o[2 * nt + 1], fma2(w0, pair2(bf_lo(e0[nt]), bf_hi(e0[nt])), x));
         }
     }
     __device__ __forceinline__ void leave(const BranchArgs& a, int64_t piece, int j, int h, int lane) {
@@ -375,8 +377,9 @@ struct SixteenRows {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int nt = 2 * c + p;
-                const float x0 = bf_lo(e0[nt]) * acc[nt][0], x1 = bf_hi(e0[nt]) * acc[nt][1];
-                const float y0 = bf_lo(e1[nt]) * acc[nt][2], y1 = bf_hi(e1[nt]) * acc[nt][3];
+                float x0, x1, y0, y1;
+                unpair2(x0, x1, mul2(pair2(bf_lo(e0[nt]), bf_hi(e0[nt])), pair2(acc[nt][0], acc[nt][1])));
+                unpair2(y0, y1, mul2(pair2(bf_lo(e1[nt]), bf_hi(e1[nt])), pair2(acc[nt][2], acc[nt][3])));
                 hi[0][p] = pack_bf2(x0, x1);
                 hi[1][p] = pack_bf2(y0, y1);
                 lo[0][p] = pack_bf2(x0 - bf_lo(hi[0][p]), x1 - bf_hi(hi[0][p]));
@@ -446,8 +449,10 @@ struct SixteenRows {
         }
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-            const uint32_t b0 = transpose8x8(pack_bf2(bf_lo(e0[nt]) * acc[nt][0], bf_hi(e0[nt]) * acc[nt][1]));
-            const uint32_t b1 = transpose8x8(pack_bf2(bf_lo(e1[nt]) * acc[nt][2], bf_hi(e1[nt]) * acc[nt][3]));
+            float x0, x1, y0, y1;
+            unpair2(x0, x1, mul2(pair2(bf_lo(e0[nt]), bf_hi(e0[nt])), pair2(acc[nt][0], acc[nt][1])));
+            unpair2(y0, y1, mul2(pair2(bf_lo(e1[nt]), bf_hi(e1[nt])), pair2(acc[nt][2], acc[nt][3])));
+            const uint32_t b0 = transpose8x8(pack_bf2(x0, x1)), b1 = transpose8x8(pack_bf2(y0, y1));
             mma_bf16(o[nt], P, b0, b1);
         }
     }
