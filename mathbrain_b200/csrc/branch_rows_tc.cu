@@ -10,8 +10,8 @@
 // Roles: three epilogue groups of four warps; two warps gather the E_k and E_v rows (cp.async, mbarrier arrivals), one lane copies
 // the operands, one issues the products.  With one step the groups are workers with stretches of their own, a tile each in turn; with
 // two or three steps they take the same tile, a step each.
-// 64 sequences, 3400 + 90 slots, 6 rows, 8 heads, 64 channels: 340 us (0.56e9 tanh of 16 a clock and SM would be 122).  Of a tile's 3800 cycles
-// the three epilogue warps of a scheduler have MUFU work for 1540 and instructions for about 1700; the rest are waits that three warps, which
+// 64 sequences, 3400 + 90 slots, 6 rows, 8 heads, 64 channels: 330 us (0.56e9 tanh of 16 a clock and SM would be 122).  Of a tile's 3700 cycles
+// the three epilogue warps of a scheduler have MUFU work for 1540 and instructions for about 2100; the rest are waits that three warps, which
 // is what o[64] leaves registers for, do not hide.  The two passes written out (372 us without), the mask before the waits, two FMA to an
 // instruction (10 us).  V rounded to bf16 with P . V in mixed-precision FMA needs fewer instructions, but they and the conversions run at half
 // to three quarters of the fp32 rate: an eighth slower.  The next tile's first channels loaded before this one is left: 4 % slower.
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             };
             int q_list = cur.list;                                // the list whose q has been fetched
             uint32_t q_next = q_of(q_list);
-            float m = -INFINITY, l = 0.f, o[64];
+            float m = -INFINITY, m8 = -INFINITY, l = 0.f, o[64];
             int staged = -1;
             const uint32_t* bits = nullptr;
             bool fresh = true, go = true;
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                     q_next = q_of(q_list);
                     staged = lane < j ? (prefix ? br.st_pos : br.st_own)[br_index(br, branch, lane)] : -1;
                     bits = prefix ? br.touched + (size_t)branch * ((br.Kcap + 31) / 32) : nullptr;
-                    m = -INFINITY;
+                    m = m8 = -INFINITY;
                     l = 0.f;
 #pragma unroll
                     for (int i = 0; i < 64; ++i) o[i] = 0.f;
@@ -384,10 +384,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 }
                 const bool hidden = (hide >> lane) & 1u;
                 const float x = (s0 + s1) * BR_SCORE_LOG2;
-                const bool grow = !hidden && x > m + 8.0f;        // o is scaled again only where the maximum moves by more than 2^8
+                const bool grow = !hidden && x > m8;        // o is scaled again only where the maximum moves by more than 2^8
                 if (__any_sync(0xffffffffu, grow)) {
                     const float alpha = grow ? ex2_approx(m - x) : 1.0f;
-                    if (grow) m = x;
+                    if (grow) { m = x; m8 = x + 8.0f; }
                     l *= alpha;
 #pragma unroll
                     for (int i = 0; i < 64; ++i) o[i] *= alpha;
@@ -413,13 +413,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
                 tmem_ld16_nb(t_at + 16, v1);
                 values(v0, std::integral_constant<int, 0>());
                 tmem_wait_ld16(v1);
-                values(v1, std::integral_constant<int, 1>());
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&bars->acc_empty[group][r & 1]);
-                    mbar_arrive(&bars->e_empty[st]);
-                }
+                if (lane == 0) mbar_arrive(&bars->acc_empty[group][r & 1]);
+                values(v1, std::integral_constant<int, 1>());
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->e_empty[st]);
                 int by = 0;                                       // to this worker's tile of the next round
 #pragma unroll
                 for (int x = 0; x < IG; ++x) by += (x < g ? r + 1 : r) < others[x];
