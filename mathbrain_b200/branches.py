@@ -30,7 +30,7 @@ _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 class Branches:
     """Made by DecodeState.fork.  While the branches live the state must not be updated (its own tokens are the branches'
-    prefix); a call on them after an update raises.  Memory: 6 N bytes for each of capacity slots a branch, and, with 64 or 128
+    prefix); a call on them after an update raises (one by a replayed graph is not noticed).  Memory: 6 N bytes for each of capacity slots a branch, and, with 64 or 128
     channels, 2 N bytes for each slot of the state's capacity."""
 
     def __init__(self, prefix, branches, t_now, capacity=1024, max_new=16):
