@@ -30,8 +30,8 @@ _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 class Branches:
     """Made by DecodeState.fork.  While the branches live the state must not be updated (its own tokens are the branches'
-    prefix); a call on them after an update raises (one by a replayed graph is not noticed).  Memory: 6 N bytes for each of capacity slots a branch, and, with 64 or 128
-    channels, 2 N bytes for each slot of the state's capacity."""
+    prefix); a call on them after an update raises (one by a replayed graph is not noticed).  Memory: 6 N bytes for each of
+    capacity slots a branch, and, with 64 or 128 channels, 2 N bytes for each slot of the state's capacity."""
 
     def __init__(self, prefix, branches, t_now, capacity=1024, max_new=16):
         B, V, N, Kcap = prefix.B, prefix.V, prefix.N, prefix.cap
@@ -135,8 +135,9 @@ class Branches:
         """O [B, S, n, H, 64] of q's dtype for the n staged rows of every branch.  q [B, S, n, H, 64] float32 or bfloat16;
         E_k, E_v [V, H*64] projected slot embeddings; W_pe [N, H*64].  Softmax over all V_total slots (the vocabulary by
         default), those that a row does not see with score 0 and value 0; listed_only: over the seen ones alone (a row that
-        has seen none gets 0).  E_v is taken in E_k's type.  mode: "fp32", "tc_bf16" or "auto" (the package option `mode` by default): the tensor cores
-        take bfloat16 q and tables with 64 or 128 channels, "auto" runs anything else in fp32 arithmetic."""
+        has seen none gets 0).  E_v is taken in E_k's type.  mode: "fp32", "tc_bf16" or "auto" (the package option `mode` by
+        default): the tensor cores take bfloat16 q and tables with 64 or 128 channels, "auto" runs anything else in fp32
+        arithmetic."""
         self._alive()
         dev = self._dev
         if q.get_device() != dev or E_k.get_device() != dev or E_v.get_device() != dev or W_pe.get_device() != dev:
