@@ -104,7 +104,10 @@ class Branches:
             raise _lib.MbemaError("extend: tokens %s, expected [%d, %d, 1 to %d]" % (tuple(shape), self.B, self.S, self.max_new))
         if tok.dtype != torch.int64:
             raise _lib.MbemaError("extend: tokens of %s, expected int64" % tok.dtype)
-        return self._on_device(self._extend, tok.contiguous())
+        if self._dev == _current_device():
+            return self._extend(tok.contiguous())
+        with torch.cuda.device(self._dev):
+            return self._extend(tok.contiguous())
 
     def _extend(self, tok):
         n = tok.shape[2]
@@ -123,7 +126,9 @@ class Branches:
             self._refuse(counts)
         if counts.dim() != 1 or counts.shape[0] != self.B or counts.dtype not in _INTEGERS:
             raise _lib.MbemaError("keep: counts %s of %s, expected [%d] integers" % (tuple(counts.shape), counts.dtype, self.B))
-        return self._on_device(self._keep, counts.long().contiguous())
+        if counts.dtype != torch.int64:
+            counts = counts.long()
+        return self._on_device(self._keep, counts.contiguous())
 
     def _keep(self, counts):
         rc = self._lib.mbema_branches_keep(self._ref, counts.data_ptr(), self._staged, _raw_stream(self._dev))
@@ -145,17 +150,21 @@ class Branches:
         if mode is None:
             mode = _OPTIONS["mode"]
         # checked and sized once for operands of the same shapes, types and options
-        key = (q.shape, q.dtype, E_k.shape, E_k.dtype, E_v.shape, W_pe.shape, self._staged, V_total, use_silu, listed_only, mode)
+        key = (q.shape, q.dtype, E_k.shape, E_k.dtype, E_v.shape, E_v.dtype, W_pe.shape, W_pe.dtype, self._staged, V_total, use_silu,
+               listed_only, mode)
         plan = self._plans.get(key)
         if plan is None:
             plan = self._plan(q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode)
             if len(self._plans) >= 64:
                 self._plans.clear()
             self._plans[key] = plan
-        return self._on_device(self._attend, q, E_k, E_v, W_pe, plan)
+        if dev == _current_device():
+            return self._attend(q, E_k, E_v, W_pe, plan)
+        with torch.cuda.device(dev):
+            return self._attend(q, E_k, E_v, W_pe, plan)
 
     def _plan(self, q, E_k, E_v, W_pe, V_total, use_silu, listed_only, mode):
-        """(arguments of the C call behind O, workspace bytes)."""
+        """(arguments of the C call behind O, workspace bytes, whether E_v or W_pe have to be cast)."""
         n = self._staged
         if n == 0:
             raise _lib.MbemaError("attend: no staged tokens (call extend first)")
@@ -176,12 +185,14 @@ class Branches:
         code = _lib.MODE_TC_BF16 if fits and mode != "fp32" else _lib.MODE_FP32
         flags = (_lib.FLAG_SILU if use_silu else 0) | (_lib.FLAG_LISTED_ONLY if listed_only else 0)
         need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, n, H, self.prefix.cap, self.capacity, code)
-        return q_dt, e_dt, n, H, int(self.V if V_total is None else V_total), flags, code, need
+        cast = E_v.dtype != E_k.dtype or W_pe.dtype != torch.float32
+        return q_dt, e_dt, n, H, int(self.V if V_total is None else V_total), flags, code, need, cast
 
     def _attend(self, q, E_k, E_v, W_pe, plan):
-        q_dt, e_dt, n, H, V_total, flags, code, need = plan
-        q, E_k, W = q.contiguous(), E_k.contiguous(), W_pe.float().contiguous()
-        E_v = E_v.to(E_k.dtype).contiguous()
+        q_dt, e_dt, n, H, V_total, flags, code, need, cast = plan
+        if cast:
+            E_v, W_pe = E_v.to(E_k.dtype), W_pe.float()
+        q, E_k, E_v, W = q.contiguous(), E_k.contiguous(), E_v.contiguous(), W_pe.contiguous()
         O = torch.empty_like(q)
         ws = torch.empty(need, dtype=torch.uint8, device=self._device)
         rc = self._lib.mbema_branches_attend(self._ref, q.data_ptr(), q_dt, E_k.data_ptr(), E_v.data_ptr(), e_dt, W.data_ptr(), O.data_ptr(),
