@@ -406,3 +406,20 @@ def test_captured_behind_copies_and_joined_streams(S, dt):
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
     assert torch.equal(br.lengths, ref.lengths)
     br.check_overflow()
+
+
+@pytest.mark.parametrize("B,S,n,V,N,H", [(5000, 1, 2, 40, 64, 1), (1500, 1, 4, 50, 128, 1), (2000, 3, 2, 40, 64, 1),
+                                         (1, 4000, 1, 300, 64, 1), (1, 1, 1, 50257, 64, 1), (1, 3, 1, 50257, 64, 1)])
+def test_many_sequences_many_branches_and_the_whole_vocabulary(B, S, n, V, N, H):
+    """Thousands of short lists and the longest list there is: the tensor cores against fp32 arithmetic (2e-2 and 1e-4 of the exact)."""
+    listed = [(0, V, 7 * i % (V + 1))[i % 3] for i in range(B)] if B > 1 else [V]
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, listed, torch.bfloat16, 81)
+    br = st.fork(S, t0, capacity=64, max_new=8)
+    br.extend(torch.randint(0, V, (B, S, 8), generator=g).cuda())
+    br.extend(torch.randint(0, V, (B, S, n), generator=g).cuda())
+    q = torch.randn(B, S, n, H, 64, generator=g).bfloat16().cuda()
+    tabs = E_k.cuda(), E_v.cuda(), W.cuda()
+    O, exact = br.attend(q, *tabs), br.attend(q, *tabs, mode="fp32")
+    assert rel_err(O.float().cpu(), exact.float().cpu()) < 2e-2 + 1e-4 + 2 ** -8
+    assert br.device_status() == 0
+    br.check_overflow()
