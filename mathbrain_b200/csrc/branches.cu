@@ -177,11 +177,17 @@ __device__ void running_sum(int2* out, int lists, Count count_of) {
     if (tid == 0) out[lists] = make_int2(base, 0);
 }
 
+// the largest fp16 at most; NaN stays (fminf would return the other operand: a state that is lost would count as one of 4.19 million)
+__device__ __forceinline__ float half_range(float x) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(65504.f));
+    return r;
+}
 __device__ __forceinline__ void decayed(float (&f)[8], const float* src, float dt, const float (&l2r)[8]) {
     const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
     const float in[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fminf(in[e] * exp2f(dt * l2r[e]) * BR_OP_SCALE, 65504.f);
+    for (int e = 0; e < 8; ++e) f[e] = half_range(in[e] * exp2f(dt * l2r[e]) * BR_OP_SCALE);
 }
 __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
     const __half2 o = __floats2half2_rn(lo, hi);

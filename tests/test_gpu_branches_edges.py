@@ -1,0 +1,52 @@
+"""Branches of a decode state where values, options and reports are unusual; results are equal, or NaN, or not."""
+import pytest
+import torch
+
+from test_gpu_branches_use import _made_up
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [(1, torch.bfloat16, 64, None), (3, torch.bfloat16, 64, None), (1, torch.bfloat16, 128, None), (3, torch.bfloat16, 128, None),
+         (1, torch.bfloat16, 64, "fp32"), (3, torch.float32, 20, None)]
+
+
+@pytest.mark.parametrize("S,dt,N,mode", FORMS)
+def test_a_state_that_is_nan_reaches_the_rows_that_see_it(S, dt, N, mode):
+    """In a prefix slot: every row of the sequence, not the other sequence's.  In an own slot: the rows of its branch."""
+    B, n, V, H = 2, 2, 300, 2
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [200, 40], dt, 91)
+    tabs = E_k.cuda(), E_v.cuda(), W.cuda()
+    q = torch.randn(B, S, n, H, 64, generator=g).to(dt).cuda()
+    first = torch.randint(0, V, (B, S, n), generator=g).cuda()
+    tok = torch.randint(0, V, (B, S, n), generator=g).cuda()
+
+    def run(into):
+        br = st.fork(S, t0, capacity=8, max_new=n)
+        br.extend(first)
+        br.keep(torch.full((B,), n).cuda())
+        into(br)
+        br.extend(tok)
+        return br.attend(q, *tabs, mode=mode).isnan()
+
+    assert not run(lambda br: None).any()
+
+    def own(br):
+        br._hold["own_state"][1, S - 1, 0, N // 2] = float("nan")
+    seen = run(own)
+    assert seen[1, S - 1].all() and not seen[0].any() and not seen[1, :S - 1].any()
+    slot = next(v for v in st.active[0, :200].tolist() if v not in first[0].flatten().tolist() + tok[0].flatten().tolist())
+    st.state[0, slot, 5] = float("nan")
+    seen = run(lambda br: None)
+    assert seen[0].all() and not seen[1].any()
+
+
+@pytest.mark.parametrize("S,dt,N,mode", FORMS)
+def test_a_gate_weight_that_is_nan_reaches_its_head(S, dt, N, mode):
+    B, n, V, H = 1, 2, 100, 2
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [60], dt, 92)
+    W[N - 1, 64 + 7] = float("nan")
+    br = st.fork(S, t0, capacity=8, max_new=n)
+    br.extend(torch.randint(0, V, (B, S, n), generator=g).cuda())
+    q = torch.randn(B, S, n, H, 64, generator=g).to(dt).cuda()
+    O = br.attend(q, E_k.cuda(), E_v.cuda(), W.cuda(), mode=mode)
+    assert O[..., 1, :].isnan().all() and O[..., 0, :].isfinite().all()
