@@ -348,7 +348,8 @@ int mbema_decode_advance(int32_t* t_now_dev, void* stream);
  *   B sequences, S branches of each; a branch holds `len` kept tokens of its own behind the sequence's prefix and up to
  *   max_new (<= 32) staged ones.  Row (b, s, j) of a call with n staged tokens is step t0 + len + j: it sees the prefix, the
  *   branch's kept tokens and its staged tokens before j.  All branches of a sequence have the same length.
- * The prefix (state, last_t, active, n_active: the layout above) is read and left alone until mbema_branches_adopt; the other
+ * The prefix (state, last_t, active, n_active: the layout above; without the operand copies below a state may start at any
+ * float) is read and left alone until mbema_branches_adopt; the other
  * buffers belong to the branches and are filled by the calls below (no initial values needed).
  *   mbema_branches_init    empty branches at step t_now (or *t_now_dev)
  *   mbema_branches_extend  keeps the n_pending tokens staged by the call before (0 after mbema_branches_keep; a captured call
@@ -388,7 +389,7 @@ typedef struct mbema_branches {
     int32_t* st_new;        /* [B,S,max_new] 1: this place lists a slot that nothing before it lists */
     float* st_state;        /* [B,S,max_new,N] C_q of the staged tokens */
     void* pre_op;           /* [B,ceil128(Kcap),N] fp16 or NULL (with the next three): prefix states at the first staged step, */
-    void* own_op;           /* [B,S,ceil128(cap),N] fp16 or NULL: the same of the own slots; operands of the tensor cores, 16-byte aligned */
+    void* own_op;           /* [B,S,ceil128(cap),N] fp16 or NULL: the same of the own slots; operands of the tensor cores, 16-byte aligned, as state and own_state have to be with them */
     int32_t* work;          /* [B (ceil(S/16) + S) + 1, 2] or NULL: running sum of the lists' units, by which the work is dealt, and lengths */
     int32_t* status;        /* [1] or NULL: status word of the tensor-core attends (see the conventions above) */
     int32_t* overflow;      /* [1] */

@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
     const int tid = threadIdx.x;
     const int D = H * BR_HD;
     const int tau = br.t0[0] + br.len[r0] + j0;
+    const bool whole = N % 4 == 0 && !(((uintptr_t)br.state | (uintptr_t)br.own_state) & 15);      // (a state may be a view at any offset)
     for (int i = tid; i < branches * (j0 + steps); i += BA_THREADS) {
         const int branch = i / (j0 + steps), place = i - branch * (j0 + steps);
         pos_sh[branch * BR_MAX_NEW + place] = (own ? br.st_own : br.st_pos)[br_index(br, r0 + branch, place)];
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(BA_THREADS, 2) k_branch_attend(BranchArgs a) {
             const int words = (int)((br.Kcap + 31) / 32), word = (k0 >> 5) + (tid & 1);
             hid_sh[tid] = !own && word < words ? br.touched[(size_t)(r0 + (tid >> 1)) * words + word] : 0u;
         }
-        if (N % 4 == 0) {                                 // whole rows, 16 bytes a thread
+        if (whole) {                                      // whole rows, 16 bytes a thread
             for (int i = tid; i < BA_TILE * (N / 4); i += BA_THREADS) {
                 const int k = i / (N / 4), c = (i - k * (N / 4)) * 4;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -50,3 +50,25 @@ def test_a_gate_weight_that_is_nan_reaches_its_head(S, dt, N, mode):
     q = torch.randn(B, S, n, H, 64, generator=g).to(dt).cuda()
     O = br.attend(q, E_k.cuda(), E_v.cuda(), W.cuda(), mode=mode)
     assert O[..., 1, :].isnan().all() and O[..., 0, :].isfinite().all()
+
+
+@pytest.mark.parametrize("N,S,offset", [(32, 3, 1), (96, 1, 2), (4, 2, 3), (20, 1, 1)])
+def test_a_state_at_any_offset(N, S, offset):
+    """A contiguous view that starts between two 16-byte pieces: the same results."""
+    B, n, V, H = 2, 2, 90, 1
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [70, 12], torch.float32, 90)
+    tabs = E_k.cuda(), E_v.cuda(), W.cuda()
+    tok = torch.randint(0, V, (2, B, S, n), generator=g).cuda()
+    q = torch.randn(B, S, n, H, 64, generator=g).cuda()
+
+    def run():
+        br = st.fork(S, t0, capacity=8, max_new=n)
+        br.extend(tok[0])
+        return br.extend(tok[1]), br.attend(q, *tabs)
+
+    want = run()
+    buf = torch.empty(st.state.numel() + 4, device="cuda")
+    view = buf[offset:offset + st.state.numel()].view_as(st.state)
+    view.copy_(st.state)
+    st.state = view
+    assert view.data_ptr() % 16 != 0 and all(torch.equal(a, b) for a, b in zip(run(), want))
