@@ -603,12 +603,13 @@ extern "C" size_t mbema_branches_attend_workspace_bytes(int64_t B, int64_t S, in
 extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype,
                                      const float* W_pe, void* O, int64_t n, int64_t H, int64_t hd, int64_t V_total, int flags, int mode,
                                      void* workspace, size_t workspace_bytes, void* stream) {
-    if (!br) return MBEMA_ERR_NULL;
-    if (!plan_sizes_ok(br->B, br->S, n, H, br->Kcap, br->cap) || n > br->max_new || br->V < 1 || br->N < 1) return MBEMA_ERR_SHAPE;
-    if (hd != BR_HD || br->N > 128 || br->max_new > BR_MAX_NEW || (mode != MBEMA_MODE_FP32 && mode != MBEMA_MODE_TC_BF16)) return MBEMA_ERR_UNSUPPORTED;
+    int rc = check_branches(br);
+    if (rc != MBEMA_OK) return rc;
+    if (!plan_sizes_ok(br->B, br->S, n, H, br->Kcap, br->cap) || n > br->max_new) return MBEMA_ERR_SHAPE;
+    if (hd != BR_HD || (mode != MBEMA_MODE_FP32 && mode != MBEMA_MODE_TC_BF16)) return MBEMA_ERR_UNSUPPORTED;
     if (mode == MBEMA_MODE_TC_BF16 && (!branch_tc_supported(br->N) || q_dtype != MBEMA_BF16 || e_dtype != MBEMA_BF16)) return MBEMA_ERR_UNSUPPORTED;
     if (br->B == 0) return MBEMA_OK;
-    if (!q || !E_k || !E_v || !W_pe || !O || !workspace || !br->state || !br->active || !br->own_state || !br->st_state) return MBEMA_ERR_NULL;
+    if (!q || !E_k || !E_v || !W_pe || !O || !workspace) return MBEMA_ERR_NULL;
     if ((q_dtype != MBEMA_F32 && q_dtype != MBEMA_BF16) || (e_dtype != MBEMA_F32 && e_dtype != MBEMA_BF16)) return MBEMA_ERR_DTYPE;
     if (((uintptr_t)q | (uintptr_t)E_k | (uintptr_t)E_v | (uintptr_t)W_pe | (uintptr_t)O | (uintptr_t)workspace) & 15) return MBEMA_ERR_ALIGN;
     if (workspace_bytes < mbema_branches_attend_workspace_bytes(br->B, br->S, n, H, br->Kcap, br->cap, mode)) return MBEMA_ERR_WORKSPACE;
@@ -625,7 +626,7 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     a.ml = reinterpret_cast<float2*>(a.po + (size_t)parts * BR_HD);
     cudaStream_t st = (cudaStream_t)stream;
     const bool tc = mode == MBEMA_MODE_TC_BF16;
-    int rc = !tc ? launch_branch_attend_fp32(a, st)
-             : br->S == 1 ? launch_branch_rows(a, branch_rows(n, H), st) : launch_branch_attend_tc(a, branch_shape(br->S, n, H), st);
+    rc = !tc ? launch_branch_attend_fp32(a, st)
+         : br->S == 1 ? launch_branch_rows(a, branch_rows(n, H), st) : launch_branch_attend_tc(a, branch_shape(br->S, n, H), st);
     return rc != MBEMA_OK ? rc : launch_branch_merge(a, tc, st);
 }

@@ -318,7 +318,7 @@ __global__ void k_branch_adopt(mbema_branches br, const long long* __restrict__ 
     for (int k = tid; k < s_na; k += blockDim.x) br.last_t[(size_t)b * br.V + br.active[(size_t)b * Kcap + k]] += (int)shift;
 }
 
-static int check_branches(const mbema_branches* br) {
+int check_branches(const mbema_branches* br) {
     if (!br) return MBEMA_ERR_NULL;
     if (br->B < 0 || br->S < 1 || br->V < 1 || br->N < 1 || br->Kcap < 1 || br->cap < 1 || br->max_new < 1) return MBEMA_ERR_SHAPE;
     if (br->N > 128 || br->max_new > BR_MAX_NEW || br->B > 65535 || br->B * br->S > 0x7fffffff / 2 || br->V > 0x7fffffff ||
@@ -333,7 +333,7 @@ static int check_branches(const mbema_branches* br) {
     if (br->pre_op || br->own_op || br->work || br->status) {              // all four or none
         if (!branch_tc_supported(br->N) || br->S >= 65535 || br->B >= 65535) return MBEMA_ERR_UNSUPPORTED;
         if (!br->pre_op || !br->own_op || !br->work || !br->status) return MBEMA_ERR_NULL;
-        if (((uintptr_t)br->pre_op | (uintptr_t)br->own_op | (uintptr_t)br->state | (uintptr_t)br->own_state) & 15) return MBEMA_ERR_ALIGN;
+        if (((uintptr_t)br->pre_op | (uintptr_t)br->own_op | (uintptr_t)br->state | (uintptr_t)br->own_state) & 15 || (uintptr_t)br->work & 7) return MBEMA_ERR_ALIGN;
         const int64_t blocks = (br->S + BR_BLOCK - 1) / BR_BLOCK;                   // the running sums stay below 2^30
         if (br->B * blocks * (br->Kcap / 16 + 1) * BR_COST_BLOCK + br->B * br->S * (br->cap / 16 + 1) * BR_COST_OWN >= 1ll << 30) return MBEMA_ERR_UNSUPPORTED;
     }

@@ -177,6 +177,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
+int check_branches(const mbema_branches* br);         // sizes, pointers and alignment: what every entry point refuses
 bool branch_tc_supported(int64_t N);
 BranchShape branch_shape(int64_t S, int64_t n, int64_t H);
 BranchRows branch_rows(int64_t n, int64_t H);
