@@ -314,8 +314,8 @@ int mbema_accumulate_bf16(float* dst, const void* src, int64_t n, int add, void*
  *   K = E_k * gate(M W_pe), V = E_v * gate(M W_pe), M[v] = state[v] * rho^(t_now - last_t[v]); call it BEFORE
  *   mbema_decode_update of the same step.   q [B,H,64], E_k/E_v [V,H*64] (shared by all sequences), O [B,H,64] f32.
  * mbema_decode_update: C_q[b,:] = M[tok[b]] (query-side state, 0 if never seen), then state[tok] = C_q + 1,
- *   last_t[tok] = t_now, and tok joins the active list.  *overflow is set to 1 if a list is full, 2 if a token
- *   is outside [0, V).
+ *   last_t[tok] = t_now, and tok joins the active list.  *overflow: 1 is set if a list is full, 2 if a
+ *   token is outside [0, V) (both stay: 3).
  * ---------------------------------------------------------------------------------------------- */
 int mbema_decode_attend(const void* q, int q_dtype, const void* E_k, const void* E_v, int e_dtype, const float* W_pe,
                         const float* rhos, const float* state, const int32_t* last_t, const int32_t* active,
@@ -364,8 +364,8 @@ int mbema_decode_advance(int32_t* t_now_dev, void* stream);
  *                          with workspaces of their own may run at once
  *   mbema_branches_adopt   moves branch[b] (i64) of every sequence into its prefix; step numbers move so that the next step of
  *                          every sequence is t_next (>= t0 + len)
- * *overflow: 1 an own or active list is full, 2 a token is outside [0, V) (and not -1), 3 branch[b] is outside [0, S),
- * 4 t_next lies before a branch's end (that sequence stays as it was).
+ * *overflow, a sum of: 1 an own or active list is full, 2 a token is outside [0, V) (and not -1), 4 t_next lies before a branch's
+ * end, 8 branch[b] is outside [0, S) (with these two that sequence stays as it was).
  * ---------------------------------------------------------------------------------------------- */
 typedef struct mbema_branches {
     const float* rhos;      /* [N] */

@@ -23,6 +23,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .decode import raise_reports
 from .ops import _OPTIONS, _current_device, _dt, _ptr, _raw_stream, _require_cuda
 
 _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
@@ -204,7 +205,8 @@ class Branches:
     def adopt(self, branch, t_next):
         """Branch branch[b] (integers [B] on the GPU) of every sequence becomes the state's own: its tokens join the resident
         state and the active list.  Staged tokens are kept unless `keep` has decided on them.  The next step of every sequence
-        is t_next afterwards, whatever the branches' lengths (not before the longest one's end).  Ends these branches."""
+        is t_next afterwards, whatever the branches' lengths (not before the longest one's end).  Ends these branches; what
+        they have to report goes to the state's overflow word."""
         self._alive()
         self._refuse(branch)
         if branch.shape != (self.B,) or branch.dtype not in _INTEGERS:
@@ -217,7 +219,7 @@ class Branches:
             self._keep(torch.full((self.B,), self._staged, dtype=torch.int64, device=branch.device))
         _lib.check(self._lib.mbema_branches_adopt(self._ref, _ptr(branch), t_next, _raw_stream(self._dev)), "mbema_branches_adopt")
         st._epoch += 1
-        st.overflow.copy_(torch.where(self._hold["overflow"] == 1, self._hold["overflow"], st.overflow))
+        st.overflow.bitwise_or_(self._hold["overflow"])
         if st.t_dev is not None:
             st.t_dev.fill_(t_next)
         self.prefix = None
@@ -235,8 +237,4 @@ class Branches:
     def check_overflow(self):
         """Synchronises; raises if a list overflowed, a token was out of range, or adopt was given a branch or a step that it
         cannot take."""
-        code = int(self._hold["overflow"].item())
-        if code:
-            raise _lib.MbemaError("branches: " + {1: "a list of touched slots (or the state's active list) is full",
-                                                  2: "token outside the vocabulary", 3: "adopt: no such branch",
-                                                  4: "adopt: t_next lies before the end of a branch"}.get(code, "status %d" % code))
+        raise_reports(self._hold["overflow"], "branches")

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
             s_dst[lane] = last && dst < cap ? dst : -1;
             if (first && own < 0) {
                 if (dst < cap) br.own_slot[(size_t)r * cap + dst] = v;
-                else atomicExch(br.overflow, 1);
+                else atomicOr(br.overflow, 1);
             }
             if (last && dst < cap) br.own_t[(size_t)r * cap + dst] = t0 + len + lane;
             if (first && pos >= 0) atomicOr(&br.touched[(size_t)r * words + (pos >> 5)], 1u << (pos & 31));
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
     if (tid < 32) {
         const long long v = lane < n ? tok[r * n + lane] : -1;
         const bool some = lane < n && v >= 0 && v < br.V;
-        if (lane < n && !some && v != -1) atomicExch(br.overflow, 2);
+        if (lane < n && !some && v != -1) atomicOr(br.overflow, 2);
         const unsigned same = __match_any_sync(0xffffffffu, some ? (int)v : -2 - lane);
         s_tok[lane] = some ? (int)v : -1;
         s_same[lane] = same;
@@ -288,10 +288,10 @@ __global__ void k_branch_adopt(mbema_branches br, const long long* __restrict__ 
     const int b = blockIdx.x, tid = threadIdx.x;
     const int N = (int)br.N, cap = (int)br.cap, Kcap = (int)br.Kcap;
     const long long s = branch[b];
-    if (s < 0 || s >= br.S) { if (tid == 0) atomicExch(br.overflow, 3); return; }
+    if (s < 0 || s >= br.S) { if (tid == 0) atomicOr(br.overflow, 8); return; }
     const int64_t r = (int64_t)b * br.S + s;
     const long long shift = t_next - ((long long)br.t0[0] + br.len[r]);
-    if (shift < 0) { if (tid == 0) atomicExch(br.overflow, 4); return; }
+    if (shift < 0) { if (tid == 0) atomicOr(br.overflow, 4); return; }
     const int own_n = br.own_n[r];
     for (size_t e = tid; e < (size_t)own_n * N; e += blockDim.x) {
         const int u = (int)(e / N), c = (int)(e - (size_t)u * N);
@@ -310,7 +310,7 @@ __global__ void k_branch_adopt(mbema_branches br, const long long* __restrict__ 
             const int at = na + __popc(m & ((1u << tid) - 1u));
             if (add && at < Kcap) br.active[(size_t)b * Kcap + at] = v;
             na += __popc(m);
-            if (na > Kcap) { na = Kcap; if (tid == 0) atomicExch(br.overflow, 1); }
+            if (na > Kcap) { na = Kcap; if (tid == 0) atomicOr(br.overflow, 1); }
         }
         if (tid == 0) { br.n_active[b] = na; s_na = na; }
     }

@@ -148,7 +148,7 @@ __global__ void k_decode_update(const long long* __restrict__ tok, const float* 
     const int lane = threadIdx.x & 31;
     if (b >= B) return;
     const long long v = tok[b];
-    if (v < 0 || v >= V) { if (lane == 0) atomicExch(overflow, 2); return; }
+    if (v < 0 || v >= V) { if (lane == 0) atomicOr(overflow, 2); return; }
     const int lt = last_t[(size_t)b * V + v];
     const double dt = (double)(t_now - lt);
     for (int n = lane; n < N; n += 32) {
@@ -162,7 +162,7 @@ __global__ void k_decode_update(const long long* __restrict__ tok, const float* 
         if (lt < 0) {
             const int pos = n_active[b];
             if (pos < Kcap) { active[(size_t)b * Kcap + pos] = (int)v; n_active[b] = pos + 1; }
-            else atomicExch(overflow, 1);
+            else atomicOr(overflow, 1);
         }
         last_t[(size_t)b * V + v] = t_now;
     }

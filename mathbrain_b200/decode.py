@@ -13,6 +13,17 @@ import torch
 from . import _lib
 from .ops import _dt, _ptr, _require_cuda, _stream, get_options
 
+# bits of the overflow words of the state and of its branches
+_REPORTS = ((1, "active-slot list full (the state's, or a branch's of touched slots)"), (2, "token outside the vocabulary"),
+            (4, "adopt: t_next lies before the end of a branch"), (8, "adopt: no such branch"))
+
+
+def raise_reports(word, who):
+    """Synchronises; raises if the overflow word holds anything."""
+    code = int(word.item())
+    if code:
+        raise _lib.MbemaError(who + ": " + "; ".join(text for bit, text in _REPORTS if code & bit))
+
 
 class DecodeState:
     def __init__(self, batch, vocab, rhos, capacity=4096, device="cuda"):
@@ -161,7 +172,6 @@ class DecodeState:
         return 0 if self._ws is None else int(self._ws[:4].view(torch.int32).item())
 
     def check_overflow(self):
-        """Synchronises; raises if an active list overflowed or a token was out of range."""
-        code = int(self.overflow.item())
-        if code:
-            raise _lib.MbemaError("decode state: " + ("active-slot list full" if code == 1 else "token outside the vocabulary"))
+        """Synchronises; raises if an active list overflowed, a token was out of range, or branches that were adopted report
+        such a thing."""
+        raise_reports(self.overflow, "decode state")

@@ -72,3 +72,25 @@ def test_a_state_at_any_offset(N, S, offset):
     view.copy_(st.state)
     st.state = view
     assert view.data_ptr() % 16 != 0 and all(torch.equal(a, b) for a, b in zip(run(), want))
+
+
+def test_reports_do_not_replace_one_another():
+    """A full own list, then a token outside the vocabulary: both are reported, by the branches and, after adopt, by the state."""
+    from mathbrain_b200 import _lib
+    B, V, N, H = 1, 60, 16, 1
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [20], torch.float32, 95)
+    br = st.fork(1, t0, capacity=2, max_new=3)
+    br.extend(torch.tensor([[[10, 11, 12]]]).cuda())
+    br.keep(torch.tensor([3]).cuda())
+    br.extend(torch.tensor([[[V, 11, -1]]]).cuda())
+    br.adopt(torch.tensor([0]).cuda(), t0 + 6)
+    for who in (br, st):
+        for what in ("full", "vocabulary"):
+            with pytest.raises(_lib.MbemaError, match=what):
+                who.check_overflow()
+    other = type(st)(B, V, rhos.cuda(), capacity=1)                   # the state's own reports
+    for t, tok in enumerate((3, 4, V, 5, -2)):
+        other.update(torch.tensor([tok]).cuda(), t)
+    for what in ("full", "vocabulary"):
+        with pytest.raises(_lib.MbemaError, match=what):
+            other.check_overflow()
