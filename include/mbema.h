@@ -364,8 +364,8 @@ int mbema_decode_advance(int32_t* t_now_dev, void* stream);
  *                          with workspaces of their own may run at once
  *   mbema_branches_adopt   moves branch[b] (i64) of every sequence into its prefix; step numbers move so that the next step of
  *                          every sequence is t_next (>= t0 + len)
- * *overflow, a sum of: 1 an own or active list is full, 2 a token is outside [0, V) (and not -1), 4 t_next lies before a branch's
- * end, 8 branch[b] is outside [0, S) (with these two that sequence stays as it was).
+ * *overflow, a sum of: 1 an own or active list is full, 2 a token is outside [0, V) (and not -1), 4 t_next lies before the end of a
+ * branch[b], 8 a branch[b] is outside [0, S) (with these two no sequence is adopted: the whole prefix stays as it was).
  * ---------------------------------------------------------------------------------------------- */
 typedef struct mbema_branches {
     const float* rhos;      /* [N] */

@@ -205,8 +205,9 @@ class Branches:
     def adopt(self, branch, t_next):
         """Branch branch[b] (integers [B] on the GPU) of every sequence becomes the state's own: its tokens join the resident
         state and the active list.  Staged tokens are kept unless `keep` has decided on them.  The next step of every sequence
-        is t_next afterwards, whatever the branches' lengths (not before the longest one's end).  Ends these branches; what
-        they have to report goes to the state's overflow word."""
+        is t_next afterwards, whatever the branches' lengths (not before the longest one's end).  A branch that does
+        not exist or ends behind t_next, in any sequence, leaves the whole state and its step as they were.  Ends these branches
+        in either case; what they have to report goes to the state's overflow word."""
         self._alive()
         self._refuse(branch)
         if branch.shape != (self.B,) or branch.dtype not in _INTEGERS:
@@ -221,7 +222,7 @@ class Branches:
         st._epoch += 1
         st.overflow.bitwise_or_(self._hold["overflow"])
         if st.t_dev is not None:
-            st.t_dev.fill_(t_next)
+            st.t_dev.copy_(torch.where(self._hold["overflow"] >= 4, st.t_dev, t_next))
         self.prefix = None
 
     @property

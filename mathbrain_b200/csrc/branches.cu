@@ -283,15 +283,25 @@ __global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br, int 
     if (!pending) br_wait_for_kernel_before();      // the kernels behind this one wait for it alone
 }
 
-// One branch of every sequence moves into the prefix; step numbers move with it.
+// One branch of every sequence moves into the prefix; step numbers move with it.  All sequences or none: every CTA looks all of them over
+// (nothing that is looked at is written here).
 __global__ void k_branch_adopt(mbema_branches br, const long long* __restrict__ branch, long long t_next) {
     const int b = blockIdx.x, tid = threadIdx.x;
     const int N = (int)br.N, cap = (int)br.cap, Kcap = (int)br.Kcap;
-    const long long s = branch[b];
-    if (s < 0 || s >= br.S) { if (tid == 0) atomicOr(br.overflow, 8); return; }
-    const int64_t r = (int64_t)b * br.S + s;
-    const long long shift = t_next - ((long long)br.t0[0] + br.len[r]);
-    if (shift < 0) { if (tid == 0) atomicOr(br.overflow, 4); return; }
+    const long long t0 = br.t0[0];
+    int bad = 0;
+    for (int i = tid; i < br.B; i += blockDim.x) {
+        const long long s = branch[i];
+        if (s < 0 || s >= br.S) bad |= 8;
+        else if (t_next < t0 + br.len[(int64_t)i * br.S + s]) bad |= 4;
+    }
+    const int no_branch = __syncthreads_or(bad & 8), too_early = __syncthreads_or(bad & 4);
+    if (no_branch || too_early) {
+        if (b == 0 && tid == 0) atomicOr(br.overflow, (no_branch ? 8 : 0) | (too_early ? 4 : 0));
+        return;
+    }
+    const int64_t r = (int64_t)b * br.S + branch[b];
+    const long long shift = t_next - (t0 + br.len[r]);
     const int own_n = br.own_n[r];
     for (size_t e = tid; e < (size_t)own_n * N; e += blockDim.x) {
         const int u = (int)(e / N), c = (int)(e - (size_t)u * N);

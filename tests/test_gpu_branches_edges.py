@@ -94,3 +94,50 @@ def test_reports_do_not_replace_one_another():
     for what in ("full", "vocabulary"):
         with pytest.raises(_lib.MbemaError, match=what):
             other.check_overflow()
+
+
+def _state_of(st):
+    return [getattr(st, k).clone() for k in ("state", "last_t", "active", "n_active")]
+
+
+@pytest.mark.parametrize("what", ["branch", "t_next"])
+@pytest.mark.parametrize("device_step", [False, True])
+def test_a_refused_adopt_moves_no_sequence_and_is_reported(what, device_step):
+    """One sequence's branch (or end) cannot be taken: the whole batch stays where it was, step number included, and the state says so."""
+    from mathbrain_b200 import _lib
+    B, S, V, N, H = 3, 2, 50, 16, 1
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [20, 5, 0], torch.float32, 93)
+    if device_step:
+        st.use_device_step(t0)
+    br = st.fork(S, t0, capacity=8, max_new=3)
+    br.extend(torch.randint(0, V, (B, S, 3), generator=g).cuda())
+    br.keep(torch.tensor([1, 3, 2]).cuda())
+    before = _state_of(st)
+    branch, t_next = (torch.tensor([0, 1, S]), t0 + 3) if what == "branch" else (torch.tensor([0, 1, 1]), t0 + 2)
+    br.adopt(branch.cuda(), t_next)
+    assert all(torch.equal(a, b) for a, b in zip(before, _state_of(st)))
+    if device_step:
+        assert int(st.t_dev) == t0
+    for who in (br, st):
+        with pytest.raises(_lib.MbemaError, match=what):
+            who.check_overflow()
+    # the state goes on from where it stands, and the report stays
+    st.update(torch.tensor([1, 2, V + 3]).cuda(), t0)
+    with pytest.raises(_lib.MbemaError, match=what):
+        st.check_overflow()
+    with pytest.raises(_lib.MbemaError, match="vocabulary"):
+        st.check_overflow()
+
+
+def test_an_adopt_moves_the_device_step():
+    B, S, V, N, H = 2, 2, 50, 16, 1
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [20, 5], torch.float32, 94)
+    st.use_device_step(t0)
+    br = st.fork(S, 0, capacity=8, max_new=3)
+    br.extend(torch.randint(0, V, (B, S, 3), generator=g).cuda())
+    br.keep(torch.tensor([1, 3]).cuda())
+    before = _state_of(st)
+    br.adopt(torch.tensor([1, 0]).cuda(), t0 + 9)
+    assert int(st.t_dev) == t0 + 9 and not torch.equal(before[1], st.last_t)
+    st.check_overflow()
+    br.check_overflow()
