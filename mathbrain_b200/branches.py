@@ -60,7 +60,7 @@ class Branches:
             own_state=torch.empty(B, S, cap, N, **f32), touched=torch.empty(B, S, (Kcap + 31) // 32, **i32),
             st_tok=torch.empty(B, S, max_new, **i32), st_own=torch.empty(B, S, max_new, **i32),
             st_pos=torch.empty(B, S, max_new, **i32), st_same=torch.empty(B, S, max_new, **i32),
-            st_new=torch.empty(B, S, max_new, **i32), st_state=torch.empty(B, S, max_new, N, **f32), overflow=torch.empty(1, **i32))
+            st_new=torch.empty(B, S, max_new, **i32), st_state=torch.empty(B, S, max_new, N, **f32), overflow=torch.zeros(1, **i32))
         self._tensor_cores = N in (64, 128)
         if self._tensor_cores:
             self._hold.update(pre_op=torch.empty(B, (Kcap + 127) // 128 * 128, N, dtype=torch.float16, device=dev),

@@ -141,3 +141,18 @@ def test_an_adopt_moves_the_device_step():
     assert int(st.t_dev) == t0 + 9 and not torch.equal(before[1], st.last_t)
     st.check_overflow()
     br.check_overflow()
+
+
+def test_branches_of_no_sequences_report_nothing():
+    from mathbrain_b200 import synth
+    from mathbrain_b200.decode import DecodeState
+    rhos = synth.make_rhos(64, 2.0, 64.0).cuda()
+    junk = [torch.full((1,), 5, dtype=torch.int32).cuda() for _ in range(64)]          # small blocks that the next allocations get
+    del junk
+    st = DecodeState(0, 30, rhos, capacity=8)
+    br = st.fork(2, 0, capacity=4, max_new=2)
+    br.extend(torch.zeros(0, 2, 1, dtype=torch.int64).cuda())
+    br.check_overflow()
+    br.adopt(torch.zeros(0, dtype=torch.int64).cuda(), 3)
+    br.check_overflow()
+    st.check_overflow()
