@@ -141,15 +141,15 @@ class Branches:
         """O [B, S, n, H, 64] of q's dtype for the n staged rows of every branch.  q [B, S, n, H, 64] float32 or bfloat16;
         E_k, E_v [V, H*64] projected slot embeddings; W_pe [N, H*64].  Softmax over all V_total slots (the vocabulary by
         default), those that a row does not see with score 0 and value 0; listed_only: over the seen ones alone (a row that
-        has seen none gets 0).  E_v is taken in E_k's type.  mode: "fp32", "tc_bf16" or "auto" (the package option `mode` by
-        default): the tensor cores take bfloat16 q and tables with 64 or 128 channels, "auto" runs anything else in fp32
-        arithmetic."""
+        has seen none gets 0).  E_v is taken in E_k's type.  mode: "fp32", "tc_bf16" or "auto".  The tensor cores take
+        bfloat16 q and tables with 64 or 128 channels; "auto" runs anything else in fp32 arithmetic, "tc_bf16" refuses it.
+        Without one the package option `mode` decides: "fp32" as such, the others as "auto"."""
         self._alive()
         dev = self._dev
         if q.get_device() != dev or E_k.get_device() != dev or E_v.get_device() != dev or W_pe.get_device() != dev:
             self._refuse(q, E_k, E_v, W_pe)
-        if mode is None:
-            mode = _OPTIONS["mode"]
+        if mode is None:                       # (the option is a preference, as for a decode step: it refuses nothing)
+            mode = "fp32" if _OPTIONS["mode"] == "fp32" else "auto"
         # checked and sized once for operands of the same shapes, types and options
         key = (q.shape, q.dtype, E_k.shape, E_k.dtype, E_v.shape, E_v.dtype, W_pe.shape, W_pe.dtype, self._staged, V_total, use_silu,
                listed_only, mode)

@@ -156,3 +156,26 @@ def test_branches_of_no_sequences_report_nothing():
     br.adopt(torch.zeros(0, dtype=torch.int64).cuda(), 3)
     br.check_overflow()
     st.check_overflow()
+
+
+@pytest.mark.parametrize("N,dt,qd", [(64, torch.float32, torch.float32), (64, torch.bfloat16, torch.float32), (20, torch.bfloat16, torch.bfloat16)])
+def test_the_package_option_is_a_preference(N, dt, qd):
+    """mode 'tc_bf16' as the package option: operands that the tensor cores do not take go through fp32 arithmetic, as a decode step
+    does; asked for in the call it is refused."""
+    import mathbrain_b200 as mb
+    from mathbrain_b200 import _lib
+    B, S, n, V, H = 1, 2, 2, 60, 1
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [30], dt, 96)
+    tabs = E_k.cuda(), E_v.cuda(), W.cuda()
+    q = torch.randn(B, S, n, H, 64, generator=g).to(qd).cuda()
+    br = st.fork(S, t0, capacity=8, max_new=n)
+    br.extend(torch.randint(0, V, (B, S, n), generator=g).cuda())
+    exact = br.attend(q, *tabs, mode="fp32")
+    was = mb.get_options()["mode"]
+    try:
+        mb.set_options(mode="tc_bf16")
+        assert torch.equal(br.attend(q, *tabs), exact)
+        with pytest.raises(_lib.MbemaError, match="tc_bf16"):
+            br.attend(q, *tabs, mode="tc_bf16")
+    finally:
+        mb.set_options(mode=was)
