@@ -150,6 +150,9 @@ class Branches:
             self._refuse(q, E_k, E_v, W_pe)
         if mode is None:                       # (the option is a preference, as for a decode step: it refuses nothing)
             mode = "fp32" if _OPTIONS["mode"] == "fp32" else "auto"
+        if V_total is not None:                # (numbers: a tensor's value may change between calls)
+            V_total = int(V_total)
+        use_silu, listed_only = bool(use_silu), bool(listed_only)
         # checked and sized once for operands of the same shapes, types and options
         key = (q.shape, q.dtype, E_k.shape, E_k.dtype, E_v.shape, E_v.dtype, W_pe.shape, W_pe.dtype, self._staged, V_total, use_silu,
                listed_only, mode)
@@ -187,7 +190,7 @@ class Branches:
         flags = (_lib.FLAG_SILU if use_silu else 0) | (_lib.FLAG_LISTED_ONLY if listed_only else 0)
         need = self._lib.mbema_branches_attend_workspace_bytes(self.B, self.S, n, H, self.prefix.cap, self.capacity, code)
         cast = E_v.dtype != E_k.dtype or W_pe.dtype != torch.float32
-        return q_dt, e_dt, n, H, int(self.V if V_total is None else V_total), flags, code, need, cast
+        return q_dt, e_dt, n, H, self.V if V_total is None else V_total, flags, code, need, cast
 
     def _attend(self, q, E_k, E_v, W_pe, plan):
         q_dt, e_dt, n, H, V_total, flags, code, need, cast = plan

@@ -179,3 +179,16 @@ def test_the_package_option_is_a_preference(N, dt, qd):
             br.attend(q, *tabs, mode="tc_bf16")
     finally:
         mb.set_options(mode=was)
+
+
+def test_the_number_of_slots_is_read_at_every_call():
+    B, S, n, V, N, H = 1, 2, 1, 60, 16, 1
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [30], torch.float32, 97)
+    tabs = E_k.cuda(), E_v.cuda(), W.cuda()
+    q = torch.randn(B, S, n, H, 64, generator=g).cuda()
+    br = st.fork(S, t0, capacity=8, max_new=n)
+    br.extend(torch.randint(0, V, (B, S, n), generator=g).cuda())
+    total = torch.tensor(V)
+    for v in (V, 4 * V, 40):
+        total.fill_(v)
+        assert torch.equal(br.attend(q, *tabs, V_total=total), br.attend(q, *tabs, V_total=v)), v
