@@ -356,7 +356,9 @@ using namespace mbema;
 
 extern "C" int mbema_branches_init(const mbema_branches* br, int64_t t_now, const int32_t* t_now_dev, void* stream) {
     int rc = check_branches(br);
-    if (rc != MBEMA_OK || br->B == 0) return rc;
+    if (rc != MBEMA_OK) return rc;
+    if (!t_now_dev && (t_now < 0 || t_now > 0x7fffffff)) return MBEMA_ERR_SHAPE;
+    if (br->B == 0) return MBEMA_OK;
     MBEMA_CUDA_TRY(cudaMemsetAsync(br->pos, 0xff, (size_t)br->B * br->V * sizeof(int32_t), (cudaStream_t)stream));
     dim3 grid((unsigned)((br->Kcap + 255) / 256), (unsigned)br->B);
     k_branch_init<<<grid, 256, 0, (cudaStream_t)stream>>>(*br, (int)t_now, t_now_dev);

@@ -32,3 +32,9 @@ def test_buffers_of_the_tensor_cores_are_aligned(lib, name):
     setattr(c, name, addr + 4)
     assert _attend(lib, c, addr, mode=1, dt=1) == 7
     assert lib.mbema_branches_extend(ctypes.byref(c), addr, 1, 0, addr, None) == 7
+
+
+@pytest.mark.parametrize("t_now", [-1, 1 << 31, 1 << 32])
+def test_a_step_outside_its_type_is_refused(lib, t_now):
+    c, _, addr = _branches()
+    assert lib.mbema_branches_init(ctypes.byref(c), t_now, None, None) == 2
