@@ -540,7 +540,7 @@ static BranchPlan branch_plan(int64_t B, int64_t S, int64_t n, int64_t H, int64_
 int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
     const mbema_branches& br = a.br;
     const int64_t jobs = br.B * ((br.S + BA_ROWS - 1) / BA_ROWS) * a.plan.SP * a.plan.JP + br.B * br.S * a.plan.SO;
-    if (jobs > 0x7fffffff || a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
+    if (jobs > 0x7fffffff) return MBEMA_ERR_UNSUPPORTED;
     const size_t smem = ba_smem((int)br.N);
     static std::atomic<unsigned long long> done{0};
     MBEMA_CUDA_TRY(allow_smem(k_branch_attend, ba_smem(128), done));
@@ -606,7 +606,7 @@ extern "C" int mbema_branches_attend(const mbema_branches* br, const void* q, in
     int rc = check_branches(br);
     if (rc != MBEMA_OK) return rc;
     if (!plan_sizes_ok(br->B, br->S, n, H, br->Kcap, br->cap) || n > br->max_new) return MBEMA_ERR_SHAPE;
-    if (hd != BR_HD || (mode != MBEMA_MODE_FP32 && mode != MBEMA_MODE_TC_BF16)) return MBEMA_ERR_UNSUPPORTED;
+    if (hd != BR_HD || H > 65535 || (mode != MBEMA_MODE_FP32 && mode != MBEMA_MODE_TC_BF16)) return MBEMA_ERR_UNSUPPORTED;
     if (mode == MBEMA_MODE_TC_BF16 && (!branch_tc_supported(br->N) || q_dtype != MBEMA_BF16 || e_dtype != MBEMA_BF16)) return MBEMA_ERR_UNSUPPORTED;
     if (br->B == 0) return MBEMA_OK;
     if (!q || !E_k || !E_v || !W_pe || !O || !workspace) return MBEMA_ERR_NULL;

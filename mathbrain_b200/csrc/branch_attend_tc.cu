@@ -682,7 +682,6 @@ static int launch_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
 }
 
 int launch_branch_attend_tc(BranchArgs& a, const BranchShape& p, cudaStream_t st) {
-    if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
     return a.br.N == 64 ? launch_tc<4, 4>(a, p, st) : launch_tc<8, 3>(a, p, st);
 }
 

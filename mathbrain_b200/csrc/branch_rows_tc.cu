@@ -486,7 +486,6 @@ BranchRows branch_rows(int64_t n, int64_t H) {
 }
 
 int launch_branch_rows(const BranchArgs& a, const BranchRows& p, cudaStream_t st) {
-    if (a.H > 65535) return MBEMA_ERR_UNSUPPORTED;
     return a.br.N == 64 ? brows::launch_silu<1>(a, p, st) : brows::launch_silu<2>(a, p, st);
 }
 

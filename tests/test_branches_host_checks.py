@@ -38,3 +38,10 @@ def test_buffers_of_the_tensor_cores_are_aligned(lib, name):
 def test_a_step_outside_its_type_is_refused(lib, t_now):
     c, _, addr = _branches()
     assert lib.mbema_branches_init(ctypes.byref(c), t_now, None, None) == 2
+
+
+@pytest.mark.parametrize("H", [65536, (1 << 32) + 8])
+@pytest.mark.parametrize("S,mode,dt", [(3, 0, 0), (3, 1, 1), (1, 1, 1)])
+def test_more_heads_than_a_grid_holds_are_refused(lib, H, S, mode, dt):
+    c, _, addr = _branches(S=S)
+    assert _attend(lib, c, addr, H=H, mode=mode, dt=dt, nbytes=1 << 62) == 3
