@@ -412,7 +412,8 @@ int mbema_branches_adopt(const mbema_branches* br, const int64_t* branch, int64_
  *   next token: smallest i with sum_{k<=i} w_k > uniforms[G] * sum w, w = max(p_a - q_a, 0) where draft a was rejected (p_a if
  *   that is zero everywhere), w = p_a where the drafts ended; entries that are negative or not finite count as 0; -1: no mass
  *   tokens [R,G+1] i64: the drafts that stand, the next token, then -1
- * Products, differences and sums in 64 bits.
+ * Products, differences and sums in 64 bits, but for a thread's share of a sum: pairs of fp32 (2^-47 relative; in 64 bits where the
+ * share passes fp32's range).  An entry of w that passes it counts as 0, as one that is not finite.
  * ---------------------------------------------------------------------------------------------- */
 int mbema_verify_drafts(const void* p, int64_t p_row, int64_t p_pos, const void* q, int64_t q_row, int64_t q_pos, int dtype,
                         const int64_t* drafted, const float* uniforms, int64_t* n_accepted, int64_t* tokens, int64_t R,

@@ -3,12 +3,14 @@
 // Draft j, drawn from q_j, stands with probability min(1, p_j(x) / q_j(x)): u q < p.  Behind the drafts that stand one token is
 // drawn by inversion, from max(p - q, 0) where a draft was rejected, else from p; the whole then has the target's distribution.
 // Products of two fp32 values, differences and sums are taken in (or with the exactness of) double, so that the token does not depend on
-// how the sum over the vocabulary is split (a border between tokens lies within the rounding of an fp32 sum of 50 000 terms once in a
+// how the sum over the vocabulary is split: a lane's sum of a few dozen weights is a pair of fp32 (2^-47), again in double where it leaves
+// fp32's range, all others are double (a border between tokens lies within the rounding of an fp32 sum of 50 000 terms once in a
 // hundred draws).
 // Bound by the bytes of one row of p (and of q) per sequence, behind a chain of three dependent loads that finds the row.  A
 // cluster of CTAs takes a sequence, so that one sequence alone is not bound by what one SM can load: a warp sums its
 // stretch of the vocabulary, the stretches' sums are exchanged through distributed shared memory, and the CTA whose
-// stretch holds the threshold deals it to its warps once more, so that no warp walks more than a hundred tokens one after another.
+// stretch holds the threshold deals it to its warps once more, so that a warp walks a 288th to a 1152nd of the vocabulary (175 to 44 of
+// 50 257 tokens), 32 at a time.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -164,7 +166,12 @@ __global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
         int i0 = lo + lane;
         for (; i0 + 32 * (VD_BATCH - 1) < hi; i0 += 32 * VD_BATCH) batch(i0, std::true_type());
         if (i0 < hi) batch(i0, std::false_type());
-        const double sum = warp_sum_d((double)s + (double)e);
+        double sum = warp_sum_d((double)s + (double)e);
+        if (!(sum <= 1.7976931348623157e308)) {          // a lane's sum has left fp32's range (the weights themselves are finite): in double
+            sum = 0.0;
+            for (int i = lo + lane; i < hi; i += 32) sum += weight(i);
+            sum = warp_sum_d(sum);
+        }
         if (pass == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         if (lane < VD_CTAS) cluster.map_shared_rank(s_sum, lane)[w_id] = sum;
         cluster.sync();
