@@ -13,7 +13,7 @@
 
 namespace mbema {
 
-static constexpr int BS_THREADS = 128;
+static constexpr int BS_THREADS = 128, OPERAND_THREADS = 256;
 
 // pos[b, active[b, k]] = k over a buffer of -1; empty branches
 __global__ void k_branch_init(mbema_branches br, int t_host, const int* t_dev) {
@@ -37,15 +37,13 @@ __global__ void k_branch_init(mbema_branches br, int t_host, const int* t_dev) {
     }
 }
 
-// One CTA per branch: keeps staged tokens of the call before, then stages the new ones.
-__global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, const long long* __restrict__ tok, int n,
-                                                             const long long* __restrict__ counts, int pending, float* __restrict__ C_q) {
+// One CTA of T threads per branch r: keeps staged tokens of the call before, then stages the new ones.
+template <int T>
+__device__ __forceinline__ void stage_branch(const mbema_branches& br, int64_t r, const long long* __restrict__ tok, int n,
+                                             const long long* __restrict__ counts, int pending, float* __restrict__ C_q) {
     __shared__ int s_tok[BR_MAX_NEW], s_own[BR_MAX_NEW], s_dst[BR_MAX_NEW];
     __shared__ unsigned s_same[BR_MAX_NEW];
     __shared__ int s_n, s_len;
-    br_wait_for_kernel_before();
-    br_let_next_kernel_start();
-    const int64_t r = blockIdx.x;
     const int b = (int)(r / br.S);
     const int tid = threadIdx.x, lane = tid & 31;
     const int N = (int)br.N, cap = (int)br.cap;
@@ -92,7 +90,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
     for (int i = 0; i < pending; ++i) {
         const int dst = s_dst[i];
         if (dst < 0) continue;
-        for (int c = tid; c < N; c += BS_THREADS)
+        for (int c = tid; c < N; c += T)
             br.own_state[((size_t)r * cap + dst) * N + c] = br.st_state[br_index(br, r, i) * N + c] + 1.0f;
     }
     if (n <= 0) return;
@@ -110,7 +108,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
     }
     __syncthreads();
     const int own_n = s_n, base_t = t0 + s_len;
-    for (int u = tid; u < own_n; u += BS_THREADS) {
+    for (int u = tid; u < own_n; u += T) {
         const int slot = br.own_slot[(size_t)r * cap + u];
         for (int i = 0; i < n; ++i)
             if (s_tok[i] == slot) s_own[i] = u;
@@ -126,7 +124,7 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
         br.st_pos[at] = first && own < 0 ? pos : -1;
         br.st_new[at] = first && own < 0 && pos < 0;
     }
-    for (int e = tid; e < n * N; e += BS_THREADS) {
+    for (int e = tid; e < n * N; e += T) {
         const int i = e / N, c = e - i * N;
         const int v = s_tok[i], own = s_own[i];
         double x = 0.0;
@@ -143,14 +141,20 @@ __global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, 
         C_q[((size_t)r * n + i) * N + c] = (float)x;
     }
 }
+__global__ void __launch_bounds__(BS_THREADS) k_branch_stage(mbema_branches br, const long long* __restrict__ tok, int n,
+                                                             const long long* __restrict__ counts, int pending, float* __restrict__ C_q) {
+    br_wait_for_kernel_before();
+    br_let_next_kernel_start();
+    stage_branch<BS_THREADS>(br, blockIdx.x, tok, n, counts, pending, C_q);
+}
 
 // Operand copies of all listed slots at the first staged step, state * rho^(t0 + len - last) / 64 in fp16 (11 significant bits; a
 // state is at most 1 / (1 - rho)): what the tensor cores read for every layer, step and head, in the layouts that branches.cuh gives.
-// grid: x = shares of a list, y = sequence, z = 0: its prefix, s + 1: branch s.  One CTA more (y = B) leaves the running sum of the
-// lists' units that the attention deals its work by.
+// CTA 0 leaves the running sum of the lists' units that the attention deals its work by; of the others `shares` take a list: of the
+// sequences' prefixes, then of their branches 0, of their branches 1 and so on.
 template <typename Count>
 __device__ void running_sum(int2* out, int lists, Count count_of) {
-    __shared__ int s_warp[8];
+    __shared__ int s_warp[OPERAND_THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31;
     int base = 0;
     for (int x0 = 0; x0 < lists; x0 += 256) {
@@ -194,12 +198,11 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&o);
 }
 
-__device__ __forceinline__ void make_operands(const mbema_branches& br) {
-    if (blockIdx.y == br.B) {
+__device__ __forceinline__ void make_operands(const mbema_branches& br, int64_t cta, int shares) {
+    if (cta == 0) {
         int2* work = reinterpret_cast<int2*>(br.work);
         const int blocks = (int)((br.S + BR_BLOCK - 1) / BR_BLOCK), n_pre = (int)br.B * blocks;
         auto prefix = [&](int b) { return min(br.n_active[b], (int)br.Kcap); };
-        if (blockIdx.x > 0 || blockIdx.z > 0) return;
         if (br.S == 1)
             running_sum(work, (int)(2 * br.B), [&](int x, int& cost) {
                 const int count = x & 1 ? br.own_n[x >> 1] : prefix(x >> 1);
@@ -214,12 +217,13 @@ __device__ __forceinline__ void make_operands(const mbema_branches& br) {
             });
         return;
     }
-    const int b = blockIdx.y, z = blockIdx.z;
+    const int64_t list = (cta - 1) / shares;
+    const int share = (int)(cta - 1 - list * shares), z = (int)(list / br.B), b = (int)(list - z * br.B);
     const int N = (int)br.N;
     const int64_t r = (int64_t)b * br.S + (z ? z - 1 : 0);
     const int count = z ? br.own_n[r] : min(br.n_active[b], (int)br.Kcap);
     const int now = br.t0[0] + br.len[r];
-    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5), warps = gridDim.x * 8;
+    const int lane = threadIdx.x & 31, warp = share * 8 + (threadIdx.x >> 5), warps = shares * 8;
     char* out = z ? reinterpret_cast<char*>(br.own_op) + (size_t)r * br_operand_bytes(br.cap, N)
                   : reinterpret_cast<char*>(br.pre_op) + (size_t)b * br_operand_bytes(br.Kcap, N);
     auto source = [&](int slot, float& dt) {
@@ -275,12 +279,14 @@ __device__ __forceinline__ void make_operands(const mbema_branches& br) {
     }
 }
 
-// Without tokens to keep, the staging kernel leaves lists and lengths alone, and the operands need not wait for it; it starts this one only
-// after its own wait, so that all calls before it have ended.
-__global__ void __launch_bounds__(256) k_branch_operands(mbema_branches br, int pending) {
-    if (pending) br_wait_for_kernel_before();
-    make_operands(br);
-    if (!pending) br_wait_for_kernel_before();      // the kernels behind this one wait for it alone
+// BESIDE: without tokens to keep, staging leaves lists and lengths alone and writes nothing that is read here; one kernel then does both,
+// its first CTAs a branch each.  Otherwise the staging kernel comes before.
+template <bool BESIDE>
+__global__ void __launch_bounds__(OPERAND_THREADS) k_branch_operands(mbema_branches br, int shares, const long long* __restrict__ tok, int n, float* __restrict__ C_q) {
+    br_wait_for_kernel_before();
+    const int64_t first = BESIDE ? br.B * br.S : 0;
+    if (blockIdx.x < first) stage_branch<OPERAND_THREADS>(br, blockIdx.x, tok, n, nullptr, 0, C_q);
+    else make_operands(br, blockIdx.x - first, shares);
 }
 
 // One branch of every sequence moves into the prefix; step numbers move with it.  All sequences or none: every CTA looks all of them over
@@ -371,13 +377,20 @@ extern "C" int mbema_branches_extend(const mbema_branches* br, const int64_t* to
     if (n < 1 || n > br->max_new || n_pending < 0 || n_pending > br->max_new) return MBEMA_ERR_SHAPE;
     if (br->B == 0) return MBEMA_OK;
     if (!tok || !C_q) return MBEMA_ERR_NULL;
-    MBEMA_CUDA_TRY(launch_early(k_branch_stage, dim3((unsigned)(br->B * br->S)), BS_THREADS, 0, (cudaStream_t)stream, *br, (const long long*)tok, (int)n, nullptr, (int)n_pending, C_q));
-    rc = check_launch();
-    if (rc != MBEMA_OK || !br->pre_op) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    const long long* tk = (const long long*)tok;
+    const int64_t branches = br->B * br->S;
+    const bool beside = br->pre_op && n_pending == 0;
+    if (!beside) {
+        MBEMA_CUDA_TRY(launch_early(k_branch_stage, dim3((unsigned)branches), BS_THREADS, 0, st, *br, tk, (int)n, nullptr, (int)n_pending, C_q));
+        rc = check_launch();
+        if (rc != MBEMA_OK || !br->pre_op) return rc;
+    }
     // shares of a list: eight CTAs an SM over all lists, one for every 32 or 16 slots where that is enough
-    const int64_t items = 32 / (br->N / 64), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
-    const int64_t x = std::min(longest, std::max<int64_t>(1, 8 * 148 / (br->B * (br->S + 1)) + 1));
-    MBEMA_CUDA_TRY(launch_early(k_branch_operands, dim3((unsigned)x, (unsigned)br->B + 1, (unsigned)(br->S + 1)), 256, 0, (cudaStream_t)stream, *br, (int)n_pending));
+    const int64_t lists = branches + br->B, items = 32 / (br->N / 64), longest = (std::max(br->Kcap, br->cap) + items - 1) / items;
+    const int64_t shares = std::min(longest, std::max<int64_t>(1, 8 * 148 / lists + 1)), ctas = lists * shares + 1;
+    if (beside) MBEMA_CUDA_TRY(launch_early(k_branch_operands<true>, dim3((unsigned)(branches + ctas)), OPERAND_THREADS, 0, st, *br, (int)shares, tk, (int)n, C_q));
+    else MBEMA_CUDA_TRY(launch_early(k_branch_operands<false>, dim3((unsigned)ctas), OPERAND_THREADS, 0, st, *br, (int)shares, tk, (int)n, C_q));
     return check_launch();
 }
 

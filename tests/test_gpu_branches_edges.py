@@ -192,3 +192,42 @@ def test_the_number_of_slots_is_read_at_every_call():
     for v in (V, 4 * V, 40):
         total.fill_(v)
         assert torch.equal(br.attend(q, *tabs, V_total=total), br.attend(q, *tabs, V_total=v)), v
+
+
+@pytest.mark.parametrize("B,S,n,N,H,dt", [(1, 1, 5, 64, 2, torch.bfloat16), (1, 3, 4, 64, 1, torch.bfloat16), (20, 1, 9, 128, 2, torch.bfloat16),
+                                          (2, 2, 6, 24, 2, torch.float32)])
+def test_every_call_sees_what_was_written_before_it(B, S, n, N, H, dt):
+    """Tables, weights, queries and tokens rewritten in place between calls that follow one another without a pause, tokens kept and
+    dropped in turn, against the same calls with the device at rest between them."""
+    V, rounds = 200, 12
+    g, rhos, E_k, E_v, W, st, *_, t0 = _made_up(B, V, N, H, [150 - i for i in range(B)], dt, 98)
+    toks = torch.randint(0, V, (rounds, B, S, n), generator=g).cuda()
+    qs = torch.randn(rounds, B, S, n, H, 64, generator=g).to(dt).cuda()
+    Es = (torch.randn(rounds, 2, V, 64 * H, generator=g) * 0.2).to(dt).cuda()
+    Ws = (torch.randn(rounds, N, 64 * H, generator=g) * 0.1).cuda()
+    counts = torch.randint(0, n + 1, (rounds, B), generator=g).cuda()
+
+    def run(pause):
+        br = st.fork(S, t0, capacity=rounds * n, max_new=n)
+        tok, q, E, w = toks[0].clone(), qs[0].clone(), Es[0].clone(), Ws[0].clone()
+        out = []
+        for i in range(rounds):
+            for dst, src in ((tok, toks), (E, Es), (q, qs), (w, Ws)):
+                dst.copy_(src[i])
+            pause()
+            C = br.extend(tok)
+            pause()
+            O = br.attend(q, E[0], E[1], w)
+            w.mul_(0.5)
+            q.mul_(2.0)
+            pause()
+            O2 = br.attend(q, E[0], E[1], w)
+            pause()
+            if i % 3:
+                br.keep(counts[i])
+                pause()
+            out += [C, O, O2]
+        br.check_overflow()
+        return out
+
+    assert all(torch.equal(a, b) for a, b in zip(run(lambda: None), run(torch.cuda.synchronize)))
