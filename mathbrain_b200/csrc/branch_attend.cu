@@ -312,47 +312,66 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a, in
     const int j_first = (int)(rest_id - r * JB) * RJ, rows = min(RJ, n - j_first);
     const int b = (int)(r / br.S), s = (int)(r - (int64_t)b * br.S);
     const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
-    // the staged tokens do not wait for the kernel before, which has seen the calls before it end
+    // The staged tokens do not wait for the kernel before, and no ordinary load reads global memory up to the wait.  (With the wait here: 8 drafted
+    // rows of one sequence 19.4 us for 17.3, 64 sequences of 6 rows 360 for 342, the same lists in fp32 arithmetic 36.5 for 33.3.)
     for (int jj = 0; jj < rows; ++jj) {
         const int j = j_first + jj;
         float M = -INFINITY, L = 0.f;
         float2 o = make_float2(0.f, 0.f);
         for (int i0 = 0; i0 < j; i0 += BM_STAGED) {
             const int cnt = min(BM_STAGED, j - i0);
-            // loads that depend on no other first: eight rows of W, the states; a warp's two tokens' E rows are on their way while the
-            // states are made
+            // loads that depend on no other first: a warp's two tokens, eight rows of W, a thread's first states; then the tokens' E rows
             auto W_rows = [&](float2 (&w)[8], int c0) {
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     const int c = c0 + u * BM_WARPS;
-                    w[u] = c < N ? Wc[(size_t)c * (D / 2)] : make_float2(0.f, 0.f);
+                    w[u] = c < N ? ld_gpu(Wc + (size_t)c * (D / 2)) : make_float2(0.f, 0.f);
                 }
             };
             float2 w[8];
+            int token[2];
+            unsigned same[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const size_t at = br_index(br, r, min(i0 + warp + e * BM_WARPS, j - 1));
+                token[e] = ld_gpu(br.st_tok + at);
+                same[e] = (unsigned)ld_gpu(reinterpret_cast<const int*>(br.st_same) + at);
+            }
             W_rows(w, warp);
+            float x[4], rho[4];
+            auto load_states = [&](int e0) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = min(e0 + u * BM_WARPS * 32, cnt * N - 1), i = e / N, c = e - i * N;
+                    x[u] = ld_gpu(br.st_state + br_index(br, r, i0 + i) * N + c);
+                    rho[u] = ld_gpu(br.rhos + c);
+                }
+            };
+            load_states(threadIdx.x);
             float2 ek[2], ev[2], q = make_float2(0.f, 0.f);
             bool see[2];
             const size_t qoff = (((size_t)r * n + j) * H + h) * BR_HD + 2 * lane;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int place = i0 + warp + e * BM_WARPS;
-                see[e] = place < j;
-                const size_t at = br_index(br, r, see[e] ? place : 0);
-                const int v = br.st_tok[at];
                 // none, or repeated before this row (j <= 31)
-                see[e] = see[e] && v >= 0 && ((br.st_same[at] & ((1u << j) - 1u)) >> place) == 1u;
+                see[e] = place < j && token[e] >= 0 && ((same[e] & ((1u << j) - 1u)) >> place) == 1u;
                 ek[e] = ev[e] = make_float2(0.f, 0.f);
                 if (see[e]) {
-                    const size_t off = (size_t)v * D + h * BR_HD + 2 * lane;
-                    ek[e] = make_float2(ld_dyn_f32(a.Ek, a.e_dt, off), ld_dyn_f32(a.Ek, a.e_dt, off + 1));
-                    ev[e] = make_float2(ld_dyn_f32(a.Ev, a.e_dt, off), ld_dyn_f32(a.Ev, a.e_dt, off + 1));
-                    q = make_float2(ld_dyn_f32(a.q, a.q_dt, qoff), ld_dyn_f32(a.q, a.q_dt, qoff + 1));
+                    const size_t off = (size_t)token[e] * D + h * BR_HD + 2 * lane;
+                    ek[e] = ld_gpu_pair(a.Ek, a.e_dt, off);
+                    ev[e] = ld_gpu_pair(a.Ev, a.e_dt, off);
+                    q = ld_gpu_pair(a.q, a.q_dt, qoff);
                 }
             }
             __syncthreads();
-            for (int e = threadIdx.x; e < cnt * N; e += BM_WARPS * 32) {
-                const int i = e / N, c = e - i * N;
-                s_c[c][i] = (br.st_state[br_index(br, r, i0 + i) * N + c] + 1.0f) * exp2f((float)(j - i0 - i) * br_log2(br.rhos[c]));
+            for (int e0 = threadIdx.x; e0 < cnt * N; e0 += 4 * BM_WARPS * 32) {
+                if (e0 >= 4 * BM_WARPS * 32) load_states(e0);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = e0 + u * BM_WARPS * 32, i = e / N, c = e - i * N;
+                    if (e < cnt * N) s_c[c][i] = (x[u] + 1.0f) * exp2f((float)(j - i0 - i) * br_log2(rho[u]));
+                }
             }
             __syncthreads();
             float x0[BM_STAGED], x1[BM_STAGED];
@@ -398,27 +417,30 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a, in
         if (lane == 0) s_ml[jj][warp] = make_float2(M, L);
         s_o[jj][warp][lane] = o;
     }
-    const int na = min(br.n_active[b], (int)br.Kcap);
+    const int na = min(ld_gpu(br.n_active + b), (int)br.Kcap);
+    const int own_new = ld_gpu(br.own_new + r);
     // partials of step j_first: np of the prefix from p0 on, then nq of the own slots from q0 on, p_step and q_step apart; of the next step
     // j_step further
     int np, nq;
     size_t p0, q0, p_step, q_step, j_step;
     if constexpr (PIECES) {
-        const int2* work = reinterpret_cast<const int2*>(br.work);
+        auto unit_at = [&](int list) { return ld_gpu(br.work + 2 * (size_t)list); };          // the running sum of the lists' units
+        struct Units { int lo, hi; };
         const size_t each = (size_t)n * H, at = (size_t)j_first * H + h;
         const bool one = br.S == 1;
-        const int total = work[a.lists].x, workers = branch_workers(total, a.max_workers, one ? 1 : BR_LEAST_COST);
-        auto pieces = [&](int list, int unit, int& first) {
-            const int lo = work[list].x, hi = work[list + 1].x;
-            first = 0;
-            if (hi == lo) return 0;
-            first = branch_worker_of(total, workers, lo);
-            return branch_worker_of(total, workers, hi - unit) - first + 1;
-        };
         const int pre = one ? 2 * b : b * a.blocks + s / BR_BLOCK, own = one ? 2 * b + 1 : a.n_pre + (int)r;
+        const int total = unit_at(a.lists);
+        const Units in_pre = {unit_at(pre), unit_at(pre + 1)}, in_own = {unit_at(own), unit_at(own + 1)};
+        const int workers = branch_workers(total, a.max_workers, one ? 1 : BR_LEAST_COST);
+        auto pieces = [&](Units u, int unit, int& first) {
+            first = 0;
+            if (u.hi == u.lo) return 0;
+            first = branch_worker_of(total, workers, u.lo);
+            return branch_worker_of(total, workers, u.hi - unit) - first + 1;
+        };
         int wp, wq;
-        np = pieces(pre, one ? 1 : BR_COST_BLOCK, wp);
-        nq = pieces(own, one ? 1 : BR_COST_OWN, wq);
+        np = pieces(in_pre, one ? 1 : BR_COST_BLOCK, wp);
+        nq = pieces(in_own, one ? 1 : BR_COST_OWN, wq);
         q_step = each;
         j_step = H;
         if (one) {
@@ -435,13 +457,12 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a, in
     } else {
         const int SP = a.plan.SP, SO = a.plan.SO;
         np = (na + a.plan.chp - 1) / a.plan.chp;
-        nq = (br.own_n[r] + a.plan.cho - 1) / a.plan.cho;
+        nq = (ld_gpu(br.own_n + r) + a.plan.cho - 1) / a.plan.cho;
         p_step = q_step = 1;
         j_step = (size_t)H * (SP + SO);
         p0 = (((size_t)r * n + j_first) * H + h) * (SP + SO);
         q0 = p0 + SP;
     }
-    const int own_new = br.own_new[r];
     br_wait_for_kernel_before();
     // joins the warp's share of a step's partials (every share-th) to (M, L, o)
     auto join = [&](int jj, int first, int share, float& M, float& L, float2& o) {

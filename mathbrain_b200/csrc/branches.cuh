@@ -140,8 +140,8 @@ inline cudaError_t allow_smem(Kernel kernel, size_t most, std::atomic<unsigned l
 }
 
 // A kernel whose CTAs may start while the kernel before it still runs; it waits for that one's end with br_wait_for_kernel_before.  All
-// kernels here wait before their first access and only then let the next one start (the merge and the operands reach further: see there);
-// so a kernel's end means the end of all before it.  A launch costs about 2 us less.
+// kernels here wait before their first access and only then let the next one start (but for the merge, which begins with ld_gpu); so a
+// kernel's end means the end of all before it.  A launch costs about 2 us less.
 template <typename... Params, typename... Args>
 inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
@@ -158,6 +158,31 @@ inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int thread
 }
 __device__ __forceinline__ void br_wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void br_let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Loads of a kernel that has not waited yet, of what the kernels before the one directly before it wrote.  It starts only after every CTA of
+// that one has waited, so those have ended and their writes are in L2; but it is the own wait that makes them visible to ordinary loads,
+// which might be served from a line that L1 holds from before.  Loads at the scope of the GPU are not.  (volatile: an asm without it may
+// run ahead of the condition that guards its address.)
+__device__ __forceinline__ int ld_gpu(const int* p) {
+    int x;
+    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(x) : "l"(p));
+    return x;
+}
+__device__ __forceinline__ float ld_gpu(const float* p) {
+    float x;
+    asm volatile("ld.relaxed.gpu.global.f32 %0, [%1];" : "=f"(x) : "l"(p));
+    return x;
+}
+__device__ __forceinline__ float2 ld_gpu(const float2* p) {
+    float2 x;
+    asm volatile("ld.relaxed.gpu.global.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "l"(p));
+    return x;
+}
+__device__ __forceinline__ float2 ld_gpu_pair(const void* p, int dt, size_t i) {       // elements i, i + 1 (i even) of fp32 or bf16
+    if (dt == MBEMA_F32) return ld_gpu(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p) + i));
+    const uint32_t x = (uint32_t)ld_gpu(reinterpret_cast<const int*>(reinterpret_cast<const __nv_bfloat16*>(p) + i));
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
 
 // Two fp32 values as one operand: one instruction for two FMA, at the same rate (it is issue slots that run short).
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
