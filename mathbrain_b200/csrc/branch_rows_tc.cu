@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             const int sub = lane >> 3;
             const uint32_t base = smem_u32(sm) + (warp == WARP_K ? L::EK : L::EV);
             const uint32_t even = base + sub * 128 + (((lane & 7) ^ sub) << 4), odd = base + (sub + 4) * 128 + (((lane & 7) ^ (sub + 4)) << 4);
-            Cursor cur[IG];
+            Cursor cur[IG] = {};
             int ids[IG][4];                                       // of each worker's next tile
             auto fetch_ids = [&](int g) {
                 const int* slots = a.row_slots(cur[g].list);
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_branch_rows(BranchArgs a, int JW
             asm volatile("cp.async.wait_all;" ::: "memory");
         } else if (warp == WARP_A) {
             // ------------------------------------------------------------ operand copies
-            Cursor cur[IG];
+            Cursor cur[IG] = {};
 #pragma unroll 1
             for (int g = 0; g < IG; ++g)
                 if (count_of[g] > 0) cur[g].start(search, work, lists, total, workers, me0 + g, lane);
