@@ -31,8 +31,9 @@ _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 class Branches:
     """Made by DecodeState.fork.  While the branches live the state must not be updated (its own tokens are the branches'
-    prefix); a call on them after an update raises (one by a replayed graph is not noticed).  Memory: 6 N bytes for each of
-    capacity slots a branch, and, with 64 or 128 channels, 2 N bytes for each slot of the state's capacity."""
+    prefix); a call on them after an update raises (one by a replayed graph is not noticed).  Memory: 4 bytes for each token of the
+    vocabulary a sequence, 4 N (with 64 or 128 channels 6 N) for each of capacity slots a branch, and, with 64 or 128 channels, 2 N for
+    each slot of the state's capacity."""
 
     def __init__(self, prefix, branches, t_now, capacity=1024, max_new=16):
         B, V, N, Kcap = prefix.B, prefix.V, prefix.N, prefix.cap
@@ -143,7 +144,8 @@ class Branches:
         default), those that a row does not see with score 0 and value 0; listed_only: over the seen ones alone (a row that
         has seen none gets 0).  E_v is taken in E_k's type.  mode: "fp32", "tc_bf16" or "auto".  The tensor cores take
         bfloat16 q and tables with 64 or 128 channels; "auto" runs anything else in fp32 arithmetic, "tc_bf16" refuses it.
-        Without one the package option `mode` decides: "fp32" as such, the others as "auto"."""
+        Without one the package option `mode` decides: "fp32" as such, the others as "auto".
+        On the tensor cores states and W_pe are fp16 operands: states above 4.19 million and |W_pe| above 1023 count as that."""
         self._alive()
         dev = self._dev
         if q.get_device() != dev or E_k.get_device() != dev or E_v.get_device() != dev or W_pe.get_device() != dev:

@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(BM_WARPS * 32) k_branch_merge(BranchArgs a, in
     const int b = (int)(r / br.S), s = (int)(r - (int64_t)b * br.S);
     const float2* Wc = reinterpret_cast<const float2*>(a.W + h * BR_HD + 2 * lane);
     // The staged tokens do not wait for the kernel before, and no ordinary load reads global memory up to the wait.  (With the wait here: 8 drafted
-    // rows of one sequence 19.4 us for 17.3, 64 sequences of 6 rows 360 for 342, the same lists in fp32 arithmetic 36.5 for 33.3.)
+    // rows of one sequence 2 us more of 17, 64 sequences of 6 rows 18 of 335, 2 x 5 branches of 3 rows in fp32 arithmetic 3 of 33.)
     for (int jj = 0; jj < rows; ++jj) {
         const int j = j_first + jj;
         float M = -INFINITY, L = 0.f;
@@ -570,9 +570,9 @@ int launch_branch_attend_fp32(const BranchArgs& a, cudaStream_t st) {
 }
 
 int launch_branch_merge(const BranchArgs& a, bool pieces, cudaStream_t st) {
-    // eight steps a CTA where three CTAs an SM are left: W then crosses L2 less often (64 sequences of 6 drafted rows with their attention: 394 us,
-    // with a step a CTA 9 more); a step a CTA otherwise, as its loads then do not wait for one another (8 drafted rows of one sequence: 17 us,
-    // with eight 12 more)
+    // eight steps a CTA where three CTAs an SM are left: W then crosses L2 less often (64 sequences of 6 drafted rows with their attention: 335 us,
+    // with a step a CTA 14 more); a step a CTA otherwise, as its loads then do not wait for one another (8 drafted rows of one sequence: 17 us,
+    // with eight 15 more)
     const int64_t heads = a.br.B * a.br.S * a.H;
     const int RJ = heads * ((a.n + BM_ROWS - 1) / BM_ROWS) >= 3 * 148 ? std::min(a.n, BM_ROWS) : 1;
     const int64_t ctas = heads * ((a.n + RJ - 1) / RJ);

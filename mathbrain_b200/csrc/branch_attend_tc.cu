@@ -16,7 +16,7 @@
 // Own slots go through tcgen05 in branch_rows_tc.cu's tiles of 128 slots too, but not faster: with its two gathering warps and a list's start
 // and end (own lists are short) 4 x 16 branches of 400 own slots took half as long again, 64 branches of 180 a quarter.
 // 64 branches of 180 own slots behind a prefix of 3400, 8 heads, 64 channels: 24 us with 11 units a warp, of which 5 us until the first
-// unit is there, 3 for the ends of lists and 13 for the units' arithmetic (750 instructions each, 39 % of the issue slots: two warps a
+// unit is there, 3 for the ends of lists and 13 for the units' arithmetic (690 instructions each, 37 % of the issue slots: two warps a
 // scheduler, as W and the accumulators leave registers for).
 #include <algorithm>
 

@@ -10,7 +10,7 @@
 // Roles: three epilogue groups of four warps; two warps gather the E_k and E_v rows (cp.async, mbarrier arrivals), one lane copies
 // the operands, one issues the products.  With one step the groups are workers with stretches of their own, a tile each in turn; with
 // two or three steps they take the same tile, a step each.
-// 64 sequences, 3400 + 90 slots, 6 rows, 8 heads, 64 channels: 330 us (0.56e9 tanh of 16 a clock and SM would be 122).  Of a tile's 3700 cycles
+// 64 sequences, 3400 + 90 slots, 6 rows, 8 heads, 64 channels: 323 us (0.56e9 tanh of 16 a clock and SM would be 122).  Of a tile's 3700 cycles
 // the three epilogue warps of a scheduler have MUFU work for 1540 and instructions for about 2100; the rest are waits that three warps, which
 // is what o[64] leaves registers for, do not hide.  The two passes written out (372 us without), the mask before the waits, two FMA to an
 // instruction (10 us).  V rounded to bf16 with P . V in mixed-precision FMA needs fewer instructions, but they and the conversions run at half

@@ -5,8 +5,8 @@
 //     C_i = kept value * rho^(t_i - t_kept) + sum over staged i' < i with the same token of rho^(t_i - t_i'),
 // linear in its occurrences, so all staged tokens are independent of one another; powers and sums in double, rounded once (a
 // token repeated at every step amplifies a bias of rho by 1/(1 - rho)).
-// Bound by latency: chains of a few dependent loads for B S n rows of 4 N bytes (5 us).  The operand copies beside it move 6 N bytes a
-// listed slot: 84 MB for 64 x 3400 slots of 64 channels, 16 us (13 at the memory's measured rate).
+// Bound by latency: chains of a few dependent loads for B S n rows of 4 N bytes (3 us).  The operand copies beside it move 6 N bytes a
+// listed slot: 84 MB for 64 x 3400 slots of 64 channels, 17 us (13 at the memory's measured rate).
 #include <algorithm>
 
 #include "branches.cuh"

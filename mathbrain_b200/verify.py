@@ -21,8 +21,8 @@ def verify_drafts(p_target, drafted, uniforms, p_draft=None):
     p_draft [R, G, V] probabilities the drafts were drawn from (p_target's dtype), or None for drafts that were not drawn: draft
         j then stands with probability p_j and its token is left out of the draw otherwise.
 
-    A draw takes the smallest i whose running sum of weights passes uniform * their total; probabilities that are negative or
-    not finite count as 0 there.  G = 0 draws from p_target alone."""
+    A draw takes the smallest i whose running sum of weights (p, or p - q where a draft was rejected) passes uniform * their total;
+    weights that are negative, not finite or beyond fp32 count as 0.  G = 0 draws from p_target alone."""
     dev = p_target.get_device()
     if dev < 0 or drafted.get_device() != dev or uniforms.get_device() != dev or (p_draft is not None and p_draft.get_device() != dev):
         _require_cuda(p_target, drafted, uniforms, p_draft)
