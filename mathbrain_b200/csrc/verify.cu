@@ -94,9 +94,10 @@ __device__ __forceinline__ int pick(const double* sums, double thr, double& befo
     return __shfl_sync(0xffffffffu, hits ? hit : some, from);
 }
 
-// CTAS: of a cluster, 2 to 8
+// CTAS: of a cluster, 2 to 8.  Four CTAs an SM, which the choice of the cluster below counts on: 42 registers a thread (with 44, 109 sequences of
+// 7 drafts and 32 000 tokens take two waves, 14 us for 11).
 template <int DT, int VD_CTAS>
-__global__ void __launch_bounds__(VD_THREADS) k_verify(VerifyArgs a) {
+__global__ void __launch_bounds__(VD_THREADS, 4) k_verify(VerifyArgs a) {
     constexpr int VD_LANE = (VD_CTAS * VD_WARPS + 31) / 32;      // stretches a lane holds
     __shared__ double s_sum[VD_LANE * 32];         // sums of all stretches of the row, in vocabulary order, then zeros
     __shared__ double s_sub[32];
